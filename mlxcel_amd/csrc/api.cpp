@@ -27,106 +27,12 @@
 
 #include "../../include/mlxq.h"
 #include "common.hpp"
+#include "host.hpp"
 #include "kernels.hpp"
 
 namespace {
 
-using Shape = std::vector<int64_t>;
-
-thread_local std::string g_last_error;
-
-struct Error {
-  mlxq_status code;
-  std::string msg;
-};
-
-[[noreturn]] void fail(mlxq_status code, const std::string& msg) { throw Error{code, msg}; }
-[[noreturn]] void invalid(const std::ostringstream& os) { fail(MLXQ_EINVAL, os.str()); }
-[[noreturn]] void unsupported(const std::string& msg) { fail(MLXQ_EUNSUPPORTED, "[mlxq] " + msg); }
-
-void hip_check(hipError_t e, const char* what) {
-  if (e != hipSuccess) fail(MLXQ_EHIP, std::string("[mlxq] ") + what + ": " + hipGetErrorString(e));
-}
-
-template <typename F>
-mlxq_status guarded(F&& f) {
-  try {
-    f();
-    g_last_error.clear();
-    return MLXQ_OK;
-  } catch (const Error& e) {
-    g_last_error = e.msg;
-    return e.code;
-  } catch (const std::exception& e) {
-    g_last_error = std::string("[mlxq] internal error: ") + e.what();
-    return MLXQ_EHIP;
-  }
-}
-
-// ---- dtype facts (mlx::core::Dtype order) ----------------------------------
-
-const char* dtype_name(int d) {
-  static const char* names[] = {"bool",  "uint8",   "uint16",  "uint32",  "uint64",
-                                "int8",  "int16",   "int32",   "int64",   "float16",
-                                "float32", "float64", "bfloat16", "complex64"};
-  return (d >= 0 && d <= 13) ? names[d] : "unknown";
-}
-bool is_floating(int d) { return d == MLXQ_FLOAT16 || d == MLXQ_FLOAT32 || d == MLXQ_FLOAT64 || d == MLXQ_BFLOAT16; }
-bool is_integral(int d) { return d >= MLXQ_BOOL + 1 && d <= MLXQ_INT64; }
-int dtype_size(int d) {
-  static const int sz[] = {1, 1, 2, 4, 8, 1, 2, 4, 8, 2, 4, 8, 2, 8};
-  return (d >= 0 && d <= 13) ? sz[d] : 0;
-}
-
-// Upstream MLX promote_types for the floating types this op layer meets
-// (jax-style lattice: f16+bf16 -> f32, anything with f32/f64 -> the wider).
-int promote(int a, int b) {
-  if (a == b) return a;
-  if (!is_floating(a) && !is_floating(b)) return a < b ? b : a;  // stays integral
-  if (a == MLXQ_FLOAT64 || b == MLXQ_FLOAT64) return MLXQ_FLOAT64;
-  if (is_floating(a) && !is_floating(b)) return a;
-  if (is_floating(b) && !is_floating(a)) return b;
-  return MLXQ_FLOAT32;  // f16/bf16/f32 mixes
-}
-
-// ---- array views -------------------------------------------------------------
-
-struct View {
-  const mlxq_array* a = nullptr;
-  int64_t dim(int i) const { return a->shape[i < 0 ? i + a->ndim : i]; }
-  int ndim() const { return a->ndim; }
-  Shape shape() const { return Shape(a->shape, a->shape + a->ndim); }
-  int dtype() const { return a->dtype; }
-  int64_t size() const {
-    int64_t s = 1;
-    for (int i = 0; i < a->ndim; i++) s *= a->shape[i];
-    return s;
-  }
-  bool row_contiguous() const {
-    int64_t st = 1;
-    for (int i = a->ndim - 1; i >= 0; i--) {
-      if (a->shape[i] != 1 && a->strides[i] != st) return false;
-      st *= a->shape[i];
-    }
-    return true;
-  }
-};
-
-std::string fmt_shape(const Shape& s) {
-  std::ostringstream os;
-  os << "(";
-  for (size_t i = 0; i < s.size(); i++) os << s[i] << (i + 1 == s.size() ? "" : ",");
-  os << ")";
-  return os.str();
-}
-
-void check_array(const mlxq_array* a, const char* name) {
-  if (!a) fail(MLXQ_EINVAL, std::string("[mlxq] ") + name + " must not be NULL");
-  if (a->ndim < 0 || a->ndim > MLXQ_MAX_DIMS)
-    fail(MLXQ_EINVAL, std::string("[mlxq] ") + name + " has an invalid ndim");
-  for (int i = 0; i < a->ndim; i++)
-    if (a->shape[i] < 0) fail(MLXQ_EINVAL, std::string("[mlxq] ") + name + " has a negative dimension");
-}
+using namespace mlxq::host;
 
 Shape broadcast_shapes(const Shape& s1, const Shape& s2) {
   const size_t nd = std::max(s1.size(), s2.size());
@@ -410,7 +316,9 @@ void write_shape(const Shape& s, int dtype, int32_t* ndim, int64_t* shape, int32
   if (out_dtype) *out_dtype = dtype;
 }
 
-void check_out(const mlxq_array* out, const Shape& shape, int dtype, const char* tag) {
+}  // namespace
+
+void mlxq::host::check_out(const mlxq_array* out, const Shape& shape, int dtype, const char* tag) {
   check_array(out, "out");
   if (View{out}.shape() != shape || out->dtype != dtype) {
     std::ostringstream os;
@@ -419,6 +327,8 @@ void check_out(const mlxq_array* out, const Shape& shape, int dtype, const char*
     invalid(os);
   }
 }
+
+namespace {
 
 void require_contiguous(const mlxq_array* a, const char* name) {
   if (a && !View{a}.row_contiguous())
@@ -448,16 +358,18 @@ struct Workspace {
   std::vector<void*> retired;
   size_t retired_bytes = 0;
 };
-// key: (device, stream, slot); slot 0 holds kernel scratch, slot 1 the
-// row-contiguous copies of strided operands, slot 2 the flat index lists of
-// gathers run in chunks
+// key: (device, stream, slot); the slots are listed in host.hpp
 std::map<std::tuple<int, hipStream_t, int>, Workspace> g_ws;
 
-int current_device() {
+}  // namespace
+
+int mlxq::host::current_device() {
   int dev = 0;
   hip_check(hipGetDevice(&dev), "hipGetDevice");
   return dev;
 }
+
+namespace {
 
 DevInfo device_info(int dev) {
   std::lock_guard<std::mutex> lk(g_mu);
@@ -526,6 +438,26 @@ void alloc_counters(Workspace& w, hipStream_t stream) {
   grow_workspace(w, (size_t)mlxq::kSplitCounters * sizeof(uint32_t));
   hip_check(hipMemsetAsync(w.data, 0, w.bytes, stream), "hipMemsetAsync (stream-K counters)");
 }
+
+}  // namespace
+
+int mlxq::host::device_cus(int dev) { return device_info(dev).cus; }
+
+void* mlxq::host::stream_workspace(int dev, hipStream_t stream, size_t bytes, int slot) {
+  return workspace(dev, stream, bytes, ScratchSrc{}, slot);
+}
+
+uint32_t* mlxq::host::stream_counters(int dev, hipStream_t stream) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  Workspace& c = g_ws[{dev, stream, 3}];
+  if (!c.data) {
+    if (stream_capturing(stream)) return nullptr;
+    alloc_counters(c, stream);
+  }
+  return static_cast<uint32_t*>(c.data);
+}
+
+namespace {
 
 // Whether a call may take `bytes` of scratch without allocating under a
 // capture (or past the fixed scratch).
@@ -932,12 +864,14 @@ QmmSpec check_quantized_matmul(const mlxq_array* x, const mlxq_array* w, const m
 
 // ---- row-contiguous staging of strided operands --------------------------
 
-bool needs_staging(const mlxq_array* a) {
+}  // namespace
+
+bool mlxq::host::needs_staging(const mlxq_array* a) {
   if (!a || View{a}.size() == 0) return false;
   return !View{a}.row_contiguous() || (reinterpret_cast<uintptr_t>(a->data) & 15u) != 0;
 }
 
-mlxq_array contiguous_like(const mlxq_array* a, void* data) {
+mlxq_array mlxq::host::contiguous_like(const mlxq_array* a, void* data) {
   mlxq_array c = *a;
   c.data = data;
   int64_t st = 1;
@@ -948,7 +882,7 @@ mlxq_array contiguous_like(const mlxq_array* a, void* data) {
   return c;
 }
 
-void copy_view(const mlxq_array* src, const mlxq_array* dst, hipStream_t stream) {
+void mlxq::host::copy_view(const mlxq_array* src, const mlxq_array* dst, hipStream_t stream) {
   mlxq::CopyArgs c{};
   c.src = src->data;
   c.dst = dst->data;
@@ -962,6 +896,8 @@ void copy_view(const mlxq_array* src, const mlxq_array* dst, hipStream_t stream)
   }
   hip_check(mlxq::launch_strided_copy(c, stream), "strided copy launch");
 }
+
+namespace {
 
 // The operands of one call as the kernels need them: row-contiguous and
 // 16-byte aligned.  Others are first copied into the stream's staging
