@@ -334,6 +334,101 @@ mlxq_status mlxq_fused_moe_geglu(const mlxq_array* x, const mlxq_array* indices,
                                  int32_t dff, int32_t k, int32_t gu_bits, int32_t d_bits,
                                  int32_t group_size, mlxq_array* out, void* stream);
 
+/* ---- serving operators around the projections ------------------------------
+ * Their errors read "[operator] what is wrong": MLXQ_EINVAL for arguments that
+ * do not fit together, MLXQ_EUNSUPPORTED for layouts and sizes that are not
+ * implemented.  Values of device arrays (lengths, page numbers, rows, tokens)
+ * are not read by the host; the kernels never follow one that is out of range.
+ *
+ * The cache: pools [pages][kv heads][page][width] of keys and of values, one
+ * pair per layer; table (rows, width) int32, the pages of each sequence in
+ * order; lengths (rows) int32, its tokens; refs (pages) int32, how many
+ * sequences hold a page (0: free).  A sequence of n tokens holds the first
+ * ceil(n / page) entries of its row; what the others hold is never read.
+ * Bookkeeping arrays have dense rows. */
+
+/* out[b][h] = sum_t p_t v_t over the sequence's keys, p = softmax of
+ * softcap * tanh(q . k_t * scale / softcap) (softcap 0: of q . k_t * scale),
+ * for one query token per sequence.
+ * q, out: (B, query heads, width), bfloat16, float16 or float32, any strides;
+ * k_pool, v_pool: of the same type, the last axis contiguous, any other
+ * strides; query heads a multiple of the pools'; width a multiple of 8 up to
+ * 256.  table (B, n), lengths (B): a length is cut to the n pages, one of 0 or
+ * less gives zeros.  window > 0: only the last `window` keys.  sinks: NULL or
+ * float32 (query heads), logits that join each head's sum without a value.
+ * Keys outside the sequence are not read; page numbers out of range are
+ * clamped.  Scores, probabilities and sums are held in 32 bits, the result is
+ * rounded once. */
+mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool,
+                                 const mlxq_array* v_pool, const mlxq_array* table,
+                                 const mlxq_array* lengths, const mlxq_array* sinks, float scale,
+                                 float softcap, int32_t window, mlxq_array* out, void* stream);
+
+/* Pages for counts[r] more tokens of every row r, in the rows' order, the
+ * lowest free pages first: enters them in the table, sets their refs to 1 and
+ * lengths[r] += counts[r].  granted[r] (int32) is 0 for a row that the free
+ * pages or the table's width do not hold, or whose count or length is
+ * negative: it stays as it was, and the rows after it are still served. */
+mlxq_status mlxq_cache_reserve(const mlxq_array* table, const mlxq_array* lengths,
+                               const mlxq_array* refs, const mlxq_array* counts, int32_t page,
+                               mlxq_array* granted, void* stream);
+
+/* Writes the keys and values of T tokens, k and v (T, kv heads, width), to
+ * where the table has position positions[t] of row rows[t] (int32).  Tokens
+ * with a row, position or page out of range are left out, and, where lengths
+ * is not NULL, tokens at or past their row's length (of rows that were not
+ * granted their pages). */
+mlxq_status mlxq_cache_append(const mlxq_array* k, const mlxq_array* v, const mlxq_array* k_pool,
+                              const mlxq_array* v_pool, const mlxq_array* table,
+                              const mlxq_array* positions, const mlxq_array* rows,
+                              const mlxq_array* lengths, void* stream);
+
+/* Makes the empty row dst[i] a copy of row src[i]: the full pages are shared
+ * (their refs grow), a last page that is part full is copied to the lowest
+ * free page in each of the n pools.  Pairs are served in order; sources are
+ * read as they were before the call.  granted[i] (int32) is 0 where dst[i] is
+ * not empty or an earlier pair's too, no page is free for the copy, or a row
+ * is out of range.  Pools of one shape and type, each page dense. */
+mlxq_status mlxq_cache_fork(int32_t n, const mlxq_array* const* pools, const mlxq_array* table,
+                            const mlxq_array* lengths, const mlxq_array* refs,
+                            const mlxq_array* src, const mlxq_array* dst, mlxq_array* granted,
+                            void* stream);
+
+/* Empties the rows: their pages lose a reference, their lengths become 0 (the
+ * table keeps its entries).  A row named twice is freed once. */
+mlxq_status mlxq_cache_free(const mlxq_array* table, const mlxq_array* lengths,
+                            const mlxq_array* refs, const mlxq_array* rows, int32_t page,
+                            void* stream);
+
+/* Moves the held pages to the front of every pool: with `live` of them (int32
+ * (1)), the i-th held page at or past `live` goes to the i-th free page below
+ * it; refs and the sequences' table entries follow. */
+mlxq_status mlxq_cache_compact(int32_t n, const mlxq_array* const* pools, const mlxq_array* table,
+                               const mlxq_array* lengths, const mlxq_array* refs, mlxq_array* live,
+                               void* stream);
+
+/* h = x + scale * gate * post(y) and n = pre(h), where post and pre are
+ * t * rsqrt(mean(t^2) + eps) * (weight + weight_offset) over the last axis,
+ * post the identity without post_weight; n is NULL without pre_weight.  32-bit
+ * arithmetic, h and n rounded once each (n from the unrounded h).  x, y, gate,
+ * h, n of one type (bfloat16, float16, float32), weights of that type or
+ * float32; gate broadcasts over the last axis, over all rows or over the rows
+ * of a batch entry.  Rows of at most 32768 elements; any strides. */
+mlxq_status mlxq_residual_norm(const mlxq_array* x, const mlxq_array* y,
+                               const mlxq_array* post_weight, const mlxq_array* gate, float scale,
+                               const mlxq_array* pre_weight, float eps, float weight_offset,
+                               mlxq_array* h, mlxq_array* n, void* stream);
+
+/* For each row of logits (T, V), with log p = log_softmax(scale * logits):
+ * logprobs (T, m) float32, log p of tokens (T, m) int32 (NaN for one outside
+ * the row); entropy (T) float32; the top_k <= 64 most probable tokens, top_ids
+ * int32 and top_logprobs float32 (T, top_k), equal logits by the lower token
+ * (both NULL where top_k is 0).  -inf logits have probability 0; a row of them
+ * alone gives -inf and entropy 0, one with NaN or +inf gives NaN. */
+mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* tokens, int32_t top_k,
+                                float scale, mlxq_array* logprobs, mlxq_array* entropy,
+                                mlxq_array* top_logprobs, mlxq_array* top_ids, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

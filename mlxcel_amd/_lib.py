@@ -51,6 +51,14 @@ SYMBOLS = (
     "mlxq_clear_cache",
     "mlxq_reload_options",
     "mlxq_quantized_matmul_noalloc",
+    "mlxq_paged_attention",
+    "mlxq_cache_reserve",
+    "mlxq_cache_append",
+    "mlxq_cache_fork",
+    "mlxq_cache_free",
+    "mlxq_cache_compact",
+    "mlxq_residual_norm",
+    "mlxq_token_logprobs",
 )
 
 _lib = None
@@ -93,6 +101,15 @@ def load() -> ctypes.CDLL:
     lib.mlxq_fused_moe_expert.argtypes = [A] * 12 + [I32] * 6 + [A, P]
     lib.mlxq_fused_moe_geglu.argtypes = [A] * 12 + [I32] * 6 + [A, P]
     lib.mlxq_quantized_matmul_noalloc.argtypes = [A, A, A, A, B, I32, I32, S, A, P]
+    F = ctypes.c_float
+    lib.mlxq_paged_attention.argtypes = [A] * 6 + [F, F, I32, A, P]
+    lib.mlxq_cache_reserve.argtypes = [A] * 4 + [I32, A, P]
+    lib.mlxq_cache_append.argtypes = [A] * 8 + [P]
+    lib.mlxq_cache_fork.argtypes = [I32, AA] + [A] * 6 + [P]
+    lib.mlxq_cache_free.argtypes = [A] * 4 + [I32, P]
+    lib.mlxq_cache_compact.argtypes = [I32, AA] + [A] * 4 + [P]
+    lib.mlxq_residual_norm.argtypes = [A] * 4 + [F, A, F, F, A, A, P]
+    lib.mlxq_token_logprobs.argtypes = [A, A, I32, F, A, A, A, A, P]
     lib.mlxq_workspace_reserve.argtypes = [ctypes.c_size_t, P]
     lib.mlxq_get_cache_memory.argtypes = []
     lib.mlxq_clear_cache.argtypes = []

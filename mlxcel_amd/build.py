@@ -40,6 +40,7 @@ COMMON = [
 # reference's CPU code, so no FMA contraction there.
 SOURCES = {
     "api.cpp": [],
+    "api_decode.cpp": [],
     "qmv.hip": [],
     "qmv_rs.hip": [],
     "qmv_fr.hip": [],
@@ -57,6 +58,10 @@ SOURCES = {
     "moe.hip": [],
     "bias.hip": [],
     "copy.hip": [],
+    "paged.hip": [],
+    "pages.hip": [],
+    "norm.hip": [],
+    "logprobs.hip": [],
     "scratch.hip": [],
     "dequant.hip": ["-ffp-contract=off"],
 }

@@ -561,4 +561,99 @@ hipError_t launch_bias_add(void* out, const void* bias, int64_t n, int64_t bias_
 size_t static_scratch_bytes();
 hipError_t static_scratch(int dev, void** ptr);
 
+// ---- serving operators (api_decode.cpp): attention over a paged cache, the
+// ---- cache's pages, residual norms, token log probabilities ---------------------
+
+// Element types of these operators: GEN_BF16, GEN_F16, GEN_F32.
+
+// One query token per sequence over pages of keys and values (paged.hip).
+struct PagedAttnArgs {
+  const void *q, *k, *v;   // [B][Hq][D], [pages][Hkv][page][D] (the last axis dense, any other strides)
+  void* out;               // [B][Hq][D], row-contiguous
+  const int32_t* table;    // [B][width] page numbers
+  const int32_t* lengths;  // [B]
+  const float* sinks;      // [Hq] or null
+  int64_t q_b, q_h;        // strides in elements
+  int64_t k_page, k_head, k_tok, v_page, v_head, v_tok;
+  int64_t table_row;
+  int B, Hq, Hkv, D, pages, page, width;
+  int window;              // keys from length - window on (0: all)
+  float scale, softcap;    // scores: q . k * scale, then softcap * tanh(. / softcap) (0: none)
+  int type;
+};
+hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
+
+// The cache's bookkeeping (pages.hip): a table of pages per sequence, the
+// sequences' lengths in tokens, and how many sequences hold each page.
+struct CacheBook {
+  int32_t *table, *lengths, *refs;
+  int64_t table_row;
+  int rows, width, pages, page;
+};
+// scratch: pages words
+hipError_t launch_cache_reserve(const CacheBook& b, const int32_t* counts, int32_t* granted, int32_t* scratch,
+                                hipStream_t stream);
+
+struct CacheAppendArgs {
+  const void *k, *v;  // [T][Hkv][D]
+  void *kp, *vp;      // [pages][Hkv][page][D]
+  int64_t k_tok, k_head, v_tok, v_head;
+  int64_t kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok;
+  const int32_t *table, *positions, *rows, *lengths;  // lengths: null, or tokens past them are left out
+  int64_t table_row;
+  int T, Hkv, D, esz, table_rows, width, pages, page;
+};
+hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream);
+
+// Pools whose pages are copied within each pool: `bytes` of one page, pages
+// `stride` bytes apart.
+constexpr int kPoolsPerLaunch = 256;
+struct PoolList {
+  char* base[kPoolsPerLaunch];
+  int n;
+  int64_t bytes, stride;
+};
+// scratch: pages + 4 n words (fork), 3 pages + 16 words (compact)
+int64_t cache_fork_words(int pages, int n);
+int64_t cache_compact_words(int pages);
+hipError_t launch_cache_fork_plan(const CacheBook& b, const int32_t* src, const int32_t* dst, int n, int32_t* granted,
+                                  int32_t* scratch, hipStream_t stream);
+// the copies of one list of pools; `book` also forks the tables (once a call)
+hipError_t launch_cache_fork_copy(const CacheBook& b, const int32_t* src, const int32_t* dst, int n,
+                                  const int32_t* scratch, const PoolList& pools, bool book, hipStream_t stream);
+hipError_t launch_cache_free(const CacheBook& b, const int32_t* rows, int n, hipStream_t stream);
+hipError_t launch_cache_compact_plan(const CacheBook& b, int32_t* live, int32_t* scratch, hipStream_t stream);
+hipError_t launch_cache_compact_copy(const CacheBook& b, const int32_t* scratch, const PoolList& pools, bool book,
+                                     int cus, hipStream_t stream);
+
+// h = x + scale * gate * norm(y), n = norm(h) (norm.hip)
+constexpr int kNormMaxH = 32768;
+struct ResidualNormArgs {
+  const void *x, *y, *post, *gate, *pre;  // post, gate, pre nullable
+  void *h, *n;                            // row-contiguous; n null without pre
+  int64_t x_row, y_row, gate_row;         // strides in elements
+  int64_t gate_div;                       // gate row of row t: t / gate_div
+  int gate_col;                           // 1, or 0: one gate a row
+  int64_t T;
+  int H;
+  float scale, eps, offset;
+  int type, post_type, pre_type;
+};
+hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t stream);
+
+// log softmax of scaled logits at given tokens, entropy, largest entries (logprobs.hip)
+constexpr int kTopMax = 64;
+struct LogprobArgs {
+  const void* logits;     // [T][V]
+  int64_t row;            // stride in elements
+  const int32_t* tokens;  // [T][n_tok]
+  float *given, *entropy, *top;  // [T][n_tok], [T], [T][k]
+  int32_t* ids;           // [T][k]
+  int64_t T;
+  int V, n_tok, k;
+  float scale;
+  int type;
+};
+hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream);
+
 }  // namespace mlxq

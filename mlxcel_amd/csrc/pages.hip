@@ -1,0 +1,419 @@
+// pages.hip — the pages of a paged key-value cache on gfx950: reserving them
+// for new tokens, writing the tokens' keys and values, sharing them between
+// sequences, freeing them and moving them together.
+//
+// A sequence (a row of the table) of n tokens holds the first
+// ceil(n / page) entries of its row; refs counts the sequences that hold a
+// page, 0 for a free one.  Free pages are given out in ascending order and
+// requests served in their order, so every result is one fixed function of the
+// inputs.  The bookkeeping is a few thousand words and runs in one workgroup
+// (launch latency and its barriers bound it); the copies of pages run on the
+// whole card and are bound by HBM.
+//
+// Page numbers out of range are never followed; such an entry is copied or
+// kept as it stands.
+#include <hip/hip_runtime.h>
+
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace mlxq {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive sum over the workgroup's kPlanThreads threads, and the total.
+// wsum: one word per wave.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* wsum, int64_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t x = v;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int64_t o = __shfl_up((long long)x, s);
+    if (lane >= s) x += o;
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 63) wsum[wave] = x;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    if (w < wave) before += wsum[w];
+    total += wsum[w];
+  }
+  return before + x - v;
+}
+
+__device__ __forceinline__ int pages_of(int64_t tokens, int page) { return (int)((tokens + page - 1) / page); }
+
+// Appends the next free pages to list until it has `want` of them or refs is
+// at its end; at / have: where the scan stands and what the list holds (the
+// same in every thread).
+__device__ void extend_free(const int32_t* refs, int pages, int32_t* list, int64_t want, int& at, int64_t& have,
+                            int64_t* wsum) {
+  while (have < want && at < pages) {
+    const int p = at + threadIdx.x;
+    const bool free = p < pages && refs[p] == 0;
+    int64_t total;
+    const int64_t r = block_scan(free, wsum, total);
+    if (free) list[have + r] = p;
+    have += total;
+    at += kPlanThreads;
+  }
+  __syncthreads();  // the list's new entries are read by other threads
+}
+
+// The first of n ascending numbers that is above v, minus one.
+__device__ __forceinline__ int owner_of(const int64_t* first, int n, int64_t v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void cache_reserve_kernel(const CacheBook b, const int32_t* counts,
+                                                                     int32_t* granted, int32_t* list) {
+  __shared__ int64_t wsum[kPlanThreads / 64];
+  __shared__ int64_t first[kPlanThreads];
+  __shared__ int32_t need_s[kPlanThreads];
+  __shared__ int64_t taken_s;
+  const int tid = threadIdx.x;
+  int at = 0;
+  int64_t have = 0, used = 0;
+  for (int r0 = 0; r0 < b.rows; r0 += kPlanThreads) {
+    const int r = r0 + tid, n = min(kPlanThreads, b.rows - r0);
+    int64_t len = 0, cnt = 0;
+    int had = 0, need = 0;
+    bool ok = false;
+    if (r < b.rows) {
+      len = b.lengths[r];
+      cnt = counts[r];
+      // a row that cannot hold its tokens, or counts below zero, are refused
+      ok = len >= 0 && cnt >= 0 && len + cnt <= (int64_t)b.width * b.page;
+      if (ok) {
+        had = pages_of(len, b.page);
+        need = pages_of(len + cnt, b.page) - had;
+      }
+    }
+    int64_t total;
+    int64_t before = block_scan(need, wsum, total);
+    extend_free(b.refs, b.pages, list, used + total, at, have, wsum);
+    if (have - used < total) {
+      // too few pages: row by row, each that still fits
+      need_s[tid] = need;
+      __syncthreads();
+      if (tid == 0) {
+        int64_t left = have - used, sum = 0;
+        for (int i = 0; i < n; i++) {
+          first[i] = sum;
+          if (need_s[i] > left) need_s[i] = -1;
+          else {
+            left -= need_s[i];
+            sum += need_s[i];
+          }
+        }
+        taken_s = sum;
+      }
+      __syncthreads();
+      if (need_s[tid] < 0) {
+        ok = false;
+        need = 0;
+      }
+      before = first[tid];
+      total = taken_s;
+    }
+    __syncthreads();
+    first[tid] = r < b.rows ? before : INT64_MAX;
+    need_s[tid] = had;
+    __syncthreads();
+    for (int64_t i = tid; i < total; i += kPlanThreads) {
+      const int o = owner_of(first, n, i);
+      const int32_t p = list[used + i];
+      b.table[(int64_t)(r0 + o) * b.table_row + need_s[o] + (i - first[o])] = p;
+      b.refs[p] = 1;
+    }
+    if (r < b.rows) {
+      granted[r] = ok;
+      if (ok) b.lengths[r] = (int32_t)(len + cnt);
+    }
+    used += total;
+    __syncthreads();
+  }
+}
+
+// ---- append ------------------------------------------------------------------
+
+// One workgroup a token; the token's page number is the same for all its
+// elements.  VEC: 16 bytes at a time, else one element.
+template <typename W>
+__global__ __launch_bounds__(256) void cache_append_kernel(const CacheAppendArgs a) {
+  const int t = blockIdx.x, row = a.rows[t], pos = a.positions[t];
+  if (row < 0 || row >= a.table_rows || pos < 0 || pos / a.page >= a.width) return;
+  if (a.lengths && pos >= a.lengths[row]) return;
+  const int pid = a.table[row * a.table_row + pos / a.page], off = pos % a.page;
+  if (pid < 0 || pid >= a.pages) return;
+  const int per = a.D * a.esz / (int)sizeof(W);  // words of a head
+  for (int i = threadIdx.x; i < 2 * a.Hkv * per; i += 256) {
+    const int v = i >= a.Hkv * per, j = v ? i - a.Hkv * per : i, h = j / per, w = j - h * per;
+    const char* src = static_cast<const char*>(v ? a.v : a.k) +
+                      (v ? t * a.v_tok + h * a.v_head : t * a.k_tok + h * a.k_head) * a.esz;
+    char* dst = static_cast<char*>(v ? a.vp : a.kp) +
+                (v ? pid * a.vp_page + h * a.vp_head + off * a.vp_tok
+                   : pid * a.kp_page + h * a.kp_head + off * a.kp_tok) * a.esz;
+    reinterpret_cast<W*>(dst)[w] = reinterpret_cast<const W*>(src)[w];
+  }
+}
+
+// ---- copies of pages -----------------------------------------------------------
+
+template <typename W>
+__device__ __forceinline__ void copy_page(char* base, int64_t stride, int64_t bytes, int from, int to) {
+  const W* s = reinterpret_cast<const W*>(base + from * stride);
+  W* d = reinterpret_cast<W*>(base + to * stride);
+  const int64_t n = bytes / (int64_t)sizeof(W);
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) d[i] = s[i];
+}
+
+// ---- fork ----------------------------------------------------------------------
+
+// scratch: the list of free pages, then per pair {tokens or -1, fresh page or -1}
+__global__ __launch_bounds__(kPlanThreads) void cache_fork_plan_kernel(const CacheBook b, const int32_t* src,
+                                                                       const int32_t* dst, int n, int32_t* granted,
+                                                                       int32_t* list, int32_t* pair) {
+  __shared__ int64_t wsum[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  int at = 0;
+  int64_t have = 0, used = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    bool ok = false;
+    int64_t len = 0;
+    if (i < n) {
+      const int s = src[i], d = dst[i];
+      ok = s >= 0 && s < b.rows && d >= 0 && d < b.rows;
+      if (ok) {
+        len = b.lengths[s];
+        ok = len >= 0 && len <= (int64_t)b.width * b.page && b.lengths[d] == 0;
+      }
+      for (int j = 0; ok && j < i; j++) ok = dst[j] != d;  // the first pair of a row takes it
+    }
+    const int part = ok && len % b.page != 0;
+    int64_t total;
+    const int64_t r = block_scan(part, wsum, total);
+    extend_free(b.refs, b.pages, list, used + total, at, have, wsum);
+    int fresh = -1;
+    if (part) {
+      if (used + r < have) {
+        fresh = list[used + r];
+        b.refs[fresh] = 1;
+      } else {
+        ok = false;
+      }
+    }
+    if (i < n) {
+      granted[i] = ok;
+      pair[2 * i] = ok ? (int32_t)len : -1;
+      pair[2 * i + 1] = fresh;
+    }
+    used = min(used + total, have);
+    __syncthreads();
+  }
+}
+
+// blockIdx.x: a pair; blockIdx.y: a pool, the last one the table's row.
+template <typename W>
+__global__ __launch_bounds__(256) void cache_fork_copy_kernel(const CacheBook b, const int32_t* src, const int32_t* dst,
+                                                              const int32_t* pair, const PoolList pools) {
+  const int i = blockIdx.x, len = pair[2 * i], fresh = pair[2 * i + 1];
+  if (len < 0) return;
+  const int full = len / b.page;
+  const int32_t* from = b.table + src[i] * b.table_row;
+  if ((int)blockIdx.y == pools.n) {
+    int32_t* to = b.table + dst[i] * b.table_row;
+    for (int j = threadIdx.x; j < full; j += blockDim.x) {
+      const int32_t p = from[j];
+      to[j] = p;
+      if (p >= 0 && p < b.pages) atomicAdd(b.refs + p, 1);
+    }
+    if (threadIdx.x == 0) {
+      if (fresh >= 0) to[full] = fresh;
+      b.lengths[dst[i]] = len;
+    }
+    return;
+  }
+  if (fresh < 0) return;
+  const int old = from[full];
+  if (old < 0 || old >= b.pages) return;
+  copy_page<W>(pools.base[blockIdx.y], pools.stride, pools.bytes, old, fresh);
+}
+
+// ---- free ------------------------------------------------------------------------
+
+__global__ __launch_bounds__(256) void cache_free_kernel(const CacheBook b, const int32_t* rows) {
+  __shared__ int len_s;
+  const int row = rows[blockIdx.x];
+  if (row < 0 || row >= b.rows) return;
+  // of several requests for one row one gets its length
+  if (threadIdx.x == 0) len_s = atomicExch(b.lengths + row, 0);
+  __syncthreads();
+  const int64_t len = min((int64_t)max(len_s, 0), (int64_t)b.width * b.page);
+  const int held = pages_of(len, b.page);
+  for (int j = threadIdx.x; j < held; j += blockDim.x) {
+    const int32_t p = b.table[row * b.table_row + j];
+    if (p >= 0 && p < b.pages) atomicSub(b.refs + p, 1);
+  }
+}
+
+// ---- compact ---------------------------------------------------------------------
+
+// scratch: the number of moves (16 words), to[pages], holes[pages], movers[pages]
+__global__ __launch_bounds__(kPlanThreads) void cache_compact_plan_kernel(const CacheBook b, int32_t* live_out,
+                                                                          int32_t* moves, int32_t* to, int32_t* holes,
+                                                                          int32_t* movers) {
+  __shared__ int64_t wsum[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  int64_t live = 0, total;
+  for (int p = tid; p < b.pages; p += kPlanThreads) live += b.refs[p] > 0;
+  block_scan(live, wsum, total);
+  const int n = (int)total;
+  // holes are the free pages below n, movers the held ones from n on: as many
+  int64_t nh = 0, nm = 0;
+  for (int p0 = 0; p0 < b.pages; p0 += kPlanThreads) {
+    const int p = p0 + tid;
+    const bool held = p < b.pages && b.refs[p] > 0;
+    const bool hole = p < n && !held, mover = p >= n && held;
+    int64_t th, tm;
+    const int64_t rh = block_scan(hole, wsum, th);
+    const int64_t rm = block_scan(mover, wsum, tm);
+    if (hole) holes[nh + rh] = p;
+    if (mover) movers[nm + rm] = p;
+    if (p < b.pages) to[p] = p;
+    nh += th;
+    nm += tm;
+  }
+  __syncthreads();
+  for (int i = tid; i < nm; i += kPlanThreads) {
+    const int h = holes[i], m = movers[i];
+    to[m] = h;
+    b.refs[h] = b.refs[m];
+    b.refs[m] = 0;
+  }
+  if (tid == 0) {
+    moves[0] = (int)nm;
+    live_out[0] = n;
+  }
+}
+
+// Workgroups take (move, pool) pairs in turn; the last `rows` workgroups
+// rewrite a row of the table each.
+template <typename W>
+__global__ __launch_bounds__(256) void cache_compact_copy_kernel(const CacheBook b, const int32_t* moves,
+                                                                 const int32_t* to, const int32_t* holes,
+                                                                 const int32_t* movers, const PoolList pools,
+                                                                 int movers_wgs) {
+  if ((int)blockIdx.x >= movers_wgs) {
+    const int row = blockIdx.x - movers_wgs;
+    const int64_t len = min((int64_t)max(b.lengths[row], 0), (int64_t)b.width * b.page);
+    int32_t* t = b.table + row * b.table_row;
+    for (int j = threadIdx.x; j < pages_of(len, b.page); j += blockDim.x) {
+      const int32_t p = t[j];
+      if (p >= 0 && p < b.pages) t[j] = to[p];
+    }
+    return;
+  }
+  const int64_t n = (int64_t)moves[0] * pools.n;
+  for (int64_t i = blockIdx.x; i < n; i += movers_wgs) {
+    const int m = (int)(i / pools.n), q = (int)(i - (int64_t)m * pools.n);
+    copy_page<W>(pools.base[q], pools.stride, pools.bytes, movers[m], holes[m]);
+  }
+}
+
+// 16-byte words where every page of every pool allows them
+bool wide(const PoolList& p) {
+  uintptr_t v = (uintptr_t)p.bytes | (uintptr_t)p.stride;
+  for (int i = 0; i < p.n; i++) v |= reinterpret_cast<uintptr_t>(p.base[i]);
+  return (v & 15) == 0;
+}
+
+}  // namespace
+
+hipError_t launch_cache_reserve(const CacheBook& b, const int32_t* counts, int32_t* granted, int32_t* scratch,
+                                hipStream_t stream) {
+  if (b.rows == 0) return hipSuccess;
+  hipLaunchKernelGGL(cache_reserve_kernel, dim3(1), dim3(kPlanThreads), 0, stream, b, counts, granted, scratch);
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
+  if (a.T == 0 || a.Hkv == 0 || a.D == 0) return hipSuccess;
+  if (a.pages < 1 || a.page < 1) return hipErrorInvalidValue;
+  uintptr_t v = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                reinterpret_cast<uintptr_t>(a.kp) | reinterpret_cast<uintptr_t>(a.vp);
+  const int64_t st[] = {a.k_tok, a.k_head, a.v_tok, a.v_head, a.kp_page, a.kp_head, a.kp_tok,
+                        a.vp_page, a.vp_head, a.vp_tok, (int64_t)a.D};
+  for (int64_t s : st) v |= (uintptr_t)(s * a.esz);
+  const dim3 grid((unsigned)a.T), block(256);
+  if ((v & 15) == 0) hipLaunchKernelGGL(cache_append_kernel<u32x4>, grid, block, 0, stream, a);
+  else if (a.esz == 2) hipLaunchKernelGGL(cache_append_kernel<uint16_t>, grid, block, 0, stream, a);
+  else hipLaunchKernelGGL(cache_append_kernel<uint32_t>, grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+int64_t cache_fork_words(int pages, int n) { return (int64_t)pages + 2 * (int64_t)n; }
+int64_t cache_compact_words(int pages) { return 16 + 3 * (int64_t)pages; }
+
+hipError_t launch_cache_fork_plan(const CacheBook& b, const int32_t* src, const int32_t* dst, int n, int32_t* granted,
+                                  int32_t* scratch, hipStream_t stream) {
+  if (n == 0) return hipSuccess;
+  hipLaunchKernelGGL(cache_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, b, src, dst, n, granted, scratch,
+                     scratch + b.pages);
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_fork_copy(const CacheBook& b, const int32_t* src, const int32_t* dst, int n,
+                                  const int32_t* scratch, const PoolList& pools, bool book, hipStream_t stream) {
+  if (n == 0) return hipSuccess;
+  const dim3 grid((unsigned)n, (unsigned)(pools.n + (book ? 1 : 0))), block(256);
+  const int32_t* pair = scratch + b.pages;
+  if (grid.y == 0) return hipSuccess;
+  if (wide(pools)) hipLaunchKernelGGL(cache_fork_copy_kernel<u32x4>, grid, block, 0, stream, b, src, dst, pair, pools);
+  else hipLaunchKernelGGL(cache_fork_copy_kernel<uint16_t>, grid, block, 0, stream, b, src, dst, pair, pools);
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_free(const CacheBook& b, const int32_t* rows, int n, hipStream_t stream) {
+  if (n == 0 || b.rows == 0) return hipSuccess;
+  hipLaunchKernelGGL(cache_free_kernel, dim3((unsigned)n), dim3(256), 0, stream, b, rows);
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_compact_plan(const CacheBook& b, int32_t* live, int32_t* scratch, hipStream_t stream) {
+  int32_t* to = scratch + 16;
+  hipLaunchKernelGGL(cache_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, b, live, scratch, to,
+                     to + b.pages, to + 2 * (int64_t)b.pages);
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_compact_copy(const CacheBook& b, const int32_t* scratch, const PoolList& pools, bool book,
+                                     int cus, hipStream_t stream) {
+  const int wgs = pools.n > 0 && b.pages > 0 ? cus * 8 : 0;
+  const int64_t grid = (int64_t)wgs + (book ? b.rows : 0);
+  if (grid == 0) return hipSuccess;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const int32_t* to = scratch + 16;
+  const int32_t *holes = to + b.pages, *movers = to + 2 * (int64_t)b.pages;
+  if (wide(pools))
+    hipLaunchKernelGGL(cache_compact_copy_kernel<u32x4>, dim3((unsigned)grid), dim3(256), 0, stream, b, scratch, to,
+                       holes, movers, pools, wgs);
+  else
+    hipLaunchKernelGGL(cache_compact_copy_kernel<uint16_t>, dim3((unsigned)grid), dim3(256), 0, stream, b, scratch, to,
+                       holes, movers, pools, wgs);
+  return hipGetLastError();
+}
+
+}  // namespace mlxq

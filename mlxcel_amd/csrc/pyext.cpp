@@ -17,6 +17,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <vector>
+
 #include "../../include/mlxq.h"
 
 namespace {
@@ -190,6 +192,8 @@ constexpr int kMulti = 4;
 // while the GIL is released.
 struct Held {
   PyObject* o = nullptr;
+  Held() = default;
+  Held(const Held&) = delete;
   ~Held() { Py_XDECREF(o); }
 };
 
@@ -342,9 +346,213 @@ PyObject* fused_moe(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// ---- serving operators -----------------------------------------------------------
+
+// a tensor (or None) on the call's device
+Arr on(PyObject* o, const at::Device& dev) {
+  if (o != Py_None && tensor(o).device() != dev) throw NotHandled{};
+  return arr(o);
+}
+
+float number(PyObject* o) {
+  if (PyFloat_CheckExact(o)) return (float)PyFloat_AS_DOUBLE(o);
+  return (float)integer(o);
+}
+
+// (q, k_pool, v_pool, table, lengths, sinks, scale, softcap, window, out)
+PyObject* paged_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 10, [&]() -> PyObject* {
+    const at::Tensor& q = tensor(v[0]);
+    const at::Device dev = q.device();
+    Arr a[6];
+    for (int i = 0; i < 6; i++) a[i] = on(v[i], dev);
+    const float scale = number(v[6]), softcap = number(v[7]);
+    const int window = integer(v[8], 0);
+    at::Tensor out;
+    Arr o;
+    if (v[9] == Py_None) {
+      out = at::empty(q.sizes(), q.options().requires_grad(false));
+      fill(o, out);
+    } else {
+      o = on(v[9], dev);
+    }
+    call(dev, [&](void* stream) {
+      return mlxq_paged_attention(a[0].p(), a[1].p(), a[2].p(), a[3].p(), a[4].p(), a[5].p(), scale, softcap, window,
+                                  &o.a, stream);
+    });
+    return keep(v[9], out);
+  });
+}
+
+at::Tensor int32s(at::IntArrayRef shape, const at::Device& dev) {
+  return at::empty(shape, at::TensorOptions().dtype(at::kInt).device(dev));
+}
+
+// (table, lengths, refs, counts, page)
+PyObject* cache_reserve(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 5, [&]() -> PyObject* {
+    const at::Device dev = tensor(v[0]).device();
+    Arr a[4];
+    for (int i = 0; i < 4; i++) a[i] = on(v[i], dev);
+    const int page = integer(v[4]);
+    const at::Tensor granted = int32s(tensor(v[3]).sizes(), dev);
+    Arr g;
+    fill(g, granted);
+    call(dev, [&](void* stream) {
+      return mlxq_cache_reserve(a[0].p(), a[1].p(), a[2].p(), a[3].p(), page, &g.a, stream);
+    });
+    return THPVariable_Wrap(granted);
+  });
+}
+
+// (k, v, k_pool, v_pool, table, positions, rows, lengths)
+PyObject* cache_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 8, [&]() -> PyObject* {
+    const at::Device dev = tensor(v[0]).device();
+    Arr a[8];
+    for (int i = 0; i < 8; i++) a[i] = on(v[i], dev);
+    call(dev, [&](void* stream) {
+      return mlxq_cache_append(a[0].p(), a[1].p(), a[2].p(), a[3].p(), a[4].p(), a[5].p(), a[6].p(), a[7].p(), stream);
+    });
+    Py_RETURN_TRUE;
+  });
+}
+
+// A list or tuple of tensors of the call's device; each is held for the call.
+struct Pools {
+  std::vector<Held> held;
+  std::vector<Arr> arrs;
+  std::vector<const mlxq_array*> ptrs;
+  Pools(PyObject* o, const at::Device& dev) {
+    const bool l = PyList_CheckExact(o), t = PyTuple_CheckExact(o);
+    if (!l && !t) throw NotHandled{};
+    const Py_ssize_t n = l ? PyList_GET_SIZE(o) : PyTuple_GET_SIZE(o);
+    held = std::vector<Held>(n);
+    arrs.resize(n);
+    for (Py_ssize_t i = 0; i < n; i++) {
+      held[i].o = l ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i);
+      Py_INCREF(held[i].o);
+      if (held[i].o == Py_None) throw NotHandled{};
+      arrs[i] = on(held[i].o, dev);
+    }
+    for (const Arr& a : arrs) ptrs.push_back(a.p());
+  }
+};
+
+// (pools, table, lengths, refs, src, dst)
+PyObject* cache_fork(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 6, [&]() -> PyObject* {
+    const at::Device dev = tensor(v[1]).device();
+    const Pools pools(v[0], dev);
+    Arr a[5];
+    for (int i = 0; i < 5; i++) a[i] = on(v[1 + i], dev);
+    const at::Tensor granted = int32s(tensor(v[4]).sizes(), dev);
+    Arr g;
+    fill(g, granted);
+    call(dev, [&](void* stream) {
+      return mlxq_cache_fork((int32_t)pools.ptrs.size(), pools.ptrs.data(), a[0].p(), a[1].p(), a[2].p(), a[3].p(),
+                             a[4].p(), &g.a, stream);
+    });
+    return THPVariable_Wrap(granted);
+  });
+}
+
+// (table, lengths, refs, rows, page)
+PyObject* cache_free(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 5, [&]() -> PyObject* {
+    const at::Device dev = tensor(v[0]).device();
+    Arr a[4];
+    for (int i = 0; i < 4; i++) a[i] = on(v[i], dev);
+    const int page = integer(v[4]);
+    call(dev, [&](void* stream) { return mlxq_cache_free(a[0].p(), a[1].p(), a[2].p(), a[3].p(), page, stream); });
+    Py_RETURN_TRUE;
+  });
+}
+
+// (pools, table, lengths, refs)
+PyObject* cache_compact(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 4, [&]() -> PyObject* {
+    const at::Device dev = tensor(v[1]).device();
+    const Pools pools(v[0], dev);
+    Arr a[3];
+    for (int i = 0; i < 3; i++) a[i] = on(v[1 + i], dev);
+    const at::Tensor live = int32s({1}, dev);
+    Arr l;
+    fill(l, live);
+    call(dev, [&](void* stream) {
+      return mlxq_cache_compact((int32_t)pools.ptrs.size(), pools.ptrs.data(), a[0].p(), a[1].p(), a[2].p(), &l.a,
+                                stream);
+    });
+    return THPVariable_Wrap(live);
+  });
+}
+
+// (x, y, post_weight, gate, scale, pre_weight, eps, weight_offset): (h, n or None)
+PyObject* residual_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 8, [&]() -> PyObject* {
+    const at::Tensor& x = tensor(v[0]);
+    const at::Device dev = x.device();
+    const Arr xa = arr(v[0]), ya = on(v[1], dev), post = on(v[2], dev), gate = on(v[3], dev), pre = on(v[5], dev);
+    const float scale = number(v[4]), eps = number(v[6]), offset = number(v[7]);
+    const auto opts = x.options().requires_grad(false);
+    const at::Tensor h = at::empty(x.sizes(), opts);
+    at::Tensor nt;
+    Arr ha, na;
+    fill(ha, h);
+    if (pre.on) {
+      nt = at::empty(x.sizes(), opts);
+      fill(na, nt);
+    }
+    call(dev, [&](void* stream) {
+      return mlxq_residual_norm(xa.p(), ya.p(), post.p(), gate.p(), scale, pre.p(), eps, offset, &ha.a,
+                                pre.on ? &na.a : nullptr, stream);
+    });
+    PyObject* r = PyTuple_New(2);
+    if (!r) return nullptr;
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(h));
+    if (!pre.on) Py_INCREF(Py_None);
+    PyTuple_SET_ITEM(r, 1, pre.on ? THPVariable_Wrap(nt) : Py_None);
+    return r;
+  });
+}
+
+// (logits, tokens, top_k, scale): (logprobs, entropy, top_logprobs or None, top_ids or None)
+PyObject* token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 4, [&]() -> PyObject* {
+    const at::Tensor &x = tensor(v[0]), &t = tensor(v[1]);
+    const at::Device dev = x.device();
+    const Arr xa = arr(v[0]), ta = on(v[1], dev);
+    const int k = integer(v[2]);
+    const float scale = number(v[3]);
+    if (x.dim() != 2 || k < 0) throw NotHandled{};
+    const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
+    at::Tensor r[4] = {at::empty(t.sizes(), f32), at::empty({x.size(0)}, f32)};
+    Arr a[4];
+    if (k > 0) {
+      r[2] = at::empty({x.size(0), k}, f32);
+      r[3] = int32s({x.size(0), k}, dev);
+    }
+    for (int i = 0; i < (k > 0 ? 4 : 2); i++) fill(a[i], r[i]);
+    call(dev, [&](void* stream) {
+      return mlxq_token_logprobs(xa.p(), ta.p(), k, scale, &a[0].a, &a[1].a, k > 0 ? &a[2].a : nullptr,
+                                 k > 0 ? &a[3].a : nullptr, stream);
+    });
+    PyObject* out = PyTuple_New(4);
+    if (!out) return nullptr;
+    for (int i = 0; i < 4; i++) {
+      if (!a[i].on) Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(out, i, a[i].on ? THPVariable_Wrap(r[i]) : Py_None);
+    }
+    return out;
+  });
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quantized_matmul), FAST(quantized_matmul_multi), FAST(gather_qmm), FAST(dequantize),
-                         FAST(quantize),         FAST(fused_moe),              {nullptr, nullptr, 0, nullptr}};
+                         FAST(quantize),         FAST(fused_moe),
+                         FAST(paged_attention),  FAST(cache_reserve),          FAST(cache_append), FAST(cache_fork),
+                         FAST(cache_free),       FAST(cache_compact),          FAST(residual_norm), FAST(token_logprobs),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mlxq_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

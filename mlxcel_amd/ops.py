@@ -33,6 +33,8 @@ class _ctypes_only:
     """Stands in for the native module: every call takes the ctypes binding."""
     quantized_matmul = quantized_matmul_multi = gather_qmm = staticmethod(lambda *a: None)
     dequantize = quantize = fused_moe = staticmethod(lambda *a: None)
+    paged_attention = residual_norm = token_logprobs = staticmethod(lambda *a: None)
+    cache_reserve = cache_append = cache_fork = cache_free = cache_compact = staticmethod(lambda *a: None)
 
 
 def _load_native():
@@ -379,6 +381,163 @@ def fused_moe_geglu(x, indices, gate_w, gate_s, gate_b, up_w, up_s, up_b, down_w
     GELU of the gate times up)."""
     return _fused_moe("mlxq_fused_moe_geglu", x, indices, gate_w, gate_s, gate_b, up_w, up_s, up_b, down_w,
                       down_s, down_b, scores, din, dff, k, gu_bits, d_bits, group_size, out)
+
+
+def _together(*tensors: Optional[torch.Tensor]) -> torch.device:
+    """The device of the call's tensors, which must be one HIP device."""
+    dev = _device_of(tensors[0])
+    for t in tensors[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"[mlxq] tensors must live on one device but are on {dev} and {t.device}")
+    return dev
+
+
+def _run(name: str, dev: torch.device, *args) -> None:
+    """One C call on the device's current stream: tensors (or None) and numbers."""
+    arrs = [_arr(a) if isinstance(a, torch.Tensor) else None for a in args]
+    with torch.cuda.device(dev):
+        st = getattr(_lib.load(), name)(*[a if r is None else _ref(r) for a, r in zip(args, arrs)], _stream(dev))
+    if st:
+        _raise(st)
+
+
+def _pointers(pools: Sequence[torch.Tensor]):
+    """An array of pointers to the pools' structs (kept alive by it)."""
+    P = ctypes.POINTER(_lib.MlxqArray)
+    return (P * len(pools))(*[ctypes.pointer(_arr(t)[1]) for t in pools])
+
+
+def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
+                    lengths: torch.Tensor, *, window: int = 0, softcap: float = 0.0,
+                    sinks: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one query token per sequence over a paged cache.
+
+    ``q`` (B, query heads, width); ``k_pool``, ``v_pool`` (pages, kv heads, page,
+    width) of q's type (bfloat16, float16, float32) with a contiguous last axis;
+    ``table`` (B, n) and ``lengths`` (B) int32: sequence b's tokens are
+    ``lengths[b]`` ones on the pages ``table[b]``, the last of them the query's own.  A
+    length of 0 gives zeros.  ``scale`` is ``width ** -0.5`` by default;
+    ``softcap`` c > 0 makes a score s ``c tanh(s / c)``; ``window`` w > 0 keeps
+    the last w tokens; ``sinks`` (query heads) float32 join each head's softmax
+    sum."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+    r = _native.paged_attention(q, k_pool, v_pool, table, lengths, sinks, scale, softcap, window, out)
+    if r is not None:
+        return _done(r)
+    dev = _together(q, k_pool, v_pool, table, lengths, sinks, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _run("mlxq_paged_attention", dev, q, k_pool, v_pool, table, lengths, sinks, scale, softcap, window, out)
+    return out
+
+
+def cache_reserve(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, counts: torch.Tensor,
+                  page: int) -> torch.Tensor:
+    """Pages for ``counts[r]`` more tokens of every row, the lowest free pages
+    first; updates ``table`` (rows, n), ``lengths`` (rows) and ``refs`` (pages),
+    all int32, in place.  Returns int32 flags: 0 for a row that the free pages or
+    the table do not hold, which stays as it was."""
+    r = _native.cache_reserve(table, lengths, refs, counts, page)
+    if r is not None:
+        return _done(r)
+    dev = _together(table, lengths, refs, counts)
+    granted = torch.empty(counts.shape, dtype=torch.int32, device=dev)
+    _run("mlxq_cache_reserve", dev, table, lengths, refs, counts, int(page), granted)
+    return granted
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
+                 positions: torch.Tensor, rows: torch.Tensor, *, lengths: Optional[torch.Tensor] = None) -> None:
+    """Writes the keys and values of tokens, ``k`` and ``v`` (T, kv heads,
+    width), to position ``positions[t]`` of sequence ``rows[t]`` (int32).  Where a
+    reservation may have been refused pass ``lengths``: tokens at or past their
+    sequence's length are then left out, like those whose row, position or page
+    is out of range."""
+    r = _native.cache_append(k, v, k_pool, v_pool, table, positions, rows, lengths)
+    if r is not None:
+        return None if r is True else _raise(r)
+    dev = _together(k, v, k_pool, v_pool, table, positions, rows, lengths)
+    _run("mlxq_cache_append", dev, k, v, k_pool, v_pool, table, positions, rows, lengths)
+
+
+def cache_fork(pools: Sequence[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
+               src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
+    """Makes each empty row ``dst[i]`` a copy of row ``src[i]``: full pages are
+    shared, a part-full last page is copied in every pool to the lowest free
+    page.  Returns int32 flags: 0 for a pair that could not be served."""
+    pools = list(pools)
+    r = _native.cache_fork(pools, table, lengths, refs, src, dst)
+    if r is not None:
+        return _done(r)
+    dev = _together(table, lengths, refs, src, dst, *pools)
+    granted = torch.empty(src.shape, dtype=torch.int32, device=dev)
+    _run("mlxq_cache_fork", dev, len(pools), _pointers(pools), table, lengths, refs, src, dst, granted)
+    return granted
+
+
+def cache_free(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor,
+               page: int) -> None:
+    """Empties the sequences ``rows``: their pages lose a reference, their
+    lengths become 0."""
+    r = _native.cache_free(table, lengths, refs, rows, page)
+    if r is not None:
+        return None if r is True else _raise(r)
+    _run("mlxq_cache_free", _together(table, lengths, refs, rows), table, lengths, refs, rows, int(page))
+
+
+def cache_compact(pools: Sequence[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor,
+                  refs: torch.Tensor) -> torch.Tensor:
+    """Moves the held pages to the front of every pool, with their refs and the
+    table's entries; returns their number, int32 (1)."""
+    pools = list(pools)
+    r = _native.cache_compact(pools, table, lengths, refs)
+    if r is not None:
+        return _done(r)
+    dev = _together(table, lengths, refs, *pools)
+    live = torch.empty(1, dtype=torch.int32, device=dev)
+    _run("mlxq_cache_compact", dev, len(pools), _pointers(pools), table, lengths, refs, live)
+    return live
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, scale: float = 1.0,
+                  pre_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, weight_offset: float = 0.0):
+    """The residual update of a block and the norms on its sides:
+    ``h = x + scale * gate * rms(y, post_weight)``, ``n = rms(h, pre_weight)`` with
+    ``rms(t, w) = t * rsqrt(mean(t**2) + eps) * (w + weight_offset)``.  Returns
+    ``(h, n)``; without ``post_weight`` y is taken as it is, without ``pre_weight`` n
+    is None.  ``gate`` broadcasts over the last axis, all rows, or the rows of a
+    batch entry."""
+    r = _native.residual_norm(x, y, post_weight, gate, scale, pre_weight, eps, weight_offset)
+    if r is not None:
+        return _done(r)
+    dev = _together(x, y, post_weight, gate, pre_weight)
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    n = None if pre_weight is None else torch.empty_like(h)
+    _run("mlxq_residual_norm", dev, x, y, post_weight, gate, scale, pre_weight, eps, weight_offset, h, n)
+    return h, n
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top_k: int = 0, scale: float = 1.0):
+    """Of each row of ``logits`` (T, V), under ``log_softmax(scale * logits)``:
+    the log probabilities of ``tokens`` (T, m) int32, the entropy (T), and the
+    ``top_k`` <= 64 most probable tokens with theirs (equal logits by the lower
+    token).  Returns ``(logprobs, entropy, top_logprobs, top_ids)``, float32 and
+    int32, the last two None for ``top_k`` 0."""
+    r = _native.token_logprobs(logits, tokens, top_k, scale)
+    if r is not None:
+        return _done(r)
+    dev = _together(logits, tokens)
+    rows = logits.shape[0] if logits.dim() else 0
+    f32 = dict(dtype=torch.float32, device=dev)
+    out = [torch.empty(tokens.shape, **f32), torch.empty(rows, **f32), None, None]
+    if top_k > 0:
+        out[2] = torch.empty(rows, top_k, **f32)
+        out[3] = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+    _run("mlxq_token_logprobs", dev, logits, tokens, int(top_k), scale, *out)
+    return tuple(out)
 
 
 def workspace_reserve(nbytes: int, device: Optional[torch.device] = None) -> None:

@@ -118,6 +118,43 @@ pub mod sys {
             dff: i32, k: i32, gu_bits: i32, d_bits: i32, group_size: i32, out: *mut mlxq_array,
             stream: *mut c_void,
         ) -> i32;
+        pub fn mlxq_paged_attention(
+            q: *const mlxq_array, k_pool: *const mlxq_array, v_pool: *const mlxq_array, table: *const mlxq_array,
+            lengths: *const mlxq_array, sinks: *const mlxq_array, scale: f32, softcap: f32, window: i32,
+            out: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_cache_reserve(
+            table: *const mlxq_array, lengths: *const mlxq_array, refs: *const mlxq_array,
+            counts: *const mlxq_array, page: i32, granted: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_cache_append(
+            k: *const mlxq_array, v: *const mlxq_array, k_pool: *const mlxq_array, v_pool: *const mlxq_array,
+            table: *const mlxq_array, positions: *const mlxq_array, rows: *const mlxq_array,
+            lengths: *const mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_cache_fork(
+            n: i32, pools: *const *const mlxq_array, table: *const mlxq_array, lengths: *const mlxq_array,
+            refs: *const mlxq_array, src: *const mlxq_array, dst: *const mlxq_array, granted: *mut mlxq_array,
+            stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_cache_free(
+            table: *const mlxq_array, lengths: *const mlxq_array, refs: *const mlxq_array,
+            rows: *const mlxq_array, page: i32, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_cache_compact(
+            n: i32, pools: *const *const mlxq_array, table: *const mlxq_array, lengths: *const mlxq_array,
+            refs: *const mlxq_array, live: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_residual_norm(
+            x: *const mlxq_array, y: *const mlxq_array, post_weight: *const mlxq_array, gate: *const mlxq_array,
+            scale: f32, pre_weight: *const mlxq_array, eps: f32, weight_offset: f32, h: *mut mlxq_array,
+            n: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_token_logprobs(
+            logits: *const mlxq_array, tokens: *const mlxq_array, top_k: i32, scale: f32,
+            logprobs: *mut mlxq_array, entropy: *mut mlxq_array, top_logprobs: *mut mlxq_array,
+            top_ids: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
     }
 }
 
