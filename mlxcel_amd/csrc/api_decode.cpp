@@ -253,8 +253,7 @@ mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool, 
     mlxq_array qc = *q, oc = *out;
     const bool stage_q = !unit_last(x), stage_out = !View{out}.row_contiguous();
     if (stage_q || stage_out) {
-      const int dev = current_device();
-      char* p = static_cast<char*>(stream_workspace(dev, stream, 2 * padded(x), 1));
+      char* p = static_cast<char*>(stream_workspace(current_device(), stream, 2 * padded(x), 1));
       if (stage_q) {
         qc = contiguous_like(q, p);
         copy_view(q, &qc, stream);
@@ -265,6 +264,14 @@ mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool, 
     a.q_b = qc.strides[0];
     a.q_h = qc.strides[1];
     a.out = oc.data;
+    const int dev = current_device();
+    int64_t part_bytes = 0;
+    mlxq::paged_attention_plan(a, device_cus(dev), &part_bytes);
+    a.part = static_cast<float*>(stream_workspace(dev, stream, part_bytes, 0));
+    a.cnt = stream_counters(dev, stream);
+    if (!a.cnt)
+      fail(MLXQ_ENOMEM, "[paged_attention] this stream has no counters yet and is being captured; run the call once "
+                        "before the capture or reserve with mlxq_workspace_reserve");
     hip_check(mlxq::launch_paged_attention(a, stream), "paged attention launch");
     if (stage_out) copy_view(&oc, out, stream);
   });

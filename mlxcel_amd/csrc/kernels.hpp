@@ -580,7 +580,15 @@ struct PagedAttnArgs {
   int window;              // keys from length - window on (0: all)
   float scale, softcap;    // scores: q . k * scale, then softcap * tanh(. / softcap) (0: none)
   int type;
+  // how the keys are split (paged_attention_plan)
+  uint32_t page_mul;       // key / page = key * page_mul >> page_shift
+  int page_shift;
+  int wgs, least;          // workgroups; 64-key steps a workgroup takes at least
+  float* part;             // [2 wgs] partial results of part_words each
+  uint32_t* cnt;           // [wgs], zero between launches
 };
+// Sets the plan; part_bytes of scratch (and wgs counters) are needed.
+void paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes);
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
 
 // The cache's bookkeeping (pages.hip): a table of pages per sequence, the
