@@ -583,7 +583,7 @@ struct PagedAttnArgs {
   // how the keys are split (paged_attention_plan)
   uint32_t page_mul;       // key / page = key * page_mul >> page_shift
   int page_shift;
-  int wgs, least;          // workgroups; 64-key steps a workgroup takes at least
+  int wgs, least, whole;   // workgroups; steps a workgroup takes at least; steps of a head that is not cut
   float* part;             // [2 wgs] partial results of part_words each
   uint32_t* cnt;           // [wgs], zero between launches
 };

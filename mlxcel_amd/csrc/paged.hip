@@ -26,17 +26,20 @@
 //   S^T[key][head] = K Q^T: lane (c, g) = (lane % 16, lane / 16) loads 16 bytes
 //     of key c, so the tile's keys are read in 16 rows of 64 contiguous bytes;
 //     it ends with the scores of keys 4 g + r (r < 4) of head c.
-//   O^T[d][head] += V^T P^T in 32-bit MFMAs of 4 keys: step r takes keys
-//     4 g + r, for which lane (c, g) already holds P of head c; it loads V of
-//     key 4 g + r, columns VE c .. VE c + VE - 1, so a key's row is read as one
-//     contiguous run.  Accumulator j is column VE c + j, rows 4 g + r' of
-//     O^T: d = VE (4 g + r') + j, head c, the lane whose maximum rescales it.
-// P stays in 32 bits (no rounding of probabilities); the 32-bit MFMAs cost
-// 64 cycles a key of 128 columns on one SIMD where the read of a key takes a
-// CU 64 cycles, a quarter of the four SIMDs' time.
+//   O^T[d][head] += V^T P^T: lane (c, g) loads V of keys 4 g + r (r < 4), columns
+//     VE c .. VE c + VE - 1, so a key's row is read as one contiguous run and the
+//     lane holds P of the same keys for head c.  Accumulator j is column VE c + j,
+//     rows 4 g + r' of O^T: d = VE (4 g + r') + j, head c, the lane whose maximum
+//     rescales it.  16-bit pools: one MFMA of 32 keys, slot 4 t + r of group g key
+//     4 g + r of tile t; a column's keys are put side by side with byte permutes,
+//     and P goes in as the sum of two 16-bit numbers (2^-17 of it is lost in
+//     bfloat16, 2^-22 in float16, against 2^-9 and 2^-12 of the result's own
+//     rounding), for two MFMAs of 16 cycles a column instead of the 256 cycles of
+//     32-bit ones.  32-bit pools: MFMAs of 4 keys, step r taking keys 4 g + r.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"
@@ -64,15 +67,28 @@ struct Geo {
   static constexpr int NB = (DP + 16 * VE - 1) / (16 * VE);  // V loads of a lane and key
   static constexpr int VW = VE * ES / 4;           // words of one
   static constexpr int LD = DP + 4;                // LDS row of O (floats)
-  // Workgroups a CU holds: by registers (K, V, Q and O of a lane)
-  static constexpr int WGS = DP * ES <= 128 ? 4 : DP * ES <= 256 ? 3 : DP * ES <= 512 ? 2 : 1;
+  // 16-key tiles a wave takes at a time: 16-bit products of 32 keys; 32-bit
+  // ones have no shape to fill and take two tiles where they fit the registers
+  static constexpr int KT = !F32 || DP <= 64 ? 2 : 1;
+  static constexpr int KEYS = 16 * KT * 4;         // keys of a step (4 waves)
+  // Workgroups a CU holds: by registers (K, V and O of a lane)
+  static constexpr int WGS = DP * ES * KT <= 256 ? 3 : DP * ES * KT <= 512 ? 2 : 1;
 };
 
+// Two 32-bit values as a pair of 16-bit ones, rounded to nearest.
 template <int XT>
-__device__ __forceinline__ float element(uint32_t w, int hi) {
-  if constexpr (XT == GEN_BF16) return __uint_as_float(hi ? w & 0xFFFF0000u : w << 16);
-  else if constexpr (XT == GEN_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(hi ? w >> 16 : w & 0xFFFFu));
-  else return __uint_as_float(w);
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if constexpr (XT == GEN_BF16) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)lo, (_Float16)hi});
+  }
+}
+template <int XT>
+__device__ __forceinline__ float half(uint32_t w, int hi) {
+  return xt_to_f32<XT == GEN_F16 ? 1 : 0>(hi ? w >> 16 : w & 0xFFFFu);
 }
 
 template <int XT>
@@ -81,19 +97,28 @@ __device__ __forceinline__ void store_element(void* p, int64_t i, float v) {
   else static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_xt<XT == GEN_F16 ? 1 : 0>(v);
 }
 
+template <int XT>
+__device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) store_element<XT>(p, i + e, v[e]);
+}
+
+// Probabilities are held as 2^lift p: in float16 their largest is then 2^14, and
+// those down to 2^-28 of it keep all their bits.
+template <int XT>
+constexpr float kLift = XT == GEN_F16 ? 14.f : 0.f;
+
 // exp2(a - b), 0 where a is -inf (also where b is)
 __device__ __forceinline__ float exp2_diff(float a, float b) {
   return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
 }
 
-constexpr int kStep = 16 * kWaves;  // keys of a step
-
-// First 16-key tile and number of steps of a sequence.
+// Keys [lo, hi) of a sequence, and its steps.
+template <int KEYS>
 __device__ __forceinline__ int steps_of(int len, int64_t cap, int window, int& lo, int& hi) {
   hi = (int)min((int64_t)max(len, 0), cap);
   lo = window > 0 ? max(0, hi - window) : 0;
-  const int tiles = (hi + 15) / 16 - lo / 16;
-  return (tiles + kWaves - 1) / kWaves;
+  return (hi - lo + KEYS - 1) / KEYS;
 }
 
 // Words of one partial result: O [heads][DP], then (m, l) [heads][2].
@@ -105,8 +130,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   extern __shared__ __align__(16) float lds[];
   __shared__ u32x4 qs[G::KC * 64];
   __shared__ int64_t scan[kWaves];
-  __shared__ int64_t first_off;  // of this workgroup's first step in its sequence
-  __shared__ int first_b;
+  __shared__ int64_t bound[2][2];  // where this workgroup's steps begin and end: step among all, step in its sequence
+  __shared__ int bound_b[2];       // and the sequences
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -115,12 +140,12 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   const int heads_b = a.Hkv * tiles_h;  // (key head, 16 query heads) of a sequence
 
   // the sequences' steps: thread i sums those of its share
-  int64_t total, n, at, end;
+  int64_t n;
   {
     const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
     int64_t mine = 0;
     int lo, hi;
-    for (int b = b0; b < b1; b++) mine += (int64_t)heads_b * steps_of(a.lengths[b], cap, a.window, lo, hi);
+    for (int b = b0; b < b1; b++) mine += (int64_t)heads_b * steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
     int64_t sum = mine;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -129,43 +154,57 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     }
     if (lane == 63) scan[wave] = sum;
     __syncthreads();
-    int64_t before = sum - mine;
-    total = 0;
+    int64_t before = sum - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
       if (w < wave) before += scan[w];
       total += scan[w];
     }
     n = max((total + a.wgs - 1) / a.wgs, (int64_t)a.least);
-    at = blockIdx.x * n;
-    end = min(at + n, total);
-    if (at < end && before <= at && at < before + mine) {
-      int64_t off = at - before;
-      int b = b0;
-      for (;; b++) {
-        const int64_t s = (int64_t)heads_b * steps_of(a.lengths[b], cap, a.window, lo, hi);
-        if (off < s) break;
-        off -= s;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      int64_t p = (blockIdx.x + i) * n;
+      if (p >= total) {
+        if (tid == 0) bound[i][0] = total;
+      } else if (before <= p && p < before + mine) {
+        int64_t off = p - before, s;
+        int b = b0;
+        for (;; b++) {
+          s = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
+          if (off < s * heads_b) break;
+          off -= s * heads_b;
+        }
+        // a head of few steps is not cut: it belongs to the workgroup of its first one
+        if (s <= a.whole && off % s) {
+          p += s - off % s;
+          off += s - off % s;
+        }
+        bound[i][0] = p;
+        bound[i][1] = off;
+        bound_b[i] = b;
       }
-      first_b = b;
-      first_off = off;
     }
     __syncthreads();
   }
   // a sequence without keys has no steps: its output is zeros
   for (int b = blockIdx.x; b < a.B; b += a.wgs) {
     int lo, hi;
-    if (steps_of(a.lengths[b], cap, a.window, lo, hi) == 0)
+    if (steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi) == 0)
       for (int i = tid; i < a.Hq * a.D; i += 256) store_element<XT>(a.out, (int64_t)b * a.Hq * a.D + i, 0.f);
   }
+  int64_t at = bound[0][0];
+  const int64_t end = bound[1][0];
   if (at >= end) return;
-  int b = __builtin_amdgcn_readfirstlane(first_b);
-  int64_t off = first_off;
-  const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)2 * a.wgs * part_words(min(per, 16), DP) * 4));
+  int b = __builtin_amdgcn_readfirstlane(bound_b[0]);
+  int64_t off = bound[0][1];
+  // scores in units of log2 e
+  const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
+  const int slot_words = part_words(min(per, 16), DP);
+  const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)2 * a.wgs * slot_words * 4));
 
   while (at < end) {
     int lo, hi;
-    const int steps = steps_of(a.lengths[b], cap, a.window, lo, hi);
+    const int steps = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
     if (steps == 0 || off >= (int64_t)steps * heads_b) {
       b++;
       off = 0;
@@ -176,15 +215,6 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
     const int heads = min(16, per - 16 * ht), head0 = hk * per + 16 * ht;
 
-    // Q of head c in LDS, a lane's 16 bytes after the other: B operand, the d
-    // order of the K loads
-    for (int i = wave; i < G::KC; i += kWaves) {
-      const char* qp = static_cast<const char*>(a.q) + (b * a.q_b + (head0 + min(c, heads - 1)) * a.q_h) * G::ES;
-      const int d = 4 * G::KE * i + G::KE * g;
-      const u32x4_e w = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
-      qs[i * 64 + lane] = d < a.D ? u32x4{w[0], w[1], w[2], w[3]} : u32x4{0u, 0u, 0u, 0u};
-    }
-    __syncthreads();
     const int32_t* table = a.table + b * a.table_row;
     const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES;
     const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES;
@@ -195,30 +225,34 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
 #pragma unroll
       for (int j = 0; j < G::VE; j++) o[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    uint32_t kr[G::KC][4], vr[4][G::NB][G::VW];
-    int pid = 0, pid_next = 0, key_off = 0;
+    uint32_t kr[G::KT][G::KC][4], vr[G::KT][4][G::NB][G::VW];
+    int pid[G::KT], entry[G::KT], key_off[G::KT];  // pages of the keys in hand, table entries of the next ones
+    // this wave's keys of the segment: 16 KT from k0 on, every KEYS
+    const int k0 = lo + s0 * G::KEYS + wave * (16 * G::KT), k1 = (int)min((int64_t)hi, lo + (int64_t)s1 * G::KEYS);
 
-    // the lane's key of tile t, inside the sequence (rows past its ends are never read)
-    auto page_of = [&](int t, int& in_page) -> int {
-      const int key = min(max(16 * t + c, lo), hi - 1);
+    // The lane's key of the tile from `from` on.  Past the segment it is the
+    // segment's last key: rows outside the sequence are never read, and loads
+    // past the end need no branch (they ask for one row, which is at hand).
+    auto page_of = [&](int from, int& in_page) -> int {
+      const int key = min(from + c, k1 - 1);
       const int slot = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
       in_page = key - slot * a.page;
       return slot;
     };
-    auto load_k = [&]() {
-      const char* kp = kb + (pid * a.k_page + key_off * a.k_tok) * G::ES;
+    auto load_k = [&](int t) {
+      const char* kp = kb + (pid[t] * a.k_page + key_off[t] * a.k_tok) * G::ES;
 #pragma unroll
       for (int i = 0; i < G::KC; i++) {
         const int d = 4 * G::KE * i + G::KE * g;
         const u32x4_e w = *reinterpret_cast<const u32x4_e*>(kp + (d < a.D ? d : 0) * G::ES);
 #pragma unroll
-        for (int e = 0; e < 4; e++) kr[i][e] = w[e];
+        for (int e = 0; e < 4; e++) kr[t][i][e] = w[e];
       }
     };
-    auto load_v = [&]() {
+    auto load_v = [&](int t) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int vpid = __shfl(pid, 4 * g + r), voff = __shfl(key_off, 4 * g + r);
+        const int vpid = __shfl(pid[t], 4 * g + r), voff = __shfl(key_off[t], 4 * g + r);
         const char* vp = vb + (vpid * a.v_page + voff * a.v_tok) * G::ES;
 #pragma unroll
         for (int i = 0; i < G::NB; i++) {
@@ -227,68 +261,100 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
           if constexpr (G::VW == 4) {
             const u32x4_e w = *reinterpret_cast<const u32x4_e*>(p);
 #pragma unroll
-            for (int e = 0; e < 4; e++) vr[r][i][e] = w[e];
+            for (int e = 0; e < 4; e++) vr[t][r][i][e] = w[e];
           } else {
             const u32x2_e w = *reinterpret_cast<const u32x2_e*>(p);
 #pragma unroll
-            for (int e = 0; e < 2; e++) vr[r][i][e] = w[e];
+            for (int e = 0; e < 2; e++) vr[t][r][i][e] = w[e];
           }
         }
       }
     };
-    auto page_id = [&](int slot) { return min(max(table[slot], 0), a.pages - 1); };
+    // the keys in hand become those from `from` on; the ones after them have their table entries loaded
+    auto advance = [&](int from) {
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) {
+        int unused;
+        pid[t] = min(max(entry[t], 0), a.pages - 1);
+        page_of(from + 16 * t, key_off[t]);
+        entry[t] = table[page_of(from + G::KEYS + 16 * t, unused)];
+      }
+    };
 
-    // this wave's tiles of the segment
-    const int t0 = lo / 16 + s0 * kWaves + wave, t1 = min((hi + 15) / 16, lo / 16 + s1 * kWaves);
-    if (t0 < t1) {
-      const int slot = page_of(t0, key_off);
-      int unused;
-      const int slot2 = t0 + kWaves < t1 ? page_of(t0 + kWaves, unused) : slot;
-      pid = page_id(slot);
-      pid_next = page_id(slot2);
-      load_k();
-      load_v();
+    // Q of head c in LDS, a lane's 16 bytes after the other: B operand, the d
+    // order of the K loads
+    u32x4 q0[(G::KC + kWaves - 1) / kWaves];
+#pragma unroll
+    for (int i = wave, j = 0; j < (G::KC + kWaves - 1) / kWaves; i += kWaves, j++) {
+      const int d = 4 * G::KE * i + G::KE * g;
+      const char* qp = static_cast<const char*>(a.q) + (b * a.q_b + (head0 + min(c, heads - 1)) * a.q_h) * G::ES;
+      const u32x4_e w = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
+      q0[j] = d < a.D ? u32x4{w[0], w[1], w[2], w[3]} : u32x4{0u, 0u, 0u, 0u};
     }
-    for (int t = t0; t < t1; t += kWaves) {
-      const bool whole = 16 * t >= lo && 16 * t + 16 <= hi, more = t + kWaves < t1;
+    if (k0 < k1) {
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) entry[t] = table[page_of(k0 + 16 * t, key_off[t])];
+      advance(k0);
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) load_k(t);
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) load_v(t);
+    }
+#pragma unroll
+    for (int i = wave, j = 0; j < (G::KC + kWaves - 1) / kWaves; i += kWaves, j++)
+      if (i < G::KC) qs[i * 64 + lane] = q0[j];
+    __syncthreads();
+    for (int k = k0; k < k1; k += G::KEYS) {
       if (DP != a.D) {  // columns past the head are zero on both sides
 #pragma unroll
-        for (int i = 0; i < G::KC; i++)
+        for (int t = 0; t < G::KT; t++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) kr[i][e] = 4 * G::KE * i + G::KE * g < a.D ? kr[i][e] : 0u;
+          for (int i = 0; i < G::KC; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) kr[t][i][e] = 4 * G::KE * i + G::KE * g < a.D ? kr[t][i][e] : 0u;
       }
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
-      asm volatile("" ::: "memory");  // Q is read again each tile, not kept in registers
+      f32x4 s[G::KT];
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      asm volatile("" ::: "memory");  // Q is read again each time, not kept in registers
 #pragma unroll
       for (int i = 0; i < G::KC; i++) {
         const u32x4 q = qs[i * 64 + lane];
-        if constexpr (G::F32) {
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[i][e]), __uint_as_float(q[e]), s, 0, 0, 0);
-        } else {
-          s = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(u32x4{kr[i][0], kr[i][1], kr[i][2], kr[i][3]}, q, s);
+        for (int t = 0; t < G::KT; t++) {
+          if constexpr (G::F32) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][i][e]), __uint_as_float(q[e]), s[t], 0,
+                                                          0, 0);
+          } else {
+            s[t] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(
+                u32x4{kr[t][i][0], kr[t][i][1], kr[t][i][2], kr[t][i][3]}, q, s[t]);
+          }
         }
       }
-      if (more) {
-        pid = pid_next;
-        page_of(t + kWaves, key_off);
-        if (t + 2 * kWaves < t1) {
-          int unused;
-          pid_next = page_id(page_of(t + 2 * kWaves, unused));
-        }
-        load_k();
+      advance(k + G::KEYS);
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) load_k(t);
+      if (a.softcap > 0.f) {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[t][r] = cap_log2e * tanhf(s[t][r] * scale);
+      } else {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[t][r] *= scale;
       }
       float mt = m;
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        float x = s[r] * a.scale;
-        if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-        x *= kLog2e;
-        const int sk = 16 * t + 4 * g + r;
-        s[r] = whole || (sk >= lo && sk < hi) ? x : -INFINITY;
-        mt = fmaxf(mt, s[r]);
-      }
+      for (int t = 0; t < G::KT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          s[t][r] = k + 16 * t + 4 * g + r < k1 ? s[t][r] : -INFINITY;
+          mt = fmaxf(mt, s[t][r]);
+        }
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = fmaxf(mt, __shfl_xor(mt, 32));
       if (__any(mt > m)) {
@@ -302,30 +368,62 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
 #pragma unroll
             for (int r = 0; r < 4; r++) o[i][j][r] *= f;
       }
-      if (!whole) {  // the values of keys outside count as zero, also where they are not numbers
+      if (k + 16 * G::KT > k1) {
+        // past the segment p is 0, and the row read in its place has to count as 0 also where it is not finite
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int vk = 16 * t + 4 * g + r;
-          const bool live = vk >= lo && vk < hi;
+        for (int t = 0; t < G::KT; t++)
 #pragma unroll
-          for (int i = 0; i < G::NB; i++)
+          for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int e = 0; e < G::VW; e++) vr[r][i][e] = live ? vr[r][i][e] : 0u;
-        }
+            for (int i = 0; i < G::NB; i++)
+#pragma unroll
+              for (int e = 0; e < G::VW; e++) vr[t][r][i][e] = k + 16 * t + 4 * g + r < k1 ? vr[t][r][i][e] : 0u;
       }
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const float p = exp2_diff(s[r], m);
-        l += p;
+      for (int t = 0; t < G::KT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          s[t][r] = exp2_diff(s[t][r] + kLift<XT>, m);
+          l += s[t][r];
+        }
+      if constexpr (G::F32) {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int i = 0; i < G::NB; i++)
+#pragma unroll
+              for (int j = 0; j < G::VE; j++)
+                o[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][r][i][j]), s[t][r], o[i][j], 0, 0, 0);
+      } else {
+        // P = ph + pl
+        u32x4 ph, pl;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            const uint32_t h = pack<XT>(s[t][r], s[t][r + 1]);
+            ph[2 * t + r / 2] = h;
+            pl[2 * t + r / 2] = pack<XT>(s[t][r] - half<XT>(h, 0), s[t][r + 1] - half<XT>(h, 1));
+          }
 #pragma unroll
         for (int i = 0; i < G::NB; i++)
 #pragma unroll
           for (int j = 0; j < G::VE; j++) {
-            const float v = element<XT>(vr[r][i][G::F32 ? j : j >> 1], j & 1);
-            o[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p, o[i][j], 0, 0, 0);
+            const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+            u32x4 v;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+              for (int r = 0; r < 4; r += 2)
+                v[2 * t + r / 2] = __builtin_amdgcn_perm(vr[t][r + 1][i][j / 2], vr[t][r][i][j / 2], sel);
+            o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, ph, o[i][j]);
+            o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, pl, o[i][j]);
           }
       }
-      if (more) load_v();
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) load_v(t);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -346,46 +444,45 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
           }
         }
       if (g == 0) {
-        ml[(wave * 16 + c) * 2] = m;
+        ml[(wave * 16 + c) * 2] = m - kLift<XT>;
         ml[(wave * 16 + c) * 2 + 1] = l;
       }
     }
     __syncthreads();
-    const int64_t u0 = at - s0, u1 = u0 + steps;  // the head's steps among all
-    const int w0 = (int)(u0 / n), w1 = (int)((u1 - 1) / n);
-    const int words = part_words(heads, DP);
-    auto part_at = [&](int w) -> uint32_t {  // bytes; a workgroup's first head that began before it, or its last
-      return (uint32_t)((2 * w + (w == w0)) * part_words(min(per, 16), DP)) * 4u;
-    };
-    auto finish = [&](int h, int d, float M, float L, float acc) {
+    const int64_t u0 = at - s0;  // the head's first step among all
+    const int w0 = (int)(u0 / n), w1 = steps <= a.whole ? w0 : (int)((u0 + steps - 1) / n);
+    // bytes of a workgroup's partial result: of its last head (slot 1), or of one that began before it (slot 0)
+    auto part_at = [&](int w) -> uint32_t { return (uint32_t)((2 * w + (w == w0)) * slot_words) * 4u; };
+    auto finish = [&](int h, int d, float M, float L, f32x4 acc) {
+      float f = 1.f;
       if (a.sinks) {
-        const float sink = a.sinks[head0 + h] * kLog2e, M2 = fmaxf(M, sink), f = exp2_diff(M, M2);
+        const float sink = a.sinks[head0 + h] * kLog2e, M2 = fmaxf(M, sink);
+        f = exp2_diff(M, M2);
         L = L * f + exp2_diff(sink, M2);
-        acc *= f;
       }
-      store_element<XT>(a.out, ((int64_t)b * a.Hq + head0 + h) * a.D + d, L == 0.f ? 0.f : acc / L);
+      const float r = L == 0.f ? 0.f : f / L;
+      if (d < a.D) store4<XT>(a.out, ((int64_t)b * a.Hq + head0 + h) * a.D + d, acc * r);
     };
-    for (int e = tid; e < heads * DP; e += 256) {
-      const int h = e / DP, d = e - h * DP;
-      float M = -INFINITY, L = 0.f, acc = 0.f;
+    for (int e = tid; e < heads * (DP / 4); e += 256) {
+      const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
+      float M = -INFINITY, L = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWaves; w++) M = fmaxf(M, ml[(w * 16 + h) * 2]);
 #pragma unroll
       for (int w = 0; w < kWaves; w++) {
         const float f = exp2_diff(ml[(w * 16 + h) * 2], M);
         L += f * ml[(w * 16 + h) * 2 + 1];
-        acc += f * lds[(w * heads + h) * G::LD + d];
+        acc += f * *reinterpret_cast<const f32x4*>(lds + (w * heads + h) * G::LD + d);
       }
       if (w0 == w1) {
-        if (d < a.D) finish(h, d, M, L, acc);
+        finish(h, d, M, L, acc);
       } else {
         const uint32_t p = part_at(blockIdx.x);
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc), parts, p + e * 4, 0, kAgentScope);
-        if (d == 0) {
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(M), parts, p + (heads * DP + 2 * h) * 4, 0, kAgentScope);
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(L), parts, p + (heads * DP + 2 * h + 1) * 4, 0,
-                                                kAgentScope);
-        }
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + e * 16, 0, kAgentScope);
+        if (d == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
+                                                p + (heads * DP + 2 * h) * 4, 0, kAgentScope);
       }
     }
     if (w0 != w1) {
@@ -395,20 +492,32 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
       __syncthreads();
       if (arrived == (uint32_t)(w1 - w0)) {  // the last one joins, in the order of the keys
         if (tid == 0) __hip_atomic_store(a.cnt + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (int e = tid; e < heads * DP; e += 256) {
-          const int h = e / DP, d = e - h * DP;
-          float M = -INFINITY, L = 0.f, acc = 0.f;
-          for (int w = w0; w <= w1; w++) {
-            const uint32_t p = part_at(w), pm = p + (heads * DP + 2 * h) * 4;
-            const float mw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, pm, 0, kAgentScope));
-            const float lw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, pm + 4, 0, kAgentScope));
-            const float ow = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, p + e * 4, 0, kAgentScope));
-            const float M2 = fmaxf(M, mw), f = exp2_diff(M, M2), fw = exp2_diff(mw, M2);
-            M = M2;
-            L = L * f + lw * fw;
-            acc = acc * f + ow * fw;
+        for (int e = tid; e < heads * (DP / 4); e += 256) {
+          const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
+          float M = -INFINITY, L = 0.f;
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+          constexpr int U = G::NB * G::VE <= 8 ? 8 : 4;  // partial results in flight
+          for (int w = w0; w <= w1; w += U) {
+            u32x4 ow[U];
+            u32x2 mw[U];
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+              const uint32_t p = part_at(min(w + i, w1));
+              mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(
+                                                    parts, p + (heads * DP + 2 * h) * 4, 0, kAgentScope));
+              ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + e * 16, 0, kAgentScope));
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+              if (w + i > w1) break;
+              const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
+              const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
+              M = M2;
+              L = L * f + __uint_as_float(mw[i][1]) * fi;
+              acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
+            }
           }
-          if (d < a.D) finish(h, d, M, L, acc);
+          finish(h, d, M, L, acc);
         }
       }
     }
@@ -444,8 +553,8 @@ auto with_kernel(const PagedAttnArgs& a, F&& f) {
 
 }  // namespace
 
-// Steps a workgroup takes at least: below that, joining costs more than it saves.
-constexpr int kLeastSteps = 4;
+// Steps a workgroup takes at least, and steps of a head that is never cut.
+constexpr int kLeastSteps = 1, kWholeSteps = 4;
 
 void paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
   a.page_shift = 30;
@@ -453,10 +562,19 @@ void paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
   // exact for keys below 2^30: the error of page_mul, below page <= 2^(shift - 30), times the key stays below 2^shift
   a.page_mul = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page - 1) / a.page);
   const int per = a.Hq / a.Hkv;
-  const int64_t keys = a.window > 0 ? std::min<int64_t>(a.window + 15, (int64_t)a.width * a.page) : (int64_t)a.width * a.page;
-  const int64_t most = (int64_t)a.B * a.Hkv * ((per + 15) / 16) * ((keys + 15 + kStep - 1) / kStep);
+  const int64_t cap = (int64_t)a.width * a.page, keys = a.window > 0 ? std::min<int64_t>(a.window, cap) : cap;
+  int step = 0, resident = 0;
+  with_kernel(a, [&](auto xt, auto dp) {
+    step = Geo<decltype(xt)::value, decltype(dp)::value>::KEYS;
+    resident = Geo<decltype(xt)::value, decltype(dp)::value>::WGS;
+    return 0;
+  });
+  const int64_t most = (int64_t)a.B * a.Hkv * ((per + 15) / 16) * ((keys + step - 1) / step);
   a.least = kLeastSteps;
-  const int resident = with_kernel(a, [](auto xt, auto dp) { return Geo<decltype(xt)::value, decltype(dp)::value>::WGS; });
+  a.whole = kWholeSteps;
+  if (getenv("PA_LEAST")) a.least = atoi(getenv("PA_LEAST"));
+  if (getenv("PA_WHOLE")) a.whole = atoi(getenv("PA_WHOLE"));
+  if (getenv("PA_RES")) resident = atoi(getenv("PA_RES"));
   a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>((most + a.least - 1) / a.least, (int64_t)cus * resident));
   const int words = with_kernel(a, [&](auto, auto dp) { return part_words(std::min(per, 16), decltype(dp)::value); });
   *part_bytes = (int64_t)2 * a.wgs * words * 4;

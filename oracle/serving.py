@@ -10,8 +10,10 @@ import numpy as np
 U = 2.0 ** -24
 
 
-def attention(q, k, v, table, lengths, scale, softcap=0.0, window=0, sinks=None):
+def attention(q, k, v, table, lengths, scale, softcap=0.0, window=0, sinks=None, split=0.0):
     """q (B, Hq, D), pools (pages, Hkv, page, D) as float64; (out, slack).
+    split: what a probability loses where it enters a product as two 16-bit
+    numbers (2^-17 of it in bfloat16, 2^-22 in float16).
 
     Slack: a score of D products differs by (D + 8) u sum|q k| scale (its
     rounding, the cap and the change of base included); p then by twice the
@@ -38,7 +40,7 @@ def attention(q, k, v, table, lengths, scale, softcap=0.0, window=0, sinks=None)
             total = p.sum() + (0 if sinks is None else np.exp(sinks[h] - m))
             d += 4 * U * np.abs(s).max()
             out[b, h] = p @ vv / total
-            slack[b, h] = p @ np.abs(vv) / total * (2 * d + (len(at) + 32) * U)
+            slack[b, h] = p @ np.abs(vv) / total * (2 * d + split + (len(at) + 32) * U)
     return out, slack
 
 

@@ -12,6 +12,8 @@ from serving import DTYPES, Cache, f64, i32, within
 
 pytestmark = pytest.mark.gpu
 
+# what a probability loses as the sum of two 16-bit numbers
+SPLIT = {torch.bfloat16: 2.0 ** -17, torch.float16: 2.0 ** -22, torch.float32: 0.0}
 LENGTHS = [1, 0, 15, 16, 17, 33, 64, 65, 100, 257]
 
 
@@ -22,7 +24,7 @@ def check(c, q, window=0, softcap=0.0, sinks=None, scale=None, lengths=None, tab
     got = mq.paged_attention(q, c.k, c.v, i32(table), i32(lengths), window=window, softcap=softcap, sinks=s,
                              scale=scale, **kw)
     want, slack = ref.attention(f64(q), f64(c.k), f64(c.v), table, lengths, c.D ** -0.5 if scale is None else scale,
-                                softcap, window, None if s is None else f64(s))
+                                softcap, window, None if s is None else f64(s), SPLIT[q.dtype])
     within(got, want, slack)
     return got
 
@@ -197,7 +199,7 @@ def test_graph_and_another_stream():
         torch.cuda.synchronize()
         g.replay()
         torch.cuda.synchronize()
-        want, slack = ref.attention(f64(q), f64(c.k), f64(c.v), c.table, lens, 64 ** -0.5)
+        want, slack = ref.attention(f64(q), f64(c.k), f64(c.v), c.table, lens, 64 ** -0.5, split=SPLIT[q.dtype])
         within(out, want, slack, lens)
 
 
