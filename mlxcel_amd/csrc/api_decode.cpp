@@ -266,7 +266,9 @@ mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool, 
     a.out = oc.data;
     const int dev = current_device();
     int64_t part_bytes = 0;
-    mlxq::paged_attention_plan(a, device_cus(dev), &part_bytes);
+    if (!mlxq::paged_attention_plan(a, device_cus(dev), &part_bytes))
+      (Refusal(tag) << "a table of " << a.B << " rows of " << t.dim(1) << " pages holds too many keys for one call.")
+          .unsupported();
     a.part = static_cast<float*>(stream_workspace(dev, stream, part_bytes, 0));
     a.cnt = stream_counters(dev, stream);
     if (!a.cnt)

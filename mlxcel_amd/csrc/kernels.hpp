@@ -583,12 +583,13 @@ struct PagedAttnArgs {
   // how the keys are split (paged_attention_plan)
   uint32_t page_mul;       // key / page = key * page_mul >> page_shift
   int page_shift;
-  int wgs, least, whole;   // workgroups; steps a workgroup takes at least; steps of a head that is not cut
+  int wgs, whole;          // workgroups; steps of a head that is not cut
   float* part;             // [2 wgs] partial results of part_words each
-  uint32_t* cnt;           // [wgs], zero between launches
+  uint32_t* cnt;           // [2 wgs], zero between launches
 };
-// Sets the plan; part_bytes of scratch (and wgs counters) are needed.
-void paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes);
+// Sets the plan; part_bytes of scratch are needed.  False where
+// the steps cannot be counted in 32 bits.
+bool paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes);
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
 
 // The cache's bookkeeping (pages.hip): a table of pages per sequence, the

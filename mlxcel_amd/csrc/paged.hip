@@ -39,7 +39,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"
@@ -72,7 +71,7 @@ struct Geo {
   static constexpr int KT = !F32 || DP <= 64 ? 2 : 1;
   static constexpr int KEYS = 16 * KT * 4;         // keys of a step (4 waves)
   // Workgroups a CU holds: by registers (K, V and O of a lane)
-  static constexpr int WGS = DP * ES * KT <= 256 ? 3 : DP * ES * KT <= 512 ? 2 : 1;
+  static constexpr int WGS = DP * ES * KT <= 256 ? 4 : DP * ES * KT <= 512 ? 2 : 1;
 };
 
 // Two 32-bit values as a pair of 16-bit ones, rounded to nearest.
@@ -121,6 +120,9 @@ __device__ __forceinline__ int steps_of(int len, int64_t cap, int window, int& l
   return (hi - lo + KEYS - 1) / KEYS;
 }
 
+// Workgroups whose results one of them joins, and how many are read at a time.
+constexpr int kJoin = 16, kFlight = 8;
+
 // Words of one partial result: O [heads][DP], then (m, l) [heads][2].
 constexpr int part_words(int heads, int DP) { return heads * (DP + 2); }
 
@@ -129,9 +131,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   using G = Geo<XT, DP>;
   extern __shared__ __align__(16) float lds[];
   __shared__ u32x4 qs[G::KC * 64];
-  __shared__ int64_t scan[kWaves];
-  __shared__ int64_t bound[2][2];  // where this workgroup's steps begin and end: step among all, step in its sequence
-  __shared__ int bound_b[2];       // and the sequences
+  __shared__ int scan[kWaves];
+  __shared__ int bound[2][3];  // where this workgroup's steps begin and end: step among all, step in its sequence, sequence
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -140,35 +141,33 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   const int heads_b = a.Hkv * tiles_h;  // (key head, 16 query heads) of a sequence
 
   // the sequences' steps: thread i sums those of its share
-  int64_t n;
+  int n;
   {
     const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
-    int64_t mine = 0;
-    int lo, hi;
-    for (int b = b0; b < b1; b++) mine += (int64_t)heads_b * steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
-    int64_t sum = mine;
+    int mine = 0, lo, hi;
+    for (int b = b0; b < b1; b++) mine += heads_b * steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
+    int sum = mine;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-      const int64_t o = __shfl_up((long long)sum, s);
+      const int o = __shfl_up(sum, s);
       if (lane >= s) sum += o;
     }
     if (lane == 63) scan[wave] = sum;
     __syncthreads();
-    int64_t before = sum - mine, total = 0;
+    int before = sum - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
       if (w < wave) before += scan[w];
       total += scan[w];
     }
-    n = max((total + a.wgs - 1) / a.wgs, (int64_t)a.least);
+    n = (total + a.wgs - 1) / a.wgs;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      int64_t p = (blockIdx.x + i) * n;
+      int p = ((int)blockIdx.x + i) * n;
       if (p >= total) {
         if (tid == 0) bound[i][0] = total;
       } else if (before <= p && p < before + mine) {
-        int64_t off = p - before, s;
-        int b = b0;
+        int off = p - before, b = b0, s;
         for (;; b++) {
           s = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
           if (off < s * heads_b) break;
@@ -181,7 +180,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
         }
         bound[i][0] = p;
         bound[i][1] = off;
-        bound_b[i] = b;
+        bound[i][2] = b;
       }
     }
     __syncthreads();
@@ -192,11 +191,10 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     if (steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi) == 0)
       for (int i = tid; i < a.Hq * a.D; i += 256) store_element<XT>(a.out, (int64_t)b * a.Hq * a.D + i, 0.f);
   }
-  int64_t at = bound[0][0];
-  const int64_t end = bound[1][0];
+  int at = __builtin_amdgcn_readfirstlane(bound[0][0]);
+  const int end = __builtin_amdgcn_readfirstlane(bound[1][0]);
   if (at >= end) return;
-  int b = __builtin_amdgcn_readfirstlane(bound_b[0]);
-  int64_t off = bound[0][1];
+  int off = __builtin_amdgcn_readfirstlane(bound[0][1]), b = __builtin_amdgcn_readfirstlane(bound[0][2]);
   // scores in units of log2 e
   const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
   const int slot_words = part_words(min(per, 16), DP);
@@ -205,13 +203,12 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   while (at < end) {
     int lo, hi;
     const int steps = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
-    if (steps == 0 || off >= (int64_t)steps * heads_b) {
+    if (steps == 0 || off >= steps * heads_b) {
       b++;
       off = 0;
       continue;
     }
-    const int hh = (int)(off / steps), s0 = (int)(off - (int64_t)hh * steps);
-    const int s1 = (int)min((int64_t)steps, s0 + (end - at));
+    const int hh = off / steps, s0 = off - hh * steps, s1 = min(steps, s0 + (end - at));
     const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
     const int heads = min(16, per - 16 * ht), head0 = hk * per + 16 * ht;
 
@@ -228,7 +225,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     uint32_t kr[G::KT][G::KC][4], vr[G::KT][4][G::NB][G::VW];
     int pid[G::KT], entry[G::KT], key_off[G::KT];  // pages of the keys in hand, table entries of the next ones
     // this wave's keys of the segment: 16 KT from k0 on, every KEYS
-    const int k0 = lo + s0 * G::KEYS + wave * (16 * G::KT), k1 = (int)min((int64_t)hi, lo + (int64_t)s1 * G::KEYS);
+    const int k0 = lo + s0 * G::KEYS + wave * (16 * G::KT), k1 = min(hi, lo + s1 * G::KEYS);
 
     // The lane's key of the tile from `from` on.  Past the segment it is the
     // segment's last key: rows outside the sequence are never read, and loads
@@ -449,10 +446,17 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
       }
     }
     __syncthreads();
-    const int64_t u0 = at - s0;  // the head's first step among all
-    const int w0 = (int)(u0 / n), w1 = steps <= a.whole ? w0 : (int)((u0 + steps - 1) / n);
+    const int u0 = at - s0;  // the head's first step among all
+    const int w0 = u0 / n, w1 = steps <= a.whole ? w0 : (u0 + steps - 1) / n;
     // bytes of a workgroup's partial result: of its last head (slot 1), or of one that began before it (slot 0)
     auto part_at = [&](int w) -> uint32_t { return (uint32_t)((2 * w + (w == w0)) * slot_words) * 4u; };
+    auto put = [&](int w, int e, float M, float L, f32x4 acc) {
+      const uint32_t p = part_at(w);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + e * 16, 0, kAgentScope);
+      if (e % (DP / 4) == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
+                                              p + (heads * DP + 2 * (e / (DP / 4))) * 4, 0, kAgentScope);
+    };
     auto finish = [&](int h, int d, float M, float L, f32x4 acc) {
       float f = 1.f;
       if (a.sinks) {
@@ -478,46 +482,67 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
       if (w0 == w1) {
         finish(h, d, M, L, acc);
       } else {
-        const uint32_t p = part_at(blockIdx.x);
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + e * 16, 0, kAgentScope);
-        if (d == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
-                                                p + (heads * DP + 2 * h) * 4, 0, kAgentScope);
+        put(blockIdx.x, e, M, L, acc);
       }
     }
     if (w0 != w1) {
-      __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
-      __syncthreads();
-      if (tid == 0) arrived = __hip_atomic_fetch_add(a.cnt + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      if (arrived == (uint32_t)(w1 - w0)) {  // the last one joins, in the order of the keys
-        if (tid == 0) __hip_atomic_store(a.cnt + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      // The last of up to kJoin neighbours to arrive joins them; of more, the
+      // last to have joined its neighbours joins the results.
+      auto last_of = [&](uint32_t* cnt, int of) -> bool {
+        __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
+        __syncthreads();
+        if (tid == 0) {
+          const uint32_t old = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          arrived = old == (uint32_t)(of - 1);
+          if (arrived) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        return arrived != 0;
+      };
+      // sum of the results of workgroups w, w + by, .. (of them), in the order of the keys
+      auto join = [&](int w, int by, int of, int e, float& M, float& L, f32x4& acc) {
+        const int h = e / (DP / 4);
+        M = -INFINITY, L = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < of; i0 += kFlight) {
+          u32x4 ow[kFlight];
+          u32x2 mw[kFlight];
+#pragma unroll
+          for (int i = 0; i < kFlight; i++) {
+            const uint32_t p = part_at(w + by * min(i0 + i, of - 1));
+            mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + (heads * DP + 2 * h) * 4,
+                                                                                   0, kAgentScope));
+            ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + e * 16, 0, kAgentScope));
+          }
+#pragma unroll
+          for (int i = 0; i < kFlight; i++) {
+            if (i0 + i >= of) break;
+            const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
+            const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
+            M = M2;
+            L = L * f + __uint_as_float(mw[i][1]) * fi;
+            acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
+          }
+        }
+      };
+      const int of = w1 - w0 + 1, mine = ((int)blockIdx.x - w0) / kJoin * kJoin, near = min(kJoin, of - mine);
+      if (last_of(a.cnt + w0 + mine, near)) {
         for (int e = tid; e < heads * (DP / 4); e += 256) {
           const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
-          float M = -INFINITY, L = 0.f;
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-          constexpr int U = G::NB * G::VE <= 8 ? 8 : 4;  // partial results in flight
-          for (int w = w0; w <= w1; w += U) {
-            u32x4 ow[U];
-            u32x2 mw[U];
-#pragma unroll
-            for (int i = 0; i < U; i++) {
-              const uint32_t p = part_at(min(w + i, w1));
-              mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(
-                                                    parts, p + (heads * DP + 2 * h) * 4, 0, kAgentScope));
-              ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + e * 16, 0, kAgentScope));
-            }
-#pragma unroll
-            for (int i = 0; i < U; i++) {
-              if (w + i > w1) break;
-              const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
-              const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
-              M = M2;
-              L = L * f + __uint_as_float(mw[i][1]) * fi;
-              acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
-            }
+          float M, L;
+          f32x4 acc;
+          join(w0 + mine, 1, near, e, M, L, acc);
+          if (of <= kJoin) finish(h, d, M, L, acc);
+          else put(w0 + mine, e, M, L, acc);
+        }
+        const int groups = (of + kJoin - 1) / kJoin;
+        if (of > kJoin && last_of(a.cnt + a.wgs + w0, groups)) {
+          for (int e = tid; e < heads * (DP / 4); e += 256) {
+            const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
+            float M, L;
+            f32x4 acc;
+            join(w0, kJoin, groups, e, M, L, acc);
+            finish(h, d, M, L, acc);
           }
-          finish(h, d, M, L, acc);
         }
       }
     }
@@ -553,10 +578,12 @@ auto with_kernel(const PagedAttnArgs& a, F&& f) {
 
 }  // namespace
 
-// Steps a workgroup takes at least, and steps of a head that is never cut.
-constexpr int kLeastSteps = 1, kWholeSteps = 4;
+// Steps of a head that is not cut: taking them one after the other costs about
+// what a join costs (one sequence of 1000 keys, 8 steps a head: 11.1 us cut, 24.8
+// whole; 200 sequences of 1 to 4 steps: 15.5 us whole, 16.5 cut at every step).
+constexpr int kWholeSteps = 4;
 
-void paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
+bool paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
   a.page_shift = 30;
   while (((int64_t)1 << (a.page_shift - 30)) < a.page) a.page_shift++;
   // exact for keys below 2^30: the error of page_mul, below page <= 2^(shift - 30), times the key stays below 2^shift
@@ -570,19 +597,16 @@ void paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
     return 0;
   });
   const int64_t most = (int64_t)a.B * a.Hkv * ((per + 15) / 16) * ((keys + step - 1) / step);
-  a.least = kLeastSteps;
   a.whole = kWholeSteps;
-  if (getenv("PA_LEAST")) a.least = atoi(getenv("PA_LEAST"));
-  if (getenv("PA_WHOLE")) a.whole = atoi(getenv("PA_WHOLE"));
-  if (getenv("PA_RES")) resident = atoi(getenv("PA_RES"));
-  a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>((most + a.least - 1) / a.least, (int64_t)cus * resident));
+  a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)cus * resident));
   const int words = with_kernel(a, [&](auto, auto dp) { return part_words(std::min(per, 16), decltype(dp)::value); });
   *part_bytes = (int64_t)2 * a.wgs * words * 4;
+  return most <= (1 << 30);
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
   if (a.B == 0) return hipSuccess;
-  if (a.D < 8 || a.D > 256 || a.D % 8 || a.pages < 1 || a.page < 1 || a.wgs < 1 || a.wgs > kSplitCounters)
+  if (a.D < 8 || a.D > 256 || a.D % 8 || a.pages < 1 || a.page < 1 || a.wgs < 1 || 2 * a.wgs > kSplitCounters)
     return hipErrorInvalidValue;
   return with_kernel(a, [&](auto xt, auto dp) { return launch<decltype(xt)::value, decltype(dp)::value>(a, stream); });
 }
