@@ -107,6 +107,13 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
 template <int XT>
 constexpr float kLift = XT == GEN_F16 ? 14.f : 0.f;
 
+// A load that leaves the caches to others (ONCE), or an ordinary one.
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load(const char* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else return *reinterpret_cast<const T*>(p);
+}
+
 // exp2(a - b), 0 where a is -inf (also where b is)
 __device__ __forceinline__ float exp2_diff(float a, float b) {
   return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
@@ -119,6 +126,8 @@ __device__ __forceinline__ int steps_of(int len, int64_t cap, int window, int& l
   lo = window > 0 ? max(0, hi - window) : 0;
   return (hi - lo + KEYS - 1) / KEYS;
 }
+
+constexpr int64_t kLastCache = (int64_t)256 << 20;
 
 // Workgroups whose results one of them joins, and how many are read at a time.
 constexpr int kJoin = 16, kFlight = 8;
@@ -142,6 +151,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
 
   // the sequences' steps: thread i sums those of its share
   int n;
+  bool once;
   {
     const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
     int mine = 0, lo, hi;
@@ -161,6 +171,9 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
       total += scan[w];
     }
     n = (total + a.wgs - 1) / a.wgs;
+    // More keys and values than the last cache holds are not kept there for
+    // the next call: 2.1 GB 360 -> 325 us; 174 MB, read again and again, 37 -> 44 us.
+    once = (int64_t)total * (G::KEYS * 2 * G::ES) * a.D > kLastCache;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       int p = ((int)blockIdx.x + i) * n;
@@ -200,356 +213,360 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   const int slot_words = part_words(min(per, 16), DP);
   const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)2 * a.wgs * slot_words * 4));
 
-  while (at < end) {
-    int lo, hi;
-    const int steps = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
-    if (steps == 0 || off >= steps * heads_b) {
-      b++;
-      off = 0;
-      continue;
-    }
-    const int hh = off / steps, s0 = off - hh * steps, s1 = min(steps, s0 + (end - at));
-    const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
-    const int heads = min(16, per - 16 * ht), head0 = hk * per + 16 * ht;
+  auto run = [&](auto ONCE) {
+    while (at < end) {
+      int lo, hi;
+      const int steps = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
+      if (steps == 0 || off >= steps * heads_b) {
+        b++;
+        off = 0;
+        continue;
+      }
+      const int hh = off / steps, s0 = off - hh * steps, s1 = min(steps, s0 + (end - at));
+      const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
+      const int heads = min(16, per - 16 * ht), head0 = hk * per + 16 * ht;
 
-    const int32_t* table = a.table + b * a.table_row;
-    const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES;
-    const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES;
+      const int32_t* table = a.table + b * a.table_row;
+      const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES;
+      const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES;
 
-    f32x4 o[G::NB][G::VE];
-#pragma unroll
-    for (int i = 0; i < G::NB; i++)
-#pragma unroll
-      for (int j = 0; j < G::VE; j++) o[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    uint32_t kr[G::KT][G::KC][4], vr[G::KT][4][G::NB][G::VW];
-    int pid[G::KT], entry[G::KT], key_off[G::KT];  // pages of the keys in hand, table entries of the next ones
-    // this wave's keys of the segment: 16 KT from k0 on, every KEYS
-    const int k0 = lo + s0 * G::KEYS + wave * (16 * G::KT), k1 = min(hi, lo + s1 * G::KEYS);
-
-    // The lane's key of the tile from `from` on.  Past the segment it is the
-    // segment's last key: rows outside the sequence are never read, and loads
-    // past the end need no branch (they ask for one row, which is at hand).
-    auto page_of = [&](int from, int& in_page) -> int {
-      const int key = min(from + c, k1 - 1);
-      const int slot = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
-      in_page = key - slot * a.page;
-      return slot;
-    };
-    auto load_k = [&](int t) {
-      const char* kp = kb + (pid[t] * a.k_page + key_off[t] * a.k_tok) * G::ES;
-#pragma unroll
-      for (int i = 0; i < G::KC; i++) {
-        const int d = 4 * G::KE * i + G::KE * g;
-        const u32x4_e w = *reinterpret_cast<const u32x4_e*>(kp + (d < a.D ? d : 0) * G::ES);
-#pragma unroll
-        for (int e = 0; e < 4; e++) kr[t][i][e] = w[e];
-      }
-    };
-    auto load_v = [&](int t) {
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int vpid = __shfl(pid[t], 4 * g + r), voff = __shfl(key_off[t], 4 * g + r);
-        const char* vp = vb + (vpid * a.v_page + voff * a.v_tok) * G::ES;
-#pragma unroll
-        for (int i = 0; i < G::NB; i++) {
-          const int d = 16 * G::VE * i + G::VE * c;
-          const char* p = vp + (d < a.D ? d : 0) * G::ES;  // columns past the head are dropped at the end
-          if constexpr (G::VW == 4) {
-            const u32x4_e w = *reinterpret_cast<const u32x4_e*>(p);
-#pragma unroll
-            for (int e = 0; e < 4; e++) vr[t][r][i][e] = w[e];
-          } else {
-            const u32x2_e w = *reinterpret_cast<const u32x2_e*>(p);
-#pragma unroll
-            for (int e = 0; e < 2; e++) vr[t][r][i][e] = w[e];
-          }
-        }
-      }
-    };
-    // the keys in hand become those from `from` on; the ones after them have their table entries loaded
-    auto advance = [&](int from) {
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) {
-        int unused;
-        pid[t] = min(max(entry[t], 0), a.pages - 1);
-        page_of(from + 16 * t, key_off[t]);
-        entry[t] = table[page_of(from + G::KEYS + 16 * t, unused)];
-      }
-    };
-
-    // Q of head c in LDS, a lane's 16 bytes after the other: B operand, the d
-    // order of the K loads
-    u32x4 q0[(G::KC + kWaves - 1) / kWaves];
-#pragma unroll
-    for (int i = wave, j = 0; j < (G::KC + kWaves - 1) / kWaves; i += kWaves, j++) {
-      const int d = 4 * G::KE * i + G::KE * g;
-      const char* qp = static_cast<const char*>(a.q) + (b * a.q_b + (head0 + min(c, heads - 1)) * a.q_h) * G::ES;
-      const u32x4_e w = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
-      q0[j] = d < a.D ? u32x4{w[0], w[1], w[2], w[3]} : u32x4{0u, 0u, 0u, 0u};
-    }
-    if (k0 < k1) {
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) entry[t] = table[page_of(k0 + 16 * t, key_off[t])];
-      advance(k0);
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) load_k(t);
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) load_v(t);
-    }
-#pragma unroll
-    for (int i = wave, j = 0; j < (G::KC + kWaves - 1) / kWaves; i += kWaves, j++)
-      if (i < G::KC) qs[i * 64 + lane] = q0[j];
-    __syncthreads();
-    for (int k = k0; k < k1; k += G::KEYS) {
-      if (DP != a.D) {  // columns past the head are zero on both sides
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int i = 0; i < G::KC; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) kr[t][i][e] = 4 * G::KE * i + G::KE * g < a.D ? kr[t][i][e] : 0u;
-      }
-      f32x4 s[G::KT];
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      asm volatile("" ::: "memory");  // Q is read again each time, not kept in registers
-#pragma unroll
-      for (int i = 0; i < G::KC; i++) {
-        const u32x4 q = qs[i * 64 + lane];
-#pragma unroll
-        for (int t = 0; t < G::KT; t++) {
-          if constexpr (G::F32) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][i][e]), __uint_as_float(q[e]), s[t], 0,
-                                                          0, 0);
-          } else {
-            s[t] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(
-                u32x4{kr[t][i][0], kr[t][i][1], kr[t][i][2], kr[t][i][3]}, q, s[t]);
-          }
-        }
-      }
-      advance(k + G::KEYS);
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) load_k(t);
-      if (a.softcap > 0.f) {
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) s[t][r] = cap_log2e * tanhf(s[t][r] * scale);
-      } else {
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) s[t][r] *= scale;
-      }
-      float mt = m;
-#pragma unroll
-      for (int t = 0; t < G::KT; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          s[t][r] = k + 16 * t + 4 * g + r < k1 ? s[t][r] : -INFINITY;
-          mt = fmaxf(mt, s[t][r]);
-        }
-      mt = fmaxf(mt, __shfl_xor(mt, 16));
-      mt = fmaxf(mt, __shfl_xor(mt, 32));
-      if (__any(mt > m)) {
-        const float f = exp2_diff(m, mt);
-        m = mt;
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < G::NB; i++)
-#pragma unroll
-          for (int j = 0; j < G::VE; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) o[i][j][r] *= f;
-      }
-      if (k + 16 * G::KT > k1) {
-        // past the segment p is 0, and the row read in its place has to count as 0 also where it is not finite
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int i = 0; i < G::NB; i++)
-#pragma unroll
-              for (int e = 0; e < G::VW; e++) vr[t][r][i][e] = k + 16 * t + 4 * g + r < k1 ? vr[t][r][i][e] : 0u;
-      }
-#pragma unroll
-      for (int t = 0; t < G::KT; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          s[t][r] = exp2_diff(s[t][r] + kLift<XT>, m);
-          l += s[t][r];
-        }
-      if constexpr (G::F32) {
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int i = 0; i < G::NB; i++)
-#pragma unroll
-              for (int j = 0; j < G::VE; j++)
-                o[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][r][i][j]), s[t][r], o[i][j], 0, 0, 0);
-      } else {
-        // P = ph + pl
-        u32x4 ph, pl;
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-          for (int r = 0; r < 4; r += 2) {
-            const uint32_t h = pack<XT>(s[t][r], s[t][r + 1]);
-            ph[2 * t + r / 2] = h;
-            pl[2 * t + r / 2] = pack<XT>(s[t][r] - half<XT>(h, 0), s[t][r + 1] - half<XT>(h, 1));
-          }
-#pragma unroll
-        for (int i = 0; i < G::NB; i++)
-#pragma unroll
-          for (int j = 0; j < G::VE; j++) {
-            const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
-            u32x4 v;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-              for (int r = 0; r < 4; r += 2)
-                v[2 * t + r / 2] = __builtin_amdgcn_perm(vr[t][r + 1][i][j / 2], vr[t][r][i][j / 2], sel);
-            o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, ph, o[i][j]);
-            o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, pl, o[i][j]);
-          }
-      }
-#pragma unroll
-      for (int t = 0; t < G::KT; t++) load_v(t);
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-
-    // join the waves: O rows [wave][head][LD], then (m, l) [wave][16][2]
-    float* ml = lds + kWaves * heads * G::LD;
-    if (c < heads) {
-      float* row = lds + (wave * heads + c) * G::LD;
+      f32x4 o[G::NB][G::VE];
 #pragma unroll
       for (int i = 0; i < G::NB; i++)
 #pragma unroll
+        for (int j = 0; j < G::VE; j++) o[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      float m = -INFINITY, l = 0.f;
+      uint32_t kr[G::KT][G::KC][4], vr[G::KT][4][G::NB][G::VW];
+      int pid[G::KT], entry[G::KT], key_off[G::KT];  // pages of the keys in hand, table entries of the next ones
+      // this wave's keys of the segment: 16 KT from k0 on, every KEYS
+      const int k0 = lo + s0 * G::KEYS + wave * (16 * G::KT), k1 = min(hi, lo + s1 * G::KEYS);
+
+      // The lane's key of the tile from `from` on.  Past the segment it is the
+      // segment's last key: rows outside the sequence are never read, and loads
+      // past the end need no branch (they ask for one row, which is at hand).
+      auto page_of = [&](int from, int& in_page) -> int {
+        const int key = min(from + c, k1 - 1);
+        const int slot = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
+        in_page = key - slot * a.page;
+        return slot;
+      };
+      auto load_k = [&](auto ONCE, int t) {
+        const char* kp = kb + (pid[t] * a.k_page + key_off[t] * a.k_tok) * G::ES;
+#pragma unroll
+        for (int i = 0; i < G::KC; i++) {
+          const int d = 4 * G::KE * i + G::KE * g;
+          const u32x4_e w = load<decltype(ONCE)::value, u32x4_e>(kp + (d < a.D ? d : 0) * G::ES);
+#pragma unroll
+          for (int e = 0; e < 4; e++) kr[t][i][e] = w[e];
+        }
+      };
+      auto load_v = [&](auto ONCE, int t) {
+#pragma unroll
         for (int r = 0; r < 4; r++) {
-          const int d = 16 * G::VE * i + G::VE * (4 * g + r);
-          if (d < DP) {
+          const int vpid = __shfl(pid[t], 4 * g + r), voff = __shfl(key_off[t], 4 * g + r);
+          const char* vp = vb + (vpid * a.v_page + voff * a.v_tok) * G::ES;
 #pragma unroll
-            for (int j = 0; j < G::VE; j += 4)
-              *reinterpret_cast<f32x4*>(row + d + j) = f32x4{o[i][j][r], o[i][j + 1][r], o[i][j + 2][r], o[i][j + 3][r]};
-          }
-        }
-      if (g == 0) {
-        ml[(wave * 16 + c) * 2] = m - kLift<XT>;
-        ml[(wave * 16 + c) * 2 + 1] = l;
-      }
-    }
-    __syncthreads();
-    const int u0 = at - s0;  // the head's first step among all
-    const int w0 = u0 / n, w1 = steps <= a.whole ? w0 : (u0 + steps - 1) / n;
-    // bytes of a workgroup's partial result: of its last head (slot 1), or of one that began before it (slot 0)
-    auto part_at = [&](int w) -> uint32_t { return (uint32_t)((2 * w + (w == w0)) * slot_words) * 4u; };
-    auto put = [&](int w, int e, float M, float L, f32x4 acc) {
-      const uint32_t p = part_at(w);
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + e * 16, 0, kAgentScope);
-      if (e % (DP / 4) == 0)
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
-                                              p + (heads * DP + 2 * (e / (DP / 4))) * 4, 0, kAgentScope);
-    };
-    auto finish = [&](int h, int d, float M, float L, f32x4 acc) {
-      float f = 1.f;
-      if (a.sinks) {
-        const float sink = a.sinks[head0 + h] * kLog2e, M2 = fmaxf(M, sink);
-        f = exp2_diff(M, M2);
-        L = L * f + exp2_diff(sink, M2);
-      }
-      const float r = L == 0.f ? 0.f : f / L;
-      if (d < a.D) store4<XT>(a.out, ((int64_t)b * a.Hq + head0 + h) * a.D + d, acc * r);
-    };
-    for (int e = tid; e < heads * (DP / 4); e += 256) {
-      const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
-      float M = -INFINITY, L = 0.f;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < G::NB; i++) {
+            const int d = 16 * G::VE * i + G::VE * c;
+            const char* p = vp + (d < a.D ? d : 0) * G::ES;  // columns past the head are dropped at the end
+            if constexpr (G::VW == 4) {
+              const u32x4_e w = load<decltype(ONCE)::value, u32x4_e>(p);
 #pragma unroll
-      for (int w = 0; w < kWaves; w++) M = fmaxf(M, ml[(w * 16 + h) * 2]);
+              for (int e = 0; e < 4; e++) vr[t][r][i][e] = w[e];
+            } else {
+              const u32x2_e w = load<decltype(ONCE)::value, u32x2_e>(p);
 #pragma unroll
-      for (int w = 0; w < kWaves; w++) {
-        const float f = exp2_diff(ml[(w * 16 + h) * 2], M);
-        L += f * ml[(w * 16 + h) * 2 + 1];
-        acc += f * *reinterpret_cast<const f32x4*>(lds + (w * heads + h) * G::LD + d);
-      }
-      if (w0 == w1) {
-        finish(h, d, M, L, acc);
-      } else {
-        put(blockIdx.x, e, M, L, acc);
-      }
-    }
-    if (w0 != w1) {
-      // The last of up to kJoin neighbours to arrive joins them; of more, the
-      // last to have joined its neighbours joins the results.
-      auto last_of = [&](uint32_t* cnt, int of) -> bool {
-        __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
-        __syncthreads();
-        if (tid == 0) {
-          const uint32_t old = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          arrived = old == (uint32_t)(of - 1);
-          if (arrived) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        return arrived != 0;
-      };
-      // sum of the results of workgroups w, w + by, .. (of them), in the order of the keys
-      auto join = [&](int w, int by, int of, int e, float& M, float& L, f32x4& acc) {
-        const int h = e / (DP / 4);
-        M = -INFINITY, L = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 0; i0 < of; i0 += kFlight) {
-          u32x4 ow[kFlight];
-          u32x2 mw[kFlight];
-#pragma unroll
-          for (int i = 0; i < kFlight; i++) {
-            const uint32_t p = part_at(w + by * min(i0 + i, of - 1));
-            mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + (heads * DP + 2 * h) * 4,
-                                                                                   0, kAgentScope));
-            ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + e * 16, 0, kAgentScope));
-          }
-#pragma unroll
-          for (int i = 0; i < kFlight; i++) {
-            if (i0 + i >= of) break;
-            const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
-            const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
-            M = M2;
-            L = L * f + __uint_as_float(mw[i][1]) * fi;
-            acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
+              for (int e = 0; e < 2; e++) vr[t][r][i][e] = w[e];
+            }
           }
         }
       };
-      const int of = w1 - w0 + 1, mine = ((int)blockIdx.x - w0) / kJoin * kJoin, near = min(kJoin, of - mine);
-      if (last_of(a.cnt + w0 + mine, near)) {
-        for (int e = tid; e < heads * (DP / 4); e += 256) {
-          const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
-          float M, L;
-          f32x4 acc;
-          join(w0 + mine, 1, near, e, M, L, acc);
-          if (of <= kJoin) finish(h, d, M, L, acc);
-          else put(w0 + mine, e, M, L, acc);
+      // the keys in hand become those from `from` on; the ones after them have their table entries loaded
+      auto advance = [&](int from) {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) {
+          int unused;
+          pid[t] = min(max(entry[t], 0), a.pages - 1);
+          page_of(from + 16 * t, key_off[t]);
+          entry[t] = table[page_of(from + G::KEYS + 16 * t, unused)];
         }
-        const int groups = (of + kJoin - 1) / kJoin;
-        if (of > kJoin && last_of(a.cnt + a.wgs + w0, groups)) {
+      };
+
+      // Q of head c in LDS, a lane's 16 bytes after the other: B operand, the d
+      // order of the K loads
+      u32x4 q0[(G::KC + kWaves - 1) / kWaves];
+#pragma unroll
+      for (int i = wave, j = 0; j < (G::KC + kWaves - 1) / kWaves; i += kWaves, j++) {
+        const int d = 4 * G::KE * i + G::KE * g;
+        const char* qp = static_cast<const char*>(a.q) + (b * a.q_b + (head0 + min(c, heads - 1)) * a.q_h) * G::ES;
+        const u32x4_e w = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
+        q0[j] = d < a.D ? u32x4{w[0], w[1], w[2], w[3]} : u32x4{0u, 0u, 0u, 0u};
+      }
+      if (k0 < k1) {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) entry[t] = table[page_of(k0 + 16 * t, key_off[t])];
+        advance(k0);
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) load_k(ONCE, t);
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) load_v(ONCE, t);
+      }
+#pragma unroll
+      for (int i = wave, j = 0; j < (G::KC + kWaves - 1) / kWaves; i += kWaves, j++)
+        if (i < G::KC) qs[i * 64 + lane] = q0[j];
+      __syncthreads();
+      for (int k = k0; k < k1; k += G::KEYS) {
+        if (DP != a.D) {  // columns past the head are zero on both sides
+#pragma unroll
+          for (int t = 0; t < G::KT; t++)
+#pragma unroll
+            for (int i = 0; i < G::KC; i++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) kr[t][i][e] = 4 * G::KE * i + G::KE * g < a.D ? kr[t][i][e] : 0u;
+        }
+        f32x4 s[G::KT];
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        asm volatile("" ::: "memory");  // Q is read again each time, not kept in registers
+#pragma unroll
+        for (int i = 0; i < G::KC; i++) {
+          const u32x4 q = qs[i * 64 + lane];
+#pragma unroll
+          for (int t = 0; t < G::KT; t++) {
+            if constexpr (G::F32) {
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][i][e]), __uint_as_float(q[e]), s[t], 0,
+                                                            0, 0);
+            } else {
+              s[t] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(
+                  u32x4{kr[t][i][0], kr[t][i][1], kr[t][i][2], kr[t][i][3]}, q, s[t]);
+            }
+          }
+        }
+        advance(k + G::KEYS);
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) load_k(ONCE, t);
+        if (a.softcap > 0.f) {
+#pragma unroll
+          for (int t = 0; t < G::KT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[t][r] = cap_log2e * tanhf(s[t][r] * scale);
+        } else {
+#pragma unroll
+          for (int t = 0; t < G::KT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[t][r] *= scale;
+        }
+        float mt = m;
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            s[t][r] = k + 16 * t + 4 * g + r < k1 ? s[t][r] : -INFINITY;
+            mt = fmaxf(mt, s[t][r]);
+          }
+        mt = fmaxf(mt, __shfl_xor(mt, 16));
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        if (__any(mt > m)) {
+          const float f = exp2_diff(m, mt);
+          m = mt;
+          l *= f;
+#pragma unroll
+          for (int i = 0; i < G::NB; i++)
+#pragma unroll
+            for (int j = 0; j < G::VE; j++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) o[i][j][r] *= f;
+        }
+        if (k + 16 * G::KT > k1) {
+          // past the segment p is 0, and the row read in its place has to count as 0 also where it is not finite
+#pragma unroll
+          for (int t = 0; t < G::KT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+              for (int i = 0; i < G::NB; i++)
+#pragma unroll
+                for (int e = 0; e < G::VW; e++) vr[t][r][i][e] = k + 16 * t + 4 * g + r < k1 ? vr[t][r][i][e] : 0u;
+        }
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            s[t][r] = exp2_diff(s[t][r] + kLift<XT>, m);
+            l += s[t][r];
+          }
+        if constexpr (G::F32) {
+#pragma unroll
+          for (int t = 0; t < G::KT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+              for (int i = 0; i < G::NB; i++)
+#pragma unroll
+                for (int j = 0; j < G::VE; j++)
+                  o[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][r][i][j]), s[t][r], o[i][j], 0, 0, 0);
+        } else {
+          // P = ph + pl
+          u32x4 ph, pl;
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+              const uint32_t h = pack<XT>(s[t][r], s[t][r + 1]);
+              ph[2 * t + r / 2] = h;
+              pl[2 * t + r / 2] = pack<XT>(s[t][r] - half<XT>(h, 0), s[t][r + 1] - half<XT>(h, 1));
+            }
+#pragma unroll
+          for (int i = 0; i < G::NB; i++)
+#pragma unroll
+            for (int j = 0; j < G::VE; j++) {
+              const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+              u32x4 v;
+#pragma unroll
+              for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                  v[2 * t + r / 2] = __builtin_amdgcn_perm(vr[t][r + 1][i][j / 2], vr[t][r][i][j / 2], sel);
+              o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, ph, o[i][j]);
+              o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, pl, o[i][j]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) load_v(ONCE, t);
+      }
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+
+      // join the waves: O rows [wave][head][LD], then (m, l) [wave][16][2]
+      float* ml = lds + kWaves * heads * G::LD;
+      if (c < heads) {
+        float* row = lds + (wave * heads + c) * G::LD;
+#pragma unroll
+        for (int i = 0; i < G::NB; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int d = 16 * G::VE * i + G::VE * (4 * g + r);
+            if (d < DP) {
+#pragma unroll
+              for (int j = 0; j < G::VE; j += 4)
+                *reinterpret_cast<f32x4*>(row + d + j) = f32x4{o[i][j][r], o[i][j + 1][r], o[i][j + 2][r], o[i][j + 3][r]};
+            }
+          }
+        if (g == 0) {
+          ml[(wave * 16 + c) * 2] = m - kLift<XT>;
+          ml[(wave * 16 + c) * 2 + 1] = l;
+        }
+      }
+      __syncthreads();
+      const int u0 = at - s0;  // the head's first step among all
+      const int w0 = u0 / n, w1 = steps <= a.whole ? w0 : (u0 + steps - 1) / n;
+      // bytes of a workgroup's partial result: of its last head (slot 1), or of one that began before it (slot 0)
+      auto part_at = [&](int w) -> uint32_t { return (uint32_t)((2 * w + (w == w0)) * slot_words) * 4u; };
+      auto put = [&](int w, int e, float M, float L, f32x4 acc) {
+        const uint32_t p = part_at(w);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + e * 16, 0, kAgentScope);
+        if (e % (DP / 4) == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
+                                                p + (heads * DP + 2 * (e / (DP / 4))) * 4, 0, kAgentScope);
+      };
+      auto finish = [&](int h, int d, float M, float L, f32x4 acc) {
+        float f = 1.f;
+        if (a.sinks) {
+          const float sink = a.sinks[head0 + h] * kLog2e, M2 = fmaxf(M, sink);
+          f = exp2_diff(M, M2);
+          L = L * f + exp2_diff(sink, M2);
+        }
+        const float r = L == 0.f ? 0.f : f / L;
+        if (d < a.D) store4<XT>(a.out, ((int64_t)b * a.Hq + head0 + h) * a.D + d, acc * r);
+      };
+      for (int e = tid; e < heads * (DP / 4); e += 256) {
+        const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
+        float M = -INFINITY, L = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) M = fmaxf(M, ml[(w * 16 + h) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+          const float f = exp2_diff(ml[(w * 16 + h) * 2], M);
+          L += f * ml[(w * 16 + h) * 2 + 1];
+          acc += f * *reinterpret_cast<const f32x4*>(lds + (w * heads + h) * G::LD + d);
+        }
+        if (w0 == w1) {
+          finish(h, d, M, L, acc);
+        } else {
+          put(blockIdx.x, e, M, L, acc);
+        }
+      }
+      if (w0 != w1) {
+        // The last of up to kJoin neighbours to arrive joins them; of more, the
+        // last to have joined its neighbours joins the results.
+        auto last_of = [&](uint32_t* cnt, int of) -> bool {
+          __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
+          __syncthreads();
+          if (tid == 0) {
+            const uint32_t old = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            arrived = old == (uint32_t)(of - 1);
+            if (arrived) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+          __syncthreads();
+          return arrived != 0;
+        };
+        // sum of the results of workgroups w, w + by, .. (of them), in the order of the keys
+        auto join = [&](int w, int by, int of, int e, float& M, float& L, f32x4& acc) {
+          const int h = e / (DP / 4);
+          M = -INFINITY, L = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int i0 = 0; i0 < of; i0 += kFlight) {
+            u32x4 ow[kFlight];
+            u32x2 mw[kFlight];
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+              const uint32_t p = part_at(w + by * min(i0 + i, of - 1));
+              mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + (heads * DP + 2 * h) * 4,
+                                                                                     0, kAgentScope));
+              ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + e * 16, 0, kAgentScope));
+            }
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+              if (i0 + i >= of) break;
+              const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
+              const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
+              M = M2;
+              L = L * f + __uint_as_float(mw[i][1]) * fi;
+              acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
+            }
+          }
+        };
+        const int of = w1 - w0 + 1, mine = ((int)blockIdx.x - w0) / kJoin * kJoin, near = min(kJoin, of - mine);
+        if (last_of(a.cnt + w0 + mine, near)) {
           for (int e = tid; e < heads * (DP / 4); e += 256) {
             const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
             float M, L;
             f32x4 acc;
-            join(w0, kJoin, groups, e, M, L, acc);
-            finish(h, d, M, L, acc);
+            join(w0 + mine, 1, near, e, M, L, acc);
+            if (of <= kJoin) finish(h, d, M, L, acc);
+            else put(w0 + mine, e, M, L, acc);
+          }
+          const int groups = (of + kJoin - 1) / kJoin;
+          if (of > kJoin && last_of(a.cnt + a.wgs + w0, groups)) {
+            for (int e = tid; e < heads * (DP / 4); e += 256) {
+              const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
+              float M, L;
+              f32x4 acc;
+              join(w0, kJoin, groups, e, M, L, acc);
+              finish(h, d, M, L, acc);
+            }
           }
         }
       }
+      __syncthreads();  // the LDS rows are free again
+      off += s1 - s0;
+      at += s1 - s0;
     }
-    __syncthreads();  // the LDS rows are free again
-    off += s1 - s0;
-    at += s1 - s0;
-  }
+  };
+  if (once) run(std::true_type{});
+  else run(std::false_type{});
 }
 
 template <int XT, int DP>
