@@ -170,6 +170,14 @@ int32_t* page_lists(hipStream_t stream, int64_t words) {
   return static_cast<int32_t*>(stream_workspace(current_device(), stream, (size_t)words * sizeof(int32_t), 4));
 }
 
+uint32_t* counters(int dev, hipStream_t stream, const char* tag) {
+  uint32_t* c = stream_counters(dev, stream);
+  if (!c)
+    fail(MLXQ_ENOMEM, std::string("[") + tag + "] this stream has no counters yet and is being captured; run the call "
+                      "once before the capture or reserve with mlxq_workspace_reserve");
+  return c;
+}
+
 // A row-contiguous copy of an operand whose strides the kernel does not take,
 // at `at` of the staging workspace.
 size_t padded(View v) { return ((size_t)v.size() * dtype_size(v.dtype()) + 255) & ~(size_t)255; }
@@ -270,10 +278,7 @@ mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool, 
       (Refusal(tag) << "a table of " << a.B << " rows of " << t.dim(1) << " pages holds too many keys for one call.")
           .unsupported();
     a.part = static_cast<float*>(stream_workspace(dev, stream, part_bytes, 0));
-    a.cnt = stream_counters(dev, stream);
-    if (!a.cnt)
-      fail(MLXQ_ENOMEM, "[paged_attention] this stream has no counters yet and is being captured; run the call once "
-                        "before the capture or reserve with mlxq_workspace_reserve");
+    a.cnt = counters(dev, stream, tag);
     hip_check(mlxq::launch_paged_attention(a, stream), "paged attention launch");
     if (stage_out) copy_view(&oc, out, stream);
   });
@@ -560,6 +565,13 @@ mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* toke
     }
     a.logits = xc.data;
     a.row = xc.strides[0];
+    const int dev = current_device();
+    int64_t part_bytes = 0;
+    mlxq::token_logprobs_plan(a, device_cus(dev), &part_bytes);
+    if (part_bytes > 0) {
+      a.part = static_cast<float*>(stream_workspace(dev, stream, part_bytes, 0));
+      a.cnt = counters(dev, stream, tag);
+    }
     hip_check(mlxq::launch_token_logprobs(a, stream), "token log probabilities launch");
   });
 }

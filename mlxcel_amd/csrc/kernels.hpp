@@ -662,7 +662,12 @@ struct LogprobArgs {
   int V, n_tok, k;
   float scale;
   int type;
+  int split;              // workgroups a row (token_logprobs_plan)
+  float* part;            // their partial results
+  uint32_t* cnt;          // [T], zero between launches
 };
+// Sets the plan; part_bytes of scratch are needed (0: none, and no counters).
+void token_logprobs_plan(LogprobArgs& a, int cus, int64_t* part_bytes);
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream);
 
 }  // namespace mlxq
