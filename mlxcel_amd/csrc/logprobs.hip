@@ -58,24 +58,33 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 
 // ---- sorted lists of 64 keys, one a lane --------------------------------------
 
+// The value of the lane whose number differs in bit J: vector operations only
+// (4 is 3 then 7; halves and rows of 16 are swapped between two registers).
 template <int J>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int lane) {
   if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);
   else if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
+  else if constexpr (J == 4)
+    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x1B, 0xF, 0xF, false), 0x141, 0xF, 0xF, false);
   else if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, false);
-  else if constexpr (J < 32) return __builtin_amdgcn_ds_swizzle(v, (J << 10) | 0x1F);
-  else return __shfl_xor(v, J);
+  else if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
 }
 template <int J>
-__device__ __forceinline__ uint64_t lane_xor64(uint64_t v) {
-  return ((uint64_t)lane_xor<J>((uint32_t)(v >> 32)) << 32) | lane_xor<J>((uint32_t)v);
+__device__ __forceinline__ uint64_t lane_xor64(uint64_t v, int lane) {
+  return ((uint64_t)lane_xor<J>((uint32_t)(v >> 32), lane) << 32) | lane_xor<J>((uint32_t)v, lane);
 }
 
 // One step of a bitonic network: lanes J apart, the larger to the lower lane
 // where `down`.
 template <int J>
 __device__ __forceinline__ void exchange(uint64_t& v, int lane, bool down) {
-  const uint64_t o = lane_xor64<J>(v);
+  const uint64_t o = lane_xor64<J>(v, lane);
   const bool larger = ((lane & J) == 0) == down;
   v = (o > v) == larger ? o : v;
 }
@@ -84,14 +93,14 @@ __device__ __forceinline__ void bitonic(uint64_t& v, int lane) {
   exchange<J>(v, lane, SIZE == 64 || (lane & SIZE) == 0);
   if constexpr (J > 1) bitonic<SIZE, J / 2>(v, lane);
 }
-// Largest first.
-__device__ __forceinline__ void sort64(uint64_t& v, int lane) {
+// Largest first, where lanes from n on hold 0.
+__device__ __forceinline__ void sort64(uint64_t& v, int lane, int n) {
   bitonic<2, 1>(v, lane);
   bitonic<4, 2>(v, lane);
   bitonic<8, 4>(v, lane);
   bitonic<16, 8>(v, lane);
-  bitonic<32, 16>(v, lane);
-  bitonic<64, 32>(v, lane);
+  if (n > 16) bitonic<32, 16>(v, lane);
+  if (n > 32) bitonic<64, 32>(v, lane);
 }
 // The 64 largest of two sorted lists, sorted.
 __device__ __forceinline__ void merge64(uint64_t& v, uint64_t o, int lane) {
@@ -121,7 +130,7 @@ __device__ __forceinline__ Sums add(Sums x, Sums y, float a) {
 }
 
 template <int XT>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArgs a) {
   constexpr int PER = XT == GEN_F32 ? 4 : 8;  // values of a 16-byte load
   constexpr int NL = 16 / PER;                // loads of a lane and chunk
   __shared__ uint64_t cand[kWaves][128], lists[kWaves][64];
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
     __builtin_amdgcn_wave_barrier();
     uint64_t v = lane < n ? cand[wave][lane] : 0;
     const uint64_t rest = cand[wave][64 + lane];
-    sort64(v, lane);
+    sort64(v, lane, n);
     merge64(list, v, lane);
     if (waiting > 64) cand[wave][lane] = rest;
     waiting -= n;
@@ -202,37 +211,55 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
     const float m = mine.m == -INFINITY ? 0.f : mine.m;
 #pragma unroll
     for (int v = 0; v < 16; v++) {
-      float z = (value(w, v) - m) * sc;
-      z = z < -1000.f ? -1000.f : z;  // 2^-1000 is 0, and so is its product with z
-      const float p = __builtin_amdgcn_exp2f(z);
+      const float z = (value(w, v) - m) * sc, p = __builtin_amdgcn_exp2f(z);
       mine.s += p;
-      mine.e += p * z;
+      mine.e += p * fmaxf(z, -1000.f);  // 2^-1000 is 0, and so is its product with z
     }
     if (a.k == 0) continue;
     // Later values equal to the floor's lose to it: a strict comparison will
     // do.  A sum that is not a number may hide one among the values.
     if (__any(!begun || top > floor_value || mine.s != mine.s)) {
-      auto key = [&](int v) -> uint64_t {
-        const int i = c * kChunk + ((v / PER) * 64 + lane) * PER + v % PER;
-        return i < a.V ? order_key(value(w, v), (uint32_t)i) : 0;
-      };
+      auto index = [&](int v) { return c * kChunk + ((v / PER) * 64 + lane) * PER + v % PER; };
+      float above = floor_value;
       if (!begun) {
         uint64_t best = 0;
 #pragma unroll
-        for (int v = 0; v < 16; v++) best = key(v) > best ? key(v) : best;
-        sort64(best, lane);
+        for (int v = 0; v < 16; v++) {
+          const uint64_t kv = index(v) < a.V ? order_key(value(w, v), (uint32_t)index(v)) : 0;
+          best = kv > best ? kv : best;
+        }
+        sort64(best, lane, 64);
         const uint64_t kth = __shfl((unsigned long long)best, a.k - 1);
         floor = kth ? kth - 1 : 0;
         floor_value = kth ? key_value(kth) : -INFINITY;
+        // this chunk's values equal to the floor's count: compare with the next
+        // lower one (below 0 past -0; below -inf it is not a number, and
+        // everything counts)
+        above = !kth ? NAN : floor_value == 0.f ? -__uint_as_float(1u) : key_value(kth - (1ull << 32));
         begun = true;
       }
+      // each lane's values above, one a lane at a time
+      uint32_t left = 0;
 #pragma unroll
-      for (int v = 0; v < 16; v++) {
-        const uint64_t kv = key(v);
+      for (int v = 0; v < 16; v++) left |= !(value(w, v) <= above) ? 1u << v : 0u;
+      while (__any(left)) {
+        const int v = left ? __builtin_ctz(left) : 0;
+        uint32_t word[16 / PER * 4];
+#pragma unroll
+        for (int i = 0; i < 16 / PER * 4; i++) word[i] = w[i / 4][i % 4];
+        const int wi = XT == GEN_F32 ? v : v / 2;
+#pragma unroll
+        for (int bit = 8 / PER * 4; bit; bit /= 2)
+#pragma unroll
+          for (int i = 0; i < bit; i++) word[i] = wi & bit ? word[i + bit] : word[i];
+        float x;
+        if constexpr (XT == GEN_F32) x = __uint_as_float(word[0]);
+        else x = xt_to_f32<XT == GEN_F16 ? 1 : 0>(v & 1 ? word[0] >> 16 : word[0] & 0xFFFFu);
+        const uint64_t kv = left && index(v) < a.V ? order_key(x, (uint32_t)index(v)) : 0;
         const uint64_t hits = __ballot(kv > floor);
-        if (hits == 0) continue;
         if (kv > floor) cand[wave][waiting + __popcll(hits & ((1ull << lane) - 1))] = kv;
         waiting += __popcll(hits);
+        left &= left - 1;
         if (waiting >= 64) merge(64);
       }
     }
@@ -329,7 +356,8 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
 }  // namespace
 
 void token_logprobs_plan(LogprobArgs& a, int cus, int64_t* part_bytes) {
-  const int chunks = (a.V + kChunk - 1) / kChunk, most = (chunks + kWaves - 1) / kWaves;
+  const int cpw = getenv("LP_CPW") ? atoi(getenv("LP_CPW")) : 1;
+  const int chunks = (a.V + kChunk - 1) / kChunk, most = (chunks + kWaves * cpw - 1) / (kWaves * cpw);
   const int rw = getenv("LP_RW") ? atoi(getenv("LP_RW")) : kRowWgs;
   const int64_t want = ((int64_t)cus * rw + a.T - 1) / std::max<int64_t>(a.T, 1);
   a.split = (int)std::max<int64_t>(1, std::min<int64_t>(most, want));
