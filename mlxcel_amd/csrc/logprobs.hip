@@ -12,14 +12,15 @@
 // HBM-bound: each logit is read once.  A row is cut over `split` workgroups
 // where there are few rows; in each, a wave takes chunks of 64 lanes x 16 values
 // in turn.  A lane keeps a running maximum with S and sum_i exp(z_i) z_i relative
-// to it, rescaled once a chunk.  The wave keeps its 64 largest values so far
-// sorted over its lanes, as numbers that order (value, index) pairs; of a chunk
-// only values above the k-th of them are looked at (a comparison of each lane's
-// largest with that value, and mostly nothing more), collected in LDS and merged
-// 64 at a time.  The first chunk starts from the k-th largest of the lanes'
-// maxima, which at least k values reach.  The waves' and workgroups' lists and
-// sums are joined at the end, the last workgroup of a row to arrive joining the
-// row's.
+// to it, rescaled once a chunk.  Alternatives are picked in the same pass.  If
+// each of the workgroup's A waves has ceil(k / A) lanes whose maxima reach f, k
+// values do, and only values that reach f can be among the k largest; each wave
+// sorts its lanes' maxima after its 1st, 2nd, 4th, .. chunk, and the least of the
+// waves' ceil(k / A)-th ones is f.  Few values of a chunk pass (k / 4 or so of the
+// first 1024 a wave, then fewer): they are collected in LDS as numbers that order
+// (value, index) pairs and merged 64 at a time into the wave's 64 largest, sorted
+// over its lanes.  The waves' and workgroups' lists and sums are joined at the
+// end, the last workgroup of a row to arrive joining the row's.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -102,6 +103,30 @@ __device__ __forceinline__ void sort64(uint64_t& v, int lane, int n) {
   if (n > 16) bitonic<32, 16>(v, lane);
   if (n > 32) bitonic<64, 32>(v, lane);
 }
+// Largest first.
+template <int SIZE, int J>
+__device__ __forceinline__ void bitonic_values(float& v, int lane) {
+  const float o = __uint_as_float(lane_xor<J>(__float_as_uint(v), lane));
+  v = ((lane & J) == 0) == (SIZE == 64 || (lane & SIZE) == 0) ? fmaxf(v, o) : fminf(v, o);
+  if constexpr (J > 1) bitonic_values<SIZE, J / 2>(v, lane);
+}
+__device__ __forceinline__ float sorted_values(float v, int lane) {
+  bitonic_values<2, 1>(v, lane);
+  bitonic_values<4, 2>(v, lane);
+  bitonic_values<8, 4>(v, lane);
+  bitonic_values<16, 8>(v, lane);
+  bitonic_values<32, 16>(v, lane);
+  bitonic_values<64, 32>(v, lane);
+  return v;
+}
+
+// The next value below (not a number below -inf; -0 is 0).
+__device__ __forceinline__ float below(float f) {
+  if (f == -INFINITY) return NAN;
+  const uint32_t u = __float_as_uint(f);
+  return __uint_as_float(f == 0.f ? 0x80000001u : f > 0.f ? u - 1 : u + 1);
+}
+
 // The 64 largest of two sorted lists, sorted.
 __device__ __forceinline__ void merge64(uint64_t& v, uint64_t o, int lane) {
   o = __shfl((unsigned long long)o, 63 - lane);
@@ -135,6 +160,7 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
   constexpr int NL = 16 / PER;                // loads of a lane and chunk
   __shared__ uint64_t cand[kWaves][128], lists[kWaves][64];
   __shared__ Sums sums[kWaves];
+  __shared__ float reached[kWaves];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t = blockIdx.x / a.split;
@@ -146,9 +172,8 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
 
   Sums mine = {-INFINITY, 0.f, 0.f};
   uint64_t list = 0, floor = 0;  // keys up to `floor` cannot be among the k largest
-  float floor_value = -INFINITY;
-  int waiting = 0;  // candidates in LDS
-  bool begun = false;
+  float floor_value = NAN;       // their value; not a number: there are none
+  int waiting = 0;               // candidates in LDS
   auto merge = [&](int n) {  // the first n <= 64 candidates
     __builtin_amdgcn_wave_barrier();
     uint64_t v = lane < n ? cand[wave][lane] : 0;
@@ -196,14 +221,7 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
     }
   };
 
-  u32x4 next[NL];
-  int c = part * kWaves + wave;
-  if (c < chunks) load_chunk(c, next);
-  for (; c < chunks; c += step) {
-    u32x4 w[NL];
-#pragma unroll
-    for (int j = 0; j < NL; j++) w[j] = next[j];
-    if (c + step < chunks) load_chunk(c + step, next);
+  auto add_chunk = [&](const u32x4 (&w)[NL]) -> float {  // the lane's largest value of it
     float top = value(w, 0);
 #pragma unroll
     for (int v = 1; v < 16; v++) top = fmaxf(top, value(w, v));
@@ -215,54 +233,74 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
       mine.s += p;
       mine.e += p * fmaxf(z, -1000.f);  // 2^-1000 is 0, and so is its product with z
     }
-    if (a.k == 0) continue;
-    // Later values equal to the floor's lose to it: a strict comparison will
-    // do.  A sum that is not a number may hide one among the values.
-    if (__any(!begun || top > floor_value || mine.s != mine.s)) {
-      auto index = [&](int v) { return c * kChunk + ((v / PER) * 64 + lane) * PER + v % PER; };
-      float above = floor_value;
-      if (!begun) {
-        uint64_t best = 0;
+    return top;
+  };
+  // waves of this workgroup that have values; what they all reach
+  const int active = min(kWaves, chunks - part * kWaves), each = (a.k + active - 1) / active;
+  auto post = [&]() {
+    const float v = sorted_values(mine.m, lane);
+    if (lane == each - 1) __hip_atomic_store(&reached[wave], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  auto collect = [&](int c, const u32x4 (&w)[NL], float top) {
+    float f = INFINITY;
 #pragma unroll
-        for (int v = 0; v < 16; v++) {
-          const uint64_t kv = index(v) < a.V ? order_key(value(w, v), (uint32_t)index(v)) : 0;
-          best = kv > best ? kv : best;
-        }
-        sort64(best, lane, 64);
-        const uint64_t kth = __shfl((unsigned long long)best, a.k - 1);
-        floor = kth ? kth - 1 : 0;
-        floor_value = kth ? key_value(kth) : -INFINITY;
-        // this chunk's values equal to the floor's count: compare with the next
-        // lower one (below 0 past -0; below -inf it is not a number, and
-        // everything counts)
-        above = !kth ? NAN : floor_value == 0.f ? -__uint_as_float(1u) : key_value(kth - (1ull << 32));
-        begun = true;
-      }
-      // each lane's values above, one a lane at a time
-      uint32_t left = 0;
+    for (int i = 0; i < kWaves; i++)
+      f = fminf(f, __hip_atomic_load(&reached[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    // Values equal to f count; those equal to the list's floor come later and
+    // lose to it.  A sum that is not a number may hide one among the values.
+    const float above = fmaxf(floor_value, below(f));
+    if (!__any(!(top <= above) || mine.s != mine.s)) return;
+    auto index = [&](int v) { return c * kChunk + ((v / PER) * 64 + lane) * PER + v % PER; };
+    uint32_t left = 0;  // the lane's values that pass, taken one a lane at a time
 #pragma unroll
-      for (int v = 0; v < 16; v++) left |= !(value(w, v) <= above) ? 1u << v : 0u;
-      while (__any(left)) {
-        const int v = left ? __builtin_ctz(left) : 0;
-        uint32_t word[16 / PER * 4];
+    for (int v = 0; v < 16; v++) left |= !(value(w, v) <= above) ? 1u << v : 0u;
+    while (__any(left)) {
+      const int v = left ? __builtin_ctz(left) : 0;
+      constexpr int W = 4 * NL;
+      uint32_t word[W];
 #pragma unroll
-        for (int i = 0; i < 16 / PER * 4; i++) word[i] = w[i / 4][i % 4];
-        const int wi = XT == GEN_F32 ? v : v / 2;
+      for (int i = 0; i < W; i++) word[i] = w[i / 4][i % 4];
+      const int wi = XT == GEN_F32 ? v : v / 2;
 #pragma unroll
-        for (int bit = 8 / PER * 4; bit; bit /= 2)
+      for (int bit = W / 2; bit; bit /= 2)
 #pragma unroll
-          for (int i = 0; i < bit; i++) word[i] = wi & bit ? word[i + bit] : word[i];
-        float x;
-        if constexpr (XT == GEN_F32) x = __uint_as_float(word[0]);
-        else x = xt_to_f32<XT == GEN_F16 ? 1 : 0>(v & 1 ? word[0] >> 16 : word[0] & 0xFFFFu);
-        const uint64_t kv = left && index(v) < a.V ? order_key(x, (uint32_t)index(v)) : 0;
-        const uint64_t hits = __ballot(kv > floor);
-        if (kv > floor) cand[wave][waiting + __popcll(hits & ((1ull << lane) - 1))] = kv;
-        waiting += __popcll(hits);
-        left &= left - 1;
-        if (waiting >= 64) merge(64);
-      }
+        for (int i = 0; i < bit; i++) word[i] = wi & bit ? word[i + bit] : word[i];
+      float x;
+      if constexpr (XT == GEN_F32) x = __uint_as_float(word[0]);
+      else x = xt_to_f32<XT == GEN_F16 ? 1 : 0>(v & 1 ? word[0] >> 16 : word[0] & 0xFFFFu);
+      const uint64_t kv = left && index(v) < a.V ? order_key(x, (uint32_t)index(v)) : 0;
+      const uint64_t hits = __ballot(kv > floor);
+      if (kv > floor) cand[wave][waiting + __popcll(hits & ((1ull << lane) - 1))] = kv;
+      waiting += __popcll(hits);
+      left &= left - 1;
+      if (waiting >= 64) merge(64);
     }
+  };
+
+  u32x4 next[NL], w[NL];
+  int c = part * kWaves + wave;
+  if (c < chunks) {
+    load_chunk(c, w);
+    if (c + step < chunks) load_chunk(c + step, next);
+    const float top = add_chunk(w);
+    if (a.k > 0) {
+      post();
+      __syncthreads();
+      collect(c, w, top);
+    }
+  } else if (a.k > 0) {
+    if (lane == 0) reached[wave] = INFINITY;
+    __syncthreads();
+  }
+  c += step;
+  for (int n = 2; c < chunks; c += step, n++) {
+#pragma unroll
+    for (int j = 0; j < NL; j++) w[j] = next[j];
+    if (c + step < chunks) load_chunk(c + step, next);
+    const float top = add_chunk(w);
+    if (a.k == 0) continue;
+    if ((n & (n - 1)) == 0) post();
+    collect(c, w, top);
   }
   if (waiting > 0) merge(waiting);
 
