@@ -12,19 +12,22 @@
 // HBM-bound: each logit is read once.  A row is cut over `split` workgroups
 // where there are few rows; in each, a wave takes chunks of 64 lanes x 16 values
 // in turn.  A lane keeps a running maximum with S and sum_i exp(z_i) z_i relative
-// to it, rescaled once a chunk.  Alternatives are picked in the same pass.  If
-// each of the workgroup's A waves has ceil(k / A) lanes whose maxima reach f, k
-// values do, and only values that reach f can be among the k largest; each wave
-// sorts its lanes' maxima after its 1st, 2nd, 4th, .. chunk, and the least of the
-// waves' ceil(k / A)-th ones is f.  Few values of a chunk pass (k / 4 or so of the
-// first 1024 a wave, then fewer): they are collected in LDS as numbers that order
-// (value, index) pairs and merged 64 at a time into the wave's 64 largest, sorted
-// over its lanes.  The waves' and workgroups' lists and sums are joined at the
-// end, the last workgroup of a row to arrive joining the row's.
+// to it, rescaled once a chunk.
+//
+// The alternatives are found in the same pass.  If each of the workgroup's A
+// waves has ceil(k / A) lanes whose maxima so far reach f, or one wave k of them,
+// then k values reach f and no lower one is among the k largest.  Each wave
+// sorts its lanes' maxima after its 2nd, 8th, 32nd, .. chunk, which gives the
+// workgroup its f.  A lane whose 16 values of a chunk reach f notes the chunk and
+// its largest (a few instructions where none does); the notes are weighed against
+// the last f at the end, when all but about k of them fall away, and the rest's
+// values are read again, as numbers that order (value, index) pairs.  Mostly a
+// few more than k reach f, and are sorted at once.  Where there are more than 256
+// (many equal values), they are merged 64 at a time into sorted lists of the 64
+// largest, one a wave.  The last workgroup of a row to arrive joins the row's in the same way.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -34,7 +37,12 @@ namespace mlxq {
 namespace {
 
 constexpr int kWaves = 4, kChunk = 1024;  // values of a wave's chunk
-constexpr int kRowWgs = 4;                // workgroups a CU is given where rows are cut
+constexpr int kFew = 256;                 // values that a workgroup sorts at once
+// Workgroups a CU is given where rows are cut, each of at least two chunks a
+// wave: 300 rows of 151936 float32 logits 43.7 us with 2, 44.7 with 3, 52 with 4
+// (each pays for its own start and end); 8 rows of 262144 16 us, 21 with one chunk
+// a wave.
+constexpr int kRowWgs = 2;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
@@ -154,14 +162,38 @@ __device__ __forceinline__ Sums add(Sums x, Sums y, float a) {
   return Sums{M, x.s + y.s, x.e + y.e};
 }
 
+// Over the wave's lanes, the same in each.
+__device__ __forceinline__ Sums wave_sums(Sums v, float a, int lane) {
+  float M = v.m;
+  M = fmaxf(M, __uint_as_float(lane_xor<1>(__float_as_uint(M), lane)));
+  M = fmaxf(M, __uint_as_float(lane_xor<2>(__float_as_uint(M), lane)));
+  M = fmaxf(M, __uint_as_float(lane_xor<4>(__float_as_uint(M), lane)));
+  M = fmaxf(M, __uint_as_float(lane_xor<8>(__float_as_uint(M), lane)));
+  M = fmaxf(M, __uint_as_float(lane_xor<16>(__float_as_uint(M), lane)));
+  M = fmaxf(M, __uint_as_float(lane_xor<32>(__float_as_uint(M), lane)));
+  v = rebase(v, M, a);
+  auto sum = [&](float x) {
+    x += __uint_as_float(lane_xor<1>(__float_as_uint(x), lane));
+    x += __uint_as_float(lane_xor<2>(__float_as_uint(x), lane));
+    x += __uint_as_float(lane_xor<4>(__float_as_uint(x), lane));
+    x += __uint_as_float(lane_xor<8>(__float_as_uint(x), lane));
+    x += __uint_as_float(lane_xor<16>(__float_as_uint(x), lane));
+    return x + __uint_as_float(lane_xor<32>(__float_as_uint(x), lane));
+  };
+  return Sums{M, sum(v.s), sum(v.e)};
+}
+
 template <int XT>
-__global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArgs a) {
   constexpr int PER = XT == GEN_F32 ? 4 : 8;  // values of a 16-byte load
   constexpr int NL = 16 / PER;                // loads of a lane and chunk
-  __shared__ uint64_t cand[kWaves][128], lists[kWaves][64];
+  constexpr uint32_t kNone = XT == GEN_F32 ? 0xFF800000u : XT == GEN_F16 ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
+  __shared__ uint64_t notes[kWaves][128], cand[kWaves][128], lists[kWaves][64];
+  __shared__ uint64_t few[kFew], marked[kFew];
   __shared__ Sums sums[kWaves];
-  __shared__ float reached[kWaves];
+  __shared__ float reached[3][kWaves];
   __shared__ uint32_t arrived;
+  __shared__ int count[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t = blockIdx.x / a.split;
   const int part = blockIdx.x - (int)t * a.split;  // of the row
@@ -171,10 +203,10 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
   const int step = a.split * kWaves;
 
   Sums mine = {-INFINITY, 0.f, 0.f};
-  uint64_t list = 0, floor = 0;  // keys up to `floor` cannot be among the k largest
+  uint64_t list = 0, floor = 0;  // of values that were too many; keys up to `floor` cannot be among the k largest
   float floor_value = NAN;       // their value; not a number: there are none
-  int waiting = 0;               // candidates in LDS
-  auto merge = [&](int n) {  // the first n <= 64 candidates
+  int waiting = 0, noted = 0;    // candidates, notes in LDS
+  auto merge = [&](int n) __attribute__((always_inline)) {      // the first n <= 64 candidates
     __builtin_amdgcn_wave_barrier();
     uint64_t v = lane < n ? cand[wave][lane] : 0;
     const uint64_t rest = cand[wave][64 + lane];
@@ -190,28 +222,39 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
     }
   };
 
+  // First value loaded for a chunk: the last chunk reaches back into the one
+  // before it, whose values are then left out, so that every load is whole.
+  auto start = [&](int c) { return min(c * kChunk, max(a.V - kChunk, 0)); };
+  // Past the row's chunks its last one again: loads that need no branch.
   auto load_chunk = [&](int c, u32x4 (&w)[NL]) {
+    c = min(c, chunks - 1);
+    if (a.V >= kChunk) {
+      const char* p = row + ((int64_t)start(c) + lane * PER) * (16 / PER);
 #pragma unroll
-    for (int j = 0; j < NL; j++) {
-      const int i = c * kChunk + (j * 64 + lane) * PER;
-      if (i + PER <= a.V) {
-        const u32x4_e v = *reinterpret_cast<const u32x4_e*>(row + (int64_t)i * (16 / PER));
+      for (int j = 0; j < NL; j++) {
+        const u32x4_e v = *reinterpret_cast<const u32x4_e*>(p + j * 1024);
         w[j] = u32x4{v[0], v[1], v[2], v[3]};
-      } else {
+      }
+      return;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          w[j][e] = XT == GEN_F32 ? 0xFF800000u : XT == GEN_F16 ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
-          if constexpr (XT == GEN_F32) {
-            if (i + e < a.V) w[j][e] = reinterpret_cast<const uint32_t*>(row)[i + e];
-          } else {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-            if (i + 2 * e < a.V) w[j][e] = (w[j][e] & 0xFFFF0000u) | p[i + 2 * e];
-            if (i + 2 * e + 1 < a.V) w[j][e] = (w[j][e] & 0xFFFFu) | (uint32_t)p[i + 2 * e + 1] << 16;
-          }
+    for (int j = 0; j < NL; j++) {  // a short row, -inf past its end
+      const int i = (j * 64 + lane) * PER;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        w[j][e] = kNone;
+        if constexpr (XT == GEN_F32) {
+          if (i + e < a.V) w[j][e] = reinterpret_cast<const uint32_t*>(row)[i + e];
+        } else {
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+          if (i + 2 * e < a.V) w[j][e] = (w[j][e] & 0xFFFF0000u) | p[i + 2 * e];
+          if (i + 2 * e + 1 < a.V) w[j][e] = (w[j][e] & 0xFFFFu) | (uint32_t)p[i + 2 * e + 1] << 16;
         }
       }
     }
   };
+  auto index = [&](int c, int v) { return start(c) + ((v / PER) * 64 + lane) * PER + v % PER; };
+  auto counts = [&](int c, int i) { return i >= c * kChunk && i < a.V; };
   auto value = [&](const u32x4 (&w)[NL], int v) -> float {  // value v of the lane's 16
     if constexpr (XT == GEN_F32) return __uint_as_float(w[v / 4][v % 4]);
     else {
@@ -221,7 +264,17 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
     }
   };
 
-  auto add_chunk = [&](const u32x4 (&w)[NL]) -> float {  // the lane's largest value of it
+  auto add_chunk = [&](int c, u32x4 (&w)[NL]) -> float {  // the lane's largest value of it
+    if (start(c) != c * kChunk) {
+#pragma unroll
+      for (int j = 0; j < NL; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int v = j * PER + e * (PER / 4);
+          if (!counts(c, index(c, v))) w[j][e] = PER == 4 ? kNone : (w[j][e] & 0xFFFF0000u) | (kNone & 0xFFFFu);
+          if (PER == 8 && !counts(c, index(c, v + 1))) w[j][e] = (w[j][e] & 0xFFFFu) | (kNone & 0xFFFF0000u);
+        }
+    }
     float top = value(w, 0);
 #pragma unroll
     for (int v = 1; v < 16; v++) top = fmaxf(top, value(w, v));
@@ -235,87 +288,164 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
     }
     return top;
   };
-  // waves of this workgroup that have values; what they all reach
+  // waves of this workgroup that have values
   const int active = min(kWaves, chunks - part * kWaves), each = (a.k + active - 1) / active;
-  auto post = [&]() {
+  auto post = [&]() __attribute__((always_inline)) {
     const float v = sorted_values(mine.m, lane);
-    if (lane == each - 1) __hip_atomic_store(&reached[wave], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    auto put = [&](int i, int r) {
+      if (lane == r - 1) __hip_atomic_store(&reached[i][wave], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    put(0, each);
+    put(1, min(2 * each, a.k));
+    put(2, a.k);
   };
-  auto collect = [&](int c, const u32x4 (&w)[NL], float top) {
-    float f = INFINITY;
+  // What k values of the workgroup reach: `each` of every wave, twice as many of
+  // two waves, or k of one.
+  auto reach = [&]() -> float {
+    float f = INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kWaves; i++)
-      f = fminf(f, __hip_atomic_load(&reached[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    for (int i = 0; i < kWaves; i++) {
+      auto get = [&](int r) { return __hip_atomic_load(&reached[r][i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
+      f = fminf(f, get(0));
+      const float x = get(1);
+      m2 = fmaxf(m2, fminf(m1, x));
+      m1 = fmaxf(m1, x);
+      m3 = fmaxf(m3, get(2));
+    }
+    return fmaxf(f, fmaxf(m2, m3));
+  };
+  // Value v of the 16 that lane l has of chunk c, its key (0: none).
+  auto key_at = [&](uint32_t c, uint32_t l, int v) -> uint64_t {
+    const int i = start(c) + ((v / PER) * 64 + (int)l) * PER + v % PER;
+    return counts(c, i) ? order_key(load<XT>(row, i), (uint32_t)i) : 0;
+  };
+  // Notes: the largest value's order above the chunk and lane.
+  auto note = [&](int c, float top) __attribute__((always_inline)) {
     // Values equal to f count; those equal to the list's floor come later and
     // lose to it.  A sum that is not a number may hide one among the values.
-    const float above = fmaxf(floor_value, below(f));
-    if (!__any(!(top <= above) || mine.s != mine.s)) return;
-    auto index = [&](int v) { return c * kChunk + ((v / PER) * 64 + lane) * PER + v % PER; };
-    uint32_t left = 0;  // the lane's values that pass, taken one a lane at a time
-#pragma unroll
-    for (int v = 0; v < 16; v++) left |= !(value(w, v) <= above) ? 1u << v : 0u;
-    while (__any(left)) {
-      const int v = left ? __builtin_ctz(left) : 0;
-      constexpr int W = 4 * NL;
-      uint32_t word[W];
-#pragma unroll
-      for (int i = 0; i < W; i++) word[i] = w[i / 4][i % 4];
-      const int wi = XT == GEN_F32 ? v : v / 2;
-#pragma unroll
-      for (int bit = W / 2; bit; bit /= 2)
-#pragma unroll
-        for (int i = 0; i < bit; i++) word[i] = wi & bit ? word[i + bit] : word[i];
-      float x;
-      if constexpr (XT == GEN_F32) x = __uint_as_float(word[0]);
-      else x = xt_to_f32<XT == GEN_F16 ? 1 : 0>(v & 1 ? word[0] >> 16 : word[0] & 0xFFFFu);
-      const uint64_t kv = left && index(v) < a.V ? order_key(x, (uint32_t)index(v)) : 0;
-      const uint64_t hits = __ballot(kv > floor);
-      if (kv > floor) cand[wave][waiting + __popcll(hits & ((1ull << lane) - 1))] = kv;
-      waiting += __popcll(hits);
-      left &= left - 1;
-      if (waiting >= 64) merge(64);
+    const float above = fmaxf(floor_value, below(reach()));
+    const bool hit = !(top <= above) || mine.s != mine.s;
+    const uint64_t hits = __ballot(hit);
+    if (hits == 0) return;
+    if (hit)
+      notes[wave][noted + __popcll(hits & ((1ull << lane) - 1))] =
+          (order_key(mine.s != mine.s ? INFINITY : top, 0) & ~0xFFFFFFFFull) | (uint32_t)(c * 64 + lane);
+    noted += __popcll(hits);
+    if (noted < 64) return;
+    // room: those that f has left behind go first
+    post();
+    const uint64_t least = order_key(reach(), 0xFFFFFFFFu);
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t n0 = notes[wave][lane], n1 = lane + 64 < noted ? notes[wave][lane + 64] : 0;
+    const uint64_t k0 = __ballot(n0 >= least), k1 = __ballot(n1 >= least);
+    __builtin_amdgcn_wave_barrier();
+    if (n0 >= least) notes[wave][__popcll(k0 & ((1ull << lane) - 1))] = n0;
+    if (n1 >= least) notes[wave][__popcll(k0) + __popcll(k1 & ((1ull << lane) - 1))] = n1;
+    noted = __popcll(k0) + __popcll(k1);
+    while (noted >= 64) {  // too many reach it: their values go through the list
+      __builtin_amdgcn_wave_barrier();
+      noted -= 64;
+      const uint32_t at = (uint32_t)notes[wave][noted + lane];
+      for (int v = 0; v < 16; v++) {
+        const uint64_t kv = key_at(at / 64, at % 64, v);
+        const uint64_t h = __ballot(kv > floor);
+        if (kv > floor) cand[wave][waiting + __popcll(h & ((1ull << lane) - 1))] = kv;
+        waiting += __popcll(h);
+        if (waiting >= 64) merge(64);
+      }
+      if (waiting > 0) merge(waiting);
     }
   };
 
-  u32x4 next[NL], w[NL];
+  // two chunks at a time, the next two on their way
+  u32x4 w0[NL], w1[NL];
   int c = part * kWaves + wave;
-  if (c < chunks) {
-    load_chunk(c, w);
-    if (c + step < chunks) load_chunk(c + step, next);
-    const float top = add_chunk(w);
-    if (a.k > 0) {
-      post();
-      __syncthreads();
-      collect(c, w, top);
+  load_chunk(c, w0);
+  load_chunk(c + step, w1);
+  if (tid < 2) count[tid] = 0;
+  if (c >= chunks) {
+    if (lane == 0) {
+      reached[0][wave] = INFINITY;
+      reached[1][wave] = reached[2][wave] = -INFINITY;
     }
-  } else if (a.k > 0) {
-    if (lane == 0) reached[wave] = INFINITY;
     __syncthreads();
   }
-  c += step;
-  for (int n = 2; c < chunks; c += step, n++) {
-#pragma unroll
-    for (int j = 0; j < NL; j++) w[j] = next[j];
-    if (c + step < chunks) load_chunk(c + step, next);
-    const float top = add_chunk(w);
-    if (a.k == 0) continue;
-    if ((n & (n - 1)) == 0) post();
-    collect(c, w, top);
+  for (int n = 1; c < chunks; n++, c += 2 * step) {
+    float top0 = add_chunk(c, w0), top1 = -INFINITY;
+    load_chunk(c + 2 * step, w0);
+    const bool two = c + step < chunks;
+    if (two) top1 = add_chunk(c + step, w1);
+    load_chunk(c + 3 * step, w1);
+    if (a.k > 0 && (n & (n - 1)) == 0 && (n & 0x55555555)) post();
+    if (n == 1) __syncthreads();  // the first maxima are shared before any value is noted
+    if (a.k > 0) {
+#pragma unroll 1
+      for (int h = 0; h <= two; h++) note(c + h * step, h ? top1 : top0);
+    }
   }
-  if (waiting > 0) merge(waiting);
 
-  // join the workgroup
-#pragma unroll
-  for (int d = 32; d; d >>= 1) mine = add(mine, Sums{__shfl_xor(mine.m, d), __shfl_xor(mine.s, d), __shfl_xor(mine.e, d)}, sc);
+  if (a.k > 0 && part * kWaves + wave < chunks) post();
+  mine = wave_sums(mine, sc, lane);
   if (lane == 0) sums[wave] = mine;
-  lists[wave][lane] = list;
+  // Puts the lanes' keys of at least `least` into `to`, while it has room, and counts them.
+  auto pick = [&](uint64_t key, uint64_t least, uint64_t* to, int* n) __attribute__((always_inline)) {
+    const bool in = key != 0 && key >= least;
+    const uint64_t hits = __ballot(in);
+    if (hits == 0) return;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(n, __popcll(hits));
+    at = __builtin_amdgcn_readfirstlane(at) + __popcll(hits & ((1ull << lane) - 1));
+    if (in && at < kFew) to[at] = key;
+  };
+  auto merge_lists = [&]() {
+    lists[wave][lane] = list;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) merge64(list, lists[w][lane], lane);
+    }
+  };
+  // The 64 largest of n <= kFew of `few`, sorted in wave 0's lanes.
+  auto sort_few = [&](int n) {
+    list = tid < n ? few[tid] : 0;
+    if (wave * 64 < n) sort64(list, lane, n - wave * 64);
+    if (n > 64) merge_lists();
+  };
   __syncthreads();
   Sums all = sums[0];
 #pragma unroll
   for (int w = 1; w < kWaves; w++) all = add(all, sums[w], sc);
-  if (wave == 0 && a.k > 0) {
+  if (a.k > 0) {
+    const uint64_t least = order_key(reach(), 0xFFFFFFFFu);
+    pick(lane < noted ? notes[wave][lane] : 0, least, marked, &count[0]);
+    pick(list, least, few, &count[1]);
+    __syncthreads();
+    if (count[0] <= kFew) {  // four lanes a note
+      for (int i0 = 0; i0 < count[0]; i0 += 64) {
+        const int i = i0 + tid / 4;
+        const uint32_t at = i < count[0] ? (uint32_t)marked[i] : 0;
+        uint64_t kv[4];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) merge64(list, lists[w][lane], lane);
+        for (int v = 0; v < 4; v++) kv[v] = i < count[0] ? key_at(at / 64, at % 64, 4 * (tid % 4) + v) : 0;
+#pragma unroll
+        for (int v = 0; v < 4; v++) pick(kv[v], least, few, &count[1]);
+      }
+      __syncthreads();
+    }
+    if (count[0] <= kFew && count[1] <= kFew) {
+      sort_few(count[1]);
+    } else {
+      for (int n = 0; n < noted; n++) {  // a note at a time, its values in 16 lanes
+        const uint32_t at = (uint32_t)notes[wave][n];
+        const uint64_t kv = lane < 16 ? key_at(at / 64, at % 64, lane) : 0;
+        const uint64_t h = __ballot(kv > floor);
+        if (kv > floor) cand[wave][waiting + __popcll(h & ((1ull << lane) - 1))] = kv;
+        waiting += __popcll(h);
+        if (waiting >= 64) merge(64);
+      }
+      if (waiting > 0) merge(waiting);
+      merge_lists();
+    }
   }
 
   // and the row's workgroups: (m, s, e, 0), then 64 keys of each
@@ -341,37 +471,56 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
     }
     __syncthreads();
     if (!arrived) return;
-    // wave w joins parts w, w + 4, .. in order, then the waves as before
+    // the sums in order, wave w those of parts w, w + 4, ..
     mine = Sums{-INFINITY, 0.f, 0.f};
     list = 0;
+    auto load_list = [&](int i) -> uint64_t {
+      const u32x2 o = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(i) + 16 + lane * 8, 0, kAgentScope));
+      return ((uint64_t)o[1] << 32) | o[0];
+    };
     constexpr int U = 8;  // parts in flight
+    // What k keys reach: of the first 64 parts the ceil(k / r)-th largest of
+    // their r-th keys, r about twice what each part has of the k.
+    uint64_t least = 0;
+    if (a.k > 0) {
+      const int n = min(a.split, 64), r = min(2 * ((a.k + n - 1) / n), a.k);
+      const u32x2 o = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(min(lane, n - 1)) + 16 + (r - 1) * 8, 0, kAgentScope));
+      uint64_t head = lane < n ? ((uint64_t)o[1] << 32) | o[0] : 0;
+      sort64(head, lane, n);
+      least = __shfl((unsigned long long)head, (a.k + r - 1) / r - 1);
+    }
+    if (tid == 0) count[1] = 0;
+    __syncthreads();
     for (int i0 = wave; i0 < a.split; i0 += kWaves * U) {
       u32x4 v[U];
-      u32x2 o[U];
+      uint64_t o[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const uint32_t p = part_at(min(i0 + u * kWaves, a.split - 1));
-        v[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p, 0, kAgentScope));
-        if (a.k > 0)
-          o[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + 16 + lane * 8, 0, kAgentScope));
+        const int i = min(i0 + u * kWaves, a.split - 1);
+        v[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, part_at(i), 0, kAgentScope));
+        if (a.k > 0) o[u] = load_list(i);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         if (i0 + u * kWaves >= a.split) break;
         mine = add(mine, Sums{__uint_as_float(v[u][0]), __uint_as_float(v[u][1]), __uint_as_float(v[u][2])}, sc);
-        if (a.k > 0) merge64(list, ((uint64_t)o[u][1] << 32) | o[u][0], lane);
+        if (a.k > 0) pick(o[u], least, few, &count[1]);
       }
     }
-    __syncthreads();
     if (lane == 0) sums[wave] = mine;
-    lists[wave][lane] = list;
     __syncthreads();
     all = sums[0];
 #pragma unroll
     for (int w = 1; w < kWaves; w++) all = add(all, sums[w], sc);
-    if (wave == 0 && a.k > 0) {
-#pragma unroll
-      for (int w = 1; w < kWaves; w++) merge64(list, lists[w][lane], lane);
+    if (a.k > 0) {
+      if (count[1] <= kFew) {
+        sort_few(count[1]);
+      } else {
+        for (int i = wave; i < a.split; i += kWaves) merge64(list, load_list(i), lane);
+        merge_lists();
+      }
     }
   }
 
@@ -394,10 +543,8 @@ __global__ __launch_bounds__(256, 5) void token_logprobs_kernel(const LogprobArg
 }  // namespace
 
 void token_logprobs_plan(LogprobArgs& a, int cus, int64_t* part_bytes) {
-  const int cpw = getenv("LP_CPW") ? atoi(getenv("LP_CPW")) : 1;
-  const int chunks = (a.V + kChunk - 1) / kChunk, most = (chunks + kWaves * cpw - 1) / (kWaves * cpw);
-  const int rw = getenv("LP_RW") ? atoi(getenv("LP_RW")) : kRowWgs;
-  const int64_t want = ((int64_t)cus * rw + a.T - 1) / std::max<int64_t>(a.T, 1);
+  const int chunks = (a.V + kChunk - 1) / kChunk, most = (chunks + 2 * kWaves - 1) / (2 * kWaves);
+  const int64_t want = ((int64_t)cus * kRowWgs + a.T - 1) / std::max<int64_t>(a.T, 1);
   a.split = (int)std::max<int64_t>(1, std::min<int64_t>(most, want));
   *part_bytes = a.split > 1 ? a.T * a.split * (4 + 128) * 4 : 0;
 }
