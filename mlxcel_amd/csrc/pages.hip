@@ -21,51 +21,85 @@ namespace mlxq {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kBlock = 4 * kPlanThreads;  // pages looked at together, four a thread
+constexpr int kNear = 4096;               // free pages listed in LDS
 
-// Exclusive sum over the workgroup's kPlanThreads threads, and the total.
-// wsum: one word per wave.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* wsum, int64_t& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t x = v;
+typedef int32_t i32x4_e __attribute__((ext_vector_type(4), aligned(4)));
+
+// Sums over the workgroup's kPlanThreads threads; two sets of words in turn, so
+// that one barrier a sum is enough.
+template <typename T>
+struct Scan {
+  T (*words)[kPlanWaves];
+  int turn = 0;
+  // exclusive, and the total
+  __device__ __forceinline__ T operator()(T v, T& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T x = v;
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int64_t o = __shfl_up((long long)x, s);
-    if (lane >= s) x += o;
-  }
-  __syncthreads();  // the last call's sums have been read
-  if (lane == 63) wsum[wave] = x;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
+    for (int s = 1; s < 64; s <<= 1) {
+      const T o = __shfl_up(x, s);
+      if (lane >= s) x += o;
+    }
+    T* w = words[turn ^= 1];
+    if (lane == 63) w[wave] = x;
+    __syncthreads();
+    T before = 0;
+    total = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; w++) {
-    if (w < wave) before += wsum[w];
-    total += wsum[w];
+    for (int i = 0; i < kPlanWaves; i++) {
+      if (i < wave) before += w[i];
+      total += w[i];
+    }
+    return before + x - v;
   }
-  return before + x - v;
-}
+};
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int page) { return (int)((tokens + page - 1) / page); }
 
-// Appends the next free pages to list until it has `want` of them or refs is
-// at its end; at / have: where the scan stands and what the list holds (the
-// same in every thread).
-__device__ void extend_free(const int32_t* refs, int pages, int32_t* list, int64_t want, int& at, int64_t& have,
-                            int64_t* wsum) {
-  while (have < want && at < pages) {
-    const int p = at + threadIdx.x;
-    const bool free = p < pages && refs[p] == 0;
-    int64_t total;
-    const int64_t r = block_scan(free, wsum, total);
-    if (free) list[have + r] = p;
-    have += total;
-    at += kPlanThreads;
-  }
-  __syncthreads();  // the list's new entries are read by other threads
+// refs of pages 4 tid .. 4 tid + 3 of the block from `at` on (past the end: held)
+__device__ __forceinline__ i32x4_e load_refs(const int32_t* refs, int pages, int at) {
+  const int p = at + 4 * (int)threadIdx.x;
+  if (p + 4 <= pages) return *reinterpret_cast<const i32x4_e*>(refs + p);
+  i32x4_e r;
+#pragma unroll
+  for (int e = 0; e < 4; e++) r[e] = p + e < pages ? refs[p + e] : 1;
+  return r;
 }
 
-// The first of n ascending numbers that is above v, minus one.
+// The free pages in ascending order, found as they are asked for: the first
+// kNear in LDS, the others in scratch.  All members are the same in every thread.
+struct FreeList {
+  const int32_t* refs;
+  int pages;
+  int32_t *near, *far;
+  i32x4_e block;  // refs at `at`, already on their way
+  int at = 0;
+  int have = 0;
+  __device__ __forceinline__ int32_t get(int i) const { return i < kNear ? near[i] : far[i]; }
+  // until there are `want` or refs is at its end
+  __device__ void extend(int64_t want, Scan<int>& scan) {
+    while (have < want && at < pages) {
+      int n = 0, total;
+#pragma unroll
+      for (int e = 0; e < 4; e++) n += block[e] == 0;
+      int r = have + scan(n, total);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (block[e] == 0) {
+          (r < kNear ? near : far)[r] = at + 4 * (int)threadIdx.x + e;
+          r++;
+        }
+      have += total;
+      at += kBlock;
+      if (have < want && at < pages) block = load_refs(refs, pages, at);
+    }
+    __syncthreads();  // the list's new entries are read by other threads
+  }
+};
+
+// The last of n ascending numbers that is at most v.
 __device__ __forceinline__ int owner_of(const int64_t* first, int n, int64_t v) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
@@ -77,14 +111,18 @@ __device__ __forceinline__ int owner_of(const int64_t* first, int n, int64_t v) 
 }
 
 __global__ __launch_bounds__(kPlanThreads) void cache_reserve_kernel(const CacheBook b, const int32_t* counts,
-                                                                     int32_t* granted, int32_t* list) {
-  __shared__ int64_t wsum[kPlanThreads / 64];
+                                                                     int32_t* granted, int32_t* far) {
+  __shared__ int64_t sums[2][kPlanWaves];
+  __shared__ int flags[2][kPlanWaves];
+  __shared__ int32_t near[kNear];
   __shared__ int64_t first[kPlanThreads];
   __shared__ int32_t need_s[kPlanThreads];
   __shared__ int64_t taken_s;
   const int tid = threadIdx.x;
-  int at = 0;
-  int64_t have = 0, used = 0;
+  Scan<int64_t> scan{sums};
+  Scan<int> count{flags};
+  FreeList free{b.refs, b.pages, near, far, load_refs(b.refs, b.pages, 0)};
+  int64_t used = 0;
   for (int r0 = 0; r0 < b.rows; r0 += kPlanThreads) {
     const int r = r0 + tid, n = min(kPlanThreads, b.rows - r0);
     int64_t len = 0, cnt = 0;
@@ -101,48 +139,50 @@ __global__ __launch_bounds__(kPlanThreads) void cache_reserve_kernel(const Cache
       }
     }
     int64_t total;
-    int64_t before = block_scan(need, wsum, total);
-    extend_free(b.refs, b.pages, list, used + total, at, have, wsum);
-    if (have - used < total) {
-      // too few pages: row by row, each that still fits
-      need_s[tid] = need;
-      __syncthreads();
-      if (tid == 0) {
-        int64_t left = have - used, sum = 0;
-        for (int i = 0; i < n; i++) {
-          first[i] = sum;
-          if (need_s[i] > left) need_s[i] = -1;
-          else {
-            left -= need_s[i];
-            sum += need_s[i];
+    int64_t before = scan(need, total);
+    if (total > 0) {
+      free.extend(used + total, count);
+      if (free.have - used < total) {
+        // too few pages: row by row, each that still fits
+        need_s[tid] = need;
+        __syncthreads();
+        if (tid == 0) {
+          int64_t left = free.have - used, sum = 0;
+          for (int i = 0; i < n; i++) {
+            first[i] = sum;
+            if (need_s[i] > left) need_s[i] = -1;
+            else {
+              left -= need_s[i];
+              sum += need_s[i];
+            }
           }
+          taken_s = sum;
         }
-        taken_s = sum;
+        __syncthreads();
+        if (need_s[tid] < 0) {
+          ok = false;
+          need = 0;
+        }
+        before = first[tid];
+        total = taken_s;
+        __syncthreads();
       }
+      first[tid] = r < b.rows ? before : INT64_MAX;
+      need_s[tid] = had;
       __syncthreads();
-      if (need_s[tid] < 0) {
-        ok = false;
-        need = 0;
+      for (int64_t i = tid; i < total; i += kPlanThreads) {
+        const int o = owner_of(first, n, i);
+        const int32_t p = free.get((int)(used + i));
+        b.table[(int64_t)(r0 + o) * b.table_row + need_s[o] + (i - first[o])] = p;
+        b.refs[p] = 1;
       }
-      before = first[tid];
-      total = taken_s;
-    }
-    __syncthreads();
-    first[tid] = r < b.rows ? before : INT64_MAX;
-    need_s[tid] = had;
-    __syncthreads();
-    for (int64_t i = tid; i < total; i += kPlanThreads) {
-      const int o = owner_of(first, n, i);
-      const int32_t p = list[used + i];
-      b.table[(int64_t)(r0 + o) * b.table_row + need_s[o] + (i - first[o])] = p;
-      b.refs[p] = 1;
+      used += total;
+      __syncthreads();
     }
     if (r < b.rows) {
       granted[r] = ok;
       if (ok) b.lengths[r] = (int32_t)(len + cnt);
     }
-    used += total;
-    __syncthreads();
   }
 }
 
@@ -171,12 +211,21 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheAppendArgs
 
 // ---- copies of pages -----------------------------------------------------------
 
+// One page by one workgroup, four words a thread on their way.
 template <typename W>
 __device__ __forceinline__ void copy_page(char* base, int64_t stride, int64_t bytes, int from, int to) {
   const W* s = reinterpret_cast<const W*>(base + from * stride);
   W* d = reinterpret_cast<W*>(base + to * stride);
   const int64_t n = bytes / (int64_t)sizeof(W);
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) d[i] = s[i];
+  int64_t i = threadIdx.x;
+  for (; i + 3 * 256 < n; i += 4 * 256) {
+    W v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v[u] = s[i + u * 256];
+#pragma unroll
+    for (int u = 0; u < 4; u++) d[i + u * 256] = v[u];
+  }
+  for (; i < n; i += 256) d[i] = s[i];
 }
 
 // ---- fork ----------------------------------------------------------------------
@@ -184,32 +233,35 @@ __device__ __forceinline__ void copy_page(char* base, int64_t stride, int64_t by
 // scratch: the list of free pages, then per pair {tokens or -1, fresh page or -1}
 __global__ __launch_bounds__(kPlanThreads) void cache_fork_plan_kernel(const CacheBook b, const int32_t* src,
                                                                        const int32_t* dst, int n, int32_t* granted,
-                                                                       int32_t* list, int32_t* pair) {
-  __shared__ int64_t wsum[kPlanThreads / 64];
+                                                                       int32_t* far, int32_t* pair) {
+  __shared__ int sums[2][kPlanWaves], flags[2][kPlanWaves];
+  __shared__ int32_t near[kNear], dst_s[kPlanThreads];
   const int tid = threadIdx.x;
-  int at = 0;
-  int64_t have = 0, used = 0;
+  Scan<int> scan{sums}, count{flags};
+  FreeList free{b.refs, b.pages, near, far, load_refs(b.refs, b.pages, 0)};
+  int used = 0;
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    bool ok = false;
-    int64_t len = 0;
-    if (i < n) {
-      const int s = src[i], d = dst[i];
-      ok = s >= 0 && s < b.rows && d >= 0 && d < b.rows;
-      if (ok) {
-        len = b.lengths[s];
-        ok = len >= 0 && len <= (int64_t)b.width * b.page && b.lengths[d] == 0;
-      }
-      for (int j = 0; ok && j < i; j++) ok = dst[j] != d;  // the first pair of a row takes it
+    const int s = i < n ? src[i] : -1, d = i < n ? dst[i] : -1;
+    bool ok = s >= 0 && s < b.rows && d >= 0 && d < b.rows;
+    const int64_t len = ok ? b.lengths[s] : 0;
+    ok = ok && len >= 0 && len <= (int64_t)b.width * b.page && b.lengths[d] == 0;
+    dst_s[tid] = d;
+    __syncthreads();
+    // the first pair of a row takes it
+    for (int j = 0; ok && j < i0; j++) ok = dst[j] != d;
+    for (int j = 0; ok && j < tid; j += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) ok = ok && (j + e >= tid || dst_s[j + e] != d);
     }
     const int part = ok && len % b.page != 0;
-    int64_t total;
-    const int64_t r = block_scan(part, wsum, total);
-    extend_free(b.refs, b.pages, list, used + total, at, have, wsum);
+    int total;
+    const int r = used + scan(part, total);
+    if (total > 0) free.extend(used + total, count);
     int fresh = -1;
     if (part) {
-      if (used + r < have) {
-        fresh = list[used + r];
+      if (r < free.have) {
+        fresh = free.get(r);
         b.refs[fresh] = 1;
       } else {
         ok = false;
@@ -220,22 +272,27 @@ __global__ __launch_bounds__(kPlanThreads) void cache_fork_plan_kernel(const Cac
       pair[2 * i] = ok ? (int32_t)len : -1;
       pair[2 * i + 1] = fresh;
     }
-    used = min(used + total, have);
+    used = min(used + total, free.have);
     __syncthreads();
   }
 }
 
-// blockIdx.x: a pair; blockIdx.y: a pool, the last one the table's row.
+// Workgroups count pools first, in eights: those of one pool then run on one XCD
+// whatever their pair, and a page that is copied several times is read into that
+// XCD's L2 once.  Past the pools, and where `book`, one more a pair for its row
+// of the table.
 template <typename W>
 __global__ __launch_bounds__(256) void cache_fork_copy_kernel(const CacheBook b, const int32_t* src, const int32_t* dst,
-                                                              const int32_t* pair, const PoolList pools) {
-  const int i = blockIdx.x, len = pair[2 * i], fresh = pair[2 * i + 1];
-  if (len < 0) return;
+                                                              const int32_t* pair, const PoolList pools, int columns,
+                                                              bool book) {
+  const int i = blockIdx.x / columns, q = blockIdx.x - i * columns;
+  const int len = pair[2 * i], fresh = pair[2 * i + 1];
+  if (len < 0 || (q >= pools.n && (q > pools.n || !book))) return;
   const int full = len / b.page;
   const int32_t* from = b.table + src[i] * b.table_row;
-  if ((int)blockIdx.y == pools.n) {
+  if (q == pools.n) {
     int32_t* to = b.table + dst[i] * b.table_row;
-    for (int j = threadIdx.x; j < full; j += blockDim.x) {
+    for (int j = threadIdx.x; j < full; j += 256) {
       const int32_t p = from[j];
       to[j] = p;
       if (p >= 0 && p < b.pages) atomicAdd(b.refs + p, 1);
@@ -249,7 +306,7 @@ __global__ __launch_bounds__(256) void cache_fork_copy_kernel(const CacheBook b,
   if (fresh < 0) return;
   const int old = from[full];
   if (old < 0 || old >= b.pages) return;
-  copy_page<W>(pools.base[blockIdx.y], pools.stride, pools.bytes, old, fresh);
+  copy_page<W>(pools.base[q], pools.stride, pools.bytes, old, fresh);
 }
 
 // ---- free ------------------------------------------------------------------------
@@ -258,13 +315,16 @@ __global__ __launch_bounds__(256) void cache_free_kernel(const CacheBook b, cons
   __shared__ int len_s;
   const int row = rows[blockIdx.x];
   if (row < 0 || row >= b.rows) return;
-  // of several requests for one row one gets its length
+  // of several requests for one row one gets its length; the first entries of
+  // the table are read meanwhile
+  const int32_t* t = b.table + row * b.table_row;
+  int32_t p = (int)threadIdx.x < b.width ? t[threadIdx.x] : -1;
   if (threadIdx.x == 0) len_s = atomicExch(b.lengths + row, 0);
   __syncthreads();
   const int64_t len = min((int64_t)max(len_s, 0), (int64_t)b.width * b.page);
   const int held = pages_of(len, b.page);
-  for (int j = threadIdx.x; j < held; j += blockDim.x) {
-    const int32_t p = b.table[row * b.table_row + j];
+  for (int j = threadIdx.x; j < held; j += 256) {
+    if (j >= 256) p = t[j];
     if (p >= 0 && p < b.pages) atomicSub(b.refs + p, 1);
   }
 }
@@ -275,26 +335,40 @@ __global__ __launch_bounds__(256) void cache_free_kernel(const CacheBook b, cons
 __global__ __launch_bounds__(kPlanThreads) void cache_compact_plan_kernel(const CacheBook b, int32_t* live_out,
                                                                           int32_t* moves, int32_t* to, int32_t* holes,
                                                                           int32_t* movers) {
-  __shared__ int64_t wsum[kPlanThreads / 64];
+  __shared__ int sums[2][kPlanWaves];
   const int tid = threadIdx.x;
-  int64_t live = 0, total;
-  for (int p = tid; p < b.pages; p += kPlanThreads) live += b.refs[p] > 0;
-  block_scan(live, wsum, total);
-  const int n = (int)total;
+  Scan<int> scan{sums};
+  const i32x4_e block = load_refs(b.refs, b.pages, 0);
+  auto held_at = [&](const i32x4_e& r, int at, int e) { return at + 4 * tid + e < b.pages && r[e] > 0; };
+  int live = 0, n;
+  for (int at = 0; at < b.pages; at += kBlock) {
+    const i32x4_e r = at ? load_refs(b.refs, b.pages, at) : block;
+#pragma unroll
+    for (int e = 0; e < 4; e++) live += held_at(r, at, e);
+  }
+  scan(live, n);
   // holes are the free pages below n, movers the held ones from n on: as many
-  int64_t nh = 0, nm = 0;
-  for (int p0 = 0; p0 < b.pages; p0 += kPlanThreads) {
-    const int p = p0 + tid;
-    const bool held = p < b.pages && b.refs[p] > 0;
-    const bool hole = p < n && !held, mover = p >= n && held;
-    int64_t th, tm;
-    const int64_t rh = block_scan(hole, wsum, th);
-    const int64_t rm = block_scan(mover, wsum, tm);
-    if (hole) holes[nh + rh] = p;
-    if (mover) movers[nm + rm] = p;
-    if (p < b.pages) to[p] = p;
-    nh += th;
-    nm += tm;
+  int nh = 0, nm = 0;
+  for (int at = 0; at < b.pages; at += kBlock) {
+    const i32x4_e r = at ? load_refs(b.refs, b.pages, at) : block;
+    const int p = at + 4 * tid;
+    int mine = 0, total;  // holes and movers, 16 bits each
+#pragma unroll
+    for (int e = 0; e < 4; e++) mine += held_at(r, at, e) ? (p + e >= n ? 1 << 16 : 0) : (p + e < n);
+    const int before = scan(mine, total);
+    int h = nh + (before & 0xFFFF), m = nm + (before >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (p + e >= b.pages) break;
+      to[p + e] = p + e;
+      if (held_at(r, at, e)) {
+        if (p + e >= n) movers[m++] = p + e;
+      } else if (p + e < n) {
+        holes[h++] = p + e;
+      }
+    }
+    nh += total & 0xFFFF;
+    nm += total >> 16;
   }
   __syncthreads();
   for (int i = tid; i < nm; i += kPlanThreads) {
@@ -378,11 +452,15 @@ hipError_t launch_cache_fork_plan(const CacheBook& b, const int32_t* src, const 
 hipError_t launch_cache_fork_copy(const CacheBook& b, const int32_t* src, const int32_t* dst, int n,
                                   const int32_t* scratch, const PoolList& pools, bool book, hipStream_t stream) {
   if (n == 0) return hipSuccess;
-  const dim3 grid((unsigned)n, (unsigned)(pools.n + (book ? 1 : 0))), block(256);
+  const int columns = (pools.n + (book ? 1 : 0) + 7) / 8 * 8;
+  if (columns == 0) return hipSuccess;
+  if ((int64_t)n * columns > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(n * columns)), block(256);
   const int32_t* pair = scratch + b.pages;
-  if (grid.y == 0) return hipSuccess;
-  if (wide(pools)) hipLaunchKernelGGL(cache_fork_copy_kernel<u32x4>, grid, block, 0, stream, b, src, dst, pair, pools);
-  else hipLaunchKernelGGL(cache_fork_copy_kernel<uint16_t>, grid, block, 0, stream, b, src, dst, pair, pools);
+  if (wide(pools))
+    hipLaunchKernelGGL(cache_fork_copy_kernel<u32x4>, grid, block, 0, stream, b, src, dst, pair, pools, columns, book);
+  else
+    hipLaunchKernelGGL(cache_fork_copy_kernel<uint16_t>, grid, block, 0, stream, b, src, dst, pair, pools, columns, book);
   return hipGetLastError();
 }
 
