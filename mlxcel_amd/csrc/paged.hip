@@ -140,8 +140,6 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   using G = Geo<XT, DP>;
   extern __shared__ __align__(16) float lds[];
   __shared__ u32x4 qs[G::KC * 64];
-  __shared__ int scan[kWaves];
-  __shared__ int bound[2][3];  // where this workgroup's steps begin and end: step among all, step in its sequence, sequence
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -149,13 +147,51 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   const int64_t cap = (int64_t)a.width * a.page;
   const int heads_b = a.Hkv * tiles_h;  // (key head, 16 query heads) of a sequence
 
-  // the sequences' steps: thread i sums those of its share
-  int n;
-  bool once;
-  {
+  // Where this workgroup's steps begin and end: step among all, step in its
+  // sequence, sequence, its length.
+  struct Bound {
+    int step, off, b, len;
+  };
+  auto steps_in = [&](int len) {
+    int lo, hi;
+    return steps_of<G::KEYS>(len, cap, a.window, lo, hi);
+  };
+  // Step p, `off` into sequence b, unless it cuts a head of few steps: that one
+  // belongs to the workgroup of its first step.
+  auto bound_at = [&](int p, int off, int b, int len) -> Bound {
+    const int s = steps_in(len), up = s <= a.whole && off % s ? s - off % s : 0;
+    return Bound{p + up, off + up, b, len};
+  };
+  auto clear = [&](int b) {  // a sequence without keys has no steps: its output is zeros
+    for (int i = tid; i < a.Hq * a.D; i += 256) store_element<XT>(a.out, (int64_t)b * a.Hq * a.D + i, 0.f);
+  };
+  int n, total;
+  Bound first, last;
+  if (a.B <= 64) {  // each wave finds them by itself, sequence i in lane i
+    const int len = lane < a.B ? a.lengths[lane] : 0, steps = steps_in(len), mine = heads_b * steps;
+    int sum = mine;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int o = __shfl_up(sum, s);
+      if (lane >= s) sum += o;
+    }
+    total = __builtin_amdgcn_readlane(sum, 63);
+    n = (total + a.wgs - 1) / a.wgs;
+    auto find = [&](int p) -> Bound {
+      if (p >= total) return Bound{total, 0, 0, 0};
+      const int i = __builtin_ctzll(__ballot(sum - mine <= p && p < sum));
+      return bound_at(p, p - __builtin_amdgcn_readlane(sum - mine, i), i, __builtin_amdgcn_readlane(len, i));
+    };
+    first = find(blockIdx.x * n);
+    last = find((blockIdx.x + 1) * n);
+    for (uint64_t none = __ballot(lane < a.B && steps == 0); none; none &= none - 1)
+      if (__builtin_ctzll(none) % a.wgs == (int)blockIdx.x) clear(__builtin_ctzll(none));
+  } else {  // thread i sums those of its share
+    __shared__ int scan[kWaves];
+    __shared__ Bound bound[2];
     const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
-    int mine = 0, lo, hi;
-    for (int b = b0; b < b1; b++) mine += heads_b * steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
+    int mine = 0;
+    for (int b = b0; b < b1; b++) mine += heads_b * steps_in(a.lengths[b]);
     int sum = mine;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -164,50 +200,40 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     }
     if (lane == 63) scan[wave] = sum;
     __syncthreads();
-    int before = sum - mine, total = 0;
+    int before = sum - mine;
+    total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
       if (w < wave) before += scan[w];
       total += scan[w];
     }
     n = (total + a.wgs - 1) / a.wgs;
-    // More keys and values than the last cache holds are not kept there for
-    // the next call: 2.1 GB 360 -> 325 us; 174 MB, read again and again, 37 -> 44 us.
-    once = (int64_t)total * (G::KEYS * 2 * G::ES) * a.D > kLastCache;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      int p = ((int)blockIdx.x + i) * n;
+      const int p = ((int)blockIdx.x + i) * n;
       if (p >= total) {
-        if (tid == 0) bound[i][0] = total;
+        if (tid == 0) bound[i] = Bound{total, 0, 0, 0};
       } else if (before <= p && p < before + mine) {
-        int off = p - before, b = b0, s;
-        for (;; b++) {
-          s = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
-          if (off < s * heads_b) break;
-          off -= s * heads_b;
-        }
-        // a head of few steps is not cut: it belongs to the workgroup of its first one
-        if (s <= a.whole && off % s) {
-          p += s - off % s;
-          off += s - off % s;
-        }
-        bound[i][0] = p;
-        bound[i][1] = off;
-        bound[i][2] = b;
+        int off = p - before, b = b0;
+        while (off >= heads_b * steps_in(a.lengths[b])) off -= heads_b * steps_in(a.lengths[b++]);
+        bound[i] = bound_at(p, off, b, a.lengths[b]);
       }
     }
+    for (int b = blockIdx.x; b < a.B; b += a.wgs)
+      if (steps_in(a.lengths[b]) == 0) clear(b);
     __syncthreads();
+    first = bound[0];
+    last = bound[1];
   }
-  // a sequence without keys has no steps: its output is zeros
-  for (int b = blockIdx.x; b < a.B; b += a.wgs) {
-    int lo, hi;
-    if (steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi) == 0)
-      for (int i = tid; i < a.Hq * a.D; i += 256) store_element<XT>(a.out, (int64_t)b * a.Hq * a.D + i, 0.f);
-  }
-  int at = __builtin_amdgcn_readfirstlane(bound[0][0]);
-  const int end = __builtin_amdgcn_readfirstlane(bound[1][0]);
+  int at = __builtin_amdgcn_readfirstlane(first.step);
+  const int end = __builtin_amdgcn_readfirstlane(last.step);
   if (at >= end) return;
-  int off = __builtin_amdgcn_readfirstlane(bound[0][1]), b = __builtin_amdgcn_readfirstlane(bound[0][2]);
+  int off = __builtin_amdgcn_readfirstlane(first.off), b = __builtin_amdgcn_readfirstlane(first.b);
+  int len = __builtin_amdgcn_readfirstlane(first.len);
+  // More keys and values than the last cache holds beside others' are not kept
+  // there for the next call: 2.1 GB 360 -> 325 us, 174 MB among other work 46 -> 44.5 us
+  // (read again and again by itself 37 -> 44 us).
+  const bool once = (int64_t)total * (G::KEYS * 2 * G::ES) * a.D > kLastCache / 2;
   // scores in units of log2 e
   const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
   const int slot_words = part_words(min(per, 16), DP);
@@ -216,9 +242,9 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   auto run = [&](auto ONCE) {
     while (at < end) {
       int lo, hi;
-      const int steps = steps_of<G::KEYS>(a.lengths[b], cap, a.window, lo, hi);
-      if (steps == 0 || off >= steps * heads_b) {
-        b++;
+      const int steps = steps_of<G::KEYS>(len, cap, a.window, lo, hi);
+      if (off >= steps * heads_b) {
+        len = __builtin_amdgcn_readfirstlane(a.lengths[++b]);
         off = 0;
         continue;
       }
