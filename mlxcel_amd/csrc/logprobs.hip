@@ -363,6 +363,10 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
   load_chunk(c, w0);
   load_chunk(c + step, w1);
   if (tid < 2) count[tid] = 0;
+  // the first given tokens' logits, needed at the end
+  const int token = tid < a.n_tok ? a.tokens[t * a.n_tok + tid] : -1;
+  const float token_logit = token >= 0 && token < a.V ? load<XT>(row, token) : NAN;
+  bool posted = true;  // this wave's maxima as they stand
   if (c >= chunks) {
     if (lane == 0) {
       reached[0][wave] = INFINITY;
@@ -376,7 +380,8 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
     const bool two = c + step < chunks;
     if (two) top1 = add_chunk(c + step, w1);
     load_chunk(c + 3 * step, w1);
-    if (a.k > 0 && (n & (n - 1)) == 0 && (n & 0x55555555)) post();
+    posted = a.k == 0 || ((n & (n - 1)) == 0 && (n & 0x55555555));
+    if (posted && a.k > 0) post();
     if (n == 1) __syncthreads();  // the first maxima are shared before any value is noted
     if (a.k > 0) {
 #pragma unroll 1
@@ -384,18 +389,29 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
     }
   }
 
-  if (a.k > 0 && part * kWaves + wave < chunks) post();
+  if (!posted) post();
   mine = wave_sums(mine, sc, lane);
   if (lane == 0) sums[wave] = mine;
-  // Puts the lanes' keys of at least `least` into `to`, while it has room, and counts them.
-  auto pick = [&](uint64_t key, uint64_t least, uint64_t* to, int* n) __attribute__((always_inline)) {
-    const bool in = key != 0 && key >= least;
-    const uint64_t hits = __ballot(in);
-    if (hits == 0) return;
+  // Puts the lanes' N keys of at least `least` into `to`, while it has room, and counts them.
+  auto pick = [&](auto& key, uint64_t least, uint64_t* to, int* n) __attribute__((always_inline)) {
+    constexpr int N = sizeof(key) / sizeof(key[0]);
+    uint64_t hits[N];
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      hits[i] = __ballot(key[i] != 0 && key[i] >= least);
+      total += __popcll(hits[i]);
+    }
+    if (total == 0) return;
     int at = 0;
-    if (lane == 0) at = atomicAdd(n, __popcll(hits));
-    at = __builtin_amdgcn_readfirstlane(at) + __popcll(hits & ((1ull << lane) - 1));
-    if (in && at < kFew) to[at] = key;
+    if (lane == 0) at = atomicAdd(n, total);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int mine = at + __popcll(hits[i] & ((1ull << lane) - 1));
+      if ((hits[i] >> lane & 1) && mine < kFew) to[mine] = key[i];
+      at += __popcll(hits[i]);
+    }
   };
   auto merge_lists = [&]() {
     lists[wave][lane] = list;
@@ -417,8 +433,9 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
   for (int w = 1; w < kWaves; w++) all = add(all, sums[w], sc);
   if (a.k > 0) {
     const uint64_t least = order_key(reach(), 0xFFFFFFFFu);
-    pick(lane < noted ? notes[wave][lane] : 0, least, marked, &count[0]);
-    pick(list, least, few, &count[1]);
+    uint64_t held[1] = {lane < noted ? notes[wave][lane] : 0}, listed[1] = {list};
+    pick(held, least, marked, &count[0]);
+    pick(listed, least, few, &count[1]);
     __syncthreads();
     if (count[0] <= kFew) {  // four lanes a note
       for (int i0 = 0; i0 < count[0]; i0 += 64) {
@@ -427,8 +444,7 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
         uint64_t kv[4];
 #pragma unroll
         for (int v = 0; v < 4; v++) kv[v] = i < count[0] ? key_at(at / 64, at % 64, 4 * (tid % 4) + v) : 0;
-#pragma unroll
-        for (int v = 0; v < 4; v++) pick(kv[v], least, few, &count[1]);
+        pick(kv, least, few, &count[1]);
       }
       __syncthreads();
     }
@@ -479,35 +495,42 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
           u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(i) + 16 + lane * 8, 0, kAgentScope));
       return ((uint64_t)o[1] << 32) | o[0];
     };
-    constexpr int U = 8;  // parts in flight
-    // What k keys reach: of the first 64 parts the ceil(k / r)-th largest of
-    // their r-th keys, r about twice what each part has of the k.
-    uint64_t least = 0;
-    if (a.k > 0) {
-      const int n = min(a.split, 64), r = min(2 * ((a.k + n - 1) / n), a.k);
-      const u32x2 o = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(min(lane, n - 1)) + 16 + (r - 1) * 8, 0, kAgentScope));
-      uint64_t head = lane < n ? ((uint64_t)o[1] << 32) | o[0] : 0;
-      sort64(head, lane, n);
-      least = __shfl((unsigned long long)head, (a.k + r - 1) / r - 1);
-    }
-    if (tid == 0) count[1] = 0;
-    __syncthreads();
-    for (int i0 = wave; i0 < a.split; i0 += kWaves * U) {
-      u32x4 v[U];
-      uint64_t o[U];
+    constexpr int U = 8;  // parts of a wave in flight
+    u32x4 v[U];
+    uint64_t o[U];
+    auto load_parts = [&](int i0) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int i = min(i0 + u * kWaves, a.split - 1);
         v[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, part_at(i), 0, kAgentScope));
         if (a.k > 0) o[u] = load_list(i);
       }
+    };
+    // What k keys reach: of the first 64 parts the ceil(k / r)-th largest of
+    // their r-th keys, r about twice what each part has of the k.
+    uint64_t least = 0, head = 0;
+    const int n = min(a.split, 64), r = min(2 * ((a.k + n - 1) / n), a.k);
+    if (a.k > 0) {
+      const u32x2 h = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(min(lane, n - 1)) + 16 + (r - 1) * 8, 0, kAgentScope));
+      head = lane < n ? ((uint64_t)h[1] << 32) | h[0] : 0;
+    }
+    load_parts(wave);
+    if (tid == 0) count[1] = 0;
+    if (a.k > 0) {
+      sort64(head, lane, n);
+      least = __shfl((unsigned long long)head, (a.k + r - 1) / r - 1);
+    }
+    __syncthreads();
+    for (int i0 = wave; i0 < a.split; i0 += kWaves * U) {
+      if (i0 != wave) load_parts(i0);
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        if (i0 + u * kWaves >= a.split) break;
-        mine = add(mine, Sums{__uint_as_float(v[u][0]), __uint_as_float(v[u][1]), __uint_as_float(v[u][2])}, sc);
-        if (a.k > 0) pick(o[u], least, few, &count[1]);
+        if (i0 + u * kWaves < a.split)
+          mine = add(mine, Sums{__uint_as_float(v[u][0]), __uint_as_float(v[u][1]), __uint_as_float(v[u][2])}, sc);
+        else o[u] = 0;
       }
+      if (a.k > 0) pick(o, least, few, &count[1]);
     }
     if (lane == 0) sums[wave] = mine;
     __syncthreads();
@@ -527,11 +550,15 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
   const bool bad = all.s != all.s, nothing = all.m == -INFINITY;
   const float ls = logf(all.s);
   auto logprob = [&](float x) -> float {
-    return bad ? NAN : x == -INFINITY ? -INFINITY : a.scale * (x - all.m) - ls;
+    return bad || x != x ? NAN : x == -INFINITY ? -INFINITY : a.scale * (x - all.m) - ls;
   };
   for (int j = tid; j < a.n_tok; j += 256) {
-    const int tok = a.tokens[t * a.n_tok + j];
-    a.given[t * a.n_tok + j] = tok >= 0 && tok < a.V ? logprob(load<XT>(row, tok)) : NAN;
+    float x = token_logit;
+    if (j >= 256) {
+      const int other = a.tokens[t * a.n_tok + j];
+      x = other >= 0 && other < a.V ? load<XT>(row, other) : NAN;
+    }
+    a.given[t * a.n_tok + j] = logprob(x);
   }
   if (tid == 0) a.entropy[t] = bad ? NAN : nothing ? 0.f : ls - kLn2 * (all.e / all.s);
   if (tid < a.k) {
