@@ -559,6 +559,134 @@ pub unsafe fn fused_moe_geglu_kernel(
     ))
 }
 
+/// Attention of one query token per sequence over a paged cache (`q`, `out`
+/// `[B, query heads, width]`, pools `[pages, kv heads, page, width]`, `table`
+/// `[B, n]` and `lengths` `[B]` int32).  `softcap` and `window` 0: none.
+///
+/// # Safety
+/// The views must describe device memory that is valid for the call's work on `stream`.
+pub unsafe fn paged_attention(
+    q: &ArrayView, k_pool: &ArrayView, v_pool: &ArrayView, table: &ArrayView, lengths: &ArrayView,
+    sinks: Option<&ArrayView>, scale: f32, softcap: f32, window: i32, out: &mut ArrayView, stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_paged_attention(
+        q.as_raw(), k_pool.as_raw(), v_pool.as_raw(), table.as_raw(), lengths.as_raw(), opt(sinks), scale, softcap,
+        window, out.as_raw_mut(), stream,
+    ))
+}
+
+/// The book of a paged cache: `table` `[rows, n]`, `lengths` `[rows]` and `refs`
+/// `[pages]`, int32, updated in place by the functions below.
+pub struct CacheBook<'a> {
+    pub table: &'a ArrayView,
+    pub lengths: &'a ArrayView,
+    pub refs: &'a ArrayView,
+}
+
+/// Pages for `counts[r]` more tokens of every row; `granted[r]` is 0 for a row that they do not hold.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn cache_reserve(
+    book: &CacheBook, counts: &ArrayView, page: i32, granted: &mut ArrayView, stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_cache_reserve(
+        book.table.as_raw(), book.lengths.as_raw(), book.refs.as_raw(), counts.as_raw(), page, granted.as_raw_mut(),
+        stream,
+    ))
+}
+
+/// Writes tokens' keys and values `[T, kv heads, width]` to their rows' pages.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn cache_append(
+    k: &ArrayView, v: &ArrayView, k_pool: &ArrayView, v_pool: &ArrayView, table: &ArrayView, positions: &ArrayView,
+    rows: &ArrayView, lengths: Option<&ArrayView>, stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_cache_append(
+        k.as_raw(), v.as_raw(), k_pool.as_raw(), v_pool.as_raw(), table.as_raw(), positions.as_raw(), rows.as_raw(),
+        opt(lengths), stream,
+    ))
+}
+
+fn raw_list(pools: &[&ArrayView]) -> Vec<*const sys::mlxq_array> {
+    pools.iter().map(|p| p.as_raw()).collect()
+}
+
+/// Makes the empty rows `dst[i]` copies of rows `src[i]`, sharing full pages.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn cache_fork(
+    pools: &[&ArrayView], book: &CacheBook, src: &ArrayView, dst: &ArrayView, granted: &mut ArrayView,
+    stream: *mut c_void,
+) -> Result<()> {
+    let p = raw_list(pools);
+    check(sys::mlxq_cache_fork(
+        p.len() as i32, p.as_ptr(), book.table.as_raw(), book.lengths.as_raw(), book.refs.as_raw(), src.as_raw(),
+        dst.as_raw(), granted.as_raw_mut(), stream,
+    ))
+}
+
+/// Empties rows.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn cache_free(book: &CacheBook, rows: &ArrayView, page: i32, stream: *mut c_void) -> Result<()> {
+    check(sys::mlxq_cache_free(
+        book.table.as_raw(), book.lengths.as_raw(), book.refs.as_raw(), rows.as_raw(), page, stream,
+    ))
+}
+
+/// Moves the held pages to the front of every pool; `live` `[1]` gets their number.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn cache_compact(
+    pools: &[&ArrayView], book: &CacheBook, live: &mut ArrayView, stream: *mut c_void,
+) -> Result<()> {
+    let p = raw_list(pools);
+    check(sys::mlxq_cache_compact(
+        p.len() as i32, p.as_ptr(), book.table.as_raw(), book.lengths.as_raw(), book.refs.as_raw(), live.as_raw_mut(),
+        stream,
+    ))
+}
+
+/// `h = x + scale * gate * post(y)`, `n = pre(h)`; `n` exactly where `pre_weight` is.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn residual_norm(
+    x: &ArrayView, y: &ArrayView, post_weight: Option<&ArrayView>, gate: Option<&ArrayView>, scale: f32,
+    pre_weight: Option<&ArrayView>, eps: f32, weight_offset: f32, h: &mut ArrayView, n: Option<&mut ArrayView>,
+    stream: *mut c_void,
+) -> Result<()> {
+    let n = n.map_or(std::ptr::null_mut(), |v| v.as_raw_mut());
+    check(sys::mlxq_residual_norm(
+        x.as_raw(), y.as_raw(), opt(post_weight), opt(gate), scale, opt(pre_weight), eps, weight_offset,
+        h.as_raw_mut(), n, stream,
+    ))
+}
+
+/// Log probabilities of `tokens` `[T, m]`, the entropy `[T]` and, where `top` is
+/// given, the most probable tokens (log probabilities and ids, `[T, k]`).
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn token_logprobs(
+    logits: &ArrayView, tokens: &ArrayView, scale: f32, logprobs: &mut ArrayView, entropy: &mut ArrayView,
+    top: Option<(i32, &mut ArrayView, &mut ArrayView)>, stream: *mut c_void,
+) -> Result<()> {
+    let (k, lp, ids) = match top {
+        Some((k, lp, ids)) => (k, lp.as_raw_mut(), ids.as_raw_mut()),
+        None => (0, std::ptr::null_mut(), std::ptr::null_mut()),
+    };
+    check(sys::mlxq_token_logprobs(
+        logits.as_raw(), tokens.as_raw(), k, scale, logprobs.as_raw_mut(), entropy.as_raw_mut(), lp, ids, stream,
+    ))
+}
+
 /// Grows `stream`'s workspace (so later calls, e.g. under graph capture,
 /// need not allocate).
 pub fn workspace_reserve(bytes: usize, stream: *mut c_void) -> Result<()> {
