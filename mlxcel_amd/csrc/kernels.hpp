@@ -585,7 +585,7 @@ struct PagedAttnArgs {
   int page_shift;
   int wgs, whole;          // workgroups; steps of a head that is not cut
   float* part;             // [2 wgs] partial results of part_words each
-  uint32_t* cnt;           // [2 wgs], zero between launches
+  uint32_t* cnt;           // [3 wgs], zero between launches
 };
 // Sets the plan; part_bytes of scratch are needed.  False where
 // the steps cannot be counted in 32 bits.

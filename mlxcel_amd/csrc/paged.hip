@@ -565,7 +565,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
           }
         };
         const int of = w1 - w0 + 1, mine = ((int)blockIdx.x - w0) / kJoin * kJoin, near = min(kJoin, of - mine);
-        if (last_of(a.cnt + w0 + mine, near)) {
+        // a workgroup may lead neighbours of a head that began before it and of its last one
+        if (last_of(a.cnt + 2 * (w0 + mine) + (mine == 0), near)) {
           for (int e = tid; e < heads * (DP / 4); e += 256) {
             const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
             float M, L;
@@ -575,7 +576,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
             else put(w0 + mine, e, M, L, acc);
           }
           const int groups = (of + kJoin - 1) / kJoin;
-          if (of > kJoin && last_of(a.cnt + a.wgs + w0, groups)) {
+          if (of > kJoin && last_of(a.cnt + 2 * a.wgs + w0, groups)) {
             for (int e = tid; e < heads * (DP / 4); e += 256) {
               const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
               float M, L;
@@ -649,7 +650,7 @@ bool paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
   if (a.B == 0) return hipSuccess;
-  if (a.D < 8 || a.D > 256 || a.D % 8 || a.pages < 1 || a.page < 1 || a.wgs < 1 || 2 * a.wgs > kSplitCounters)
+  if (a.D < 8 || a.D > 256 || a.D % 8 || a.pages < 1 || a.page < 1 || a.wgs < 1 || 3 * a.wgs > kSplitCounters)
     return hipErrorInvalidValue;
   return with_kernel(a, [&](auto xt, auto dp) { return launch<decltype(xt)::value, decltype(dp)::value>(a, stream); });
 }

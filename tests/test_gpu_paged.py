@@ -104,6 +104,17 @@ def test_one_long_sequence_of_each_split():
         check(c, query(1, 2, 64, "bf16", n + 1))
 
 
+@pytest.mark.parametrize("length", [2176, 4224, 4352, 8448, 16896])
+def test_cut_heads_that_share_a_workgroup(length):
+    """Heads of 17, 33, .. workgroups whose last one starts the next cut head."""
+    announce("paged shared workgroups", length)
+    B = max(2, 40 * 4224 // length // 2)
+    c = Cache([length] * B, 2, 64, 16, "bf16", length)
+    q = query(B, 2, 64, "bf16", length + 1)
+    for _ in range(2):
+        check(c, q)
+
+
 def test_large_scores_and_one_winner():
     announce("paged large")
     c = Cache([200], 1, 64, 16, "f32", 21)
