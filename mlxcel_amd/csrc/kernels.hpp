@@ -583,7 +583,7 @@ struct PagedAttnArgs {
   // how the keys are split (paged_attention_plan)
   uint32_t page_mul;       // key / page = key * page_mul >> page_shift
   int page_shift;
-  int wgs, whole;          // workgroups; steps of a head that is not cut
+  int wgs;                 // workgroups
   float* part;             // [2 wgs] partial results of part_words each
   uint32_t* cnt;           // [3 wgs], zero between launches
 };

@@ -10,17 +10,18 @@
 // far under the matrix rate).
 //
 // The work is cut evenly whatever the lengths: with a sequence's keys counted
-// in steps of 64 for each key head (and each 16 of its query heads), workgroup w
-// takes steps [w n, (w + 1) n) of them all.  The lengths are on the device, so
-// each workgroup finds its first step from a scan over them.  A sequence's head
-// that crosses a workgroup's end leaves its sum, maximum and output so far in
-// scratch; the last of its workgroups to arrive joins them, in the order of the
-// keys, so the result does not depend on who came last.
+// in steps of 128 (of 64 with wide 32-bit heads) for each key head and each 16 of
+// its query heads, and two more for what a head's start and end cost, workgroup w
+// takes [w n, (w + 1) n) of them all.  The lengths are on the device, so each
+// workgroup finds its first step from a scan over them.  A sequence's head that
+// crosses a workgroup's end leaves its sum, maximum and output so far in scratch;
+// the last of its workgroups to arrive joins them, in the order of the keys, so
+// the result does not depend on who came last.
 //
-// In a step each wave takes 16 keys, with a running maximum and sum of its own;
-// the waves are joined in LDS at a head's end.  The next 16 keys are loaded
+// In a step each wave takes 32 (16) keys, with a running maximum and sum of its
+// own; the waves are joined in LDS at a head's end.  Its next keys are loaded
 // right after the product that used up these ones' registers, and their page
-// numbers one step before that, so a wave keeps 4 to 8 KiB in flight (D = 128,
+// numbers one step before that, so a wave keeps 8 to 16 KiB in flight (D = 128,
 // 16 bits).  Both products run on MFMA with the layouts chosen so that nothing
 // moves between them:
 //   S^T[key][head] = K Q^T: lane (c, g) = (lane % 16, lane / 16) loads 16 bytes
@@ -127,6 +128,15 @@ __device__ __forceinline__ int steps_of(int len, int64_t cap, int window, int& l
   return (hi - lo + KEYS - 1) / KEYS;
 }
 
+// Steps of a head that is not cut: taking them one after the other costs about
+// what a join costs (one sequence of 1000 keys, 8 steps a head: 11.1 us cut, 24.8
+// whole; 200 sequences of 1 to 4 steps: 15.5 us whole, 16.5 cut at every step).
+constexpr int kWholeSteps = 4;
+
+// What a head's start and end cost, in steps: with 0 32 ragged sequences took
+// 45.8 us, with 2 42.0, with 4 44.9 (16 ragged ones of width 256 44.6, 36.5, 39.7).
+constexpr int kAround = 2;
+
 constexpr int64_t kLastCache = (int64_t)256 << 20;
 
 // Workgroups whose results one of them joins, and how many are read at a time.
@@ -147,19 +157,23 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   const int64_t cap = (int64_t)a.width * a.page;
   const int heads_b = a.Hkv * tiles_h;  // (key head, 16 query heads) of a sequence
 
-  // Where this workgroup's steps begin and end: step among all, step in its
+  // Where this workgroup's units begin and end: unit among all, unit in its
   // sequence, sequence, its length.
   struct Bound {
-    int step, off, b, len;
+    int unit, off, b, len;
   };
   auto steps_in = [&](int len) {
     int lo, hi;
     return steps_of<G::KEYS>(len, cap, a.window, lo, hi);
   };
-  // Step p, `off` into sequence b, unless it cuts a head of few steps: that one
+  auto units_in = [&](int len) {  // of one head
+    const int s = steps_in(len);
+    return s ? kAround + s : 0;
+  };
+  // Unit p, `off` into sequence b, unless it cuts a head of few steps: that one
   // belongs to the workgroup of its first step.
   auto bound_at = [&](int p, int off, int b, int len) -> Bound {
-    const int s = steps_in(len), up = s <= a.whole && off % s ? s - off % s : 0;
+    const int u = units_in(len), up = steps_in(len) <= kWholeSteps && off % u > kAround ? u - off % u : 0;
     return Bound{p + up, off + up, b, len};
   };
   auto clear = [&](int b) {  // a sequence without keys has no steps: its output is zeros
@@ -168,7 +182,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   int n, total;
   Bound first, last;
   if (a.B <= 64) {  // each wave finds them by itself, sequence i in lane i
-    const int len = lane < a.B ? a.lengths[lane] : 0, steps = steps_in(len), mine = heads_b * steps;
+    const int len = lane < a.B ? a.lengths[lane] : 0, units = units_in(len), mine = heads_b * units;
     int sum = mine;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -184,14 +198,14 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     };
     first = find(blockIdx.x * n);
     last = find((blockIdx.x + 1) * n);
-    for (uint64_t none = __ballot(lane < a.B && steps == 0); none; none &= none - 1)
+    for (uint64_t none = __ballot(lane < a.B && units == 0); none; none &= none - 1)
       if (__builtin_ctzll(none) % a.wgs == (int)blockIdx.x) clear(__builtin_ctzll(none));
   } else {  // thread i sums those of its share
     __shared__ int scan[kWaves];
     __shared__ Bound bound[2];
     const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
     int mine = 0;
-    for (int b = b0; b < b1; b++) mine += heads_b * steps_in(a.lengths[b]);
+    for (int b = b0; b < b1; b++) mine += heads_b * units_in(a.lengths[b]);
     int sum = mine;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -215,7 +229,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
         if (tid == 0) bound[i] = Bound{total, 0, 0, 0};
       } else if (before <= p && p < before + mine) {
         int off = p - before, b = b0;
-        while (off >= heads_b * steps_in(a.lengths[b])) off -= heads_b * steps_in(a.lengths[b++]);
+        while (b + 1 < b1 && off >= heads_b * units_in(a.lengths[b])) off -= heads_b * units_in(a.lengths[b++]);
         bound[i] = bound_at(p, off, b, a.lengths[b]);
       }
     }
@@ -225,15 +239,16 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
     first = bound[0];
     last = bound[1];
   }
-  int at = __builtin_amdgcn_readfirstlane(first.step);
-  const int end = __builtin_amdgcn_readfirstlane(last.step);
+  int at = __builtin_amdgcn_readfirstlane(first.unit);
+  const int end = __builtin_amdgcn_readfirstlane(last.unit);
   if (at >= end) return;
   int off = __builtin_amdgcn_readfirstlane(first.off), b = __builtin_amdgcn_readfirstlane(first.b);
   int len = __builtin_amdgcn_readfirstlane(first.len);
   // More keys and values than the last cache holds beside others' are not kept
   // there for the next call: 2.1 GB 360 -> 325 us, 174 MB among other work 46 -> 44.5 us
   // (read again and again by itself 37 -> 44 us).
-  const bool once = (int64_t)total * (G::KEYS * 2 * G::ES) * a.D > kLastCache / 2;
+  const bool once =
+      ((int64_t)total - (int64_t)kAround * heads_b * a.B) * (G::KEYS * 2 * G::ES) * a.D > kLastCache / 2;
   // scores in units of log2 e
   const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
   const int slot_words = part_words(min(per, 16), DP);
@@ -242,13 +257,18 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   auto run = [&](auto ONCE) {
     while (at < end) {
       int lo, hi;
-      const int steps = steps_of<G::KEYS>(len, cap, a.window, lo, hi);
-      if (off >= steps * heads_b) {
-        len = __builtin_amdgcn_readfirstlane(a.lengths[++b]);
+      const int steps = steps_of<G::KEYS>(len, cap, a.window, lo, hi), units = units_in(len);
+      if (off >= units * heads_b) {
+        if (++b >= a.B) break;
+        len = __builtin_amdgcn_readfirstlane(a.lengths[b]);
         off = 0;
         continue;
       }
-      const int hh = off / steps, s0 = off - hh * steps, s1 = min(steps, s0 + (end - at));
+      const int hh = off / units, skip = max(kAround - (off - hh * units), 0);
+      if (at + skip >= end) break;  // its steps begin in the next workgroup
+      at += skip;
+      off += skip;
+      const int s0 = off - hh * units - kAround, s1 = min(steps, s0 + (end - at));
       const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
       const int heads = min(16, per - 16 * ht), head0 = hk * per + 16 * ht;
 
@@ -432,7 +452,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
               for (int i = 0; i < G::NB; i++)
 #pragma unroll
                 for (int j = 0; j < G::VE; j++)
-                  o[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][r][i][j]), s[t][r], o[i][j], 0, 0, 0);
+                  o[i][j] =
+                      __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][r][i][j]), s[t][r], o[i][j], 0, 0, 0);
         } else {
           // P = ph + pl
           u32x4 ph, pl;
@@ -477,7 +498,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
             if (d < DP) {
 #pragma unroll
               for (int j = 0; j < G::VE; j += 4)
-                *reinterpret_cast<f32x4*>(row + d + j) = f32x4{o[i][j][r], o[i][j + 1][r], o[i][j + 2][r], o[i][j + 3][r]};
+                *reinterpret_cast<f32x4*>(row + d + j) =
+                    f32x4{o[i][j][r], o[i][j + 1][r], o[i][j + 2][r], o[i][j + 3][r]};
             }
           }
         if (g == 0) {
@@ -486,8 +508,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
         }
       }
       __syncthreads();
-      const int u0 = at - s0;  // the head's first step among all
-      const int w0 = u0 / n, w1 = steps <= a.whole ? w0 : (u0 + steps - 1) / n;
+      const int w0 = (at - s0) / n, w1 = steps <= kWholeSteps ? w0 : (at - s0 + steps - 1) / n;
       // bytes of a workgroup's partial result: of its last head (slot 1), or of one that began before it (slot 0)
       auto part_at = [&](int w) -> uint32_t { return (uint32_t)((2 * w + (w == w0)) * slot_words) * 4u; };
       auto put = [&](int w, int e, float M, float L, f32x4 acc) {
@@ -622,11 +643,6 @@ auto with_kernel(const PagedAttnArgs& a, F&& f) {
 
 }  // namespace
 
-// Steps of a head that is not cut: taking them one after the other costs about
-// what a join costs (one sequence of 1000 keys, 8 steps a head: 11.1 us cut, 24.8
-// whole; 200 sequences of 1 to 4 steps: 15.5 us whole, 16.5 cut at every step).
-constexpr int kWholeSteps = 4;
-
 bool paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
   a.page_shift = 30;
   while (((int64_t)1 << (a.page_shift - 30)) < a.page) a.page_shift++;
@@ -640,12 +656,11 @@ bool paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
     resident = Geo<decltype(xt)::value, decltype(dp)::value>::WGS;
     return 0;
   });
-  const int64_t most = (int64_t)a.B * a.Hkv * ((per + 15) / 16) * ((keys + step - 1) / step);
-  a.whole = kWholeSteps;
+  const int64_t heads = (int64_t)a.B * a.Hkv * ((per + 15) / 16), most = heads * ((keys + step - 1) / step);
   a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)cus * resident));
   const int words = with_kernel(a, [&](auto, auto dp) { return part_words(std::min(per, 16), decltype(dp)::value); });
   *part_bytes = (int64_t)2 * a.wgs * words * 4;
-  return most <= (1 << 30);
+  return most + kAround * heads <= (1 << 30);
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
