@@ -377,7 +377,7 @@ mlxq_status mlxq_cache_reserve(const mlxq_array* table, const mlxq_array* length
  * where the table has position positions[t] of row rows[t] (int32).  Tokens
  * with a row, position or page out of range are left out, and, where lengths
  * is not NULL, tokens at or past their row's length (of rows that were not
- * granted their pages). */
+ * granted their pages).  Of two tokens for one place either may stay. */
 mlxq_status mlxq_cache_append(const mlxq_array* k, const mlxq_array* v, const mlxq_array* k_pool,
                               const mlxq_array* v_pool, const mlxq_array* table,
                               const mlxq_array* positions, const mlxq_array* rows,
@@ -388,7 +388,7 @@ mlxq_status mlxq_cache_append(const mlxq_array* k, const mlxq_array* v, const ml
  * free page in each of the n pools.  Pairs are served in order; sources are
  * read as they were before the call.  granted[i] (int32) is 0 where dst[i] is
  * not empty or an earlier pair's too, no page is free for the copy, or a row
- * is out of range.  Pools of one shape and type, each page dense. */
+ * is out of range.  Pools of one shape and (any) type, each page dense. */
 mlxq_status mlxq_cache_fork(int32_t n, const mlxq_array* const* pools, const mlxq_array* table,
                             const mlxq_array* lengths, const mlxq_array* refs,
                             const mlxq_array* src, const mlxq_array* dst, mlxq_array* granted,

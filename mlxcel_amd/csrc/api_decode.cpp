@@ -95,6 +95,7 @@ CacheBook book(const mlxq_array* table, const mlxq_array* lengths, const mlxq_ar
   if (l.dim(0) != t.dim(0))
     (Refusal(tag) << "table and lengths must have as many rows but have shapes " << fmt_shape(t.shape()) << " and "
                   << fmt_shape(l.shape()) << ".").invalid();
+  if (r.dim(0) > (1 << 30)) (Refusal(tag) << "refs has too many pages (" << r.dim(0) << ").").unsupported();
   if (page < 1) (Refusal(tag) << "a page must hold at least one token but holds " << page << ".").invalid();
   check_capacity(t.dim(1), page, tag);
   CacheBook b{};
@@ -440,6 +441,7 @@ mlxq_status mlxq_residual_norm(const mlxq_array* x, const mlxq_array* y, const m
       // over the last of the axes before it (one gate a batch entry).
       View g = operand(gate, tag, "gate", -1, xv.dtype());
       gc = *gate;
+      if (g.ndim() < 1) (Refusal(tag) << "gate must have at least one dimension.").invalid();
       if (g.ndim() > xv.ndim()) (Refusal(tag) << "gate has more dimensions than x.").invalid();
       Shape gs = g.shape();
       while ((int)gs.size() < xv.ndim()) gs.insert(gs.begin(), 1);

@@ -61,10 +61,10 @@ __device__ __forceinline__ int pages_of(int64_t tokens, int page) { return (int)
 // refs of pages 4 tid .. 4 tid + 3 of the block from `at` on (past the end: held)
 __device__ __forceinline__ i32x4_e load_refs(const int32_t* refs, int pages, int at) {
   const int p = at + 4 * (int)threadIdx.x;
-  if (p + 4 <= pages) return *reinterpret_cast<const i32x4_e*>(refs + p);
+  if (p <= pages - 4) return *reinterpret_cast<const i32x4_e*>(refs + p);
   i32x4_e r;
 #pragma unroll
-  for (int e = 0; e < 4; e++) r[e] = p + e < pages ? refs[p + e] : 1;
+  for (int e = 0; e < 4; e++) r[e] = p < pages - e ? refs[p + e] : 1;
   return r;
 }
 
@@ -74,13 +74,14 @@ struct FreeList {
   const int32_t* refs;
   int pages;
   int32_t *near, *far;
-  i32x4_e block;  // refs at `at`, already on their way
+  i32x4_e block;  // refs at `at`, on their way
   int at = 0;
   int have = 0;
   __device__ __forceinline__ int32_t get(int i) const { return i < kNear ? near[i] : far[i]; }
   // until there are `want` or refs is at its end
   __device__ void extend(int64_t want, Scan<int>& scan) {
     while (have < want && at < pages) {
+      const i32x4_e next = load_refs(refs, pages, at + kBlock);
       int n = 0, total;
 #pragma unroll
       for (int e = 0; e < 4; e++) n += block[e] == 0;
@@ -93,7 +94,7 @@ struct FreeList {
         }
       have += total;
       at += kBlock;
-      if (have < want && at < pages) block = load_refs(refs, pages, at);
+      block = next;
     }
     __syncthreads();  // the list's new entries are read by other threads
   }
@@ -338,19 +339,24 @@ __global__ __launch_bounds__(kPlanThreads) void cache_compact_plan_kernel(const 
   __shared__ int sums[2][kPlanWaves];
   const int tid = threadIdx.x;
   Scan<int> scan{sums};
-  const i32x4_e block = load_refs(b.refs, b.pages, 0);
+  i32x4_e block = load_refs(b.refs, b.pages, 0);
   auto held_at = [&](const i32x4_e& r, int at, int e) { return at + 4 * tid + e < b.pages && r[e] > 0; };
   int live = 0, n;
-  for (int at = 0; at < b.pages; at += kBlock) {
-    const i32x4_e r = at ? load_refs(b.refs, b.pages, at) : block;
+  for (int at = 0; at < b.pages; at += 4 * kBlock) {  // four blocks on their way
+    i32x4_e r[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) live += held_at(r, at, e);
+    for (int k = 0; k < 4; k++) r[k] = load_refs(b.refs, b.pages, at + k * kBlock);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) live += held_at(r[k], at + k * kBlock, e);
   }
   scan(live, n);
   // holes are the free pages below n, movers the held ones from n on: as many
   int nh = 0, nm = 0;
   for (int at = 0; at < b.pages; at += kBlock) {
-    const i32x4_e r = at ? load_refs(b.refs, b.pages, at) : block;
+    const i32x4_e r = block;
+    block = load_refs(b.refs, b.pages, at + kBlock);
     const int p = at + 4 * tid;
     int mine = 0, total;  // holes and movers, 16 bits each
 #pragma unroll
@@ -407,11 +413,15 @@ __global__ __launch_bounds__(256) void cache_compact_copy_kernel(const CacheBook
   }
 }
 
-// 16-byte words where every page of every pool allows them
-bool wide(const PoolList& p) {
+// The widest of 16-, 2- and 1-byte words that every page of every pool allows:
+// f(word).
+template <typename F>
+void with_word(const PoolList& p, F&& f) {
   uintptr_t v = (uintptr_t)p.bytes | (uintptr_t)p.stride;
   for (int i = 0; i < p.n; i++) v |= reinterpret_cast<uintptr_t>(p.base[i]);
-  return (v & 15) == 0;
+  if ((v & 15) == 0) f(u32x4{});
+  else if ((v & 1) == 0) f(uint16_t{});
+  else f(uint8_t{});
 }
 
 }  // namespace
@@ -457,10 +467,10 @@ hipError_t launch_cache_fork_copy(const CacheBook& b, const int32_t* src, const 
   if ((int64_t)n * columns > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid((unsigned)(n * columns)), block(256);
   const int32_t* pair = scratch + b.pages;
-  if (wide(pools))
-    hipLaunchKernelGGL(cache_fork_copy_kernel<u32x4>, grid, block, 0, stream, b, src, dst, pair, pools, columns, book);
-  else
-    hipLaunchKernelGGL(cache_fork_copy_kernel<uint16_t>, grid, block, 0, stream, b, src, dst, pair, pools, columns, book);
+  with_word(pools, [&](auto w) {
+    hipLaunchKernelGGL(cache_fork_copy_kernel<decltype(w)>, grid, block, 0, stream, b, src, dst, pair, pools, columns,
+                       book);
+  });
   return hipGetLastError();
 }
 
@@ -485,12 +495,10 @@ hipError_t launch_cache_compact_copy(const CacheBook& b, const int32_t* scratch,
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   const int32_t* to = scratch + 16;
   const int32_t *holes = to + b.pages, *movers = to + 2 * (int64_t)b.pages;
-  if (wide(pools))
-    hipLaunchKernelGGL(cache_compact_copy_kernel<u32x4>, dim3((unsigned)grid), dim3(256), 0, stream, b, scratch, to,
+  with_word(pools, [&](auto w) {
+    hipLaunchKernelGGL(cache_compact_copy_kernel<decltype(w)>, dim3((unsigned)grid), dim3(256), 0, stream, b, scratch, to,
                        holes, movers, pools, wgs);
-  else
-    hipLaunchKernelGGL(cache_compact_copy_kernel<uint16_t>, dim3((unsigned)grid), dim3(256), 0, stream, b, scratch, to,
-                       holes, movers, pools, wgs);
+  });
   return hipGetLastError();
 }
 

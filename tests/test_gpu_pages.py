@@ -153,6 +153,32 @@ def test_fork(dtype, D, turned, pools):
     b.equal("compact")
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.float64])
+@pytest.mark.parametrize("D", [16, 5])
+def test_pools_of_any_element(dtype, D):
+    """Pages of odd sizes in bytes are moved whole."""
+    announce("pools of", dtype, D)
+    b = Book(30, 6, 80, 3, D, fill=0.6, pools=0, most=15)
+    b.host = [np.random.default_rng(i).integers(0, 200, (80, 1, 3, D)).astype(np.float32) for i in range(3)]
+    b.dev_pools = [torch.from_numpy(h).to(dtype).cuda() for h in b.host]
+    held, empty = np.flatnonzero(b.lengths), np.flatnonzero(b.lengths == 0)
+    b.fork(np.resize(held, len(empty)), empty)
+    b.equal("fork")
+    b.free(held[::2])
+    b.compact()
+    b.equal("compact")
+
+
+def test_many_pages():
+    announce("many pages")
+    b = Book(300, 90, 60001, 4, 37, fill=0.99, pools=1, Hkv=1, D=2)
+    b.reserve(np.random.default_rng(1).integers(0, 300, 300))
+    b.equal("reserve")
+    b.free(np.arange(0, 300, 2))
+    b.compact()
+    b.equal("compact")
+
+
 def test_fork_refusals():
     announce("fork refusals")
     b = Book(12, 6, 24, 4, 11, fill=0.75, most=14)

@@ -87,6 +87,7 @@ BOOK = [have((4, 6), I32), have((4,), I32), have((20,), I32)]
     ([*BOOK, have((4,), I32), 0, have((4,), I32)], EINVAL, "at least one token"),
     ([*BOOK, have((4,), I32), 1 << 28, have((4,), I32)], EUNSUPPORTED, "too wide"),
     ([*BOOK, have((4,), I32), 16, have((4,), F32)], EINVAL, "granted must be int32"),
+    ([BOOK[0], BOOK[1], have(((1 << 30) + 1,), I32), have((4,), I32), 16, have((4,), I32)], EUNSUPPORTED, "too many pages"),
     ([BOOK[0], have((5,), I32), BOOK[2], have((4,), I32), 16, have((4,), I32)], EINVAL, "as many rows"),
 ])
 def test_cache_reserve(lib, args, code, text):
@@ -152,6 +153,7 @@ NORM = dict(x=((3, 8), BF), y=((3, 8), BF), post=None, gate=None, scale=1.0, pre
     (dict(pre=((8,), F16)), EINVAL, "or float32"),
     (dict(pre=None), EINVAL, "n is given"),
     (dict(n=None), EINVAL, "n is given"),
+    (dict(gate=((), BF)), EINVAL, "at least one dimension"),
     (dict(gate=((2, 8), BF)), EINVAL, "does not broadcast"),
     (dict(gate=((3, 2), BF)), EINVAL, "does not broadcast"),
     (dict(gate=((1, 3, 8), BF)), EINVAL, "more dimensions"),
