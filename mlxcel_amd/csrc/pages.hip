@@ -212,8 +212,11 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const CacheAppendArgs
 
 // ---- copies of pages -----------------------------------------------------------
 
-// One page by one workgroup, four words a thread on their way.
-template <typename W>
+// One page by one workgroup, four words a thread on their way.  What is written
+// is not kept in the caches, nor, where it is copied ONCE, what is read: fork of
+// 4 into 32 over 72 pools 30.9 -> 27.7 us (36.6 with both), compact of 16 pools
+// 71.4 -> 66.3 us (inputs in turn).
+template <bool ONCE, typename W>
 __device__ __forceinline__ void copy_page(char* base, int64_t stride, int64_t bytes, int from, int to) {
   const W* s = reinterpret_cast<const W*>(base + from * stride);
   W* d = reinterpret_cast<W*>(base + to * stride);
@@ -222,9 +225,9 @@ __device__ __forceinline__ void copy_page(char* base, int64_t stride, int64_t by
   for (; i + 3 * 256 < n; i += 4 * 256) {
     W v[4];
 #pragma unroll
-    for (int u = 0; u < 4; u++) v[u] = s[i + u * 256];
+    for (int u = 0; u < 4; u++) v[u] = ONCE ? __builtin_nontemporal_load(s + i + u * 256) : s[i + u * 256];
 #pragma unroll
-    for (int u = 0; u < 4; u++) d[i + u * 256] = v[u];
+    for (int u = 0; u < 4; u++) __builtin_nontemporal_store(v[u], d + i + u * 256);
   }
   for (; i < n; i += 256) d[i] = s[i];
 }
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(256) void cache_fork_copy_kernel(const CacheBook b,
   if (fresh < 0) return;
   const int old = from[full];
   if (old < 0 || old >= b.pages) return;
-  copy_page<W>(pools.base[q], pools.stride, pools.bytes, old, fresh);
+  copy_page<false, W>(pools.base[q], pools.stride, pools.bytes, old, fresh);
 }
 
 // ---- free ------------------------------------------------------------------------
@@ -409,7 +412,7 @@ __global__ __launch_bounds__(256) void cache_compact_copy_kernel(const CacheBook
   const int64_t n = (int64_t)moves[0] * pools.n;
   for (int64_t i = blockIdx.x; i < n; i += movers_wgs) {
     const int m = (int)(i / pools.n), q = (int)(i - (int64_t)m * pools.n);
-    copy_page<W>(pools.base[q], pools.stride, pools.bytes, movers[m], holes[m]);
+    copy_page<true, W>(pools.base[q], pools.stride, pools.bytes, movers[m], holes[m]);
   }
 }
 
