@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -183,7 +184,8 @@ __device__ __forceinline__ Sums wave_sums(Sums v, float a, int lane) {
   return Sums{M, sum(v.s), sum(v.e)};
 }
 
-template <int XT>
+// ONCE: the logits are not kept in the caches.
+template <int XT, bool ONCE>
 __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArgs a) {
   constexpr int PER = XT == GEN_F32 ? 4 : 8;  // values of a 16-byte load
   constexpr int NL = 16 / PER;                // loads of a lane and chunk
@@ -232,7 +234,8 @@ __global__ __launch_bounds__(256, 4) void token_logprobs_kernel(const LogprobArg
       const char* p = row + ((int64_t)start(c) + lane * PER) * (16 / PER);
 #pragma unroll
       for (int j = 0; j < NL; j++) {
-        const u32x4_e v = *reinterpret_cast<const u32x4_e*>(p + j * 1024);
+        const u32x4_e* q = reinterpret_cast<const u32x4_e*>(p + j * 1024);
+        const u32x4_e v = ONCE ? __builtin_nontemporal_load(q) : *q;
         w[j] = u32x4{v[0], v[1], v[2], v[3]};
       }
       return;
@@ -582,9 +585,17 @@ hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream) {
       a.T * a.split > 0x7FFFFFFF)
     return hipErrorInvalidValue;
   const dim3 grid((unsigned)(a.T * a.split)), block(256);
-  if (a.type == GEN_BF16) hipLaunchKernelGGL(token_logprobs_kernel<GEN_BF16>, grid, block, 0, stream, a);
-  else if (a.type == GEN_F16) hipLaunchKernelGGL(token_logprobs_kernel<GEN_F16>, grid, block, 0, stream, a);
-  else hipLaunchKernelGGL(token_logprobs_kernel<GEN_F32>, grid, block, 0, stream, a);
+  // more logits than the caches would still hold for the next reader are not
+  // kept there: 300 x 151936 float32 43.4 -> 40.5 us, bfloat16 (91 MB) 37.3 and 37.7
+  const bool once = a.T * a.V * (a.type == GEN_F32 ? 4 : 2) > ((int64_t)128 << 20);
+  auto run = [&](auto xt) {
+    constexpr int XT = decltype(xt)::value;
+    if (once) hipLaunchKernelGGL((token_logprobs_kernel<XT, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((token_logprobs_kernel<XT, false>), grid, block, 0, stream, a);
+  };
+  if (a.type == GEN_BF16) run(std::integral_constant<int, GEN_BF16>{});
+  else if (a.type == GEN_F16) run(std::integral_constant<int, GEN_F16>{});
+  else run(std::integral_constant<int, GEN_F32>{});
   return hipGetLastError();
 }
 
