@@ -584,7 +584,7 @@ struct PagedAttnArgs {
   uint32_t page_mul;       // key / page = key * page_mul >> page_shift
   int page_shift;
   int wgs;                 // workgroups
-  float* part;             // [2 wgs] partial results of part_words each
+  float* part;             // [4 wgs] partial results of part_words each
   uint32_t* cnt;           // [3 wgs], zero between launches
 };
 // Sets the plan; part_bytes of scratch are needed.  False where

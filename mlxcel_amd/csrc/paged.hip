@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
   // scores in units of log2 e
   const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
   const int slot_words = part_words(min(per, 16), DP);
-  const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)2 * a.wgs * slot_words * 4));
+  const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)4 * a.wgs * slot_words * 4));
 
   auto run = [&](auto ONCE) {
     while (at < end) {
@@ -511,8 +511,9 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
       const int w0 = (at - s0) / n, w1 = steps <= kWholeSteps ? w0 : (at - s0 + steps - 1) / n;
       // bytes of a workgroup's partial result: of its last head (slot 1), or of one that began before it (slot 0)
       auto part_at = [&](int w) -> uint32_t { return (uint32_t)((2 * w + (w == w0)) * slot_words) * 4u; };
-      auto put = [&](int w, int e, float M, float L, f32x4 acc) {
-        const uint32_t p = part_at(w);
+      // and of the neighbours that it leads, in a place of its own: others of the joining threads may still read the first
+      const uint32_t joined = (uint32_t)(2 * a.wgs * slot_words) * 4u;
+      auto put = [&](uint32_t p, int e, float M, float L, f32x4 acc) {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + e * 16, 0, kAgentScope);
         if (e % (DP / 4) == 0)
           __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
         if (w0 == w1) {
           finish(h, d, M, L, acc);
         } else {
-          put(blockIdx.x, e, M, L, acc);
+          put(part_at(blockIdx.x), e, M, L, acc);
         }
       }
       if (w0 != w1) {
@@ -560,8 +561,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
           __syncthreads();
           return arrived != 0;
         };
-        // sum of the results of workgroups w, w + by, .. (of them), in the order of the keys
-        auto join = [&](int w, int by, int of, int e, float& M, float& L, f32x4& acc) {
+        // sum of the results, from byte `from` on, of workgroups w, w + by, .. (of them), in the order of the keys
+        auto join = [&](uint32_t from, int w, int by, int of, int e, float& M, float& L, f32x4& acc) {
           const int h = e / (DP / 4);
           M = -INFINITY, L = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
           for (int i0 = 0; i0 < of; i0 += kFlight) {
@@ -569,7 +570,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
             u32x2 mw[kFlight];
 #pragma unroll
             for (int i = 0; i < kFlight; i++) {
-              const uint32_t p = part_at(w + by * min(i0 + i, of - 1));
+              const uint32_t p = from + part_at(w + by * min(i0 + i, of - 1));
               mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + (heads * DP + 2 * h) * 4,
                                                                                      0, kAgentScope));
               ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + e * 16, 0, kAgentScope));
@@ -592,9 +593,9 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
             const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
             float M, L;
             f32x4 acc;
-            join(w0 + mine, 1, near, e, M, L, acc);
+            join(0, w0 + mine, 1, near, e, M, L, acc);
             if (of <= kJoin) finish(h, d, M, L, acc);
-            else put(w0 + mine, e, M, L, acc);
+            else put(joined + part_at(w0 + mine), e, M, L, acc);
           }
           const int groups = (of + kJoin - 1) / kJoin;
           if (of > kJoin && last_of(a.cnt + 2 * a.wgs + w0, groups)) {
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
               const int h = e / (DP / 4), d = 4 * (e - h * (DP / 4));
               float M, L;
               f32x4 acc;
-              join(w0, kJoin, groups, e, M, L, acc);
+              join(joined, w0, kJoin, groups, e, M, L, acc);
               finish(h, d, M, L, acc);
             }
           }
@@ -659,7 +660,7 @@ bool paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* part_bytes) {
   const int64_t heads = (int64_t)a.B * a.Hkv * ((per + 15) / 16), most = heads * ((keys + step - 1) / step);
   a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)cus * resident));
   const int words = with_kernel(a, [&](auto, auto dp) { return part_words(std::min(per, 16), decltype(dp)::value); });
-  *part_bytes = (int64_t)2 * a.wgs * words * 4;
+  *part_bytes = (int64_t)4 * a.wgs * words * 4;
   return most + kAround * heads <= (1 << 30);
 }
 

@@ -104,6 +104,19 @@ def test_one_long_sequence_of_each_split():
         check(c, query(1, 2, 64, "bf16", n + 1))
 
 
+@pytest.mark.parametrize("dtype,D,Hq", [("bf16", 80, 5), ("f16", 96, 16), ("bf16", 192, 16), ("f32", 72, 16),
+                                        ("f32", 192, 7), ("f32", 256, 16), ("bf16", 256, 40)])
+def test_many_joined_parts(dtype, D, Hq):
+    """One key head of 40000 keys over more than 16 workgroups, whose results
+    are joined in two levels, at widths where a head's columns span waves."""
+    announce("paged joined", dtype, D)
+    c = Cache([40000], 1, D, 64, dtype, D)
+    q = query(1, Hq, D, dtype, D + 1)
+    first = check(c, q)
+    for _ in range(5):
+        assert torch.equal(mq.paged_attention(q, c.k, c.v, i32(c.table), i32(c.lengths)), first)
+
+
 @pytest.mark.parametrize("length", [2176, 4224, 4352, 8448, 16896])
 def test_cut_heads_that_share_a_workgroup(length):
     """Heads of 17, 33, .. workgroups whose last one starts the next cut head."""
