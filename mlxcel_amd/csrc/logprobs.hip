@@ -32,6 +32,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "wave.hpp"
 
 namespace mlxq {
 
@@ -68,23 +69,6 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 
 // ---- sorted lists of 64 keys, one a lane --------------------------------------
 
-// The value of the lane whose number differs in bit J: vector operations only
-// (4 is 3 then 7; halves and rows of 16 are swapped between two registers).
-template <int J>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int lane) {
-  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);
-  else if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
-  else if constexpr (J == 4)
-    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x1B, 0xF, 0xF, false), 0x141, 0xF, 0xF, false);
-  else if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, false);
-  else if constexpr (J == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return lane & 16 ? r[0] : r[1];
-  } else {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return lane & 32 ? r[0] : r[1];
-  }
-}
 template <int J>
 __device__ __forceinline__ uint64_t lane_xor64(uint64_t v, int lane) {
   return ((uint64_t)lane_xor<J>((uint32_t)(v >> 32), lane) << 32) | lane_xor<J>((uint32_t)v, lane);
@@ -115,7 +99,7 @@ __device__ __forceinline__ void sort64(uint64_t& v, int lane, int n) {
 // Largest first.
 template <int SIZE, int J>
 __device__ __forceinline__ void bitonic_values(float& v, int lane) {
-  const float o = __uint_as_float(lane_xor<J>(__float_as_uint(v), lane));
+  const float o = lane_xor<J>(v, lane);
   v = ((lane & J) == 0) == (SIZE == 64 || (lane & SIZE) == 0) ? fmaxf(v, o) : fminf(v, o);
   if constexpr (J > 1) bitonic_values<SIZE, J / 2>(v, lane);
 }
@@ -165,23 +149,9 @@ __device__ __forceinline__ Sums add(Sums x, Sums y, float a) {
 
 // Over the wave's lanes, the same in each.
 __device__ __forceinline__ Sums wave_sums(Sums v, float a, int lane) {
-  float M = v.m;
-  M = fmaxf(M, __uint_as_float(lane_xor<1>(__float_as_uint(M), lane)));
-  M = fmaxf(M, __uint_as_float(lane_xor<2>(__float_as_uint(M), lane)));
-  M = fmaxf(M, __uint_as_float(lane_xor<4>(__float_as_uint(M), lane)));
-  M = fmaxf(M, __uint_as_float(lane_xor<8>(__float_as_uint(M), lane)));
-  M = fmaxf(M, __uint_as_float(lane_xor<16>(__float_as_uint(M), lane)));
-  M = fmaxf(M, __uint_as_float(lane_xor<32>(__float_as_uint(M), lane)));
+  const float M = wave_max(v.m, lane);
   v = rebase(v, M, a);
-  auto sum = [&](float x) {
-    x += __uint_as_float(lane_xor<1>(__float_as_uint(x), lane));
-    x += __uint_as_float(lane_xor<2>(__float_as_uint(x), lane));
-    x += __uint_as_float(lane_xor<4>(__float_as_uint(x), lane));
-    x += __uint_as_float(lane_xor<8>(__float_as_uint(x), lane));
-    x += __uint_as_float(lane_xor<16>(__float_as_uint(x), lane));
-    return x + __uint_as_float(lane_xor<32>(__float_as_uint(x), lane));
-  };
-  return Sums{M, sum(v.s), sum(v.e)};
+  return Sums{M, wave_sum(v.s, lane), wave_sum(v.e, lane)};
 }
 
 // ONCE: the logits are not kept in the caches.

@@ -18,6 +18,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "wave.hpp"
 
 namespace mlxq {
 
@@ -104,8 +105,7 @@ __device__ __forceinline__ Raw<W32 ? GEN_F32 : XT> load_weight(const void* p, in
 
 // Sum over the workgroup, the same in each thread; lds: 16 words of this sum.
 __device__ __forceinline__ float block_sum(float v, float* lds) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
+  v = wave_sum(v, threadIdx.x & 63);
   const int waves = blockDim.x >> 6;
   if (waves == 1) return v;
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;

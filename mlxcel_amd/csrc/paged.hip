@@ -44,6 +44,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "wave.hpp"
 
 namespace mlxq {
 
@@ -412,8 +413,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
             s[t][r] = k + 16 * t + 4 * g + r < k1 ? s[t][r] : -INFINITY;
             mt = fmaxf(mt, s[t][r]);
           }
-        mt = fmaxf(mt, __shfl_xor(mt, 16));
-        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        mt = fmaxf(mt, lane_xor<16>(mt, lane));
+        mt = fmaxf(mt, lane_xor<32>(mt, lane));
         if (__any(mt > m)) {
           const float f = exp2_diff(m, mt);
           m = mt;
@@ -483,8 +484,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
 #pragma unroll
         for (int t = 0; t < G::KT; t++) load_v(ONCE, t);
       }
-      l += __shfl_xor(l, 16);
-      l += __shfl_xor(l, 32);
+      l += lane_xor<16>(l, lane);
+      l += lane_xor<32>(l, lane);
 
       // join the waves: O rows [wave][head][LD], then (m, l) [wave][16][2]
       float* ml = lds + kWaves * heads * G::LD;
