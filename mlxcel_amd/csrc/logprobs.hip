@@ -41,9 +41,9 @@ namespace {
 constexpr int kWaves = 4, kChunk = 1024;  // values of a wave's chunk
 constexpr int kFew = 256;                 // values that a workgroup sorts at once
 // Workgroups a CU is given where rows are cut, each of at least two chunks a
-// wave: 300 rows of 151936 float32 logits 43.7 us with 2, 44.7 with 3, 52 with 4
-// (each pays for its own start and end); 8 rows of 262144 16 us, 21 with one chunk
-// a wave.
+// wave: 300 rows of 151936 float32 logits with 5 alternatives 40.9 us with 2, 41.3
+// with 3, 50.5 with 4 (each pays for its own start and end; bfloat16 36.9, 35.8,
+// 40.3); 8 rows of 262144 16 us, 21 with one chunk a wave.
 constexpr int kRowWgs = 2;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 

@@ -10,8 +10,8 @@
 // takes a row and holds it in registers, 8 elements (one or two 16-byte loads)
 // a lane and vector, so nothing is read twice; all loads, the weights' too, are
 // issued before the first sum, so a single row waits for memory once (1 x 4096:
-// 5.3 us, the launch's own time; 2047 x 2880 with a gate and both norms: 15.4 us,
-// 3.8 TB/s of its 59 MB).
+// 5.2 us, the launch's own time; 2047 x 2880 with a gate and both norms: 14.7 us,
+// 4.0 TB/s of its 59 MB).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -186,7 +186,9 @@ template <int XT>
 hipError_t launch(const ResidualNormArgs& a, hipStream_t stream) {
   const int vecs = (a.H + 7) / 8;
   // One vector a lane while all rows' waves are resident (256 CUs of 32), two
-  // past that: 2047 rows of 2880 15.4 us against 17.8, 700 rows 9.0 against 8.7.
+  // past that: 2047 rows of 2880 15.4 us with two and 17.3 with one, 1400 of 8192
+  // 21.0 and 23.6 (float32 43.5 and 41.4); 700 rows of 2880 8.8 and 8.2, 4096 of
+  // 64 9.1 and 5.5.
   int nv = a.T * ((vecs + 63) / 64) > 8192 ? 2 : 1;
   while ((vecs + nv - 1) / nv > 1024) nv *= 2;
   const dim3 grid((unsigned)a.T), block((unsigned)(((vecs + nv - 1) / nv + 63) / 64 * 64));
