@@ -41,9 +41,11 @@ namespace {
 constexpr int kWaves = 4, kChunk = 1024;  // values of a wave's chunk
 constexpr int kFew = 256;                 // values that a workgroup sorts at once
 // Workgroups a CU is given where rows are cut, each of at least two chunks a
-// wave: 300 rows of 151936 float32 logits with 5 alternatives 40.9 us with 2, 41.3
-// with 3, 50.5 with 4 (each pays for its own start and end; bfloat16 36.9, 35.8,
-// 40.3); 8 rows of 262144 16 us, 21 with one chunk a wave.
+// wave: each pays for its own start and end.  Rows of 100003 with 20 alternatives,
+// 2 against 3 of them: float32 100 rows 20.8 and 23.4 us, 300 31.7 and 33.4, 600
+// 47.8 and 65.0, bfloat16 300 30.3 and 30.1, 600 40.2 and 46.1; with 4,
+// 300 rows of 151936 float32 logits 50.5 against 40.9.  8 rows of 262144 take
+// 16 us, 21 with one chunk a wave.
 constexpr int kRowWgs = 2;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
