@@ -357,8 +357,9 @@ mlxq_status mlxq_fused_moe_geglu(const mlxq_array* x, const mlxq_array* indices,
  * less gives zeros.  window > 0: only the last `window` keys.  sinks: NULL or
  * float32 (query heads), logits that join each head's sum without a value.
  * Keys outside the sequence are not read; page numbers out of range are
- * clamped.  Scores, probabilities and sums are held in 32 bits, the result is
- * rounded once. */
+ * clamped.  Scores, probabilities and sums are held in 32 bits (in a product of
+ * 16-bit values a probability differs by at most 2^-24 of itself or 2^-39 of the
+ * largest), the result is rounded once. */
 mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool,
                                  const mlxq_array* v_pool, const mlxq_array* table,
                                  const mlxq_array* lengths, const mlxq_array* sinks, float scale,

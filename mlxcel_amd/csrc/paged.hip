@@ -33,10 +33,12 @@
 //     rows 4 g + r' of O^T: d = VE (4 g + r') + j, head c, the lane whose maximum
 //     rescales it.  16-bit pools: one MFMA of 32 keys, slot 4 t + r of group g key
 //     4 g + r of tile t; a column's keys are put side by side with byte permutes,
-//     and P goes in as the sum of two 16-bit numbers (2^-17 of it is lost in
-//     bfloat16, 2^-22 in float16, against 2^-9 and 2^-12 of the result's own
-//     rounding), for two MFMAs of 16 cycles a column instead of the 256 cycles of
-//     32-bit ones.  32-bit pools: MFMAs of 4 keys, step r taking keys 4 g + r.
+//     and P goes in as the sum of three bfloat16 or two float16 numbers, which
+//     leave at most 2^-24 of it out, what a 32-bit number would: three MFMAs of 16
+//     cycles a column instead of the 256 cycles of 32-bit ones.  With two bfloat16
+//     numbers (2^-17 left out) 258 of 131072 results of 32 ragged sequences were not
+//     the 64-bit ones rounded, with three 15, at 41.5 and 41.6 us (width 256 38.9 and
+//     39.3).  32-bit pools: MFMAs of 4 keys, step r taking keys 4 g + r.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -105,7 +107,7 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
 }
 
 // Probabilities are held as 2^lift p: in float16 their largest is then 2^14, and
-// those down to 2^-28 of it keep all their bits.
+// those down to 2^-28 of it keep all their bits (smaller ones differ by 2^-39 of it).
 template <int XT>
 constexpr float kLift = XT == GEN_F16 ? 14.f : 0.f;
 
@@ -456,15 +458,21 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
                   o[i][j] =
                       __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][r][i][j]), s[t][r], o[i][j], 0, 0, 0);
         } else {
-          // P = ph + pl
-          u32x4 ph, pl;
+          // P as a sum of 16-bit numbers, each what the ones before it leave of it
+          constexpr int TERMS = XT == GEN_BF16 ? 3 : 2;
+          u32x4 pt[TERMS];
 #pragma unroll
           for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {
-              const uint32_t h = pack<XT>(s[t][r], s[t][r + 1]);
-              ph[2 * t + r / 2] = h;
-              pl[2 * t + r / 2] = pack<XT>(s[t][r] - half<XT>(h, 0), s[t][r + 1] - half<XT>(h, 1));
+              float lo = s[t][r], hi = s[t][r + 1];
+#pragma unroll
+              for (int n = 0; n < TERMS; n++) {
+                const uint32_t w = pack<XT>(lo, hi);
+                pt[n][2 * t + r / 2] = w;
+                lo -= half<XT>(w, 0);
+                hi -= half<XT>(w, 1);
+              }
             }
 #pragma unroll
           for (int i = 0; i < G::NB; i++)
@@ -477,8 +485,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
 #pragma unroll
                 for (int r = 0; r < 4; r += 2)
                   v[2 * t + r / 2] = __builtin_amdgcn_perm(vr[t][r + 1][i][j / 2], vr[t][r][i][j / 2], sel);
-              o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, ph, o[i][j]);
-              o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, pl, o[i][j]);
+#pragma unroll
+              for (int n = 0; n < TERMS; n++) o[i][j] = mfma16x16x32_xt<XT == GEN_F16 ? 1 : 0>(v, pt[n], o[i][j]);
             }
         }
 #pragma unroll

@@ -235,3 +235,28 @@ def test_the_ctypes_path_gives_the_same(monkeypatch):
     want = mq.paged_attention(q, c.k, c.v, *args, window=9, softcap=20.0)
     monkeypatch.setattr(ops, "_native", ops._ctypes_only)
     assert torch.equal(mq.paged_attention(q, c.k, c.v, *args, window=9, softcap=20.0), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_probabilities_keep_32_bits(dtype):
+    """Sequences of three keys with scores 0, 0 and x < 0, values -a, -b and 1, where a is
+    p = exp(x) in the pool's type and b what is left of it: (p - a - b) / (2 + p), what a
+    probability held in two numbers of bfloat16 has lost.  Of p in 32 bits 3 |x| u
+    are the score's roundings, 2 u the exponential's, 8 u the sums', u = 2^-24."""
+    announce("paged probabilities", dtype)
+    t, n, u = DTYPES[dtype], 128, 2.0 ** -24
+    x = -torch.arange(1, n + 1, dtype=torch.float64) / 256
+    p = x.exp()
+    a = p.to(t)
+    b = (p - a.double()).to(t)
+    want = ((p - a.double() - b.double()) / (2 + p))[:, None].numpy()
+    slack = ((3 * x.abs() + 10) * u * p / (2 + p))[:, None].numpy()
+    if dtype == "bf16":
+        assert (np.abs(want) > 2 * slack).sum() > n / 4  # zeros would not do
+    k, v = torch.zeros(n, 1, 3, 8, dtype=t), torch.zeros(n, 1, 3, 8, dtype=t)
+    k[:, 0, 2, 0] = x.to(t)
+    v[:, 0] = torch.stack([-a, -b, torch.ones_like(a)], 1)[:, :, None]
+    q = torch.zeros(n, 1, 8, dtype=t)
+    q[..., 0] = 1
+    got = mq.paged_attention(q.cuda(), k.cuda(), v.cuda(), i32(np.arange(n)[:, None]), i32([3] * n), scale=1.0)
+    within(got[:, 0], np.broadcast_to(want, (n, 8)), slack)
