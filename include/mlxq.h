@@ -356,6 +356,8 @@ mlxq_status mlxq_fused_moe_geglu(const mlxq_array* x, const mlxq_array* indices,
  * 256.  table (B, n), lengths (B): a length is cut to the n pages, one of 0 or
  * less gives zeros.  window > 0: only the last `window` keys.  sinks: NULL or
  * float32 (query heads), logits that join each head's sum without a value.
+ * Keys whose score is -inf have no part in it; scores (and sink) that are all
+ * -inf give NaN, as softmax of them.
  * Keys outside the sequence are not read; page numbers out of range are
  * clamped.  Scores, probabilities and sums are held in 32 bits (in a product of
  * 16-bit values a probability differs by at most 2^-24 of itself or 2^-39 of the

@@ -42,6 +42,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.hpp"
@@ -531,11 +532,13 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
       auto finish = [&](int h, int d, float M, float L, f32x4 acc) {
         float f = 1.f;
         if (a.sinks) {
-          const float sink = a.sinks[head0 + h] * kLog2e, M2 = fmaxf(M, sink);
+          const float x = a.sinks[head0 + h];
+          // the largest finite sinks stay finite in the other base
+          const float sink = isinf(x) ? x : fminf(fmaxf(x * kLog2e, -FLT_MAX), FLT_MAX), M2 = fmaxf(M, sink);
           f = exp2_diff(M, M2);
           L = L * f + exp2_diff(sink, M2);
         }
-        const float r = L == 0.f ? 0.f : f / L;
+        const float r = f / L;  // scores and sink all -inf: 0 / 0, not a number as the definition says
         if (d < a.D) store4<XT>(a.out, ((int64_t)b * a.Hq + head0 + h) * a.D + d, acc * r);
       };
       for (int e = tid; e < heads * (DP / 4); e += 256) {

@@ -260,3 +260,40 @@ def test_probabilities_keep_32_bits(dtype):
     q[..., 0] = 1
     got = mq.paged_attention(q.cuda(), k.cuda(), v.cuda(), i32(np.arange(n)[:, None]), i32([3] * n), scale=1.0)
     within(got[:, 0], np.broadcast_to(want, (n, 8)), slack)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 40, 700, 20000])
+def test_scores_that_are_all_minus_infinity(dtype, n):
+    """NaN as softmax gives, unless a sink joins: then zeros.  Where some scores are
+    -inf, the keys that are left alone."""
+    announce("paged all -inf", dtype, n)
+    c = Cache([n], 1, 64, 16, dtype, n)
+    q = query(1, 3, 64, dtype, n + 1)
+    q[..., 0] = 1.0
+    ok = torch.isfinite(c.k[:, :, :, 0])
+    c.k[..., 0] = torch.where(ok, -float("inf"), c.k[..., 0])
+    args = (q, c.k, c.v, i32(c.table), i32(c.lengths))
+    sinks = torch.tensor([0.0, -float("inf"), -3e38], device="cuda")
+    assert torch.isnan(mq.paged_attention(*args)).all()
+    got = mq.paged_attention(*args, sinks=sinks)
+    assert not got[0, [0, 2]].any() and torch.isnan(got[0, 1]).all()
+    few = Cache([n], 1, 64, 16, dtype, n + 2)
+    at = np.arange(n)
+    pages, off = few.table[0, at // 16], at % 16
+    gone = np.random.default_rng(n).random(n) < 0.5
+    gone[n // 2] = False
+    few.k[pages[gone], 0, off[gone], 0] = -float("inf")
+    k, v = (t[pages[~gone], 0, off[~gone]][None, None] for t in (few.k, few.v))
+    want, slack = ref.attention(f64(q), f64(k), f64(v), np.zeros((1, 1), np.int32), [k.shape[2]], 0.125)
+    within(mq.paged_attention(q, few.k, few.v, i32(few.table), i32(few.lengths)), want, slack + n * ref.U * np.abs(want))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [40, 20000])
+def test_largest_finite_sinks(dtype, n):
+    announce("paged largest sinks", dtype, n)
+    top = float(torch.finfo(torch.float32).max)
+    c = Cache([n], 1, 64, 16, dtype, n)
+    got = check(c, query(1, 6, 64, dtype, n + 1), sinks=[top, 2.5e38, -top, -2.5e38, np.inf, -np.inf])
+    assert not got[0, :2].any() and torch.isnan(got[0, 4]).all()
