@@ -361,7 +361,9 @@ mlxq_status mlxq_fused_moe_geglu(const mlxq_array* x, const mlxq_array* indices,
  * Keys outside the sequence are not read; page numbers out of range are
  * clamped.  Scores, probabilities and sums are held in 32 bits (in a product of
  * 16-bit values a probability differs by at most 2^-24 of itself or 2^-39 of the
- * largest), the result is rounded once. */
+ * largest), the result is rounded once.  An infinite value of a 32-bit pool
+ * gives what the sum gives; one of a 16-bit pool makes its column of the result
+ * infinite or NaN. */
 mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool,
                                  const mlxq_array* v_pool, const mlxq_array* table,
                                  const mlxq_array* lengths, const mlxq_array* sinks, float scale,

@@ -38,7 +38,8 @@
 //     cycles a column instead of the 256 cycles of 32-bit ones.  With two bfloat16
 //     numbers (2^-17 left out) 258 of 131072 results of 32 ragged sequences were not
 //     the 64-bit ones rounded, with three 15, at 41.5 and 41.6 us (width 256 38.9 and
-//     39.3).  32-bit pools: MFMAs of 4 keys, step r taking keys 4 g + r.
+//     39.3).  A part may be 0 or below it, so an infinite value may give NaN.  32-bit
+//     pools: MFMAs of 4 keys, step r taking keys 4 g + r.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -297,3 +297,28 @@ def test_largest_finite_sinks(dtype, n):
     c = Cache([n], 1, 64, 16, dtype, n)
     got = check(c, query(1, 6, 64, dtype, n + 1), sinks=[top, 2.5e38, -top, -2.5e38, np.inf, -np.inf])
     assert not got[0, :2].any() and torch.isnan(got[0, 4]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [40, 20000])
+def test_infinite_values(dtype, n):
+    """32-bit pools add them up; in 16-bit ones an infinite value makes its column
+    infinite or NaN.  Other columns and the sequence beside it are left alone."""
+    announce("paged infinite values", dtype, n)
+    inf = float("inf")
+    c = Cache([n, 33], 1, 64, 16, dtype, n)
+    q = query(2, 3, 64, dtype, n + 1)
+    args = (q, c.k, c.v, i32(c.table), i32(c.lengths))
+    want = mq.paged_attention(*args)
+    at = lambda t: (int(c.table[0, t // 16]), 0, t % 16)
+    for t, column, value in ((0, 3, inf), (n - 1, 5, -inf), (0, 7, inf), (n - 1, 7, -inf), (n // 2, 9, float("nan"))):
+        c.v[at(t)][column] = value
+    got = mq.paged_attention(*args)
+    bad = [3, 5, 7, 9]
+    rest = [d for d in range(64) if d not in bad]
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0][:, rest], want[0][:, rest])
+    assert torch.isnan(got[0][:, [7, 9]]).all()
+    if dtype == "f32":
+        assert (got[0][:, 3] == inf).all() and (got[0][:, 5] == -inf).all()
+    else:
+        assert not torch.isfinite(got[0][:, [3, 5]]).any()
