@@ -361,7 +361,14 @@ struct Workspace {
 // key: (device, stream, slot); the slots are listed in host.hpp
 std::map<std::tuple<int, hipStream_t, int>, Workspace> g_ws;
 
+// Locks of the streams' calls, taken before g_mu; streams may share one.
+constexpr int kTurns = 64;
+std::mutex g_turns[kTurns];
+
 }  // namespace
+
+mlxq::host::StreamTurn::StreamTurn(hipStream_t stream)
+    : lk_(g_turns[(reinterpret_cast<uintptr_t>(stream) * 0x9E3779B97F4A7C15ull) >> 58]) {}
 
 int mlxq::host::current_device() {
   int dev = 0;
@@ -2295,6 +2302,7 @@ mlxq_status mlxq_quantized_matmul(const mlxq_array* x, const mlxq_array* w, cons
     const QmmSpec sp =
         check_quantized_matmul(x, w, scales, biases, transpose, group_size, bits, mode, out, "quantized_matmul");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     Staged st = stage_operands(x, w, scales, biases, out, stream, true, "quantized_matmul");
     run_quantized_matmul(sp, st.in[0], st.in[1], st.in[2], st.in[3], st.out, stream);
     st.finish();
@@ -2401,6 +2409,7 @@ mlxq_status mlxq_quantized_linear(const mlxq_array* x, const mlxq_array* w, cons
       require_contiguous(linear_bias, "linear_bias");
     }
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     Staged st = stage_operands(x, w, scales, biases, out, stream, true, tag);
     run_quantized_matmul(sp, st.in[0], st.in[1], st.in[2], st.in[3], st.out, stream);
     if (bias_n > 0 && View{out}.size() > 0)
@@ -2444,6 +2453,7 @@ mlxq_status mlxq_quantized_matmul_multi(const mlxq_array* x, int32_t n, const ml
       if (View{w[i]}.ndim() != 2) unsupported(std::string(tag) + ": 2-D weights only");
     }
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     // One launch of the row-streaming kernel over every projection when each
     // call alone would run it with the same plan (decode rows, no kernel
     // override): the results are then those of the separate calls, bit for
@@ -2544,6 +2554,7 @@ mlxq_status mlxq_gather_qmm(const mlxq_array* x_, const mlxq_array* w_, const ml
     choose_route(sp, x_, w_, scales_, biases_, tag);
     if (global_scale) unsupported("gather_qmm: global_scale (nvfp4) is not implemented");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     Staged st = stage_operands(x_, w_, scales_, biases_, out_, stream, true, tag);
     const mlxq_array* x = st.in[0];
     const mlxq_array* w = st.in[1];
@@ -2649,6 +2660,7 @@ mlxq_status mlxq_dequantize(const mlxq_array* w, const mlxq_array* scales, const
         unsupported("dequantize: group_size must be 32, 64 or 128");
     }
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     Staged st = stage_operands(nullptr, w, scales, biases, out, stream, true, tag);
     w = st.in[1];
     scales = st.in[2];
@@ -2880,6 +2892,7 @@ void fused_moe(const char* tag, const mlxq_array* x, const mlxq_array* indices, 
   a.k = k;
   a.E = (int)std::min<int64_t>(E, INT32_MAX);
   a.gs_shift = group_size == 32 ? 5 : (group_size == 64 ? 6 : 7);
+  const StreamTurn turn(stream);
   a.act = reinterpret_cast<float*>(workspace(dev, stream, (size_t)k * dff * sizeof(float)));
   hip_check(mlxq::moe_launch(a, gu_bits, d_bits, act, stream), "fused MoE launch");
 }

@@ -5,7 +5,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <mutex>
 
 #include "host.hpp"
 #include "kernels.hpp"
@@ -163,10 +162,6 @@ void each_pools(int32_t n, const mlxq_array* const* pools, F&& f) {
   }
 }
 
-// The launches of one call that share the stream's page lists follow each
-// other: no other call's come between them.
-std::mutex g_pages_mu;
-
 int32_t* page_lists(hipStream_t stream, int64_t words) {
   return static_cast<int32_t*>(stream_workspace(current_device(), stream, (size_t)words * sizeof(int32_t), 4));
 }
@@ -259,6 +254,7 @@ mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool, 
     a.table_row = table->strides[0];
     a.lengths = static_cast<const int32_t*>(lengths->data);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     mlxq_array qc = *q, oc = *out;
     const bool stage_q = !unit_last(x), stage_out = !View{out}.row_contiguous();
     if (stage_q || stage_out) {
@@ -294,7 +290,7 @@ mlxq_status mlxq_cache_reserve(const mlxq_array* table, const mlxq_array* length
     same_shape(vec32(granted, tag, "granted"), Shape{b.rows}, tag, "granted");
     if (b.rows == 0) return;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-    std::lock_guard<std::mutex> lk(g_pages_mu);
+    const StreamTurn turn(stream);
     hip_check(mlxq::launch_cache_reserve(b, static_cast<const int32_t*>(counts->data),
                                          static_cast<int32_t*>(granted->data), page_lists(stream, b.pages), stream),
               "cache reserve launch");
@@ -362,7 +358,7 @@ mlxq_status mlxq_cache_fork(int32_t n, const mlxq_array* const* pools, const mlx
     if (pairs == 0) return;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int32_t *sp = static_cast<const int32_t*>(src->data), *dp = static_cast<const int32_t*>(dst->data);
-    std::lock_guard<std::mutex> lk(g_pages_mu);
+    const StreamTurn turn(stream);
     int32_t* ws = page_lists(stream, mlxq::cache_fork_words(b.pages, pairs));
     hip_check(mlxq::launch_cache_fork_plan(b, sp, dp, pairs, static_cast<int32_t*>(granted->data), ws, stream),
               "cache fork launch");
@@ -394,7 +390,7 @@ mlxq_status mlxq_cache_compact(int32_t n, const mlxq_array* const* pools, const 
     same_shape(vec32(live, tag, "live"), Shape{1}, tag, "live");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int cus = device_cus(current_device());
-    std::lock_guard<std::mutex> lk(g_pages_mu);
+    const StreamTurn turn(stream);
     int32_t* ws = page_lists(stream, mlxq::cache_compact_words(b.pages));
     hip_check(mlxq::launch_cache_compact_plan(b, static_cast<int32_t*>(live->data), ws, stream),
               "cache compact launch");
@@ -483,6 +479,7 @@ mlxq_status mlxq_residual_norm(const mlxq_array* x, const mlxq_array* y, const m
     a.scale = scale, a.eps = eps, a.offset = weight_offset;
     // operands whose rows one stride does not describe go through a dense copy
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     mlxq_array xc = *x, yc = *y, hc = *h, nc = n ? *n : mlxq_array{};
     const bool sx = !matrix_rows(xv, a.x_row), sy = !matrix_rows(yv, a.y_row);
     const bool sg = gate && !matrix_rows(View{gate}, a.gate_row);
@@ -560,6 +557,7 @@ mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* toke
     a.k = top_k;
     a.scale = scale;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
     mlxq_array xc = *logits;
     if (!unit_last(x)) {
       xc = contiguous_like(logits, stream_workspace(current_device(), stream, padded(x), 1));

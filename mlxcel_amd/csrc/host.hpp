@@ -129,6 +129,15 @@ void* stream_workspace(int dev, hipStream_t stream, size_t bytes, int slot);
 // kSplitCounters words, all zero between launches; null where they would have
 // to be allocated under a capture.
 uint32_t* stream_counters(int dev, hipStream_t stream);
+// The launches of one call that takes a stream's workspaces follow each other on
+// the stream: held while it issues them, so that no call of another thread uses
+// the same buffers between them.
+class StreamTurn {
+  std::lock_guard<std::mutex> lk_;
+
+ public:
+  explicit StreamTurn(hipStream_t stream);
+};
 bool needs_staging(const mlxq_array* a);
 mlxq_array contiguous_like(const mlxq_array* a, void* data);
 void copy_view(const mlxq_array* src, const mlxq_array* dst, hipStream_t stream);
