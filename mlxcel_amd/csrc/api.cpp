@@ -2362,6 +2362,9 @@ size_t mlxq_get_cache_memory(void) {
 
 mlxq_status mlxq_clear_cache(void) {
   return guarded([&] {
+    // no call is between taking a buffer and its last launch
+    std::unique_lock<std::mutex> turns[kTurns];
+    for (int i = 0; i < kTurns; i++) turns[i] = std::unique_lock<std::mutex>(g_turns[i]);
     std::lock_guard<std::mutex> lk(g_mu);
     int cur = 0;
     hip_check(hipGetDevice(&cur), "hipGetDevice");

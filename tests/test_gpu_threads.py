@@ -60,3 +60,29 @@ def test_one_stream_of_two_threads():
     assert {n for n, _ in got} == set(calls)
     wrong = sorted({n for (n, _), r in got.items() if not torch.equal(r, want[n])})
     assert not wrong, wrong
+
+
+def test_buffers_freed_beside_calls():
+    """`clear_cache` of one thread waits for the launches of the calls under way."""
+    announce("clear_cache beside calls")
+    calls = strided_calls()
+    want = {name: f() for name, f in calls.items()}
+    got, done = {}, threading.Event()
+
+    def work():
+        for rep in range(200):
+            for name, f in calls.items():
+                got[name, rep] = f()
+        done.set()
+
+    t = threading.Thread(target=work)
+    t.start()
+    cleared = 0
+    while cleared < 10 and not done.is_set():
+        mq.clear_cache()
+        cleared += 1
+    t.join()
+    torch.cuda.synchronize()
+    assert cleared and mq.get_cache_memory() > 0
+    wrong = sorted({n for (n, _), r in got.items() if not torch.equal(r, want[n])})
+    assert not wrong, wrong
