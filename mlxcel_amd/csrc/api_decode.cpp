@@ -174,8 +174,7 @@ uint32_t* counters(int dev, hipStream_t stream, const char* tag) {
   return c;
 }
 
-// A row-contiguous copy of an operand whose strides the kernel does not take,
-// at `at` of the staging workspace.
+// Bytes of an operand's row-contiguous copy in the staging workspace.
 size_t padded(View v) { return ((size_t)v.size() * dtype_size(v.dtype()) + 255) & ~(size_t)255; }
 
 // x's rows as a matrix [rows][last axis]: the stride of a row where one number
@@ -258,12 +257,14 @@ mlxq_status mlxq_paged_attention(const mlxq_array* q, const mlxq_array* k_pool, 
     mlxq_array qc = *q, oc = *out;
     const bool stage_q = !unit_last(x), stage_out = !View{out}.row_contiguous();
     if (stage_q || stage_out) {
-      char* p = static_cast<char*>(stream_workspace(current_device(), stream, 2 * padded(x), 1));
+      char* p = static_cast<char*>(
+          stream_workspace(current_device(), stream, ((int)stage_q + (int)stage_out) * padded(x), 1));
       if (stage_q) {
         qc = contiguous_like(q, p);
         copy_view(q, &qc, stream);
+        p += padded(x);
       }
-      if (stage_out) oc = contiguous_like(out, p + padded(x));
+      if (stage_out) oc = contiguous_like(out, p);
     }
     a.q = qc.data;
     a.q_b = qc.strides[0];
@@ -485,16 +486,17 @@ mlxq_status mlxq_residual_norm(const mlxq_array* x, const mlxq_array* y, const m
     const bool sg = gate && !matrix_rows(View{gate}, a.gate_row);
     const bool sh = !View{h}.row_contiguous(), sn = n && !View{n}.row_contiguous();
     if (sx || sy || sg || sh || sn) {
-      char* p = static_cast<char*>(stream_workspace(current_device(), stream, 5 * padded(xv), 1));
+      const size_t bytes = ((int)sx + (int)sy + (int)sh + (int)sn) * padded(xv) + (sg ? padded(View{gate}) : 0);
+      char* p = static_cast<char*>(stream_workspace(current_device(), stream, bytes, 1));
       auto in = [&](const mlxq_array* from, mlxq_array& c, int64_t& row) {
         c = contiguous_like(from, p);
         copy_view(from, &c, stream);
         row = View{from}.dim(-1);
-        p += padded(xv);
+        p += padded(View{from});
       };
       auto result = [&](const mlxq_array* to, mlxq_array& c) {
         c = contiguous_like(to, p);
-        p += padded(xv);
+        p += padded(View{to});
       };
       if (sx) in(x, xc, a.x_row);
       if (sy) in(y, yc, a.y_row);

@@ -322,3 +322,21 @@ def test_infinite_values(dtype, n):
         assert (got[0][:, 3] == inf).all() and (got[0][:, 5] == -inf).all()
     else:
         assert not torch.isfinite(got[0][:, [3, 5]]).any()
+
+
+def test_copies_take_their_own_size():
+    announce("paged staging size")
+    B, H, mib = 64, 64, 1 << 20
+    c = Cache([5] * B, 1, 256, 16, "f32", 91)
+    q, args = query(B, H, 256, "f32", 92), (c.k, c.v, i32(c.table), i32(c.lengths))  # 4 MiB
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    out = torch.empty(B, 256, H, device="cuda").transpose(1, 2)
+    want = mq.paged_attention(q, *args)
+    torch.cuda.synchronize()
+    mq.clear_cache()
+    mq.paged_attention(q, *args)
+    held = mq.get_cache_memory()
+    assert torch.equal(mq.paged_attention(turned, *args), want)
+    assert mq.get_cache_memory() == held + 4 * mib
+    assert torch.equal(mq.paged_attention(turned, *args, out=out), want)
+    assert mq.get_cache_memory() == held + (4 + 8) * mib  # the first buffer is kept until clear_cache

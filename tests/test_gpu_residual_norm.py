@@ -122,3 +122,22 @@ def test_empty_graph_stream_and_ctypes(monkeypatch):
     monkeypatch.setattr(ops, "_native", ops._ctypes_only)
     again = mq.residual_norm(x, y, pre_weight=w, scale=0.5)
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+def test_copies_take_their_own_size():
+    """Only what is copied counts: a gate of every other element beside rows of 32 MiB, then the rows too."""
+    announce("norm staging size")
+    T, H, mib = 2048, 4096, 1 << 20
+    x, gate = torch.randn(T, H, device="cuda"), torch.randn(2 * H, device="cuda")[::2]
+    want = mq.residual_norm(x, x, gate=gate.contiguous())[0]
+    turned = x.t().contiguous().t()
+    torch.cuda.synchronize()
+    mq.clear_cache()
+    assert torch.equal(mq.residual_norm(x, x, gate=gate)[0], want)
+    assert mq.get_cache_memory() == mib
+    mq.clear_cache()
+    assert torch.equal(mq.residual_norm(turned, x, gate=gate)[0], want)
+    assert mq.get_cache_memory() == 64 * mib
+    mq.clear_cache()
+    assert torch.equal(mq.residual_norm(x, turned)[0], mq.residual_norm(x, x)[0])
+    assert mq.get_cache_memory() == 32 * mib
