@@ -97,10 +97,11 @@ typedef struct mlxq_array {
  * MLXQ_ENOMEM instead of allocating.  Callers that capture either run each
  * call shape once before the capture or reserve the workspace up front. */
 
-/* Grows `stream`'s workspace on the current device to at least `bytes`, both
- * the kernel scratch and the staging buffer that holds row-contiguous copies
- * of strided or misaligned operands (each at least `bytes`), so a capture of
- * calls needing at most that much of either allocates nothing.  Also
+/* Grows `stream`'s workspaces on the current device to at least `bytes` each:
+ * the kernel scratch, the staging buffer that holds row-contiguous copies of
+ * strided or misaligned operands, the index lists of gathers run in chunks and
+ * the page lists of the cache operators, so a capture of calls needing at
+ * most that much of each allocates nothing.  Also
  * allocates the stream's stream-K counters (1 MiB) and resolves the device
  * address of mlxq_quantized_matmul_noalloc's fixed scratch.  A captured
  * prefill call whose stream-K plan needs more scratch than the stream holds

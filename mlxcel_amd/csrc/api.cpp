@@ -2339,8 +2339,8 @@ mlxq_status mlxq_workspace_reserve(size_t bytes, void* stream_) {
     void* fixed = nullptr;
     hip_check(mlxq::static_scratch(dev, &fixed), "hipGetSymbolAddress(scratch)");
     std::lock_guard<std::mutex> lk(g_mu);
-    // kernel scratch (slot 0) and the staging copies of strided operands (slot 1)
-    for (int slot = 0; slot < 2; slot++) {
+    // every slot that calls take by size (host.hpp)
+    for (int slot : {0, 1, 2, 4}) {
       Workspace& w = g_ws[{dev, stream, slot}];
       if (w.bytes >= bytes) continue;
       if (stream_capturing(stream)) unsupported("mlxq_workspace_reserve: the stream is being captured");

@@ -258,3 +258,28 @@ def test_captured_odd_width_prefill_without_scratch_gets_a_status():
     g.replay()
     torch.cuda.synchronize()
     assert float(out.float().min()) == 1.0 == float(out.float().max())
+
+
+def test_capture_of_a_chunked_gather_after_a_reserve():
+    # its flat index lists have a buffer of their own
+    announce("graph_chunked_gather_reserve")
+    T, N, K, E = 70000, 64, 64, 3
+    g = torch.Generator().manual_seed(7)
+    w = [mq.quantize(torch.randn(N, K, generator=g).to(torch.bfloat16).cuda(), 64, 4) for _ in range(E)]
+    W, S, B = (torch.stack(t) for t in zip(*w))
+    X = torch.randn(1, 1, K, generator=g).to(torch.bfloat16).cuda()
+    lhs = torch.zeros(T, dtype=torch.int32, device="cuda")
+    rhs = torch.randint(0, E, (T,), generator=g).int().cuda()
+    eager = host_u16(mq.gather_qmm(X, W, S, B, lhs, rhs, True, 64, 4))
+    out = torch.empty(T, 1, N, dtype=torch.bfloat16, device="cuda")
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        mq.workspace_reserve(64 << 20)
+    torch.cuda.synchronize()
+    held = mq.get_cache_memory()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        mq.gather_qmm(X, W, S, B, lhs, rhs, True, 64, 4, out=out)
+    assert mq.get_cache_memory() == held
+    junk = torch.randn(1 << 20, device="cuda")
+    replay_and_check(graph, out, eager, lambda: junk.mul_(0.25))

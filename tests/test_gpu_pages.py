@@ -288,3 +288,35 @@ def test_the_ctypes_path_gives_the_same(monkeypatch):
         h[b.table[r, 0], :, 0] = k[0].float().numpy()
     b.compact()
     b.equal()
+
+
+def test_capture_after_a_reserve():
+    """On a stream that has run nothing yet."""
+    announce("pages capture after a reserve")
+    b = Book(10, 8, 80, 4, 29, fill=0.4, most=10)
+    held, empty = np.flatnonzero(b.lengths), np.flatnonzero(b.lengths == 0)
+    b.free(held[-2:])
+    src, dst = held[:2], np.concatenate([held[-2:], empty])[:2]
+    counts, s, d = i32(np.ones(10)), i32(src), i32(dst)
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        mq.workspace_reserve(1 << 20)
+    torch.cuda.synchronize()
+    size = mq.get_cache_memory()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        forked = mq.cache_fork(b.dev_pools, b.t, b.l, b.r, s, d)
+        granted = mq.cache_reserve(b.t, b.l, b.r, counts, b.page)
+        live = mq.cache_compact(b.dev_pools, b.t, b.l, b.r)
+    assert mq.get_cache_memory() == size
+    for rep in range(3):
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ref.fork(b.host, b.table, b.lengths, b.refs, src, dst, b.page)
+        np.testing.assert_array_equal(forked.cpu().numpy(), want)
+        assert rep or want.all()
+        np.testing.assert_array_equal(granted.cpu().numpy(), ref.reserve(b.table, b.lengths, b.refs, np.ones(10, np.int32),
+                                                                         b.page))
+        assert int(live) == ref.compact(b.host, b.table, b.lengths, b.refs, b.page)
+        b.equal(rep)
