@@ -357,6 +357,9 @@ mlxq_status mlxq_cache_fork(int32_t n, const mlxq_array* const* pools, const mlx
     same_shape(vec32(granted, tag, "granted"), s.shape(), tag, "granted");
     const int pairs = (int)s.dim(0);
     if (pairs == 0) return;
+    // before the plan, which changes the book
+    if (pairs * mlxq::cache_fork_columns(std::min(n, mlxq::kPoolsPerLaunch)) > mlxq::kMaxGroups)
+      (Refusal(tag) << "too many pairs (" << pairs << ") for one call.").unsupported();
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int32_t *sp = static_cast<const int32_t*>(src->data), *dp = static_cast<const int32_t*>(dst->data);
     const StreamTurn turn(stream);
@@ -389,6 +392,8 @@ mlxq_status mlxq_cache_compact(int32_t n, const mlxq_array* const* pools, const 
     const int64_t page = check_pools(n, pools, r.dim(0), tag);
     const CacheBook b = book(table, lengths, refs, page, tag);
     same_shape(vec32(live, tag, "live"), Shape{1}, tag, "live");
+    if (b.rows > mlxq::kMaxGroups - mlxq::kCompactGroups)
+      (Refusal(tag) << "a table of " << b.rows << " rows is too long.").unsupported();
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int cus = device_cus(current_device());
     const StreamTurn turn(stream);

@@ -622,7 +622,14 @@ struct PoolList {
   int n;
   int64_t bytes, stride;
 };
-// scratch: pages + 4 n words (fork), 3 pages + 16 words (compact)
+// Workgroups of 256 threads that one launch takes (2^32 threads less one).
+constexpr int64_t kMaxGroups = 0xFFFFFFFF / 256;
+// Workgroups of a fork's copies, for each pair one a pool and one for its row,
+// in eights; compaction's copies of pages take at most kCompactGroups beside one
+// a row of the table.
+inline int64_t cache_fork_columns(int pools) { return (pools + 1 + 7) / 8 * 8; }
+constexpr int kCompactGroups = 1 << 16;
+// scratch: pages + 2 n words (fork), 3 pages + 16 words (compact)
 int64_t cache_fork_words(int pages, int n);
 int64_t cache_compact_words(int pages);
 hipError_t launch_cache_fork_plan(const CacheBook& b, const int32_t* src, const int32_t* dst, int n, int32_t* granted,

@@ -14,6 +14,8 @@
 // kept as it stands.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -465,9 +467,9 @@ hipError_t launch_cache_fork_plan(const CacheBook& b, const int32_t* src, const 
 hipError_t launch_cache_fork_copy(const CacheBook& b, const int32_t* src, const int32_t* dst, int n,
                                   const int32_t* scratch, const PoolList& pools, bool book, hipStream_t stream) {
   if (n == 0) return hipSuccess;
-  const int columns = (pools.n + (book ? 1 : 0) + 7) / 8 * 8;
+  const int columns = (int)cache_fork_columns(book ? pools.n : pools.n - 1);
   if (columns == 0) return hipSuccess;
-  if ((int64_t)n * columns > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (n * (int64_t)columns > kMaxGroups) return hipErrorInvalidValue;
   const dim3 grid((unsigned)(n * columns)), block(256);
   const int32_t* pair = scratch + b.pages;
   with_word(pools, [&](auto w) {
@@ -492,10 +494,10 @@ hipError_t launch_cache_compact_plan(const CacheBook& b, int32_t* live, int32_t*
 
 hipError_t launch_cache_compact_copy(const CacheBook& b, const int32_t* scratch, const PoolList& pools, bool book,
                                      int cus, hipStream_t stream) {
-  const int wgs = pools.n > 0 && b.pages > 0 ? cus * 8 : 0;
+  const int wgs = pools.n > 0 && b.pages > 0 ? std::min(cus * 8, kCompactGroups) : 0;
   const int64_t grid = (int64_t)wgs + (book ? b.rows : 0);
   if (grid == 0) return hipSuccess;
-  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (grid > kMaxGroups) return hipErrorInvalidValue;
   const int32_t* to = scratch + 16;
   const int32_t *holes = to + b.pages, *movers = to + 2 * (int64_t)b.pages;
   with_word(pools, [&](auto w) {

@@ -123,6 +123,15 @@ def test_fork_free_and_compact(lib):
     refused(lib, "mlxq_cache_free", EINVAL, "1 dimensions", *BOOK, have((2, 1), I32), 16)
 
 
+def test_forks_and_compactions_of_more_than_a_launch(lib):
+    """Refused before the plan, which would have changed the book."""
+    many, long = have((1 << 21,), I32), [have((1 << 24, 6), I32), have((1 << 24,), I32), BOOK[2]]
+    refused(lib, "mlxq_cache_fork", EUNSUPPORTED, "too many pairs", 1, pools(POOL), *BOOK, many, many, many)
+    refused(lib, "mlxq_cache_fork", EUNSUPPORTED, "too many pairs", 300, pools(*[POOL] * 300), *BOOK,
+            *[have((1 << 16,), I32)] * 3)
+    refused(lib, "mlxq_cache_compact", EUNSUPPORTED, "too long", 1, pools(POOL), *long, have((1,), I32))
+
+
 APPEND = [have((3, 2, 8), BF), have((3, 2, 8), BF), POOL, POOL, have((4, 6), I32), have((3,), I32), have((3,), I32), None]
 
 
