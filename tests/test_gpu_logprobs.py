@@ -131,3 +131,30 @@ def test_repeatable_graph_and_ctypes(monkeypatch):
 
     monkeypatch.setattr(ops, "_native", ops._ctypes_only)
     assert all(torch.equal(a, b) for a, b in zip(mq.token_logprobs(x, tok, top_k=20), want))
+
+
+@pytest.mark.parametrize("dtype,T", [("bf16", 460), ("f16", 460), ("f32", 230), ("bf16", 700)])
+@pytest.mark.parametrize("k", [0, 20])
+def test_more_than_the_caches_hold(dtype, T, k):
+    """Past 128 MiB the logits are read past the caches; rows of one and of two workgroups."""
+    announce("logprobs past the caches", dtype, T, k)
+    V = 151937
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, V, generator=g, device="cuda", dtype=DTYPES[dtype]) * 3
+    x[3, ::2] = -float("inf")
+    x[T - 1, 5:9] = x[T - 1].max()
+    assert x.numel() * x.element_size() > 128 << 20
+    tok = np.random.default_rng(T).integers(0, V, (T, 2)).astype(np.int32)
+    given, ent, top, ids = mq.token_logprobs(x, i32(tok), top_k=k, scale=0.7)
+    few = [0, 3, T // 2, T - 1]
+    wg, we, wt, wi, dl, de = ref.token_logprobs(f64(x[few]), tok[few], k, float(np.float32(0.7)))
+    with np.errstate(invalid="ignore"):
+        slack = lambda w: np.nan_to_num(dl[:, None] + 4 * ref.U * np.abs(w), posinf=0)
+        within(given[few], wg, slack(wg), "given")
+        within(ent[few], we, de, "entropy")
+        if k:
+            np.testing.assert_array_equal(ids[few].cpu().numpy(), wi)
+            within(top[few], wt, slack(wt), "top")
+            # every row's alternatives, against a call that leaves the caches as they are
+            for r in range(0, T, 100):
+                assert torch.equal(mq.token_logprobs(x[r:r + 100], i32(tok[r:r + 100]), top_k=k)[3], ids[r:r + 100])

@@ -340,3 +340,68 @@ def test_copies_take_their_own_size():
     assert mq.get_cache_memory() == held + 4 * mib
     assert torch.equal(mq.paged_attention(turned, *args, out=out), want)
     assert mq.get_cache_memory() == held + (4 + 8) * mib  # the first buffer is kept until clear_cache
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("window", [0, 30000])
+def test_more_than_the_last_cache_holds(dtype, window):
+    """Past 128 MiB of keys and values they are read past it."""
+    announce("paged past the cache", dtype, window)
+    lengths = [40000, 1, 0, 25001]
+    c = Cache(lengths, 8, 128, 64, dtype, 95)
+    q = query(4, 16, 128, dtype, 96)
+    seen = sum(min(n, window or n) for n in lengths)
+    assert seen * 2 * 8 * 128 * q.element_size() > 128 << 20
+    got = mq.paged_attention(q, c.k, c.v, i32(c.table), i32(lengths), window=window)
+    for h in range(8):  # 64-bit keys and values of one head at a time
+        mine = slice(2 * h, 2 * h + 2)
+        want, slack = ref.attention(f64(q[:, mine]), f64(c.k[:, h:h + 1]), f64(c.v[:, h:h + 1]), c.table, lengths,
+                                    128 ** -0.5, 0.0, window)
+        within(got[:, mine], want, slack, h)
+
+
+MIXED = [0, 1, 100, 200, 300, 400, 500, 513, 2000, 3000]
+
+
+def mixed(B, seed, most=9000):
+    g = np.random.default_rng(seed)
+    lengths = g.choice(MIXED, B)
+    lengths[[0, B // 2, B - 1]] = most, 0, most - 1
+    return lengths.astype(np.int32)
+
+
+@pytest.mark.parametrize("B", [63, 64, 65, 200, 256, 257, 600])
+@pytest.mark.parametrize("window,sinks", [(0, False), (300, True), (2500, False)])
+def test_many_sequences_with_cut_heads(B, window, sinks):
+    """Sequences without keys, heads of one to four steps and cut ones, on both
+    sides of 64 sequences and of one a thread."""
+    announce("paged many cut", B, window, sinks)
+    c = Cache(mixed(B, B + window).tolist(), 2, 64, 16, "bf16", B)
+    check(c, query(B, 4, 64, "bf16", B + 1), window, 0.0, np.linspace(-2, 4, 4) if sinks else None)
+
+
+@pytest.mark.parametrize("B", [64, 65, 300])
+def test_graph_of_many_sequences(B):
+    announce("paged many graph", B)
+    most = mixed(B, 1, 9000)
+    first = np.maximum(most, 600)
+    c = Cache(first.tolist(), 2, 64, 16, "bf16", B)
+    for t in (c.k, c.v):  # lengths are changed within the rows' pages
+        t[torch.isnan(t)] = 0.5
+    q, table, n = query(B, 4, 64, "bf16", B + 1), i32(c.table), i32(first)
+    out = torch.empty_like(q)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        mq.workspace_reserve(32 << 20)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        mq.paged_attention(q, c.k, c.v, table, n, out=out)
+    for rep, lens in enumerate((first, np.minimum(first, 130), np.where(np.arange(B) % 7 == 3, first, 0), first * 0, most)):
+        n.copy_(i32(lens))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        want, slack = ref.attention(f64(q), f64(c.k), f64(c.v), c.table, lens, 64 ** -0.5)
+        within(out, want, slack, rep)
