@@ -383,7 +383,8 @@ mlxq_status mlxq_cache_reserve(const mlxq_array* table, const mlxq_array* length
  * where the table has position positions[t] of row rows[t] (int32).  Tokens
  * with a row, position or page out of range are left out, and, where lengths
  * is not NULL, tokens at or past their row's length (of rows that were not
- * granted their pages).  Of two tokens for one place either may stay. */
+ * granted their pages).  Of two tokens for one place parts of either may stay:
+ * the tokens of a call are for different places. */
 mlxq_status mlxq_cache_append(const mlxq_array* k, const mlxq_array* v, const mlxq_array* k_pool,
                               const mlxq_array* v_pool, const mlxq_array* table,
                               const mlxq_array* positions, const mlxq_array* rows,
