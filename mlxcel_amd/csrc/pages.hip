@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_reserve_kernel(const Cache
 // ---- append ------------------------------------------------------------------
 
 // One workgroup a token; the token's page number is the same for all its
-// elements.  VEC: 16 bytes at a time, else one element.
+// elements.  W: 16 bytes where everything is aligned to them, else one element.
 template <typename W>
 __global__ __launch_bounds__(256) void cache_append_kernel(const CacheAppendArgs a) {
   const int t = blockIdx.x, row = a.rows[t], pos = a.positions[t];
@@ -494,6 +494,8 @@ hipError_t launch_cache_compact_plan(const CacheBook& b, int32_t* live, int32_t*
 
 hipError_t launch_cache_compact_copy(const CacheBook& b, const int32_t* scratch, const PoolList& pools, bool book,
                                      int cus, hipStream_t stream) {
+  // 2, 4, 8, 16 and 32 workgroups a CU: 16 pools of 32 KiB pages 65.0, 67.6, 67.2, 66.2
+  // and 65.0 us, 48 pools of 4 KiB pages 36.1, 30.5, 28.6, 29.5 and 27.7
   const int wgs = pools.n > 0 && b.pages > 0 ? std::min(cus * 8, kCompactGroups) : 0;
   const int64_t grid = (int64_t)wgs + (book ? b.rows : 0);
   if (grid == 0) return hipSuccess;
