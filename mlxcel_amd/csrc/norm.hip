@@ -10,7 +10,7 @@
 // takes a row and holds it in registers, 8 elements (one or two 16-byte loads)
 // a lane and vector, so nothing is read twice; all loads, the weights' too, are
 // issued before the first sum, so a single row waits for memory once (1 x 4096:
-// 5.2 us, the launch's own time; 2047 x 2880 with a gate and both norms: 14.7 us,
+// 5.0 us, the launch's own time; 2047 x 2880 with a gate and both norms: 14.8 us,
 // 4.0 TB/s of its 59 MB).
 #include <hip/hip_runtime.h>
 
