@@ -12,8 +12,7 @@ U = 2.0 ** -24
 
 def attention(q, k, v, table, lengths, scale, softcap=0.0, window=0, sinks=None, split=0.0):
     """q (B, Hq, D), pools (pages, Hkv, page, D) as float64; (out, slack).
-    split: what a probability loses where it enters a product as two 16-bit
-    numbers (2^-17 of it in bfloat16, 2^-22 in float16).
+    split: a relative loss of each probability to allow for besides.
 
     Slack: a score of D products differs by (D + 8) u sum|q k| scale (its
     rounding, the cap and the change of base included); p then by twice the
