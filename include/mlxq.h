@@ -436,6 +436,84 @@ mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* toke
                                 float scale, mlxq_array* logprobs, mlxq_array* entropy,
                                 mlxq_array* top_logprobs, mlxq_array* top_ids, void* stream);
 
+/* As mlxq_paged_attention for several new tokens per sequence (prompts, parts
+ * of them, drafted tokens): rows starts[b] .. starts[b + 1] - 1 of q (T, query
+ * heads, width) are the last of the lengths[b] tokens of sequence b, whose keys
+ * and values are in the pages already; each sees the keys up to its own (of
+ * which the last `window`, where that is not 0).  starts (B + 1) int32
+ * ascending; rows of no sequence are left as they were, tokens before a
+ * sequence's first (more rows than its length) give zeros.  The result does not
+ * depend on how a prompt is cut into calls, up to the order of 32-bit sums.
+ * Types, layouts, sinks, infinities: as there. */
+mlxq_status mlxq_paged_attention_chunk(const mlxq_array* q, const mlxq_array* k_pool,
+                                       const mlxq_array* v_pool, const mlxq_array* table,
+                                       const mlxq_array* lengths, const mlxq_array* starts,
+                                       const mlxq_array* sinks, float scale, float softcap,
+                                       int32_t window, mlxq_array* out, void* stream);
+
+/* How the frequencies base^(-2 i / dims) of the dims / 2 pairs are scaled for
+ * contexts `factor` times the `original` number of tokens. */
+typedef enum mlxq_rotary_scaling {
+  MLXQ_ROTARY_PLAIN = 0,  /* not at all */
+  MLXQ_ROTARY_LINEAR = 1, /* all divided by factor */
+  MLXQ_ROTARY_BASE = 2,   /* base grows by factor^(dims / (dims - 2)) */
+  MLXQ_ROTARY_BANDS = 3,  /* divided where a pair turns at most `low` times over the original
+                             tokens, kept from `high` turns on, between them in proportion */
+  MLXQ_ROTARY_RAMP = 4    /* as BANDS, in proportion to the pair's number between those (rounded
+                             outwards) that turn `high` and `low` times; attention_factor is
+                             0.1 ln(factor) + 1 */
+} mlxq_rotary_scaling;
+
+/* Writes the dims / 2 frequencies and the factor of mlxq_rotary (1 except for
+ * RAMP) to HOST memory; worked out in 64 bits, rounded once.  Arguments that a
+ * scaling does not name are not looked at. */
+mlxq_status mlxq_rotary_frequencies(int32_t dims, double base, int32_t scaling, double factor,
+                                    double original, double low, double high, float* inv_freq,
+                                    float* attention_factor);
+
+/* Rotates the first 2 n elements of every head of x (T, heads, width) by the
+ * position of its token: pair i, elements (i, n + i) or, interleaved,
+ * (2 i, 2 i + 1), by positions[t] * inv_freq[i], times factor; the elements
+ * after them are copied.  positions (T) int32 of either sign (the negated
+ * positions give the gradient for x, and turn cached keys back); inv_freq (n)
+ * float32.  bfloat16, float16 or float32, any strides; heads of at most 4096
+ * elements; out may be x.  Angles are taken in 64 bits, the products in 32,
+ * the result is rounded once. */
+mlxq_status mlxq_rotary(const mlxq_array* x, const mlxq_array* positions,
+                        const mlxq_array* inv_freq, bool interleaved, float factor,
+                        mlxq_array* out, void* stream);
+
+/* mlxq_rotary of q (T, query heads, width) to out, which may be q, and of
+ * k (T, kv heads, width) on its way to where mlxq_cache_append would write it,
+ * with v beside it as it is.  Tokens that have no place there (as in
+ * mlxq_cache_append) have their queries rotated all the same. */
+mlxq_status mlxq_rotary_append(const mlxq_array* q, const mlxq_array* k, const mlxq_array* v,
+                               const mlxq_array* k_pool, const mlxq_array* v_pool,
+                               const mlxq_array* table, const mlxq_array* positions,
+                               const mlxq_array* rows, const mlxq_array* lengths,
+                               const mlxq_array* inv_freq, bool interleaved, float factor,
+                               mlxq_array* out, void* stream);
+
+/* out = logits (T, V), of the same type, after, for each row t (each step NULL:
+ * left out):
+ *   tokens among history[t][0 .. history_lengths[t] - 1]: x / repetition[t] where
+ *     x > 0, else x * repetition[t];
+ *   those among them at place prompts[t] or later, `times` of them:
+ *     x - (presence[t] + frequency[t] * times);
+ *   the token bias_ids[t][j]: x + bias[t][j] (of equal ids the last j counts);
+ *   tokens whose bit of mask[t] is 0 (bit v % 32 of word v / 32): -inf.
+ * history (T, n), history_lengths (NULL: n each), prompts (NULL: 0), bias_ids
+ * (T, m), mask (T, ceil(V / 32)) int32; repetition, presence, frequency (T),
+ * bias (T, m) float32.  Tokens outside the row are passed over.  32-bit
+ * arithmetic, rounded once; logits that no step names keep their bits.  Any
+ * strides; out may be logits. */
+mlxq_status mlxq_adjust_logits(const mlxq_array* logits, const mlxq_array* history,
+                               const mlxq_array* history_lengths, const mlxq_array* prompts,
+                               const mlxq_array* repetition, const mlxq_array* presence,
+                               const mlxq_array* frequency, const mlxq_array* bias_ids,
+                               const mlxq_array* bias, const mlxq_array* mask, mlxq_array* out,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -59,6 +59,11 @@ SYMBOLS = (
     "mlxq_cache_compact",
     "mlxq_residual_norm",
     "mlxq_token_logprobs",
+    "mlxq_paged_attention_chunk",
+    "mlxq_rotary_frequencies",
+    "mlxq_rotary",
+    "mlxq_rotary_append",
+    "mlxq_adjust_logits",
 )
 
 _lib = None
@@ -110,6 +115,12 @@ def load() -> ctypes.CDLL:
     lib.mlxq_cache_compact.argtypes = [I32, AA] + [A] * 4 + [P]
     lib.mlxq_residual_norm.argtypes = [A] * 4 + [F, A, F, F, A, A, P]
     lib.mlxq_token_logprobs.argtypes = [A, A, I32, F, A, A, A, A, P]
+    lib.mlxq_paged_attention_chunk.argtypes = [A] * 7 + [F, F, I32, A, P]
+    D, FP = ctypes.c_double, ctypes.POINTER(F)
+    lib.mlxq_rotary_frequencies.argtypes = [I32, D, I32, D, D, D, D, FP, FP]
+    lib.mlxq_rotary.argtypes = [A] * 3 + [B, F, A, P]
+    lib.mlxq_rotary_append.argtypes = [A] * 10 + [B, F, A, P]
+    lib.mlxq_adjust_logits.argtypes = [A] * 11 + [P]
     lib.mlxq_workspace_reserve.argtypes = [ctypes.c_size_t, P]
     lib.mlxq_get_cache_memory.argtypes = []
     lib.mlxq_clear_cache.argtypes = []

@@ -62,6 +62,9 @@ SOURCES = {
     "pages.hip": [],
     "norm.hip": [],
     "logprobs.hip": [],
+    "rotary.hip": [],
+    "chunk.hip": [],
+    "adjust.hip": [],
     "scratch.hip": [],
     "dequant.hip": ["-ffp-contract=off"],
 }

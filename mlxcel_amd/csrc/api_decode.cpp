@@ -1,10 +1,12 @@
 // api_decode.cpp — the C ABI of the serving operators around the quantized
 // projections (include/mlxq.h): attention over a paged cache, the cache's
-// pages, residual norms, token log probabilities.  Arguments are checked here
-// and the kernels launched; nothing waits for the device.
+// pages, position rotations, residual norms, logit adjustments, token log
+// probabilities.  Arguments are checked here and the kernels launched; nothing
+// waits for the device.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <utility>
 
 #include "host.hpp"
 #include "kernels.hpp"
@@ -190,6 +192,47 @@ bool matrix_rows(View x, int64_t& row) {
     want = x.a->strides[i] * x.dim(i);
   }
   return true;
+}
+
+// Row-contiguous copies of a call's strided operands in the staging workspace.
+struct Staging {
+  hipStream_t stream;
+  std::vector<std::pair<mlxq_array, const mlxq_array*>> back;  // results to copy out again
+  char* p = nullptr;
+  size_t bytes = 0;
+  void need(const mlxq_array* a) { bytes += padded(View{a}); }
+  void take() {
+    if (bytes) p = static_cast<char*>(stream_workspace(current_device(), stream, bytes, 1));
+  }
+  mlxq_array copy(const mlxq_array* a, bool read, bool write) {
+    mlxq_array c = contiguous_like(a, p);
+    p += padded(View{a});
+    if (read) copy_view(a, &c, stream);
+    if (write) back.push_back({c, a});
+    return c;
+  }
+  void finish() {
+    for (auto& r : back) copy_view(&r.first, r.second, stream);
+  }
+};
+
+// What rotary and rotary_append share: inv_freq, the pair layout, the factor.
+void check_rotation(mlxq::RotaryArgs& a, View x, const mlxq_array* inv_freq, float factor, const char* tag) {
+  View f = operand(inv_freq, tag, "inv_freq", 1, MLXQ_FLOAT32);
+  if (!unit_last(f)) (Refusal(tag) << "inv_freq must be contiguous.").unsupported();
+  if (2 * f.dim(0) > x.dim(2))
+    (Refusal(tag) << "inv_freq has " << f.dim(0) << " pairs but a head has " << x.dim(2) << " elements.").invalid();
+  if (!std::isfinite(factor)) (Refusal(tag) << "factor must be finite.").invalid();
+  a.inv_freq = static_cast<const float*>(inv_freq->data);
+  a.n = (int)std::min<int64_t>(f.dim(0), mlxq::kRotaryMaxD);
+  a.factor = factor;
+}
+void check_heads(int64_t heads, int64_t width, const char* tag) {
+  if (width > mlxq::kRotaryMaxD)
+    (Refusal(tag) << "heads of at most " << mlxq::kRotaryMaxD << " elements are implemented, not " << width << ".")
+        .unsupported();
+  if (heads > mlxq::kRotaryMaxHeads)
+    (Refusal(tag) << "at most " << mlxq::kRotaryMaxHeads << " heads are implemented, not " << heads << ".").unsupported();
 }
 
 }  // namespace
@@ -580,6 +623,297 @@ mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* toke
       a.cnt = counters(dev, stream, tag);
     }
     hip_check(mlxq::launch_token_logprobs(a, stream), "token log probabilities launch");
+  });
+}
+
+mlxq_status mlxq_paged_attention_chunk(const mlxq_array* q, const mlxq_array* k_pool, const mlxq_array* v_pool,
+                                       const mlxq_array* table, const mlxq_array* lengths, const mlxq_array* starts,
+                                       const mlxq_array* sinks, float scale, float softcap, int32_t window,
+                                       mlxq_array* out, void* stream_) {
+  return guarded([&] {
+    const char* tag = "paged_attention_chunk";
+    View x = operand(q, tag, "q", 3, -1);
+    mlxq::ChunkAttnArgs a{};
+    a.type = float_type(x, tag, "q");
+    View k = operand(k_pool, tag, "k_pool", 4, x.dtype()), v = operand(v_pool, tag, "v_pool", 4, x.dtype());
+    same_shape(v, k.shape(), tag, "v_pool");
+    View t = table32(table, tag), l = vec32(lengths, tag, "lengths"), s = vec32(starts, tag, "starts");
+    a.T = fits_int(x.dim(0), tag, "q");
+    a.Hq = fits_int(x.dim(1), tag, "q");
+    a.Hkv = fits_int(k.dim(1), tag, "k_pool");
+    a.B = (int)l.dim(0);
+    if (x.dim(2) != k.dim(3))
+      (Refusal(tag) << "q and the pools must have one head width but have " << x.dim(2) << " and " << k.dim(3) << ".")
+          .invalid();
+    if (a.Hkv < 1 || a.Hq % a.Hkv)
+      (Refusal(tag) << "query heads (" << a.Hq << ") must be a multiple of the pools' heads (" << a.Hkv << ").").invalid();
+    if (t.dim(0) != a.B)
+      (Refusal(tag) << "table and lengths must have as many rows but have shapes " << fmt_shape(t.shape()) << " and "
+                    << fmt_shape(l.shape()) << ".").invalid();
+    if (s.dim(0) != (int64_t)a.B + 1)
+      (Refusal(tag) << "starts must have one entry more than lengths (" << a.B << ") but has shape "
+                    << fmt_shape(s.shape()) << ".").invalid();
+    if (!std::isfinite(scale)) (Refusal(tag) << "scale must be finite.").invalid();
+    if (!std::isfinite(softcap) || softcap < 0.f)
+      (Refusal(tag) << "softcap must be finite and not negative but is " << softcap << ".").invalid();
+    if (window < 0) (Refusal(tag) << "window must not be negative but is " << window << ".").invalid();
+    if (sinks) {
+      View sv = operand(sinks, tag, "sinks", 1, MLXQ_FLOAT32);
+      same_shape(sv, Shape{a.Hq}, tag, "sinks");
+      if (!unit_last(sv)) (Refusal(tag) << "sinks must be contiguous.").unsupported();
+      a.sinks = static_cast<const float*>(sinks->data);
+    }
+    check_out(out, x.shape(), x.dtype(), tag);
+    operand(out, tag, "out", 3, -1);
+    if (x.size() == 0 || a.B == 0) return;
+    if (x.dim(2) % 8 || x.dim(2) > 256)
+      (Refusal(tag) << "head widths up to 256 that are a multiple of 8 are implemented, not " << x.dim(2) << ".")
+          .unsupported();
+    if (!unit_last(k) || !unit_last(v))
+      (Refusal(tag) << "the pools' last axis must be contiguous.").unsupported();
+    if (k.dim(0) < 1 || k.dim(2) < 1) (Refusal(tag) << "the pools have no pages.").invalid();
+    check_capacity(t.dim(1), k.dim(2), tag);
+    a.D = (int)x.dim(2);
+    a.pages = fits_int(k.dim(0), tag, "k_pool");
+    a.page = fits_int(k.dim(2), tag, "k_pool");
+    a.width = (int)t.dim(1);
+    a.window = window;
+    a.scale = scale;
+    a.softcap = softcap;
+    a.k = k_pool->data;
+    a.v = v_pool->data;
+    a.k_page = k_pool->strides[0], a.k_head = k_pool->strides[1], a.k_tok = k_pool->strides[2];
+    a.v_page = v_pool->strides[0], a.v_head = v_pool->strides[1], a.v_tok = v_pool->strides[2];
+    a.table = static_cast<const int32_t*>(table->data);
+    a.table_row = table->strides[0];
+    a.lengths = static_cast<const int32_t*>(lengths->data);
+    a.starts = static_cast<const int32_t*>(starts->data);
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
+    const bool stage_q = !unit_last(x), stage_out = !View{out}.row_contiguous();
+    Staging st{stream};
+    if (stage_q) st.need(q);
+    if (stage_out) st.need(out);
+    st.take();
+    const mlxq_array qc = stage_q ? st.copy(q, true, false) : *q;
+    // rows of no sequence stay as they are, so the copy begins as out
+    const mlxq_array oc = stage_out ? st.copy(out, true, true) : *out;
+    a.q = qc.data;
+    a.q_tok = qc.strides[0];
+    a.q_head = qc.strides[1];
+    a.out = oc.data;
+    hip_check(mlxq::launch_chunk_attention(a, stream), "chunk attention launch");
+    st.finish();
+  });
+}
+
+mlxq_status mlxq_rotary_frequencies(int32_t dims, double base, int32_t scaling, double factor, double original, double low,
+                                    double high, float* inv_freq, float* attention_factor) {
+  return guarded([&] {
+    const char* tag = "rotary_frequencies";
+    const double turn = 6.283185307179586476925;
+    if (dims < 2 || dims % 2) (Refusal(tag) << "dims must be even and at least 2 but is " << dims << ".").invalid();
+    if (!(base > 1.0) || !std::isfinite(base)) (Refusal(tag) << "base must be finite and above 1 but is " << base << ".").invalid();
+    if (scaling < MLXQ_ROTARY_PLAIN || scaling > MLXQ_ROTARY_RAMP)
+      (Refusal(tag) << "scaling " << scaling << " is not one of the header's.").invalid();
+    if (scaling != MLXQ_ROTARY_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor)))
+      (Refusal(tag) << "factor must be finite and at least 1 but is " << factor << ".").invalid();
+    if (scaling == MLXQ_ROTARY_BASE && dims < 4)
+      (Refusal(tag) << "a grown base needs at least 4 dims.").invalid();
+    if (scaling >= MLXQ_ROTARY_BANDS &&
+        (!(original > 0.0) || !std::isfinite(original) || !(low > 0.0) || !(high > low) || !std::isfinite(high)))
+      (Refusal(tag) << "original must be above zero and 0 < low < high but they are " << original << ", " << low << " and "
+                    << high << ".").invalid();
+    if (!inv_freq || !attention_factor) (Refusal(tag) << "inv_freq and attention_factor must not be NULL.").invalid();
+    if (scaling == MLXQ_ROTARY_BASE) base *= std::pow(factor, (double)dims / (dims - 2));
+    // the pair that turns r times over the original length
+    auto pair_at = [&](double r) { return dims * std::log(original / (r * turn)) / (2.0 * std::log(base)); };
+    const double first = std::max(std::floor(pair_at(high)), 0.0);
+    const double last = std::min(std::ceil(pair_at(low)), dims - 1.0);
+    for (int i = 0; i < dims / 2; i++) {
+      const double f = std::pow(base, -2.0 * i / dims);
+      double keep = 1.0;  // how much of f stays, the rest being f / factor
+      if (scaling == MLXQ_ROTARY_LINEAR) keep = 0.0;
+      // turns over the original length: all kept from `high` on, none up to `low`
+      if (scaling == MLXQ_ROTARY_BANDS) keep = std::min(std::max((original * f / turn - low) / (high - low), 0.0), 1.0);
+      if (scaling == MLXQ_ROTARY_RAMP)
+        keep = 1.0 - std::min(std::max((i - first) / std::max(last - first, 1e-3), 0.0), 1.0);
+      inv_freq[i] = (float)(keep * f + (1.0 - keep) * f / factor);
+    }
+    *attention_factor = scaling == MLXQ_ROTARY_RAMP ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
+  });
+}
+
+mlxq_status mlxq_rotary(const mlxq_array* x, const mlxq_array* positions, const mlxq_array* inv_freq, bool interleaved,
+                        float factor, mlxq_array* out, void* stream_) {
+  return guarded([&] {
+    const char* tag = "rotary";
+    View xv = operand(x, tag, "x", 3, -1);
+    mlxq::RotaryArgs a{};
+    a.type = float_type(xv, tag, "x");
+    same_shape(vec32(positions, tag, "positions"), Shape{xv.dim(0)}, tag, "positions");
+    check_rotation(a, xv, inv_freq, factor, tag);
+    check_out(out, xv.shape(), xv.dtype(), tag);
+    View ov = operand(out, tag, "out", 3, -1);
+    if (xv.size() == 0) return;
+    check_heads(xv.dim(1), xv.dim(2), tag);
+    a.T = fits_int(xv.dim(0), tag, "x");
+    a.Hq = (int)xv.dim(1);
+    a.D = (int)xv.dim(2);
+    a.interleaved = interleaved;
+    a.positions = static_cast<const int32_t*>(positions->data);
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
+    Staging st{stream};
+    if (!unit_last(xv)) st.need(x);
+    if (!unit_last(ov)) st.need(out);
+    st.take();
+    const mlxq_array xc = unit_last(xv) ? *x : st.copy(x, true, false), oc = unit_last(ov) ? *out : st.copy(out, false, true);
+    a.q = xc.data, a.q_tok = xc.strides[0], a.q_head = xc.strides[1];
+    a.out = oc.data, a.out_tok = oc.strides[0], a.out_head = oc.strides[1];
+    hip_check(mlxq::launch_rotary(a, stream), "rotary launch");
+    st.finish();
+  });
+}
+
+mlxq_status mlxq_rotary_append(const mlxq_array* q, const mlxq_array* k, const mlxq_array* v, const mlxq_array* k_pool,
+                               const mlxq_array* v_pool, const mlxq_array* table, const mlxq_array* positions,
+                               const mlxq_array* rows, const mlxq_array* lengths, const mlxq_array* inv_freq,
+                               bool interleaved, float factor, mlxq_array* out, void* stream_) {
+  return guarded([&] {
+    const char* tag = "rotary_append";
+    View qv = operand(q, tag, "q", 3, -1);
+    mlxq::RotaryArgs a{};
+    a.type = float_type(qv, tag, "q");
+    View kv = operand(k, tag, "k", 3, qv.dtype()), vv = operand(v, tag, "v", 3, qv.dtype());
+    if (kv.dim(0) != qv.dim(0) || kv.dim(2) != qv.dim(2))
+      (Refusal(tag) << "q and k must have the same tokens and width but have shapes " << fmt_shape(qv.shape()) << " and "
+                    << fmt_shape(kv.shape()) << ".").invalid();
+    same_shape(vv, kv.shape(), tag, "v");
+    View kp = operand(k_pool, tag, "k_pool", 4, qv.dtype()), vp = operand(v_pool, tag, "v_pool", 4, qv.dtype());
+    same_shape(vp, kp.shape(), tag, "v_pool");
+    if (kp.dim(1) != kv.dim(1) || kp.dim(3) != kv.dim(2))
+      (Refusal(tag) << "k and the pools must have the same heads and width but have shapes " << fmt_shape(kv.shape())
+                    << " and " << fmt_shape(kp.shape()) << ".").invalid();
+    View t = table32(table, tag);
+    same_shape(vec32(positions, tag, "positions"), Shape{kv.dim(0)}, tag, "positions");
+    same_shape(vec32(rows, tag, "rows"), Shape{kv.dim(0)}, tag, "rows");
+    if (lengths) same_shape(vec32(lengths, tag, "lengths"), Shape{t.dim(0)}, tag, "lengths");
+    check_rotation(a, qv, inv_freq, factor, tag);
+    check_out(out, qv.shape(), qv.dtype(), tag);
+    View ov = operand(out, tag, "out", 3, -1);
+    if (qv.size() == 0 && kv.size() == 0) return;
+    check_heads(qv.dim(1) + 2 * kv.dim(1), qv.dim(2), tag);
+    if (!unit_last(kp) || !unit_last(vp)) (Refusal(tag) << "the pools' last axis must be contiguous.").unsupported();
+    a.T = fits_int(qv.dim(0), tag, "q");
+    a.Hq = (int)qv.dim(1);
+    a.D = (int)qv.dim(2);
+    a.interleaved = interleaved;
+    a.positions = static_cast<const int32_t*>(positions->data);
+    if (kv.size() > 0 && t.size() > 0) {  // a table without pages takes no token
+      if (kp.dim(0) < 1 || kp.dim(2) < 1) (Refusal(tag) << "the pools have no pages.").invalid();
+      check_capacity(t.dim(1), kp.dim(2), tag);
+      a.Hkv = (int)kv.dim(1);
+      a.kp = k_pool->data, a.vp = v_pool->data;
+      a.kp_page = k_pool->strides[0], a.kp_head = k_pool->strides[1], a.kp_tok = k_pool->strides[2];
+      a.vp_page = v_pool->strides[0], a.vp_head = v_pool->strides[1], a.vp_tok = v_pool->strides[2];
+      a.table = static_cast<const int32_t*>(table->data);
+      a.table_row = table->strides[0];
+      a.rows = static_cast<const int32_t*>(rows->data);
+      a.lengths = lengths ? static_cast<const int32_t*>(lengths->data) : nullptr;
+      a.table_rows = (int)t.dim(0);
+      a.width = (int)t.dim(1);
+      a.pages = fits_int(kp.dim(0), tag, "k_pool");
+      a.page = fits_int(kp.dim(2), tag, "k_pool");
+    }
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
+    Staging st{stream};
+    if (!unit_last(qv)) st.need(q);
+    if (!unit_last(kv)) st.need(k);
+    if (!unit_last(vv)) st.need(v);
+    if (!unit_last(ov)) st.need(out);
+    st.take();
+    const mlxq_array qc = unit_last(qv) ? *q : st.copy(q, true, false), kc = unit_last(kv) ? *k : st.copy(k, true, false);
+    const mlxq_array vc = unit_last(vv) ? *v : st.copy(v, true, false), oc = unit_last(ov) ? *out : st.copy(out, false, true);
+    a.q = qc.data, a.q_tok = qc.strides[0], a.q_head = qc.strides[1];
+    a.k = kc.data, a.k_tok = kc.strides[0], a.k_head = kc.strides[1];
+    a.v = vc.data, a.v_tok = vc.strides[0], a.v_head = vc.strides[1];
+    a.out = oc.data, a.out_tok = oc.strides[0], a.out_head = oc.strides[1];
+    hip_check(mlxq::launch_rotary(a, stream), "rotary append launch");
+    st.finish();
+  });
+}
+
+mlxq_status mlxq_adjust_logits(const mlxq_array* logits, const mlxq_array* history, const mlxq_array* history_lengths,
+                               const mlxq_array* prompts, const mlxq_array* repetition, const mlxq_array* presence,
+                               const mlxq_array* frequency, const mlxq_array* bias_ids, const mlxq_array* bias,
+                               const mlxq_array* mask, mlxq_array* out, void* stream_) {
+  return guarded([&] {
+    const char* tag = "adjust_logits";
+    View x = operand(logits, tag, "logits", 2, -1);
+    mlxq::AdjustArgs a{};
+    a.type = float_type(x, tag, "logits");
+    const int64_t T = x.dim(0), V = x.dim(1);
+    // a matrix of T rows, each dense
+    auto rows = [&](const mlxq_array* r, const char* name, int dtype, int64_t& stride) -> const void* {
+      View v = operand(r, tag, name, 2, dtype);
+      if (v.dim(0) != T)
+        (Refusal(tag) << name << " must have one row a row of logits (" << T << ") but has shape " << fmt_shape(v.shape())
+                      << ".").invalid();
+      if (!unit_last(v)) (Refusal(tag) << name << "'s rows must be contiguous.").unsupported();
+      fits_int(v.dim(1), tag, name);
+      stride = r->strides[0];
+      return r->data;
+    };
+    auto each = [&](const mlxq_array* r, const char* name, int dtype) -> const void* {
+      if (!r) return nullptr;
+      if (!history) (Refusal(tag) << name << " needs a history.").invalid();
+      View v = operand(r, tag, name, 1, dtype);
+      same_shape(v, Shape{T}, tag, name);
+      if (!unit_last(v)) (Refusal(tag) << name << " must be contiguous.").unsupported();
+      return r->data;
+    };
+    if (history) {
+      a.history = static_cast<const int32_t*>(rows(history, "history", MLXQ_INT32, a.history_row));
+      a.n = (int)View{history}.dim(1);
+    }
+    a.history_lengths = static_cast<const int32_t*>(each(history_lengths, "history_lengths", MLXQ_INT32));
+    a.prompts = static_cast<const int32_t*>(each(prompts, "prompts", MLXQ_INT32));
+    a.repetition = static_cast<const float*>(each(repetition, "repetition", MLXQ_FLOAT32));
+    a.presence = static_cast<const float*>(each(presence, "presence", MLXQ_FLOAT32));
+    a.frequency = static_cast<const float*>(each(frequency, "frequency", MLXQ_FLOAT32));
+    if ((bias_ids != nullptr) != (bias != nullptr)) (Refusal(tag) << "bias_ids and bias go together.").invalid();
+    if (bias_ids) {
+      a.bias_ids = static_cast<const int32_t*>(rows(bias_ids, "bias_ids", MLXQ_INT32, a.bias_ids_row));
+      a.bias = static_cast<const float*>(rows(bias, "bias", MLXQ_FLOAT32, a.bias_row));
+      same_shape(View{bias}, View{bias_ids}.shape(), tag, "bias");
+      a.m = (int)View{bias}.dim(1);
+    }
+    if (mask) {
+      a.mask = static_cast<const uint32_t*>(rows(mask, "mask", MLXQ_INT32, a.mask_row));
+      same_shape(View{mask}, Shape{T, (V + 31) / 32}, tag, "mask");
+    }
+    check_out(out, x.shape(), x.dtype(), tag);
+    View ov = operand(out, tag, "out", 2, -1);
+    if (x.size() == 0) return;
+    if (V > ((int64_t)1 << 30)) (Refusal(tag) << "rows of " << V << " logits are too long.").unsupported();
+    a.T = fits_int(T, tag, "logits");
+    a.V = (int)V;
+    if (mlxq::adjust_logits_groups(a) > mlxq::kMaxGroups)
+      (Refusal(tag) << "too many logits (" << T << " rows of " << V << ") for one call.").unsupported();
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const StreamTurn turn(stream);
+    Staging st{stream};
+    if (!unit_last(x)) st.need(logits);
+    if (!unit_last(ov)) st.need(out);
+    st.take();
+    const mlxq_array xc = unit_last(x) ? *logits : st.copy(logits, true, false);
+    const mlxq_array oc = unit_last(ov) ? *out : st.copy(out, false, true);
+    a.x = xc.data, a.x_row = xc.strides[0];
+    a.out = oc.data, a.out_row = oc.strides[0];
+    hip_check(mlxq::launch_adjust_logits(a, stream), "adjust logits launch");
+    st.finish();
   });
 }
 

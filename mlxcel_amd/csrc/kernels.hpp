@@ -677,4 +677,61 @@ struct LogprobArgs {
 void token_logprobs_plan(LogprobArgs& a, int cus, int64_t* part_bytes);
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream);
 
+// Rotation of heads by their tokens' positions (rotary.hip); with key heads also
+// the append of keys, rotated, and values to their pages.
+constexpr int kRotaryMaxD = 4096, kRotaryMaxHeads = 1 << 15;
+struct RotaryArgs {
+  const void *q, *k, *v;   // [T][Hq][D], [T][Hkv][D] (the last axis dense)
+  void *out, *kp, *vp;     // [T][Hq][D], [pages][Hkv][page][D]
+  const float* inv_freq;   // [n]
+  int64_t q_tok, q_head, out_tok, out_head, k_tok, k_head, v_tok, v_head;  // strides in elements
+  int64_t kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok;
+  const int32_t *table, *positions, *rows, *lengths;  // with Hkv; lengths: null, or tokens past them are left out
+  int64_t table_row;
+  int T, Hq, Hkv, D, n, table_rows, width, pages, page;
+  int interleaved;         // pairs (2 i, 2 i + 1), or (i, n + i)
+  float factor;
+  int type;
+  int unit_shift;          // lanes of a head (launch_rotary)
+};
+hipError_t launch_rotary(const RotaryArgs& a, hipStream_t stream);
+
+// Several new tokens per sequence over its pages (chunk.hip): row t of q is
+// token t - starts[b] of the sequence b with starts[b] <= t < starts[b + 1], whose
+// tokens are the last of its lengths[b].
+struct ChunkAttnArgs {
+  const void *q, *k, *v;   // [T][Hq][D], [pages][Hkv][page][D] (the last axis dense, any other strides)
+  void* out;               // [T][Hq][D], row-contiguous
+  const int32_t* table;    // [B][width] page numbers
+  const int32_t *lengths, *starts;  // [B], [B + 1]
+  const float* sinks;      // [Hq] or null
+  int64_t q_tok, q_head;   // strides in elements
+  int64_t k_page, k_head, k_tok, v_page, v_head, v_tok;
+  int64_t table_row;
+  int T, B, Hq, Hkv, D, pages, page, width;
+  int window;              // keys a token sees, itself the last (0: all)
+  float scale, softcap;    // as PagedAttnArgs
+  int type;
+};
+hipError_t launch_chunk_attention(const ChunkAttnArgs& a, hipStream_t stream);
+
+// Penalties, biases and a mask on logits (adjust.hip)
+struct AdjustArgs {
+  const void* x;           // [T][V]
+  void* out;               // [T][V], may be x
+  int64_t x_row, out_row;  // strides in elements
+  const int32_t* history;  // [T][n] or null
+  int64_t history_row;
+  const int32_t *history_lengths, *prompts;             // [T] or null
+  const float *repetition, *presence, *frequency;       // [T] or null
+  const int32_t* bias_ids;  // [T][m] or null
+  const float* bias;        // [T][m]
+  int64_t bias_ids_row, bias_row;
+  const uint32_t* mask;     // [T][(V + 31) / 32] or null
+  int64_t mask_row;
+  int T, V, n, m, type;
+};
+int64_t adjust_logits_groups(const AdjustArgs& a);  // workgroups (kMaxGroups at most in a launch)
+hipError_t launch_adjust_logits(const AdjustArgs& a, hipStream_t stream);
+
 }  // namespace mlxq

@@ -547,11 +547,94 @@ PyObject* token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// The result: a new tensor of t's shape and type, or the one that is given (o: None or a tensor).
+at::Tensor result_like(const at::Tensor& t, PyObject* o, Arr& r) {
+  if (o != Py_None) {
+    r = on(o, t.device());
+    return {};
+  }
+  const at::Tensor out = at::empty(t.sizes(), t.options().requires_grad(false));
+  fill(r, out);
+  return out;
+}
+
+// (q, k_pool, v_pool, table, lengths, starts, sinks, scale, softcap, window, out)
+PyObject* paged_attention_chunk(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 11, [&]() -> PyObject* {
+    const at::Tensor& q = tensor(v[0]);
+    const at::Device dev = q.device();
+    Arr a[7];
+    for (int i = 0; i < 7; i++) a[i] = on(v[i], dev);
+    const float scale = number(v[7]), softcap = number(v[8]);
+    const int window = integer(v[9], 0);
+    Arr o;
+    const at::Tensor out = result_like(q, v[10], o);
+    call(dev, [&](void* stream) {
+      return mlxq_paged_attention_chunk(a[0].p(), a[1].p(), a[2].p(), a[3].p(), a[4].p(), a[5].p(), a[6].p(), scale,
+                                        softcap, window, &o.a, stream);
+    });
+    return keep(v[10], out);
+  });
+}
+
+// (x, positions, inv_freq, interleaved, factor, out)
+PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 6, [&]() -> PyObject* {
+    const at::Tensor& x = tensor(v[0]);
+    const at::Device dev = x.device();
+    Arr a[3];
+    for (int i = 0; i < 3; i++) a[i] = on(v[i], dev);
+    const bool interleaved = boolean(v[3]);
+    const float factor = number(v[4]);
+    Arr o;
+    const at::Tensor out = result_like(x, v[5], o);
+    call(dev, [&](void* stream) { return mlxq_rotary(a[0].p(), a[1].p(), a[2].p(), interleaved, factor, &o.a, stream); });
+    return keep(v[5], out);
+  });
+}
+
+// (q, k, v, k_pool, v_pool, table, positions, rows, lengths, inv_freq, interleaved, factor, out)
+PyObject* rotary_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 13, [&]() -> PyObject* {
+    const at::Tensor& q = tensor(v[0]);
+    const at::Device dev = q.device();
+    Arr a[10];
+    for (int i = 0; i < 10; i++) a[i] = on(v[i], dev);
+    const bool interleaved = boolean(v[10]);
+    const float factor = number(v[11]);
+    Arr o;
+    const at::Tensor out = result_like(q, v[12], o);
+    call(dev, [&](void* stream) {
+      return mlxq_rotary_append(a[0].p(), a[1].p(), a[2].p(), a[3].p(), a[4].p(), a[5].p(), a[6].p(), a[7].p(), a[8].p(),
+                                a[9].p(), interleaved, factor, &o.a, stream);
+    });
+    return keep(v[12], out);
+  });
+}
+
+// (logits, history, history_lengths, prompts, repetition, presence, frequency, bias_ids, bias, mask, out)
+PyObject* adjust_logits(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return entry(n, 11, [&]() -> PyObject* {
+    const at::Tensor& x = tensor(v[0]);
+    const at::Device dev = x.device();
+    Arr a[10];
+    for (int i = 0; i < 10; i++) a[i] = on(v[i], dev);
+    Arr o;
+    const at::Tensor out = result_like(x, v[10], o);
+    call(dev, [&](void* stream) {
+      return mlxq_adjust_logits(a[0].p(), a[1].p(), a[2].p(), a[3].p(), a[4].p(), a[5].p(), a[6].p(), a[7].p(), a[8].p(),
+                                a[9].p(), &o.a, stream);
+    });
+    return keep(v[10], out);
+  });
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quantized_matmul), FAST(quantized_matmul_multi), FAST(gather_qmm), FAST(dequantize),
                          FAST(quantize),         FAST(fused_moe),
                          FAST(paged_attention),  FAST(cache_reserve),          FAST(cache_append), FAST(cache_fork),
                          FAST(cache_free),       FAST(cache_compact),          FAST(residual_norm), FAST(token_logprobs),
+                         FAST(paged_attention_chunk), FAST(rotary),            FAST(rotary_append), FAST(adjust_logits),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mlxq_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -35,6 +35,7 @@ class _ctypes_only:
     dequantize = quantize = fused_moe = staticmethod(lambda *a: None)
     paged_attention = residual_norm = token_logprobs = staticmethod(lambda *a: None)
     cache_reserve = cache_append = cache_fork = cache_free = cache_compact = staticmethod(lambda *a: None)
+    paged_attention_chunk = rotary = rotary_append = adjust_logits = staticmethod(lambda *a: None)
 
 
 def _load_native():
@@ -538,6 +539,118 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top_k: int = 0
         out[3] = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
     _run("mlxq_token_logprobs", dev, logits, tokens, int(top_k), scale, *out)
     return tuple(out)
+
+
+def paged_attention_chunk(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
+                          lengths: torch.Tensor, starts: torch.Tensor, *, window: int = 0, softcap: float = 0.0,
+                          sinks: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attention`` for several new tokens per sequence: rows ``starts[b]``
+    to ``starts[b + 1] - 1`` of ``q`` (T, query heads, width) are the last of
+    sequence b's ``lengths[b]`` tokens, whose keys and values are in the pages
+    already; each sees the keys up to its own (the last ``window`` of them).
+    ``starts`` (B + 1) int32, ascending.  Rows of no sequence are left as they were
+    in ``out`` (undefined in a new one); tokens before a sequence's first give
+    zeros."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+    r = _native.paged_attention_chunk(q, k_pool, v_pool, table, lengths, starts, sinks, scale, softcap, window, out)
+    if r is not None:
+        return _done(r)
+    dev = _together(q, k_pool, v_pool, table, lengths, starts, sinks, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _run("mlxq_paged_attention_chunk", dev, q, k_pool, v_pool, table, lengths, starts, sinks, scale, softcap, window, out)
+    return out
+
+
+_ROTARY_SCALING = {None: 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
+
+
+def rotary_frequencies(dims: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
+                       original: float = 0.0, low: Optional[float] = None, high: Optional[float] = None, device="cuda"):
+    """``(inv_freq, attention_factor)`` for ``rotary``: ``base ** (-2 i / dims)``
+    for the ``dims / 2`` pairs, float32, and a float.  ``scaling`` for contexts
+    ``factor`` times the ``original`` tokens: "linear" divides all by factor;
+    "base" grows the base by ``factor ** (dims / (dims - 2))``; "bands" divides
+    those that turn at most ``low`` (1) times over the original tokens, keeps
+    those that turn ``high`` (4) times or more and takes the ones between in
+    proportion; "ramp" is that in proportion to the pair's number, between
+    ``high`` (32) and ``low`` (1) turns, with an attention factor of
+    ``0.1 ln(factor) + 1``."""
+    if scaling not in _ROTARY_SCALING:
+        raise ValueError(f"[rotary_frequencies] scaling must be one of {list(_ROTARY_SCALING)} but is {scaling!r}.")
+    low = 1.0 if low is None else low
+    high = (32.0 if scaling == "ramp" else 4.0) if high is None else high
+    inv, by = (ctypes.c_float * max(int(dims) // 2, 1))(), ctypes.c_float()
+    st = _lib.load().mlxq_rotary_frequencies(int(dims), base, _ROTARY_SCALING[scaling], factor, original, low, high, inv,
+                                             ctypes.byref(by))
+    if st:
+        _raise(st)
+    return torch.tensor(list(inv), dtype=torch.float32, device=device), by.value
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
+           factor: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates the first ``2 n`` elements of every head of ``x`` (T, heads, width)
+    by its token's position: pair i, elements ``(i, n + i)`` or, interleaved,
+    ``(2 i, 2 i + 1)``, by ``positions[t] * inv_freq[i]``, times ``factor``; the rest
+    is copied.  ``positions`` (T) int32, ``inv_freq`` (n) float32
+    (``rotary_frequencies``).  ``-positions`` give the gradient for x.  ``out`` may be
+    x."""
+    r = _native.rotary(x, positions, inv_freq, interleaved, factor, out)
+    if r is not None:
+        return _done(r)
+    dev = _together(x, positions, inv_freq, out)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    _run("mlxq_rotary", dev, x, positions, inv_freq, bool(interleaved), factor, out)
+    return out
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                  table: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, inv_freq: torch.Tensor, *,
+                  lengths: Optional[torch.Tensor] = None, interleaved: bool = False, factor: float = 1.0,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rotary`` of ``q`` (T, query heads, width), which it returns, and of ``k`` (T,
+    kv heads, width) on its way into the pages, with ``v`` beside it:
+    ``cache_append`` of the rotated keys in one launch.  Tokens that have no place
+    in the cache (a row, position or page out of range, at or past ``lengths``) are
+    left out of it; their queries are rotated all the same."""
+    r = _native.rotary_append(q, k, v, k_pool, v_pool, table, positions, rows, lengths, inv_freq, interleaved, factor, out)
+    if r is not None:
+        return _done(r)
+    dev = _together(q, k, v, k_pool, v_pool, table, positions, rows, lengths, inv_freq, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _run("mlxq_rotary_append", dev, q, k, v, k_pool, v_pool, table, positions, rows, lengths, inv_freq, bool(interleaved),
+         factor, out)
+    return out
+
+
+def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
+                  history_lengths: Optional[torch.Tensor] = None, prompts: Optional[torch.Tensor] = None,
+                  repetition: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                  frequency: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties, biases and a grammar's mask on ``logits`` (T, V), in this order:
+    tokens among the first ``history_lengths[t]`` of ``history`` (T, n) are divided
+    by ``repetition[t]`` where positive and multiplied by it elsewhere; those at
+    place ``prompts[t]`` or later lose ``presence[t] + frequency[t] * times``;
+    ``bias[t, j]`` is added to token ``bias_ids[t, j]`` (of equal ids the last
+    counts); tokens whose bit of ``mask`` (T, ceil(V / 32)) is 0 (bit ``v % 32`` of
+    word ``v // 32``) become -inf.  int32 and float32; steps that are not given are
+    left out.  ``out`` may be ``logits``."""
+    args = (history, history_lengths, prompts, repetition, presence, frequency, bias_ids, bias, mask)
+    r = _native.adjust_logits(logits, *args, out)
+    if r is not None:
+        return _done(r)
+    dev = _together(logits, *args, out)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    _run("mlxq_adjust_logits", dev, logits, *args, out)
+    return out
 
 
 def workspace_reserve(nbytes: int, device: Optional[torch.device] = None) -> None:

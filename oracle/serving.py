@@ -1,6 +1,7 @@
 """Plain 64-bit forms of the serving operators (test infrastructure only):
-attention of single tokens over a paged cache, the cache's bookkeeping,
-residual norms and token log probabilities.  numpy, one row at a time.
+attention of single tokens and of chunks over a paged cache, the cache's
+bookkeeping, position rotations, residual norms, logit adjustments and token
+log probabilities.  numpy, one row at a time.
 
 Each float result comes with `slack`, what 32-bit arithmetic may differ from it
 by, from the sizes of the terms (u = 2^-24, a 32-bit rounding); rounding the
@@ -165,3 +166,73 @@ def token_logprobs(x, tokens, k, scale=1.0):
     order = np.where(np.isnan(x), np.inf, x)
     ids = np.lexsort((np.broadcast_to(np.arange(V), x.shape), -order, ~np.isnan(x)), axis=-1)[:, :k]
     return given, entropy, np.take_along_axis(lp, ids, -1), ids, dl, de
+
+
+def chunk_attention(q, k, v, table, lengths, starts, scale, softcap=0.0, window=0, sinks=None, split=0.0):
+    """q (T, Hq, D): (out, slack, which rows belong to a sequence).  Token i of n
+    new ones is the last of a sequence of length - n + i + 1 tokens."""
+    out, slack, live = np.zeros(q.shape), np.zeros(q.shape), np.zeros(len(q), bool)
+    cap = table.shape[1] * k.shape[2]
+    for b, length in enumerate(lengths):
+        t = np.arange(starts[b], starts[b + 1])
+        ends = min(max(int(length), 0), cap) - (starts[b + 1] - t) + 1
+        rows = np.repeat(table[b:b + 1], len(t), 0)
+        out[t], slack[t] = attention(q[t], k, v, rows, ends, scale, softcap, window, sinks, split)
+        live[t] = True
+    return out, slack, live
+
+
+def rotary(x, positions, inv_freq, interleaved=False, factor=1.0):
+    """x (T, H, D): (y, slack).
+
+    Slack: an angle of up to 2^20 turns differs by 2^-30 turns (64 bits, two
+    roundings); what is left of it, at most pi / 4, is rounded to 32 bits and its
+    sine and cosine come from series of five terms: 4 u; the factor, a product and
+    the sum round once each."""
+    n = len(inv_freq)
+    # exact: 31 and 24 bits of a 64-bit significand, then whole turns off
+    angle = positions.astype(np.longdouble)[:, None] * inv_freq.astype(np.longdouble)
+    turn = 2 * np.longdouble("3.14159265358979323846264338327950288")
+    angle = (angle - turn * np.round(angle / turn)).astype(np.float64)[:, None]
+    c, s = factor * np.cos(angle), factor * np.sin(angle)
+    first, second = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if interleaved else (slice(0, n), slice(n, 2 * n))
+    a, b = x[..., first], x[..., second]
+    y, slack = x.copy(), np.zeros(x.shape)
+    y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+    slack[..., first] = slack[..., second] = 8 * U * abs(factor) * (np.abs(a) + np.abs(b))
+    return y, slack
+
+
+def adjust_logits(x, history=None, history_lengths=None, prompts=None, repetition=None, presence=None, frequency=None,
+                  bias_ids=None, bias=None, mask=None):
+    """x (T, V) float64: (y, slack, which logits a step changed).  Slack: a rounding of each step."""
+    T, V = x.shape
+    y, slack, changed = x.copy(), np.zeros(x.shape), np.zeros(x.shape, bool)
+    for t in range(T):
+        if history is not None:
+            n = history.shape[1] if history_lengths is None else min(max(int(history_lengths[t]), 0), history.shape[1])
+            p = 0 if prompts is None else int(prompts[t])
+            times = {}
+            for i, v in enumerate(history[t, :n].tolist()):
+                if 0 <= v < V:
+                    times[v] = times.get(v, 0) + (i >= p)
+            for v, c in times.items():
+                changed[t, v] = True
+                if repetition is not None:
+                    y[t, v] = y[t, v] / repetition[t] if y[t, v] > 0 else y[t, v] * repetition[t]
+                    slack[t, v] += U * abs(y[t, v])
+                if c:
+                    a, b = (0.0 if w is None else w[t] * k for w, k in ((presence, 1), (frequency, c)))
+                    y[t, v] -= a + b
+                    slack[t, v] += U * (2 * abs(a) + 2 * abs(b) + abs(y[t, v]))
+        if bias is not None:
+            last = {v: j for j, v in enumerate(bias_ids[t].tolist()) if 0 <= v < V}
+            for v, j in last.items():
+                changed[t, v] = True
+                y[t, v] += bias[t, j]
+                slack[t, v] += U * abs(y[t, v])
+        if mask is not None:
+            bits = (mask[t].astype(np.int64)[:, None] >> np.arange(32)) & 1
+            off = bits.reshape(-1)[:V] == 0
+            y[t, off], slack[t, off], changed[t, off] = -np.inf, 0, True
+    return y, slack, changed

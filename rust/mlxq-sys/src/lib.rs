@@ -155,6 +155,31 @@ pub mod sys {
             logprobs: *mut mlxq_array, entropy: *mut mlxq_array, top_logprobs: *mut mlxq_array,
             top_ids: *mut mlxq_array, stream: *mut c_void,
         ) -> i32;
+        pub fn mlxq_paged_attention_chunk(
+            q: *const mlxq_array, k_pool: *const mlxq_array, v_pool: *const mlxq_array, table: *const mlxq_array,
+            lengths: *const mlxq_array, starts: *const mlxq_array, sinks: *const mlxq_array, scale: f32, softcap: f32,
+            window: i32, out: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_rotary_frequencies(
+            dims: i32, base: f64, scaling: i32, factor: f64, original: f64, low: f64, high: f64, inv_freq: *mut f32,
+            attention_factor: *mut f32,
+        ) -> i32;
+        pub fn mlxq_rotary(
+            x: *const mlxq_array, positions: *const mlxq_array, inv_freq: *const mlxq_array, interleaved: bool,
+            factor: f32, out: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_rotary_append(
+            q: *const mlxq_array, k: *const mlxq_array, v: *const mlxq_array, k_pool: *const mlxq_array,
+            v_pool: *const mlxq_array, table: *const mlxq_array, positions: *const mlxq_array,
+            rows: *const mlxq_array, lengths: *const mlxq_array, inv_freq: *const mlxq_array, interleaved: bool,
+            factor: f32, out: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
+        pub fn mlxq_adjust_logits(
+            logits: *const mlxq_array, history: *const mlxq_array, history_lengths: *const mlxq_array,
+            prompts: *const mlxq_array, repetition: *const mlxq_array, presence: *const mlxq_array,
+            frequency: *const mlxq_array, bias_ids: *const mlxq_array, bias: *const mlxq_array,
+            mask: *const mlxq_array, out: *mut mlxq_array, stream: *mut c_void,
+        ) -> i32;
     }
 }
 
@@ -684,6 +709,108 @@ pub unsafe fn token_logprobs(
     };
     check(sys::mlxq_token_logprobs(
         logits.as_raw(), tokens.as_raw(), k, scale, logprobs.as_raw_mut(), entropy.as_raw_mut(), lp, ids, stream,
+    ))
+}
+
+/// Attention of several new tokens per sequence: rows `starts[b] .. starts[b + 1]`
+/// of `q` `[T, query heads, width]` are the last of `lengths[b]` tokens.  Rows of
+/// no sequence are left as they were in `out`.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn paged_attention_chunk(
+    q: &ArrayView, k_pool: &ArrayView, v_pool: &ArrayView, table: &ArrayView, lengths: &ArrayView, starts: &ArrayView,
+    sinks: Option<&ArrayView>, scale: f32, softcap: f32, window: i32, out: &mut ArrayView, stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_paged_attention_chunk(
+        q.as_raw(), k_pool.as_raw(), v_pool.as_raw(), table.as_raw(), lengths.as_raw(), starts.as_raw(), opt(sinks),
+        scale, softcap, window, out.as_raw_mut(), stream,
+    ))
+}
+
+/// How [`rotary_frequencies`] scales for contexts `factor` times `original` tokens
+/// (`mlxq_rotary_scaling` in `include/mlxq.h`).
+#[derive(Clone, Copy, Debug, PartialEq)]
+pub enum RotaryScaling {
+    Plain,
+    Linear { factor: f64 },
+    Base { factor: f64 },
+    Bands { factor: f64, original: f64, low: f64, high: f64 },
+    Ramp { factor: f64, original: f64, low: f64, high: f64 },
+}
+
+/// The `dims / 2` frequencies of [`rotary`] and its factor, worked out on the host.
+pub fn rotary_frequencies(dims: i32, base: f64, scaling: RotaryScaling) -> Result<(Vec<f32>, f32)> {
+    let (kind, factor, original, low, high) = match scaling {
+        RotaryScaling::Plain => (0, 1.0, 0.0, 0.0, 0.0),
+        RotaryScaling::Linear { factor } => (1, factor, 0.0, 0.0, 0.0),
+        RotaryScaling::Base { factor } => (2, factor, 0.0, 0.0, 0.0),
+        RotaryScaling::Bands { factor, original, low, high } => (3, factor, original, low, high),
+        RotaryScaling::Ramp { factor, original, low, high } => (4, factor, original, low, high),
+    };
+    let mut inv_freq = vec![0f32; (dims.max(2) / 2) as usize];
+    let mut by = 1f32;
+    // SAFETY: writes dims / 2 floats and one to host memory.
+    check(unsafe {
+        sys::mlxq_rotary_frequencies(dims, base, kind, factor, original, low, high, inv_freq.as_mut_ptr(), &mut by)
+    })?;
+    Ok((inv_freq, by))
+}
+
+/// Rotates the first `2 n` elements of the heads of `x` `[T, heads, width]` by
+/// `positions` `[T]` times `inv_freq` `[n]` (device memory), times `factor`.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn rotary(
+    x: &ArrayView, positions: &ArrayView, inv_freq: &ArrayView, interleaved: bool, factor: f32, out: &mut ArrayView,
+    stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_rotary(
+        x.as_raw(), positions.as_raw(), inv_freq.as_raw(), interleaved, factor, out.as_raw_mut(), stream,
+    ))
+}
+
+/// [`rotary`] of `q` to `out` and of `k` on its way into the pages, with `v` beside
+/// it: [`cache_append`] of the rotated keys in one launch.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn rotary_append(
+    q: &ArrayView, k: &ArrayView, v: &ArrayView, k_pool: &ArrayView, v_pool: &ArrayView, table: &ArrayView,
+    positions: &ArrayView, rows: &ArrayView, lengths: Option<&ArrayView>, inv_freq: &ArrayView, interleaved: bool,
+    factor: f32, out: &mut ArrayView, stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_rotary_append(
+        q.as_raw(), k.as_raw(), v.as_raw(), k_pool.as_raw(), v_pool.as_raw(), table.as_raw(), positions.as_raw(),
+        rows.as_raw(), opt(lengths), inv_freq.as_raw(), interleaved, factor, out.as_raw_mut(), stream,
+    ))
+}
+
+/// The parts of [`adjust_logits`]; what is `None` is left out.
+#[derive(Default)]
+pub struct LogitAdjustments<'a> {
+    pub history: Option<&'a ArrayView>,
+    pub history_lengths: Option<&'a ArrayView>,
+    pub prompts: Option<&'a ArrayView>,
+    pub repetition: Option<&'a ArrayView>,
+    pub presence: Option<&'a ArrayView>,
+    pub frequency: Option<&'a ArrayView>,
+    pub bias_ids: Option<&'a ArrayView>,
+    pub bias: Option<&'a ArrayView>,
+    pub mask: Option<&'a ArrayView>,
+}
+
+/// Penalties, biases and a grammar's mask on `logits` `[T, V]`.
+///
+/// # Safety
+/// As [`paged_attention`].
+pub unsafe fn adjust_logits(
+    logits: &ArrayView, a: &LogitAdjustments, out: &mut ArrayView, stream: *mut c_void,
+) -> Result<()> {
+    check(sys::mlxq_adjust_logits(
+        logits.as_raw(), opt(a.history), opt(a.history_lengths), opt(a.prompts), opt(a.repetition), opt(a.presence),
+        opt(a.frequency), opt(a.bias_ids), opt(a.bias), opt(a.mask), out.as_raw_mut(), stream,
     ))
 }
 
