@@ -702,6 +702,13 @@ mlxq_status mlxq_paged_attention_chunk(const mlxq_array* q, const mlxq_array* k_
     a.q_tok = qc.strides[0];
     a.q_head = qc.strides[1];
     a.out = oc.data;
+    const int dev = current_device();
+    int64_t part_bytes = 0;
+    if (!mlxq::chunk_attention_plan(a, device_cus(dev), &part_bytes))
+      (Refusal(tag) << a.T << " tokens over a table of " << a.B << " rows of " << t.dim(1) << " pages are too many for one call.")
+          .unsupported();
+    a.part = static_cast<float*>(stream_workspace(dev, stream, part_bytes, 0));
+    a.cnt = counters(dev, stream, tag);
     hip_check(mlxq::launch_chunk_attention(a, stream), "chunk attention launch");
     st.finish();
   });

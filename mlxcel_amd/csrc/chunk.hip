@@ -4,9 +4,33 @@
 //   s_j = cap(q_i . k_j * scale)   over the keys j that token i sees: (p - window, p], p = length - new + i
 //   o_i = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m))
 //
-// One wave a token and query head: a lane scores one of 64 keys at a time, then
-// holds some columns of the result while the 64 probabilities go round.
+// A tile is up to 128 rows, (token, query head) pairs of one key head, over the
+// keys that any of them sees.  Its workgroup takes 32 keys a step: the step's K
+// and V rows are loaded while the step before is worked on and go to LDS in the
+// order of their keys, whatever pages they come from.  Each of the four waves has
+// 32 rows, with O, the running maximum and the running sum in registers.  Both
+// products are 32x32 MFMAs whose operands need no exchange between lanes:
+//   S^T[key][row] = K Q^T: lane (c, g) = (lane % 32, lane / 32) ends with keys
+//     8 i + 4 g + e (i, e < 4) of row c, so a row's maximum and sum are taken
+//     within a lane and its neighbour lane ^ 32;
+//   O^T[d][row] += V^T P^T: the lane's keys are those it holds P of; V comes out
+//     of LDS transposed (16-bit types: four keys of a column a read).
+// 16-bit products take P as the sum of two 16-bit numbers: bfloat16 ones leave
+// out at most 2^-17 of it, float16 ones 2^-23 or 2^-39 of the largest.
+//
+// The work is cut evenly whatever the lengths: a tile counts its keys and kAround
+// more, and workgroup w takes [w n, (w + 1) n) of all tiles laid end to end,
+// rounded to whole steps.  Lengths and starts are on the device, so each workgroup
+// finds its first tile from a scan over the sequences and, among the tiles of
+// one, from the closed form of their sum.  A tile that crosses a workgroup's end
+// leaves its sum, maximum and output so far in scratch; the last of its workgroups
+// to arrive joins them, in the order of the keys, so the result does not depend on
+// who came last.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -16,89 +40,702 @@ namespace mlxq {
 
 namespace {
 
+constexpr int kWaves = 4, kRows = 32 * kWaves;
+constexpr int kKeys = 32;  // of a step
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// What a tile's start and end cost, in keys.
+constexpr int kAround = 64;
+// Keys of a tile that is not cut, and the least that a workgroup takes.
+constexpr int kWhole = 4 * kKeys, kLeast = 4 * kKeys;
+
+// Workgroups whose results one of them joins, and how many are read at a time.
+constexpr int kJoin = 16, kFlight = 8;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// 16-byte loads of element alignment (rows of any stride)
+typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
+
+// XT: GEN_BF16 / GEN_F16 / GEN_F32.  DP: head width rounded up.
+template <int XT, int DP>
+struct Geo {
+  static constexpr bool F32 = XT == GEN_F32;
+  static constexpr int ES = F32 ? 4 : 2;
+  static constexpr int CE = 16 / ES;            // elements of 16 bytes
+  static constexpr int C = DP / CE;             // 16-byte chunks of a row
+  static constexpr int DT = DP / 32;            // 32-column tiles of O
+  static constexpr int NI = (kKeys * C + 255) / 256;  // chunks of K (of V) that a thread loads
+  static constexpr int TILE = kKeys * C * 16;   // bytes of a step's K (V) in LDS
+  static constexpr int LDS = 4 * TILE + 64;     // two steps, K and V; flags
+  // Workgroups a CU holds: by registers
+  static constexpr int WGS = DP * ES <= 256 ? 2 : 1;
+  // K's chunk c of row r lies at chunk c ^ swizzle_k(r): 16 lanes that read one
+  // chunk of 16 rows then hit all banks (rows are C chunks apart).
+  static constexpr int LOW = (C & -C) < 16 ? (C & -C) : 16;
+  static __device__ __forceinline__ int swizzle_k(int r) { return (r / (16 / LOW)) & (LOW - 1); }
+  // V's: four rows are read 64 bytes each at a time, which then lie in different
+  // quarters of the banks (rows are C / 4 quarters apart).
+  static __device__ __forceinline__ int swizzle_v(int r) {
+    if constexpr (F32 || (C / 4) % 2 == 1) return 0;
+    else if constexpr ((C / 4) % 4 == 2) return ((r >> 1) & 1) * 4;
+    else return (r & 3) * 4;
+  }
+};
+
 template <int XT>
-__device__ __forceinline__ float element(const void* p, int64_t i) {
-  if constexpr (XT == GEN_F32) return static_cast<const float*>(p)[i];
-  else return xt_to_f32<XT == GEN_F16 ? 1 : 0>(static_cast<const uint16_t*>(p)[i]);
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if constexpr (XT == GEN_BF16) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)lo, (_Float16)hi});
+  }
 }
 template <int XT>
-__device__ __forceinline__ void store_element(void* p, int64_t i, float v) {
-  if constexpr (XT == GEN_F32) static_cast<float*>(p)[i] = v;
-  else static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_xt<XT == GEN_F16 ? 1 : 0>(v);
+__device__ __forceinline__ float half(uint32_t w, int hi) {
+  return xt_to_f32<XT == GEN_F16 ? 1 : 0>(hi ? w >> 16 : w & 0xFFFFu);
 }
+
+template <int XT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (XT == GEN_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Four rows of the lane's column: row i of the 16 lanes' 4 x 16 elements is read
+// by lanes 4 i .. 4 i + 3, lane j gets column j.
+__device__ __forceinline__ u32x2 read_transposed(const char* p) {
+  typedef __attribute__((address_space(3))) s16x4* ptr;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(uint32_t)(uintptr_t)(
+                                       (__attribute__((address_space(3))) const char*)p)));
+}
+
+// Four values to consecutive places.
+template <int XT>
+__device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
+  if constexpr (XT == GEN_F32) {
+    typedef float f32x4_e __attribute__((ext_vector_type(4), aligned(4)));
+    *reinterpret_cast<f32x4_e*>(static_cast<float*>(p) + i) = f32x4_e{v[0], v[1], v[2], v[3]};
+  } else {
+    typedef uint32_t u32x2_e __attribute__((ext_vector_type(2), aligned(2)));
+    uint32_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) h[e] = f32_to_xt<XT == GEN_F16 ? 1 : 0>(v[e]);
+    *reinterpret_cast<u32x2_e*>(static_cast<uint16_t*>(p) + i) = u32x2_e{h[0] | h[1] << 16, h[2] | h[3] << 16};
+  }
+}
+
+// Probabilities are held as 2^lift p: in float16 their largest is then 2^14, and
+// those down to 2^-28 of it keep all their bits (smaller ones differ by 2^-39 of it).
+template <int XT>
+constexpr float kLift = XT == GEN_F16 ? 14.f : 0.f;
+
+// exp2(a - b), 0 where a is -inf (also where b is)
 __device__ __forceinline__ float exp2_diff(float a, float b) {
   return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
 }
 
+// Whether one of the two 16-bit numbers (the 32-bit number) is infinite or NaN.
 template <int XT>
-__global__ __launch_bounds__(256) void chunk_attention_kernel(const ChunkAttnArgs a) {
-  __shared__ float qs[4][256];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
-  const bool mine = unit < (int64_t)a.T * a.Hq;
-  const int t = mine ? (int)(unit / a.Hq) : 0, h = mine ? (int)(unit % a.Hq) : 0;
-  for (int d = lane; d < a.D; d += 64) qs[wave][d] = element<XT>(a.q, t * a.q_tok + h * a.q_head + d);
-  __syncthreads();
-  if (!mine) return;
-  // the last sequence that starts at or before t
-  int lo = 0, hi = a.B;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.starts[mid] <= t) lo = mid + 1;
-    else hi = mid;
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  constexpr uint32_t E = XT == GEN_F16 ? 0x7C00u : 0x7F80u;
+  if constexpr (XT == GEN_F32) return (w & 0x7F800000u) == 0x7F800000u;
+  else return (w & E) == E || (w & E << 16) == E << 16;
+}
+
+// The new tokens of a sequence that have a position, and its tiles.
+struct Seq {
+  int first, n, p0;  // row of the first of n tokens, its position
+  int tiles;         // of a head
+  int skip;          // rows before `first` without a position
+};
+
+// Rows of a tile: tt tokens of hp heads.
+__device__ __forceinline__ Seq seq_of(const ChunkAttnArgs& a, int start, int end, int length) {
+  const int st = min(max(start, 0), a.T), all = min(max(end, st), a.T) - st;
+  const int len = (int)min((int64_t)max(length, 0), (int64_t)a.width * a.page);
+  Seq s;
+  s.skip = max(all - len, 0);
+  s.n = all - s.skip;
+  s.first = st + s.skip;
+  s.p0 = len - s.n;
+  s.tiles = (s.n + a.tile_tokens - 1) / a.tile_tokens;
+  return s;
+}
+__device__ __forceinline__ int tile_lo(const ChunkAttnArgs& a, const Seq& s, int j) {
+  return a.window > 0 ? max(0, s.p0 + j * a.tile_tokens - a.window + 1) : 0;
+}
+__device__ __forceinline__ int tile_hi(const ChunkAttnArgs& a, const Seq& s, int j) {
+  return s.p0 + min(s.n, (j + 1) * a.tile_tokens);
+}
+// sum over tiles i < j of kAround + tile_hi(i) - tile_lo(i)
+__device__ __forceinline__ int64_t before(const ChunkAttnArgs& a, const Seq& s, int j) {
+  const int64_t tt = a.tile_tokens;
+  int64_t sum = j * (int64_t)(kAround + s.p0) + tt * ((int64_t)j * (j + 1) / 2);
+  if (j == s.tiles) sum -= j * tt - s.n;
+  if (a.window > 0) {
+    const int64_t lo = (int64_t)s.p0 - a.window + 1;
+    const int i0 = lo > 0 ? 0 : (int)((uint32_t)-lo / (uint32_t)tt) + 1;  // the first tile that does not begin at key 0
+    if (j > i0) sum -= (j - i0) * lo + tt * ((int64_t)j * (j - 1) / 2 - (int64_t)i0 * (i0 - 1) / 2);
   }
-  const int b = lo - 1;
-  if (b < 0 || t >= a.starts[b + 1]) return;
-  const int64_t cap = (int64_t)a.width * a.page;
-  const int len = (int)min((int64_t)max(a.lengths[b], 0), cap);
-  const int p = len - (a.starts[b + 1] - t), k1 = p + 1, k0 = a.window > 0 ? max(0, k1 - a.window) : 0;
-  const int kh = h / (a.Hq / a.Hkv);
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = k0; k < k1; k += 64) {
-    const int key = min(k + lane, k1 - 1);
-    const int pid = min(max(a.table[b * a.table_row + key / a.page], 0), a.pages - 1), off = key % a.page;
-    float s = 0.f;
-    for (int d = 0; d < a.D; d++)
-      s = fmaf(qs[wave][d], element<XT>(a.k, pid * a.k_page + kh * a.k_head + off * a.k_tok + d), s);
-    s *= a.scale;
-    if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
-    s = k + lane < k1 ? s * kLog2e : -INFINITY;
-    const float M = fmaxf(m, wave_max(s, lane)), f = exp2_diff(m, M), e = exp2_diff(s, M);
-    m = M;
-    l = l * f + wave_sum(e, lane);
-    for (int i = 0; i < 4; i++) o[i] *= f;
-    for (int j = 0; j < min(64, k1 - k); j++) {
-      const float w = __shfl(e, j);
-      const int vp = __shfl(pid, j), vo = __shfl(off, j);
-      for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < a.D)
-          o[i] = fmaf(w, element<XT>(a.v, vp * a.v_page + kh * a.v_head + vo * a.v_tok + lane + 64 * i), o[i]);
+  return sum;
+}
+// v / d for 0 <= v < 2^52
+__device__ __forceinline__ int64_t divide(int64_t v, int64_t d) {
+  int64_t q = (int64_t)((double)v / (double)d);
+  while (q * d > v) q--;
+  while ((q + 1) * d <= v) q++;
+  return q;
+}
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// Words of one partial result: O [rows][DP], then (m, l) [rows][2].
+constexpr int part_words(int rows, int DP) { return rows * (DP + 2); }
+
+template <int XT, int DP>
+__global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kernel(const ChunkAttnArgs a) {
+  using G = Geo<XT, DP>;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ uint32_t arrived;
+  uint32_t* const bad = reinterpret_cast<uint32_t*>(lds + 4 * G::TILE);  // [2][waves]: the step's V has values that are not finite
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, g = lane >> 5;
+  // neighbours in the order of the keys on one XCD
+  const int w = a.wgs % 8 == 0 ? (int)(blockIdx.x % 8) * (a.wgs / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  const int per = a.Hq / a.Hkv, hp = a.tile_heads, tiles_h = (per + hp - 1) / hp, heads_b = a.Hkv * tiles_h;
+
+  // Where this workgroup's work begins and ends: tile among those of sequence b, key of its range.
+  struct Bound {
+    int b, tile, key;
+    int64_t base;  // of the sequence, among all units
+  };
+  auto load_seq = [&](int b) -> Seq {
+    const int s = __builtin_amdgcn_readfirstlane(a.starts[b]), e = __builtin_amdgcn_readfirstlane(a.starts[b + 1]);
+    return seq_of(a, s, e, __builtin_amdgcn_readfirstlane(a.lengths[b]));
+  };
+  auto bound_at = [&](int64_t off, int b, int64_t base) -> Bound {
+    const Seq s = load_seq(b);
+    const int64_t head = before(a, s, s.tiles);
+    const int hh = (int)divide(off, head);
+    off -= hh * head;
+    int lo = 0, hi = s.tiles - 1;  // the last tile that begins at or before off
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (before(a, s, mid) <= off) lo = mid;
+      else hi = mid - 1;
+    }
+    const int keys = tile_hi(a, s, lo) - tile_lo(a, s, lo);
+    const int64_t r = off - before(a, s, lo) - kAround;
+    int key = r > 0 ? (int)r / kKeys * kKeys : 0, tile = hh * s.tiles + lo;
+    if (keys <= kWhole && off > before(a, s, lo)) key = 0, tile++;  // it belongs to the workgroup that begins it
+    return Bound{b, tile, key, base};
+  };
+  auto clear = [&](const Seq& s) {  // rows without a position
+    const int64_t from = (int64_t)(s.first - s.skip) * a.Hq * a.D, n = (int64_t)s.skip * a.Hq * a.D;
+    for (int64_t i = 4 * tid; i < n; i += 1024) store4<XT>(a.out, from + i, f32x4{0.f, 0.f, 0.f, 0.f});
+  };
+  int64_t total, n;
+  Bound at, end;
+  {
+    auto units_of = [&](const Seq& s) { return heads_b * before(a, s, s.tiles); };
+    auto per_group = [&]() { return max((int64_t)((double)total * a.inv_wgs) + 1, (int64_t)kLeast); };
+    int64_t sum, mine;
+    auto scan = [&]() {
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const int64_t o = __shfl_up(sum, s);
+        if (lane >= s) sum += o;
+      }
+    };
+    if (a.B <= 64) {  // each wave finds them by itself, sequence i in lane i
+      const Seq s = lane < a.B ? seq_of(a, a.starts[lane], a.starts[lane + 1], a.lengths[lane]) : Seq{0, 0, 0, 0, 0};
+      sum = mine = units_of(s);
+      scan();
+      total = __shfl(sum, 63);
+      total = uniform(total);
+      n = per_group();
+      auto find = [&](int64_t p) -> Bound {
+        if (p >= total) return Bound{a.B, 0, 0, total};
+        const int i = __builtin_ctzll(__ballot(sum - mine <= p && p < sum));
+        const int64_t base = uniform(__shfl(sum - mine, i));
+        return bound_at(p - base, i, base);
+      };
+      at = find(w * n);
+      end = find((w + 1) * n);
+      for (uint64_t none = __ballot(s.skip > 0); none; none &= none - 1) {
+        const int b = __builtin_ctzll(none);
+        if (b % a.wgs == w) clear(load_seq(b));
+      }
+    } else {  // thread i sums those of its share
+      int64_t* sums = reinterpret_cast<int64_t*>(lds);
+      Bound* bound = reinterpret_cast<Bound*>(lds + 64);
+      const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
+      mine = 0;
+      for (int b = b0; b < b1; b++) mine += units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
+      sum = mine;
+      scan();
+      if (lane == 63) sums[wave] = sum;
+      __syncthreads();
+      int64_t ahead = sum - mine;
+      total = 0;
+#pragma unroll
+      for (int i = 0; i < kWaves; i++) {
+        if (i < wave) ahead += sums[i];
+        total += sums[i];
+      }
+      total = uniform(total);
+      n = per_group();
+      for (int i = 0; i < 2; i++) {
+        const int64_t p = (w + i) * n;
+        if (p >= total) {
+          if (tid == 0) bound[i] = Bound{a.B, 0, 0, total};
+        } else if (ahead <= p && p < ahead + mine) {
+          int64_t base = ahead;
+          for (int b = b0; b < b1; b++) {
+            const int64_t u = units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
+            if (p < base + u) {
+              bound[i] = Bound{b, 0, 0, base};
+              break;
+            }
+            base += u;
+          }
+        }
+      }
+      for (int b = w; b < a.B; b += a.wgs) {
+        const Seq s = load_seq(b);
+        if (s.skip > 0) clear(s);
+      }
+      __syncthreads();
+      auto find = [&](int i) -> Bound {
+        const int b = __builtin_amdgcn_readfirstlane(bound[i].b);
+        const int64_t base = uniform(bound[i].base);
+        return b >= a.B ? Bound{b, 0, 0, base} : bound_at((w + i) * n - base, b, base);
+      };
+      at = find(0);
+      end = find(1);
+      __syncthreads();  // the LDS is free again
     }
   }
-  if (a.sinks && k1 > k0) {
-    const float sink = a.sinks[h] * kLog2e, M = fmaxf(m, sink), f = exp2_diff(m, M);
-    l = l * f + exp2_diff(sink, M);
-    for (int i = 0; i < 4; i++) o[i] *= f;
+
+  // a thread's chunks of a step's rows
+  int row_i[G::NI], dofs[G::NI], kofs[G::NI], vofs[G::NI];
+  bool dead[G::NI];
+#pragma unroll
+  for (int i = 0; i < G::NI; i++) {
+    const int slot = min(i * 256 + tid, kKeys * G::C - 1), r = slot / G::C, ch = slot - r * G::C;
+    row_i[i] = r;
+    dead[i] = ch * G::CE >= a.D;
+    dofs[i] = dead[i] ? 0 : ch * 16;
+    kofs[i] = (r * G::C + (ch ^ G::swizzle_k(r))) * 16;
+    vofs[i] = (r * G::C + (ch ^ G::swizzle_v(r))) * 16;
   }
-  for (int i = 0; i < 4; i++)
-    if (lane + 64 * i < a.D)
-      store_element<XT>(a.out, ((int64_t)t * a.Hq + h) * a.D + lane + 64 * i, k1 > k0 ? o[i] / l : 0.f);
+  const bool plain = a.softcap == 0.f && a.scale > 0.f;
+  // scores in units of log2 e
+  const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
+  const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)4 * a.wgs * a.slot_words * 4));
+
+  Seq sq = at.b < a.B ? load_seq(at.b) : Seq{};
+  int64_t head_units = at.b < a.B ? before(a, sq, sq.tiles) : 0;
+  while (at.b < a.B && (at.b < end.b || (at.b == end.b && (at.tile < end.tile || (at.tile == end.tile && at.key < end.key))))) {
+    if (at.tile >= heads_b * sq.tiles) {
+      at.base += heads_b * head_units;
+      at.b++;
+      at.tile = at.key = 0;
+      if (at.b < a.B) {
+        sq = load_seq(at.b);
+        head_units = before(a, sq, sq.tiles);
+      }
+      continue;
+    }
+    const int hh = at.tile / sq.tiles, j = at.tile - hh * sq.tiles, hk = hh / tiles_h, ht = hh - hk * tiles_h;
+    const int heads = min(hp, per - hp * ht), head0 = hk * per + hp * ht;
+    const int tok0 = j * a.tile_tokens, toks = min(a.tile_tokens, sq.n - tok0), rows = toks * heads;
+    const int lo = tile_lo(a, sq, j), hi = tile_hi(a, sq, j);
+    const int k0 = lo + at.key, k1 = at.b == end.b && at.tile == end.tile ? min(hi, lo + end.key) : hi;
+    // the tile's workgroups
+    const int64_t p0 = at.base + hh * head_units + before(a, sq, j) + kAround;
+    int w0 = w, w1 = w;
+    if (hi - lo > kWhole && (k0 > lo || k1 < hi)) {
+      w0 = (int)divide(p0 + kKeys + n - 1, n) - 1;
+      w1 = (int)divide(p0 + (hi - lo) + n - 1, n) - 1;
+    }
+
+    // this wave's rows, and the keys that any of them sees
+    const int r0 = 32 * wave, my_row = min(r0 + c, rows - 1), my_tok = my_row / heads;
+    const int pos = sq.p0 + tok0 + my_tok;
+    const bool busy = r0 < rows;
+    const int see1 = pos + 1, see0 = a.window > 0 ? max(0, see1 - a.window) : 0;
+    const int wave_hi = sq.p0 + tok0 + min(r0 + 31, rows - 1) / heads + 1, first_hi = sq.p0 + tok0 + min(r0, rows - 1) / heads + 1;
+    const int wave_lo = a.window > 0 ? max(0, first_hi - a.window) : 0, last_lo = a.window > 0 ? max(0, wave_hi - a.window) : 0;
+    // steps from here on, and those up to there, are masked for some row of the tile
+    const int mask_hi = sq.p0 + tok0 + 1, mask_lo = a.window > 0 ? max(0, hi - a.window) : 0;
+
+    const char* qp = static_cast<const char*>(a.q) +
+                     ((int64_t)(sq.first + tok0 + my_tok) * a.q_tok + (head0 + my_row - my_tok * heads) * a.q_head) * G::ES;
+    u32x4 qf[G::C / 2];
+#pragma unroll
+    for (int i = 0; i < G::C / 2; i++) {
+      const int d = (2 * i + g) * G::CE;
+      const u32x4_e v = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
+      qf[i] = d < a.D ? u32x4{v[0], v[1], v[2], v[3]} : u32x4{0u, 0u, 0u, 0u};
+    }
+    f32x16 o[G::DT];
+#pragma unroll
+    for (int i = 0; i < G::DT; i++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[i][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    const int32_t* table = a.table + at.b * a.table_row;
+    const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES;
+    const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES;
+    int entry[G::NI], in_page[G::NI];
+    u32x4 kr[G::NI], vr[G::NI];
+    // table entries of the rows from key k on; past the range they are the last key's
+    auto look = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < G::NI; i++) {
+        const int key = min(k + row_i[i], hi - 1);
+        const int slot = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
+        in_page[i] = key - slot * a.page;
+        entry[i] = table[slot];
+      }
+    };
+    auto load = [&]() {
+#pragma unroll
+      for (int i = 0; i < G::NI; i++) {
+        const int64_t pid = min(max(entry[i], 0), a.pages - 1);
+        const u32x4_e x = *reinterpret_cast<const u32x4_e*>(kb + (pid * a.k_page + in_page[i] * a.k_tok) * G::ES + dofs[i]);
+        const u32x4_e y = *reinterpret_cast<const u32x4_e*>(vb + (pid * a.v_page + in_page[i] * a.v_tok) * G::ES + dofs[i]);
+        kr[i] = u32x4{x[0], x[1], x[2], x[3]};
+        vr[i] = u32x4{y[0], y[1], y[2], y[3]};
+      }
+    };
+    auto masked = [&](int k) { return k + kKeys > mask_hi || k < mask_lo; };
+    auto put = [&](int stage, int k) {
+      char* p = lds + stage * 2 * G::TILE;
+#pragma unroll
+      for (int i = 0; i < G::NI; i++) {
+        if ((i + 1) * 256 > kKeys * G::C && i * 256 + tid >= kKeys * G::C) continue;
+        *reinterpret_cast<u32x4*>(p + kofs[i]) = dead[i] ? u32x4{0u, 0u, 0u, 0u} : kr[i];
+        *reinterpret_cast<u32x4*>(p + G::TILE + vofs[i]) = vr[i];
+      }
+      if (masked(k)) {
+        bool x = false;
+#pragma unroll
+        for (int i = 0; i < G::NI; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) x |= not_finite<XT>(vr[i][e]);
+        const bool any = __any(x);
+        if (lane == 0) bad[stage * kWaves + wave] = any;
+      }
+    };
+
+    __syncthreads();  // the last tile's steps have been read
+    look(k0);
+    load();
+    if (k0 + kKeys < k1) look(k0 + kKeys);
+    put(0, k0);
+    __syncthreads();
+    for (int k = k0, stage = 0; k < k1; k += kKeys, stage ^= 1) {
+      const bool more = k + kKeys < k1;
+      if (more) {
+        load();
+        if (k + 2 * kKeys < k1) look(k + 2 * kKeys);
+      }
+      if (busy && k < wave_hi && k + kKeys > wave_lo) {
+        const char* ks = lds + stage * 2 * G::TILE;
+        const char* vs = ks + G::TILE;
+        f32x16 s;
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < G::C / 2; i++) {
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (c * G::C + ((2 * i + g) ^ G::swizzle_k(c))) * 16);
+          if constexpr (G::F32) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), s, 0, 0, 0);
+          } else {
+            s = mfma32<XT>(kf, qf[i], s);
+          }
+        }
+        float by = scale;  // what the scores still have to be multiplied with
+        if (!plain) {
+          by = 1.f;
+          if (a.softcap > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = cap_log2e * tanhf(s[e] * scale);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] *= scale;
+          }
+        }
+        const bool hidden = k + kKeys > first_hi || k < last_lo;  // some key from some row of this wave
+        if (hidden) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int key = k + 8 * (e / 4) + 4 * g + e % 4;
+            s[e] = key < see1 && key >= see0 && key < k1 ? s[e] : -INFINITY;
+          }
+        }
+        float mt = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) mt = fmaxf(mt, s[e]);
+        mt = fmaxf(mt, lane_xor<32>(mt, lane)) * by;
+        mt = fmaxf(mt, m);
+        if (__any(mt > m)) {
+          const float f = exp2_diff(m, mt);
+          m = mt;
+          l *= f;
+#pragma unroll
+          for (int i = 0; i < G::DT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[i][e] *= f;
+        }
+        const float off = (m == -INFINITY ? 0.f : m) - kLift<XT>;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], by, -off));
+          sum += s[e];
+        }
+        l += sum;
+        bool safe = false;
+        if (hidden) {
+          uint32_t x = 0;
+#pragma unroll
+          for (int i = 0; i < kWaves; i++) x |= bad[stage * kWaves + i];
+          safe = __builtin_amdgcn_readfirstlane(x) != 0;
+        }
+        if (safe) {
+          // Values that are not finite count only for the rows that see their key: one key at a time
+          for (int i = 0; i < 16; i++) {
+            const float other = lane_xor<32>(s[0], lane);
+#pragma unroll
+            for (int gg = 0; gg < 2; gg++) {
+              const int key = 8 * (i / 4) + 4 * gg + i % 4;
+              const float p = gg == g ? s[0] : other;
+#pragma unroll
+              for (int dt = 0; dt < G::DT; dt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                  const int d = 32 * dt + 8 * (e / 4) + 4 * g + e % 4, ch = d / G::CE;
+                  const char* vp = vs + (key * G::C + (ch ^ G::swizzle_v(key))) * 16 + d % G::CE * G::ES;
+                  float v;
+                  if constexpr (G::F32) v = *reinterpret_cast<const float*>(vp);
+                  else v = half<XT>(*reinterpret_cast<const uint16_t*>(vp), 0);
+                  o[dt][e] = p == 0.f ? o[dt][e] : fmaf(p, v, o[dt][e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 15; e++) s[e] = s[e + 1];
+          }
+        } else if constexpr (G::F32) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int key = 8 * (e / 4) + 4 * g + e % 4;
+#pragma unroll
+            for (int dt = 0; dt < G::DT; dt++) {
+              const float v = *reinterpret_cast<const float*>(vs + key * (G::C * 16) + (32 * dt + c) * 4);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[dt], 0, 0, 0);
+            }
+          }
+        } else {
+          u32x4 pt[2][2];  // [16 keys][term]
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
+              const uint32_t t = pack<XT>(x, y);
+              pt[u][0][e] = t;
+              pt[u][1][e] = pack<XT>(x - half<XT>(t, 0), y - half<XT>(t, 1));
+            }
+          const int i16 = lane & 15, vr4 = i16 >> 2;  // the row and the 8 bytes of it that this lane reads
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++) {
+            const int ch = 4 * dt + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              const int ka = 16 * u + 4 * g + vr4, kc = ka + 8;
+              const u32x2 x = read_transposed(vs + (ka * G::C + (ch ^ G::swizzle_v(ka))) * 16 + (i16 & 1) * 8);
+              const u32x2 y = read_transposed(vs + (kc * G::C + (ch ^ G::swizzle_v(kc))) * 16 + (i16 & 1) * 8);
+              const u32x4 vf = {x[0], x[1], y[0], y[1]};
+              o[dt] = mfma32<XT>(vf, pt[u][0], o[dt]);
+              o[dt] = mfma32<XT>(vf, pt[u][1], o[dt]);
+            }
+          }
+        }
+      }
+      if (more) put(stage ^ 1, k + kKeys);
+      __syncthreads();
+    }
+    l += lane_xor<32>(l, lane);
+
+    // row r of the tile: its place in out, its head
+    auto finish = [&](int r, int d, float M, float L, f32x4 acc) {
+      const int tok = r / heads, h = head0 + r - tok * heads;
+      float f = 1.f;
+      if (a.sinks) {
+        const float x = a.sinks[h];
+        // the largest finite sinks stay finite in the other base
+        const float sink = isinf(x) ? x : fminf(fmaxf(x * kLog2e, -FLT_MAX), FLT_MAX), M2 = fmaxf(M, sink);
+        f = exp2_diff(M, M2);
+        L = L * f + exp2_diff(sink, M2);
+      }
+      if (d < a.D) store4<XT>(a.out, ((int64_t)(sq.first + tok0 + tok) * a.Hq + h) * a.D + d, acc * (f / L));
+    };
+    const bool mine = r0 + c < rows;
+    if (w0 == w1) {
+      if (mine) {
+#pragma unroll
+        for (int dt = 0; dt < G::DT; dt++)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            finish(r0 + c, 32 * dt + 2 * e + 4 * g, m - kLift<XT>, l, f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]});
+      }
+    } else {
+      // bytes of a workgroup's partial result: of its last tile (slot 1), or of one that began before it (slot 0)
+      auto part_at = [&](int v) -> uint32_t { return (uint32_t)((2 * v + (v == w0)) * a.slot_words) * 4u; };
+      // and of the neighbours that it leads, in a place of its own: others of the joining threads may still read the first
+      const uint32_t joined = (uint32_t)(2 * a.wgs * a.slot_words) * 4u;
+      auto put_part = [&](uint32_t p, int r, int d, float M, float L, f32x4 acc) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + (r * DP + d) * 4, 0, kAgentScope);
+        if (d == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
+                                                p + (rows * DP + 2 * r) * 4, 0, kAgentScope);
+      };
+      if (mine) {
+#pragma unroll
+        for (int dt = 0; dt < G::DT; dt++)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            put_part(part_at(w), r0 + c, 32 * dt + 2 * e + 4 * g, m - kLift<XT>, l,
+                     f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]});
+      }
+      // The last of up to kJoin neighbours to arrive joins them; of more, the
+      // last to have joined its neighbours joins the results.
+      auto last_of = [&](uint32_t* cnt, int of) -> bool {
+        __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
+        __syncthreads();
+        if (tid == 0) {
+          const uint32_t old = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          arrived = old == (uint32_t)(of - 1);
+          if (arrived) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        return arrived != 0;
+      };
+      // sum of the results, from byte `from` on, of workgroups v, v + by, .. (of them), in the order of the keys
+      auto join = [&](uint32_t from, int v, int by, int of, int r, int d, float& M, float& L, f32x4& acc) {
+        M = -INFINITY, L = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < of; i0 += kFlight) {
+          u32x4 ow[kFlight];
+          u32x2 mw[kFlight];
+#pragma unroll
+          for (int i = 0; i < kFlight; i++) {
+            const uint32_t p = from + part_at(v + by * min(i0 + i, of - 1));
+            mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + (rows * DP + 2 * r) * 4, 0,
+                                                                                   kAgentScope));
+            ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + (r * DP + d) * 4, 0, kAgentScope));
+          }
+#pragma unroll
+          for (int i = 0; i < kFlight; i++) {
+            if (i0 + i >= of) break;
+            const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
+            const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
+            M = M2;
+            L = L * f + __uint_as_float(mw[i][1]) * fi;
+            acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
+          }
+        }
+      };
+      const int of = w1 - w0 + 1, lead = (w - w0) / kJoin * kJoin, near = min(kJoin, of - lead);
+      // a workgroup may lead neighbours of a tile that began before it and of its last one
+      if (last_of(a.cnt + 2 * (w0 + lead) + (lead == 0), near)) {
+        for (int e = tid; e < rows * (DP / 4); e += 256) {
+          const int r = e / (DP / 4), d = 4 * (e - r * (DP / 4));
+          float M, L;
+          f32x4 acc;
+          join(0, w0 + lead, 1, near, r, d, M, L, acc);
+          if (of <= kJoin) finish(r, d, M, L, acc);
+          else put_part(joined + part_at(w0 + lead), r, d, M, L, acc);
+        }
+        const int groups = (of + kJoin - 1) / kJoin;
+        if (of > kJoin && last_of(a.cnt + 2 * a.wgs + w0, groups)) {
+          for (int e = tid; e < rows * (DP / 4); e += 256) {
+            const int r = e / (DP / 4), d = 4 * (e - r * (DP / 4));
+            float M, L;
+            f32x4 acc;
+            join(joined, w0, kJoin, groups, r, d, M, L, acc);
+            finish(r, d, M, L, acc);
+          }
+        }
+      }
+    }
+    at.tile++;
+    at.key = 0;
+  }
+}
+
+// f(type, width of the kernel)
+template <typename F>
+auto with_kernel(const ChunkAttnArgs& a, F&& f) {
+  auto width = [&](auto xt) {
+    if (a.D <= 64) return f(xt, std::integral_constant<int, 64>{});
+    if (a.D <= 96) return f(xt, std::integral_constant<int, 96>{});
+    if (a.D <= 128) return f(xt, std::integral_constant<int, 128>{});
+    if (a.D <= 192) return f(xt, std::integral_constant<int, 192>{});
+    return f(xt, std::integral_constant<int, 256>{});
+  };
+  if (a.type == GEN_BF16) return width(std::integral_constant<int, GEN_BF16>{});
+  if (a.type == GEN_F16) return width(std::integral_constant<int, GEN_F16>{});
+  return width(std::integral_constant<int, GEN_F32>{});
 }
 
 }  // namespace
 
+bool chunk_attention_plan(ChunkAttnArgs& a, int cus, int64_t* part_bytes) {
+  a.page_shift = 30;
+  while (((int64_t)1 << (a.page_shift - 30)) < a.page) a.page_shift++;
+  // exact for keys below 2^30: the error of page_mul, below page <= 2^(shift - 30), times the key stays below 2^shift
+  a.page_mul = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page - 1) / a.page);
+  const int per = a.Hq / a.Hkv;
+  a.tile_heads = std::min(per, kRows);
+  a.tile_tokens = kRows / a.tile_heads;
+  const int64_t cap = (int64_t)a.width * a.page;
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(cap, (int64_t)a.window + a.tile_tokens) : cap;
+  const int64_t heads = (int64_t)a.Hkv * ((per + a.tile_heads - 1) / a.tile_heads);
+  const int64_t tiles = heads * (((int64_t)a.T + a.tile_tokens - 1) / a.tile_tokens + std::min(a.B, a.T));
+  const int resident = with_kernel(a, [](auto xt, auto dp) { return Geo<decltype(xt)::value, decltype(dp)::value>::WGS; });
+  // tiles are counted in 32 bits, keys of all of them below 2^52
+  if (tiles > (1 << 30) || tiles * (double)(keys + kAround) > 4e15) return false;
+  a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>((tiles * (keys + kAround) + kLeast - 1) / kLeast, (int64_t)cus * resident));
+  a.inv_wgs = 1.0 / a.wgs;
+  const int rows = (int)std::min<int64_t>(kRows, (int64_t)a.T * a.tile_heads);
+  a.slot_words = with_kernel(a, [&](auto, auto dp) { return part_words(rows, decltype(dp)::value); });
+  *part_bytes = (int64_t)4 * a.wgs * a.slot_words * 4;
+  return *part_bytes < ((int64_t)1 << 32);
+}
+
 hipError_t launch_chunk_attention(const ChunkAttnArgs& a, hipStream_t stream) {
   if (a.T == 0 || a.B == 0) return hipSuccess;
-  if (a.D < 8 || a.D > 256 || a.D % 8 || a.pages < 1 || a.page < 1) return hipErrorInvalidValue;
-  const int64_t wgs = ((int64_t)a.T * a.Hq + 3) / 4;
-  if (wgs > kMaxGroups) return hipErrorInvalidValue;
-  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(256), 0, stream, a); };
-  if (a.type == GEN_BF16) run(chunk_attention_kernel<GEN_BF16>);
-  else if (a.type == GEN_F16) run(chunk_attention_kernel<GEN_F16>);
-  else run(chunk_attention_kernel<GEN_F32>);
-  return hipGetLastError();
+  if (a.D < 8 || a.D > 256 || a.D % 8 || a.pages < 1 || a.page < 1 || a.wgs < 1 || 3 * a.wgs > kSplitCounters)
+    return hipErrorInvalidValue;
+  return with_kernel(a, [&](auto xt, auto dp) {
+    constexpr int XT = decltype(xt)::value, DP = decltype(dp)::value;
+    hipLaunchKernelGGL((chunk_attention_kernel<XT, DP>), dim3((unsigned)a.wgs), dim3(256), (Geo<XT, DP>::LDS), stream, a);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace mlxq

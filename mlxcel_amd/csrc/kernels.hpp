@@ -712,7 +712,18 @@ struct ChunkAttnArgs {
   int window;              // keys a token sees, itself the last (0: all)
   float scale, softcap;    // as PagedAttnArgs
   int type;
+  // how the work is split (chunk_attention_plan)
+  int tile_heads, tile_tokens;  // rows of a tile
+  uint32_t page_mul;       // as PagedAttnArgs
+  int page_shift;
+  int wgs;                 // workgroups
+  double inv_wgs;
+  int slot_words;          // of a partial result
+  float* part;             // [4 wgs][slot_words]
+  uint32_t* cnt;           // [3 wgs], zero between launches
 };
+// Sets the plan; part_bytes of scratch are needed.  False where the work cannot be counted.
+bool chunk_attention_plan(ChunkAttnArgs& a, int cus, int64_t* part_bytes);
 hipError_t launch_chunk_attention(const ChunkAttnArgs& a, hipStream_t stream);
 
 // Penalties, biases and a mask on logits (adjust.hip)
