@@ -41,13 +41,12 @@ namespace mlxq {
 namespace {
 
 constexpr int kWaves = 4, kRows = 32 * kWaves;
-constexpr int kKeys = 32;  // of a step
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // What a tile's start and end cost, in keys.
 constexpr int kAround = 64;
 // Keys of a tile that is not cut, and the least that a workgroup takes.
-constexpr int kWhole = 4 * kKeys, kLeast = 4 * kKeys;
+constexpr int kWhole = 128, kLeast = 128;
 
 // Workgroups whose results one of them joins, and how many are read at a time.
 constexpr int kJoin = 16, kFlight = 8;
@@ -64,24 +63,20 @@ struct Geo {
   static constexpr int ES = F32 ? 4 : 2;
   static constexpr int CE = 16 / ES;            // elements of 16 bytes
   static constexpr int C = DP / CE;             // 16-byte chunks of a row
+  static constexpr int NC = (C + 7) / 8;        // blocks of 8 chunks
   static constexpr int DT = DP / 32;            // 32-column tiles of O
-  static constexpr int NI = (kKeys * C + 255) / 256;  // chunks of K (of V) that a thread loads
-  static constexpr int TILE = kKeys * C * 16;   // bytes of a step's K (V) in LDS
-  static constexpr int LDS = 4 * TILE + 64;     // two steps, K and V; flags
+  static constexpr int KEYS = DP * ES <= 512 ? 64 : 32;  // of a step
+  static constexpr int KT = KEYS / 32;
+  // A step in LDS: K, then V; each in blocks [8 chunks of the row][KEYS rows][128 bytes],
+  // so that a wave's 64 lanes fill 8 rows of a block in their order.
+  static constexpr int TILE = NC * KEYS * 128;
   // Workgroups a CU holds: by registers
   static constexpr int WGS = DP * ES <= 256 ? 2 : 1;
-  // K's chunk c of row r lies at chunk c ^ swizzle_k(r): 16 lanes that read one
-  // chunk of 16 rows then hit all banks (rows are C chunks apart).
-  static constexpr int LOW = (C & -C) < 16 ? (C & -C) : 16;
-  static __device__ __forceinline__ int swizzle_k(int r) { return (r / (16 / LOW)) & (LOW - 1); }
-  // V's: four rows are read 64 bytes each at a time, which then lie in different
-  // quarters of the banks (rows are C / 4 quarters apart).
-  static __device__ __forceinline__ int swizzle_v(int r) {
-    if constexpr (F32 || (C / 4) % 2 == 1) return 0;
-    else if constexpr ((C / 4) % 4 == 2) return ((r >> 1) & 1) * 4;
-    else return (r & 3) * 4;
-  }
 };
+// Chunk p of row r of a block lies at place p ^ swizzle(r).  K is read one chunk
+// of 16 rows at a time, which then hit all banks; V four rows of 64 bytes.
+__device__ __forceinline__ int swizzle_k(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int swizzle_v(int r) { return (r >> 1 & 1) * 4; }
 
 template <int XT>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -114,6 +109,12 @@ __device__ __forceinline__ u32x2 read_transposed(const char* p) {
                                        (__attribute__((address_space(3))) const char*)p)));
 }
 
+// 16 bytes a lane to LDS, in the order of the lanes.
+__device__ __forceinline__ void to_lds(const char* from, char* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
 // Four values to consecutive places.
 template <int XT>
 __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
@@ -137,14 +138,6 @@ constexpr float kLift = XT == GEN_F16 ? 14.f : 0.f;
 // exp2(a - b), 0 where a is -inf (also where b is)
 __device__ __forceinline__ float exp2_diff(float a, float b) {
   return __builtin_amdgcn_exp2f(a - (b == -INFINITY ? 0.f : b));
-}
-
-// Whether one of the two 16-bit numbers (the 32-bit number) is infinite or NaN.
-template <int XT>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  constexpr uint32_t E = XT == GEN_F16 ? 0x7C00u : 0x7F80u;
-  if constexpr (XT == GEN_F32) return (w & 0x7F800000u) == 0x7F800000u;
-  else return (w & E) == E || (w & E << 16) == E << 16;
 }
 
 // The new tokens of a sequence that have a position, and its tiles.
@@ -203,9 +196,10 @@ constexpr int part_words(int rows, int DP) { return rows * (DP + 2); }
 template <int XT, int DP>
 __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kernel(const ChunkAttnArgs a) {
   using G = Geo<XT, DP>;
-  extern __shared__ __align__(16) char lds[];
+  constexpr int kKeys = G::KEYS;
+  // two steps as two objects, so that the compiler does not wait for the one that is filled before it reads the other
+  __shared__ __align__(16) char stage0[2 * G::TILE], stage1[2 * G::TILE];
   __shared__ uint32_t arrived;
-  uint32_t* const bad = reinterpret_cast<uint32_t*>(lds + 4 * G::TILE);  // [2][waves]: the step's V has values that are not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, g = lane >> 5;
   // neighbours in the order of the keys on one XCD
@@ -275,8 +269,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         if (b % a.wgs == w) clear(load_seq(b));
       }
     } else {  // thread i sums those of its share
-      int64_t* sums = reinterpret_cast<int64_t*>(lds);
-      Bound* bound = reinterpret_cast<Bound*>(lds + 64);
+      int64_t* sums = reinterpret_cast<int64_t*>(stage0);
+      Bound* bound = reinterpret_cast<Bound*>(stage0 + 64);
       const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
       mine = 0;
       for (int b = b0; b < b1; b++) mine += units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
@@ -325,21 +319,20 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     }
   }
 
-  // a thread's chunks of a step's rows
-  int row_i[G::NI], dofs[G::NI], kofs[G::NI], vofs[G::NI];
-  bool dead[G::NI];
-#pragma unroll
-  for (int i = 0; i < G::NI; i++) {
-    const int slot = min(i * 256 + tid, kKeys * G::C - 1), r = slot / G::C, ch = slot - r * G::C;
-    row_i[i] = r;
-    dead[i] = ch * G::CE >= a.D;
-    dofs[i] = dead[i] ? 0 : ch * 16;
-    kofs[i] = (r * G::C + (ch ^ G::swizzle_k(r))) * 16;
-    vofs[i] = (r * G::C + (ch ^ G::swizzle_v(r))) * 16;
+  // A thread brings place lane % 8 of every block of rows 8 wave + lane / 8 (+ 32) of a step.
+  const int my_row8 = 8 * wave + (lane >> 3), k_chunk = (lane & 7) ^ swizzle_k(my_row8), v_chunk = (lane & 7) ^ swizzle_v(my_row8);
+  const int chunks = a.D / G::CE;
+  if (DP != a.D) {  // K's chunks past the head are zero and stay so
+    for (int i = tid; i < G::TILE / 16; i += 256) {
+      reinterpret_cast<u32x4*>(stage0)[i] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(stage1)[i] = u32x4{0u, 0u, 0u, 0u};
+    }
   }
-  const bool plain = a.softcap == 0.f && a.scale > 0.f;
-  // scores in units of log2 e
-  const float scale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap_log2e = a.softcap * kLog2e;
+  // Scores in units of log2 e are `scale` times the product (the tanh of a soft
+  // cap); a negative scale's sign goes to Q, so that the largest product is the largest score.
+  // A scale of 0 is the smallest number instead: scores then do not differ either, and -inf stays what it is.
+  const float scale = fmaxf((a.softcap > 0.f ? a.softcap : fabsf(a.scale)) * kLog2e, FLT_MIN);
+  const float cap_in = a.softcap > 0.f ? fminf(2.f * kLog2e * fabsf(a.scale) / a.softcap, FLT_MAX) : 0.f;
   const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)4 * a.wgs * a.slot_words * 4));
 
   Seq sq = at.b < a.B ? load_seq(at.b) : Seq{};
@@ -375,8 +368,6 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     const int see1 = pos + 1, see0 = a.window > 0 ? max(0, see1 - a.window) : 0;
     const int wave_hi = sq.p0 + tok0 + min(r0 + 31, rows - 1) / heads + 1, first_hi = sq.p0 + tok0 + min(r0, rows - 1) / heads + 1;
     const int wave_lo = a.window > 0 ? max(0, first_hi - a.window) : 0, last_lo = a.window > 0 ? max(0, wave_hi - a.window) : 0;
-    // steps from here on, and those up to there, are masked for some row of the tile
-    const int mask_hi = sq.p0 + tok0 + 1, mask_lo = a.window > 0 ? max(0, hi - a.window) : 0;
 
     const char* qp = static_cast<const char*>(a.q) +
                      ((int64_t)(sq.first + tok0 + my_tok) * a.q_tok + (head0 + my_row - my_tok * heads) * a.q_head) * G::ES;
@@ -386,150 +377,140 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       const int d = (2 * i + g) * G::CE;
       const u32x4_e v = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
       qf[i] = d < a.D ? u32x4{v[0], v[1], v[2], v[3]} : u32x4{0u, 0u, 0u, 0u};
+      if (a.scale < 0.f) qf[i] ^= G::F32 ? 0x80000000u : 0x80008000u;
     }
     f32x16 o[G::DT];
-#pragma unroll
-    for (int i = 0; i < G::DT; i++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) o[i][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m, l;
 
     const int32_t* table = a.table + at.b * a.table_row;
-    const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES;
-    const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES;
-    int entry[G::NI], in_page[G::NI];
-    u32x4 kr[G::NI], vr[G::NI];
-    // table entries of the rows from key k on; past the range they are the last key's
-    auto look = [&](int k) {
+    const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES + k_chunk * 16;
+    const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES + v_chunk * 16;
+    int entry[G::KT], in_page[G::KT];
+    // table entries of the thread's rows from key k on; past the range they are the last key's
+    auto look = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < G::NI; i++) {
-        const int key = min(k + row_i[i], hi - 1);
+      for (int t = 0; t < G::KT; t++) {
+        const int key = min(k + 32 * t + my_row8, hi - 1);
         const int slot = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
-        in_page[i] = key - slot * a.page;
-        entry[i] = table[slot];
+        in_page[t] = key - slot * a.page;
+        entry[t] = table[slot];
       }
     };
-    auto load = [&]() {
+    // the rows that were looked up, to LDS
+    auto bring = [&](char* to) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < G::NI; i++) {
-        const int64_t pid = min(max(entry[i], 0), a.pages - 1);
-        const u32x4_e x = *reinterpret_cast<const u32x4_e*>(kb + (pid * a.k_page + in_page[i] * a.k_tok) * G::ES + dofs[i]);
-        const u32x4_e y = *reinterpret_cast<const u32x4_e*>(vb + (pid * a.v_page + in_page[i] * a.v_tok) * G::ES + dofs[i]);
-        kr[i] = u32x4{x[0], x[1], x[2], x[3]};
-        vr[i] = u32x4{y[0], y[1], y[2], y[3]};
-      }
-    };
-    auto masked = [&](int k) { return k + kKeys > mask_hi || k < mask_lo; };
-    auto put = [&](int stage, int k) {
-      char* p = lds + stage * 2 * G::TILE;
+      for (int t = 0; t < G::KT; t++) {
+        const int pid = min(max(entry[t], 0), a.pages - 1);
+        if (a.direct) {  // 16-byte aligned, strides of 32 bits
+          const char* ks = kb + ((uint64_t)(uint32_t)pid * (uint32_t)(a.k_page * G::ES) + (uint64_t)(uint32_t)in_page[t] * (uint32_t)(a.k_tok * G::ES));
+          const char* vs = vb + ((uint64_t)(uint32_t)pid * (uint32_t)(a.v_page * G::ES) + (uint64_t)(uint32_t)in_page[t] * (uint32_t)(a.v_tok * G::ES));
 #pragma unroll
-      for (int i = 0; i < G::NI; i++) {
-        if ((i + 1) * 256 > kKeys * G::C && i * 256 + tid >= kKeys * G::C) continue;
-        *reinterpret_cast<u32x4*>(p + kofs[i]) = dead[i] ? u32x4{0u, 0u, 0u, 0u} : kr[i];
-        *reinterpret_cast<u32x4*>(p + G::TILE + vofs[i]) = vr[i];
-      }
-      if (masked(k)) {
-        bool x = false;
+          for (int i = 0; i < G::NC; i++) {
+            char* dst = to + (i * kKeys + 32 * t + 8 * wave) * 128;
+            if (8 * i + k_chunk < chunks) to_lds(ks + i * 128, dst);
+            if (8 * i + v_chunk < chunks) to_lds(vs + i * 128, dst + G::TILE);
+          }
+        } else {
+          const char* ks = kb + (pid * a.k_page + in_page[t] * a.k_tok) * G::ES;
+          const char* vs = vb + (pid * a.v_page + in_page[t] * a.v_tok) * G::ES;
 #pragma unroll
-        for (int i = 0; i < G::NI; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) x |= not_finite<XT>(vr[i][e]);
-        const bool any = __any(x);
-        if (lane == 0) bad[stage * kWaves + wave] = any;
+          for (int i = 0; i < G::NC; i++) {
+            char* dst = to + (i * kKeys + 32 * t + my_row8) * 128 + (lane & 7) * 16;
+            if (8 * i + k_chunk < chunks) {
+              const u32x4_e x = *reinterpret_cast<const u32x4_e*>(ks + i * 128);
+              *reinterpret_cast<u32x4*>(dst) = u32x4{x[0], x[1], x[2], x[3]};
+            }
+            if (8 * i + v_chunk < chunks) {
+              const u32x4_e y = *reinterpret_cast<const u32x4_e*>(vs + i * 128);
+              *reinterpret_cast<u32x4*>(dst + G::TILE) = u32x4{y[0], y[1], y[2], y[3]};
+            }
+          }
+        }
       }
     };
 
-    __syncthreads();  // the last tile's steps have been read
-    look(k0);
-    load();
-    if (k0 + kKeys < k1) look(k0 + kKeys);
-    put(0, k0);
-    __syncthreads();
-    for (int k = k0, stage = 0; k < k1; k += kKeys, stage ^= 1) {
-      const bool more = k + kKeys < k1;
-      if (more) {
-        load();
-        if (k + 2 * kKeys < k1) look(k + 2 * kKeys);
-      }
-      if (busy && k < wave_hi && k + kKeys > wave_lo) {
-        const char* ks = lds + stage * 2 * G::TILE;
-        const char* vs = ks + G::TILE;
-        f32x16 s;
+    // One step on the keys from k on.  SAFE: values that are not finite count only
+    // for the rows that see their key; otherwise they may make any row NaN.
+    auto step = [&](auto SAFE, const char* ks, int k) __attribute__((always_inline)) {
+      if (!(busy && k < wave_hi && k + kKeys > wave_lo)) return;
+      const char* vs = ks + G::TILE;
+      f32x16 s[G::KT];
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = 0.f;
+      for (int t = 0; t < G::KT; t++)
 #pragma unroll
-        for (int i = 0; i < G::C / 2; i++) {
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (c * G::C + ((2 * i + g) ^ G::swizzle_k(c))) * 16);
+        for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < G::C / 2; i++)
+#pragma unroll
+        for (int t = 0; t < G::KT; t++) {
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (i / 4 * kKeys + 32 * t + c) * 128 +
+                                                           (((2 * i + g) & 7) ^ swizzle_k(c)) * 16);
           if constexpr (G::F32) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), s, 0, 0, 0);
+              s[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), s[t], 0, 0, 0);
           } else {
-            s = mfma32<XT>(kf, qf[i], s);
+            s[t] = mfma32<XT>(kf, qf[i], s[t]);
           }
         }
-        float by = scale;  // what the scores still have to be multiplied with
-        if (!plain) {
-          by = 1.f;
-          if (a.softcap > 0.f) {
+      if (a.softcap > 0.f) {
+        // tanh x = 1 - 2 / (e^2x + 1): off by three roundings of 1 at most, infinite x included
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = cap_log2e * tanhf(s[e] * scale);
-          } else {
+        for (int t = 0; t < G::KT; t++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] *= scale;
-          }
-        }
-        const bool hidden = k + kKeys > first_hi || k < last_lo;  // some key from some row of this wave
-        if (hidden) {
+          for (int e = 0; e < 16; e++)
+            s[t][e] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[t][e] * cap_in) + 1.f);
+      }
+      const bool hidden = k + kKeys > first_hi || k < last_lo;  // some key from some row of this wave
+      if (hidden) {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
 #pragma unroll
           for (int e = 0; e < 16; e++) {
-            const int key = k + 8 * (e / 4) + 4 * g + e % 4;
-            s[e] = key < see1 && key >= see0 && key < k1 ? s[e] : -INFINITY;
+            const int key = k + 32 * t + 8 * (e / 4) + 4 * g + e % 4;
+            s[t][e] = key < see1 && key >= see0 && key < k1 ? s[t][e] : -INFINITY;
           }
-        }
-        float mt = s[0];
+      }
+      float mt = s[0][0];
 #pragma unroll
-        for (int e = 1; e < 16; e++) mt = fmaxf(mt, s[e]);
-        mt = fmaxf(mt, lane_xor<32>(mt, lane)) * by;
-        mt = fmaxf(mt, m);
-        if (__any(mt > m)) {
-          const float f = exp2_diff(m, mt);
-          m = mt;
-          l *= f;
+      for (int t = 0; t < G::KT; t++)
 #pragma unroll
-          for (int i = 0; i < G::DT; i++)
+        for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[t][e]);
+      mt = fmaxf(mt, lane_xor<32>(mt, lane)) * scale;
+      mt = fmaxf(mt, m);
+      if (__any(mt > m)) {
+        const float f = exp2_diff(m, mt);
+        m = mt;
+        l *= f;
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[i][e] *= f;
-        }
-        const float off = (m == -INFINITY ? 0.f : m) - kLift<XT>;
-        float sum = 0.f;
+        for (int i = 0; i < G::DT; i++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[i][e] *= f;
+      }
+      const float off = kLift<XT> - (m == -INFINITY ? 0.f : m);
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < G::KT; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], by, -off));
-          sum += s[e];
+          s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], scale, off));
+          sum += s[t][e];
         }
-        l += sum;
-        bool safe = false;
-        if (hidden) {
-          uint32_t x = 0;
+      l += sum;
+      if (decltype(SAFE)::value && hidden) {  // one key at a time
 #pragma unroll
-          for (int i = 0; i < kWaves; i++) x |= bad[stage * kWaves + i];
-          safe = __builtin_amdgcn_readfirstlane(x) != 0;
-        }
-        if (safe) {
-          // Values that are not finite count only for the rows that see their key: one key at a time
+        for (int t = 0; t < G::KT; t++)
           for (int i = 0; i < 16; i++) {
-            const float other = lane_xor<32>(s[0], lane);
-#pragma unroll
+            const float other = lane_xor<32>(s[t][0], lane);
             for (int gg = 0; gg < 2; gg++) {
               const int key = 8 * (i / 4) + 4 * gg + i % 4;
-              const float p = gg == g ? s[0] : other;
+              const float p = gg == g ? s[t][0] : other;
 #pragma unroll
               for (int dt = 0; dt < G::DT; dt++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                   const int d = 32 * dt + 8 * (e / 4) + 4 * g + e % 4, ch = d / G::CE;
-                  const char* vp = vs + (key * G::C + (ch ^ G::swizzle_v(key))) * 16 + d % G::CE * G::ES;
+                  const char* vp = vs + (ch / 8 * kKeys + 32 * t + key) * 128 + ((ch & 7) ^ swizzle_v(key)) * 16 + d % G::CE * G::ES;
                   float v;
                   if constexpr (G::F32) v = *reinterpret_cast<const float*>(vp);
                   else v = half<XT>(*reinterpret_cast<const uint16_t*>(vp), 0);
@@ -537,52 +518,87 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 15; e++) s[e] = s[e + 1];
+            for (int e = 0; e < 15; e++) s[t][e] = s[t][e + 1];
           }
-        } else if constexpr (G::F32) {
+      } else if constexpr (G::F32) {
+#pragma unroll
+        for (int t = 0; t < G::KT; t++)
 #pragma unroll
           for (int e = 0; e < 16; e++) {
-            const int key = 8 * (e / 4) + 4 * g + e % 4;
+            const int key = 32 * t + 8 * (e / 4) + 4 * g + e % 4;
 #pragma unroll
             for (int dt = 0; dt < G::DT; dt++) {
-              const float v = *reinterpret_cast<const float*>(vs + key * (G::C * 16) + (32 * dt + c) * 4);
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[dt], 0, 0, 0);
+              const float v = *reinterpret_cast<const float*>(vs + (dt * kKeys + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[t][e], o[dt], 0, 0, 0);
             }
           }
-        } else {
-          u32x4 pt[2][2];  // [16 keys][term]
+      } else {
+        const int i16 = lane & 15, vrow = 4 * g + (i16 >> 2);  // the row and the 8 bytes of it that this lane reads
 #pragma unroll
-          for (int u = 0; u < 2; u++)
+        for (int t = 0; t < G::KT; t++)
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            u32x4 p0, p1;  // 16 keys: P as the sum of two numbers
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-              const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
-              const uint32_t t = pack<XT>(x, y);
-              pt[u][0][e] = t;
-              pt[u][1][e] = pack<XT>(x - half<XT>(t, 0), y - half<XT>(t, 1));
+              const float x = s[t][8 * u + 2 * e], y = s[t][8 * u + 2 * e + 1];
+              p0[e] = pack<XT>(x, y);
+              p1[e] = pack<XT>(x - half<XT>(p0[e], 0), y - half<XT>(p0[e], 1));
             }
-          const int i16 = lane & 15, vr4 = i16 >> 2;  // the row and the 8 bytes of it that this lane reads
+            u32x4 vf[G::DT];
 #pragma unroll
-          for (int dt = 0; dt < G::DT; dt++) {
-            const int ch = 4 * dt + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-              const int ka = 16 * u + 4 * g + vr4, kc = ka + 8;
-              const u32x2 x = read_transposed(vs + (ka * G::C + (ch ^ G::swizzle_v(ka))) * 16 + (i16 & 1) * 8);
-              const u32x2 y = read_transposed(vs + (kc * G::C + (ch ^ G::swizzle_v(kc))) * 16 + (i16 & 1) * 8);
-              const u32x4 vf = {x[0], x[1], y[0], y[1]};
-              o[dt] = mfma32<XT>(vf, pt[u][0], o[dt]);
-              o[dt] = mfma32<XT>(vf, pt[u][1], o[dt]);
+            for (int dt = 0; dt < G::DT; dt++) {
+              const int ch = 4 * (dt & 1) + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+              const char* vp = vs + (dt / 2 * kKeys + 32 * t + 16 * u + vrow) * 128 + (ch ^ swizzle_v(vrow)) * 16 + (i16 & 1) * 8;
+              const u32x2 x = read_transposed(vp), y = read_transposed(vp + 8 * 128);
+              vf[dt] = u32x4{x[0], x[1], y[0], y[1]};
             }
+#pragma unroll
+            for (int dt = 0; dt < G::DT; dt++) o[dt] = mfma32<XT>(vf[dt], p0, o[dt]);
+#pragma unroll
+            for (int dt = 0; dt < G::DT; dt++) o[dt] = mfma32<XT>(vf[dt], p1, o[dt]);
           }
-        }
       }
-      if (more) put(stage ^ 1, k + kKeys);
+    };
+    // the steps from k0 to k1: while one is worked on the next is brought, and the one after it looked up
+    auto run = [&](auto SAFE) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < G::DT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[i][e] = 0.f;
+      m = -INFINITY, l = 0.f;
+      look(k0);
+      __syncthreads();  // the last tile's steps have been read
+      bring(stage0);
+      look(k0 + kKeys);
       __syncthreads();
-    }
-    l += lane_xor<32>(l, lane);
+      for (int k = k0; k < k1; k += 2 * kKeys) {
+        if (k + kKeys < k1) {
+          bring(stage1);
+          look(k + 2 * kKeys);
+        }
+        step(SAFE, stage0, k);
+        __syncthreads();
+        if (k + kKeys >= k1) break;
+        if (k + 2 * kKeys < k1) {
+          bring(stage0);
+          look(k + 3 * kKeys);
+        }
+        step(SAFE, stage1, k + kKeys);
+        __syncthreads();
+      }
+      l += lane_xor<32>(l, lane);
+    };
+    run(std::false_type{});
+    float x = l;  // not finite where some value is not
+#pragma unroll
+    for (int i = 0; i < G::DT; i++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) x = fmaf(o[i][e], 0.f, x);
+    if (__syncthreads_or(r0 + c < rows && !isfinite(x))) run(std::true_type{});
 
     // row r of the tile: its place in out, its head
-    auto finish = [&](int r, int d, float M, float L, f32x4 acc) {
+    auto finish = [&](int r, int d, float M, float L, f32x4 acc) __attribute__((always_inline)) {
       const int tok = r / heads, h = head0 + r - tok * heads;
       float f = 1.f;
       if (a.sinks) {
@@ -709,6 +725,14 @@ bool chunk_attention_plan(ChunkAttnArgs& a, int cus, int64_t* part_bytes) {
   while (((int64_t)1 << (a.page_shift - 30)) < a.page) a.page_shift++;
   // exact for keys below 2^30: the error of page_mul, below page <= 2^(shift - 30), times the key stays below 2^shift
   a.page_mul = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page - 1) / a.page);
+  const int esz = a.type == GEN_F32 ? 4 : 2;
+  uint64_t bits = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+  a.direct = 1;
+  for (int64_t st : {a.k_page, a.k_head, a.k_tok, a.v_page, a.v_head, a.v_tok}) {
+    bits |= (uint64_t)(st * esz);
+    if (st < 0 || st * esz > 0xFFFFFFFFll) a.direct = 0;
+  }
+  if (bits & 15) a.direct = 0;
   const int per = a.Hq / a.Hkv;
   a.tile_heads = std::min(per, kRows);
   a.tile_tokens = kRows / a.tile_heads;
@@ -733,7 +757,7 @@ hipError_t launch_chunk_attention(const ChunkAttnArgs& a, hipStream_t stream) {
     return hipErrorInvalidValue;
   return with_kernel(a, [&](auto xt, auto dp) {
     constexpr int XT = decltype(xt)::value, DP = decltype(dp)::value;
-    hipLaunchKernelGGL((chunk_attention_kernel<XT, DP>), dim3((unsigned)a.wgs), dim3(256), (Geo<XT, DP>::LDS), stream, a);
+    hipLaunchKernelGGL((chunk_attention_kernel<XT, DP>), dim3((unsigned)a.wgs), dim3(256), 0, stream, a);
     return hipGetLastError();
   });
 }

@@ -714,6 +714,7 @@ struct ChunkAttnArgs {
   int type;
   // how the work is split (chunk_attention_plan)
   int tile_heads, tile_tokens;  // rows of a tile
+  int direct;              // pools of 16-byte alignment and strides of 32 bits
   uint32_t page_mul;       // as PagedAttnArgs
   int page_shift;
   int wgs;                 // workgroups
