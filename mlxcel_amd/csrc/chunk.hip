@@ -93,6 +93,16 @@ __device__ __forceinline__ float half(uint32_t w, int hi) {
   return xt_to_f32<XT == GEN_F16 ? 1 : 0>(hi ? w >> 16 : w & 0xFFFFu);
 }
 
+// v less the low (high) half of w, exact where w holds v rounded.  minus: -1 in
+// that half, 0 in the other, in a register: the compiler writes a low bfloat16 -1 as
+// the inline constant -1.0, whose bits are in the high half.
+template <int XT, int HI>
+__device__ __forceinline__ float less(float v, uint32_t w, uint32_t minus) {
+  if constexpr (XT == GEN_BF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, minus), v, false);
+  else return fmaf((float)__builtin_bit_cast(_Float16, (uint16_t)(HI ? w >> 16 : w)), -1.f, v);
+}
+
 template <int XT>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (XT == GEN_BF16)
@@ -104,15 +114,19 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // Four rows of the lane's column: row i of the 16 lanes' 4 x 16 elements is read
 // by lanes 4 i .. 4 i + 3, lane j gets column j.
 __device__ __forceinline__ u32x2 read_transposed(const char* p) {
-  typedef __attribute__((address_space(3))) s16x4* ptr;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(uint32_t)(uintptr_t)(
-                                       (__attribute__((address_space(3))) const char*)p)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
 // 16 bytes a lane to LDS, in the order of the lanes.
 __device__ __forceinline__ void to_lds(const char* from, char* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// All waves' loads to LDS have arrived, and all have read what is filled next.
+__device__ __forceinline__ void step_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
 }
 
 // Four values to consecutive places.
@@ -177,6 +191,14 @@ __device__ __forceinline__ int64_t before(const ChunkAttnArgs& a, const Seq& s, 
   }
   return sum;
 }
+// The tiles of a head are taken shortest, longest, second shortest, ..: tile number q
+// in that order, and the units of those before it.  Two neighbours together then cost
+// about the same everywhere, so that workgroups begin near the same key of their tiles
+// and find each other's keys in L2 (2048 tokens of 32768: misses XX of XX).
+__device__ __forceinline__ int tile_at(const Seq& s, int q) { return q & 1 ? s.tiles - 1 - q / 2 : q / 2; }
+__device__ __forceinline__ int64_t units_before(const ChunkAttnArgs& a, const Seq& s, int q) {
+  return before(a, s, (q + 1) / 2) + (q > 1 ? before(a, s, s.tiles) - before(a, s, s.tiles - q / 2) : 0);
+}
 // v / d for 0 <= v < 2^52
 __device__ __forceinline__ int64_t divide(int64_t v, int64_t d) {
   int64_t q = (int64_t)((double)v / (double)d);
@@ -197,8 +219,10 @@ template <int XT, int DP>
 __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kernel(const ChunkAttnArgs a) {
   using G = Geo<XT, DP>;
   constexpr int kKeys = G::KEYS;
-  // two steps as two objects, so that the compiler does not wait for the one that is filled before it reads the other
-  __shared__ __align__(16) char stage0[2 * G::TILE], stage1[2 * G::TILE];
+  // Keys and values of two steps.  Objects of their own, with one sum from each to what is
+  // read of it, so that the compiler sees that what is being filled is not what is read and
+  // does not wait for it (it did, at 1700 us for 2048 tokens of 32768).
+  __shared__ __align__(16) char k_lds0[G::TILE], v_lds0[G::TILE], k_lds1[G::TILE], v_lds1[G::TILE];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, g = lane >> 5;
@@ -223,13 +247,14 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     int lo = 0, hi = s.tiles - 1;  // the last tile that begins at or before off
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (before(a, s, mid) <= off) lo = mid;
+      if (units_before(a, s, mid) <= off) lo = mid;
       else hi = mid - 1;
     }
-    const int keys = tile_hi(a, s, lo) - tile_lo(a, s, lo);
-    const int64_t r = off - before(a, s, lo) - kAround;
+    off -= units_before(a, s, lo);
+    const int j = tile_at(s, lo), keys = tile_hi(a, s, j) - tile_lo(a, s, j);
+    const int64_t r = off - kAround;
     int key = r > 0 ? (int)r / kKeys * kKeys : 0, tile = hh * s.tiles + lo;
-    if (keys <= kWhole && off > before(a, s, lo)) key = 0, tile++;  // it belongs to the workgroup that begins it
+    if (keys <= kWhole && off > 0) key = 0, tile++;  // it belongs to the workgroup that begins it
     return Bound{b, tile, key, base};
   };
   auto clear = [&](const Seq& s) {  // rows without a position
@@ -269,8 +294,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         if (b % a.wgs == w) clear(load_seq(b));
       }
     } else {  // thread i sums those of its share
-      int64_t* sums = reinterpret_cast<int64_t*>(stage0);
-      Bound* bound = reinterpret_cast<Bound*>(stage0 + 64);
+      int64_t* sums = reinterpret_cast<int64_t*>(k_lds0);
+      Bound* bound = reinterpret_cast<Bound*>(k_lds0 + 64);
       const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
       mine = 0;
       for (int b = b0; b < b1; b++) mine += units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
@@ -319,13 +344,15 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     }
   }
 
+  uint32_t minus_lo = 0x0000BF80u, minus_hi = 0xBF800000u;
+  asm volatile("" : "+s"(minus_lo), "+s"(minus_hi));
   // A thread brings place lane % 8 of every block of rows 8 wave + lane / 8 (+ 32) of a step.
   const int my_row8 = 8 * wave + (lane >> 3), k_chunk = (lane & 7) ^ swizzle_k(my_row8), v_chunk = (lane & 7) ^ swizzle_v(my_row8);
   const int chunks = a.D / G::CE;
   if (DP != a.D) {  // K's chunks past the head are zero and stay so
     for (int i = tid; i < G::TILE / 16; i += 256) {
-      reinterpret_cast<u32x4*>(stage0)[i] = u32x4{0u, 0u, 0u, 0u};
-      reinterpret_cast<u32x4*>(stage1)[i] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(k_lds0)[i] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(k_lds1)[i] = u32x4{0u, 0u, 0u, 0u};
     }
   }
   // Scores in units of log2 e are `scale` times the product (the tanh of a soft
@@ -348,13 +375,14 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       }
       continue;
     }
-    const int hh = at.tile / sq.tiles, j = at.tile - hh * sq.tiles, hk = hh / tiles_h, ht = hh - hk * tiles_h;
+    const int hh = at.tile / sq.tiles, nth = at.tile - hh * sq.tiles, j = tile_at(sq, nth);
+    const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
     const int heads = min(hp, per - hp * ht), head0 = hk * per + hp * ht;
     const int tok0 = j * a.tile_tokens, toks = min(a.tile_tokens, sq.n - tok0), rows = toks * heads;
     const int lo = tile_lo(a, sq, j), hi = tile_hi(a, sq, j);
     const int k0 = lo + at.key, k1 = at.b == end.b && at.tile == end.tile ? min(hi, lo + end.key) : hi;
     // the tile's workgroups
-    const int64_t p0 = at.base + hh * head_units + before(a, sq, j) + kAround;
+    const int64_t p0 = at.base + hh * head_units + units_before(a, sq, nth) + kAround;
     int w0 = w, w1 = w;
     if (hi - lo > kWhole && (k0 > lo || k1 < hi)) {
       w0 = (int)divide(p0 + kKeys + n - 1, n) - 1;
@@ -380,222 +408,410 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       if (a.scale < 0.f) qf[i] ^= G::F32 ? 0x80000000u : 0x80008000u;
     }
     f32x16 o[G::DT];
-    float m, l;
+    float m, l, off;  // off: what is added to a score before its exponential is taken
 
     const int32_t* table = a.table + at.b * a.table_row;
-    const char* kb = static_cast<const char*>(a.k) + hk * a.k_head * G::ES + k_chunk * 16;
-    const char* vb = static_cast<const char*>(a.v) + hk * a.v_head * G::ES + v_chunk * 16;
+    const char* kb = static_cast<const char*>(a.k) + hk * a.k_head + k_chunk * 16;
+    const char* vb = static_cast<const char*>(a.v) + hk * a.v_head + v_chunk * 16;
+    // A thread's rows of a step from key k on are k + my_row8 (+ 32) of V and 32 keys more of K:
+    // the scores of 32 keys are worked out beside the values of the 32 before them.
     int entry[G::KT], in_page[G::KT];
-    // table entries of the thread's rows from key k on; past the range they are the last key's
-    auto look = [&](int k) __attribute__((always_inline)) {
+    int64_t v_off = 0;  // bytes to the V row that comes next
+    // table entries of keys from + my_row8 (+ 32); past the range they are the last key's
+    auto look = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < G::KT; t++) {
-        const int key = min(k + 32 * t + my_row8, hi - 1);
-        const int slot = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
+        const uint32_t key = min(from + 32 * t + my_row8, hi - 1);
+        const uint32_t slot = __umulhi(key << 2, a.page_mul) >> (a.page_shift - 30);
         in_page[t] = key - slot * a.page;
         entry[t] = table[slot];
       }
     };
-    // the rows that were looked up, to LDS
-    auto bring = [&](char* to) __attribute__((always_inline)) {
+    // bytes to the looked-up row t in a pool of these strides
+    auto place = [&](int t, int64_t page_bytes, int64_t tok_bytes) __attribute__((always_inline)) -> int64_t {
+      const int pid = min(max(entry[t], 0), a.pages - 1);
+      if (a.direct) return (int64_t)((uint64_t)(uint32_t)pid * (uint32_t)page_bytes + (uint64_t)(uint32_t)in_page[t] * (uint32_t)tok_bytes);
+      return pid * page_bytes + in_page[t] * tok_bytes;
+    };
+    // a row of full width to LDS without passing through registers
+    auto rows_to_lds = [&](const char* from, int chunk, char* to, int row) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < G::NC; i++)
+        if (8 * i + 8 <= G::C || 8 * i + chunk < G::C) to_lds(from + i * 128, to + (i * kKeys + row + 8 * wave) * 128);
+    };
+    // a row to LDS, rows `row` on of the blocks
+    auto bring_row = [&](const char* from, int chunk, char* to, int row) __attribute__((always_inline)) {
+      if (a.direct) {  // 16-byte aligned, strides of 32 bits
+        if (DP == a.D) {
+          rows_to_lds(from, chunk, to, row);
+        } else {
+#pragma unroll
+          for (int i = 0; i < G::NC; i++)
+            if (8 * i + chunk < chunks) to_lds(from + i * 128, to + (i * kKeys + row + 8 * wave) * 128);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < G::NC; i++)
+          if (8 * i + chunk < chunks) {
+            const u32x4_e x = *reinterpret_cast<const u32x4_e*>(from + i * 128);
+            *reinterpret_cast<u32x4*>(to + (i * kKeys + row + my_row8) * 128 + (lane & 7) * 16) = u32x4{x[0], x[1], x[2], x[3]};
+          }
+      }
+    };
+    // K of looked-up row t, V of the one before
+    auto bring_k = [&](int t, char* to, int row) __attribute__((always_inline)) {
+      const int64_t off = place(t, a.k_page, a.k_tok);
+      bring_row(kb + off, k_chunk, to, row);
+      v_off = a.same ? off : place(t, a.v_page, a.v_tok);
+    };
+    auto bring_v = [&](char* to, int row) __attribute__((always_inline)) { bring_row(vb + v_off, v_chunk, to, row); };
+    // a step to LDS
+    auto bring = [&](char* ks, char* vs) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < G::KT; t++) {
-        const int pid = min(max(entry[t], 0), a.pages - 1);
-        if (a.direct) {  // 16-byte aligned, strides of 32 bits
-          const char* ks = kb + ((uint64_t)(uint32_t)pid * (uint32_t)(a.k_page * G::ES) + (uint64_t)(uint32_t)in_page[t] * (uint32_t)(a.k_tok * G::ES));
-          const char* vs = vb + ((uint64_t)(uint32_t)pid * (uint32_t)(a.v_page * G::ES) + (uint64_t)(uint32_t)in_page[t] * (uint32_t)(a.v_tok * G::ES));
-#pragma unroll
-          for (int i = 0; i < G::NC; i++) {
-            char* dst = to + (i * kKeys + 32 * t + 8 * wave) * 128;
-            if (8 * i + k_chunk < chunks) to_lds(ks + i * 128, dst);
-            if (8 * i + v_chunk < chunks) to_lds(vs + i * 128, dst + G::TILE);
-          }
-        } else {
-          const char* ks = kb + (pid * a.k_page + in_page[t] * a.k_tok) * G::ES;
-          const char* vs = vb + (pid * a.v_page + in_page[t] * a.v_tok) * G::ES;
-#pragma unroll
-          for (int i = 0; i < G::NC; i++) {
-            char* dst = to + (i * kKeys + 32 * t + my_row8) * 128 + (lane & 7) * 16;
-            if (8 * i + k_chunk < chunks) {
-              const u32x4_e x = *reinterpret_cast<const u32x4_e*>(ks + i * 128);
-              *reinterpret_cast<u32x4*>(dst) = u32x4{x[0], x[1], x[2], x[3]};
-            }
-            if (8 * i + v_chunk < chunks) {
-              const u32x4_e y = *reinterpret_cast<const u32x4_e*>(vs + i * 128);
-              *reinterpret_cast<u32x4*>(dst + G::TILE) = u32x4{y[0], y[1], y[2], y[3]};
-            }
-          }
-        }
+        bring_v(vs, 32 * t);
+        bring_k(t, ks, 32 * t);
       }
     };
 
-    // One step on the keys from k on.  SAFE: values that are not finite count only
-    // for the rows that see their key; otherwise they may make any row NaN.
-    auto step = [&](auto SAFE, const char* ks, int k) __attribute__((always_inline)) {
-      if (!(busy && k < wave_hi && k + kKeys > wave_lo)) return;
-      const char* vs = ks + G::TILE;
-      f32x16 s[G::KT];
+    f32x16 s;  // scores of 32 keys
+    float mt;  // and their largest
+    auto read_k = [&](const char* ks, int row, int i) __attribute__((always_inline)) -> u32x4 {
+      return *reinterpret_cast<const u32x4*>(ks + ((i / 4 * kKeys + row + c) * 128 + (((2 * i + g) & 7) ^ swizzle_k(c)) * 16));
+    };
+    // 16 u + the lane's eight keys of column 32 dt + c
+    auto read_v = [&](const char* vs, int row, int u, int dt) __attribute__((always_inline)) -> u32x4 {
+      const int i16 = lane & 15, r = 4 * g + (i16 >> 2);  // the row and the 8 bytes of it that this lane reads
+      const int ch = 4 * (dt & 1) + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+      const int at = (dt / 2 * kKeys + row + 16 * u + r) * 128 + (ch ^ swizzle_v(r)) * 16 + (i16 & 1) * 8;
+      const u32x2 x = read_transposed(vs + at), y = read_transposed(vs + (at + 8 * 128));
+      return u32x4{x[0], x[1], y[0], y[1]};
+    };
+    auto products = [&](const char* ks, int row) __attribute__((always_inline)) -> f32x16 {
+      f32x16 r;
 #pragma unroll
-      for (int t = 0; t < G::KT; t++)
+      for (int e = 0; e < 16; e++) r[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+      for (int i = 0; i < G::C / 2; i++) {
+        const u32x4 kf = read_k(ks, row, i);
+        if constexpr (G::F32) {
 #pragma unroll
-      for (int i = 0; i < G::C / 2; i++)
-#pragma unroll
-        for (int t = 0; t < G::KT; t++) {
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (i / 4 * kKeys + 32 * t + c) * 128 +
-                                                           (((2 * i + g) & 7) ^ swizzle_k(c)) * 16);
-          if constexpr (G::F32) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              s[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), s[t], 0, 0, 0);
-          } else {
-            s[t] = mfma32<XT>(kf, qf[i], s[t]);
-          }
+          for (int e = 0; e < 4; e++)
+            r = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), r, 0, 0, 0);
+        } else {
+          r = mfma32<XT>(kf, qf[i], r);
         }
+      }
+      return r;
+    };
+    auto largest = [&]() __attribute__((always_inline)) {
+      mt = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; e++) mt = fmaxf(mt, s[e]);
+      mt = fmaxf(mt, lane_xor<32>(mt, lane)) * scale;
+    };
+    // soft cap and mask of the scores of the keys from k on
+    auto special = [&](int k) __attribute__((always_inline)) {
+      const bool hidden = k + 32 > first_hi || k < last_lo;  // some key from some row of this wave
       if (a.softcap > 0.f) {
         // tanh x = 1 - 2 / (e^2x + 1): off by three roundings of 1 at most, infinite x included
 #pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int e = 0; e < 16; e++)
-            s[t][e] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[t][e] * cap_in) + 1.f);
+        for (int e = 0; e < 16; e++)
+          s[e] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * cap_in) + 1.f);
       }
-      const bool hidden = k + kKeys > first_hi || k < last_lo;  // some key from some row of this wave
       if (hidden) {
 #pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const int key = k + 32 * t + 8 * (e / 4) + 4 * g + e % 4;
-            s[t][e] = key < see1 && key >= see0 && key < k1 ? s[t][e] : -INFINITY;
-          }
+        for (int e = 0; e < 16; e++) {
+          const int key = k + 8 * (e / 4) + 4 * g + e % 4;
+          s[e] = key < see1 && key >= see0 && key < k1 ? s[e] : -INFINITY;
+        }
       }
-      float mt = s[0][0];
-#pragma unroll
-      for (int t = 0; t < G::KT; t++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[t][e]);
-      mt = fmaxf(mt, lane_xor<32>(mt, lane)) * scale;
-      mt = fmaxf(mt, m);
+      if (a.softcap > 0.f || hidden) largest();
+    };
+    auto seen = [&](int k) __attribute__((always_inline)) -> bool { return busy && k < k1 && k < wave_hi && k + 32 > wave_lo; };
+    auto grow = [&]() __attribute__((always_inline)) {  // the running maximum
       if (__any(mt > m)) {
-        const float f = exp2_diff(m, mt);
-        m = mt;
+        const float to = fmaxf(mt, m), f = exp2_diff(m, to);
+        m = to;
+        off = kLift<XT> - (m == -INFINITY ? 0.f : m);
         l *= f;
 #pragma unroll
         for (int i = 0; i < G::DT; i++)
 #pragma unroll
           for (int e = 0; e < 16; e++) o[i][e] *= f;
       }
-      const float off = kLift<XT> - (m == -INFINITY ? 0.f : m);
+    };
+    // probabilities in place of the scores
+    auto exponentials = [&]() __attribute__((always_inline)) {
       float sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < G::KT; t++)
+      for (int e = 0; e < 16; e++) {
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, off));
+        sum += s[e];
+      }
+      l += sum;
+    };
+    auto values = [&](const char* vs, int row) __attribute__((always_inline)) {
+      if constexpr (G::F32) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-          s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], scale, off));
-          sum += s[t][e];
+          const int key = 8 * (e / 4) + 4 * g + e % 4;
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++) {
+            const float v = *reinterpret_cast<const float*>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[dt], 0, 0, 0);
+          }
         }
-      l += sum;
-      if (decltype(SAFE)::value && hidden) {  // one key at a time
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-          for (int i = 0; i < 16; i++) {
-            const float other = lane_xor<32>(s[t][0], lane);
-            for (int gg = 0; gg < 2; gg++) {
-              const int key = 8 * (i / 4) + 4 * gg + i % 4;
-              const float p = gg == g ? s[t][0] : other;
-#pragma unroll
-              for (int dt = 0; dt < G::DT; dt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                  const int d = 32 * dt + 8 * (e / 4) + 4 * g + e % 4, ch = d / G::CE;
-                  const char* vp = vs + (ch / 8 * kKeys + 32 * t + key) * 128 + ((ch & 7) ^ swizzle_v(key)) * 16 + d % G::CE * G::ES;
-                  float v;
-                  if constexpr (G::F32) v = *reinterpret_cast<const float*>(vp);
-                  else v = half<XT>(*reinterpret_cast<const uint16_t*>(vp), 0);
-                  o[dt][e] = p == 0.f ? o[dt][e] : fmaf(p, v, o[dt][e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 15; e++) s[t][e] = s[t][e + 1];
-          }
-      } else if constexpr (G::F32) {
-#pragma unroll
-        for (int t = 0; t < G::KT; t++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const int key = 32 * t + 8 * (e / 4) + 4 * g + e % 4;
-#pragma unroll
-            for (int dt = 0; dt < G::DT; dt++) {
-              const float v = *reinterpret_cast<const float*>(vs + (dt * kKeys + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4);
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[t][e], o[dt], 0, 0, 0);
-            }
-          }
       } else {
-        const int i16 = lane & 15, vrow = 4 * g + (i16 >> 2);  // the row and the 8 bytes of it that this lane reads
 #pragma unroll
-        for (int t = 0; t < G::KT; t++)
+        for (int u = 0; u < 2; u++) {
+          u32x4 p0, p1;  // 16 keys: P as the sum of two numbers
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            u32x4 p0, p1;  // 16 keys: P as the sum of two numbers
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const float x = s[t][8 * u + 2 * e], y = s[t][8 * u + 2 * e + 1];
-              p0[e] = pack<XT>(x, y);
-              p1[e] = pack<XT>(x - half<XT>(p0[e], 0), y - half<XT>(p0[e], 1));
-            }
-            u32x4 vf[G::DT];
-#pragma unroll
-            for (int dt = 0; dt < G::DT; dt++) {
-              const int ch = 4 * (dt & 1) + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-              const char* vp = vs + (dt / 2 * kKeys + 32 * t + 16 * u + vrow) * 128 + (ch ^ swizzle_v(vrow)) * 16 + (i16 & 1) * 8;
-              const u32x2 x = read_transposed(vp), y = read_transposed(vp + 8 * 128);
-              vf[dt] = u32x4{x[0], x[1], y[0], y[1]};
-            }
-#pragma unroll
-            for (int dt = 0; dt < G::DT; dt++) o[dt] = mfma32<XT>(vf[dt], p0, o[dt]);
-#pragma unroll
-            for (int dt = 0; dt < G::DT; dt++) o[dt] = mfma32<XT>(vf[dt], p1, o[dt]);
+          for (int e = 0; e < 4; e++) {
+            const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
+            p0[e] = pack<XT>(x, y);
+            p1[e] = pack<XT>(less<XT, 0>(x, p0[e], minus_lo), less<XT, 1>(y, p0[e], minus_hi));
           }
+          u32x4 vf[G::DT];
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++) vf[dt] = read_v(vs, row, u, dt);
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++) o[dt] = mfma32<XT>(vf[dt], p0, o[dt]);
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++) o[dt] = mfma32<XT>(vf[dt], p1, o[dt]);
+        }
       }
     };
-    // the steps from k0 to k1: while one is worked on the next is brought, and the one after it looked up
-    auto run = [&](auto SAFE) __attribute__((always_inline)) {
+    // The same where values that are not finite must count only for the rows that see their key: one key at a time
+    auto values_safe = [&](const char* vs) __attribute__((always_inline)) {
+      for (int i = 0; i < 16; i++) {
+        const float other = lane_xor<32>(s[0], lane);
+        for (int gg = 0; gg < 2; gg++) {
+          const int key = 8 * (i / 4) + 4 * gg + i % 4;
+          const float p = gg == g ? s[0] : other;
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const int d = 32 * dt + 8 * (e / 4) + 4 * g + e % 4, ch = d / G::CE;
+              const char* vp = vs + (ch / 8 * kKeys + key) * 128 + ((ch & 7) ^ swizzle_v(key)) * 16 + d % G::CE * G::ES;
+              float v;
+              if constexpr (G::F32) v = *reinterpret_cast<const float*>(vp);
+              else v = half<XT>(*reinterpret_cast<const uint16_t*>(vp), 0);
+              o[dt][e] = p == 0.f ? o[dt][e] : fmaf(p, v, o[dt][e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 15; e++) s[e] = s[e + 1];
+      }
+    };
+    auto reset = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < G::DT; i++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = 0.f;
-      m = -INFINITY, l = 0.f;
+      m = -INFINITY, l = 0.f, off = kLift<XT>;
       look(k0);
       __syncthreads();  // the last tile's steps have been read
-      bring(stage0);
-      look(k0 + kKeys);
-      __syncthreads();
-      for (int k = k0; k < k1; k += 2 * kKeys) {
-        if (k + kKeys < k1) {
-          bring(stage1);
-          look(k + 2 * kKeys);
-        }
-        step(SAFE, stage0, k);
-        __syncthreads();
-        if (k + kKeys >= k1) break;
-        if (k + 2 * kKeys < k1) {
-          bring(stage0);
-          look(k + 3 * kKeys);
-        }
-        step(SAFE, stage1, k + kKeys);
-        __syncthreads();
-      }
-      l += lane_xor<32>(l, lane);
+      bring_k(0, k_lds1, 0);
+      look(k0 + 32);
     };
-    run(std::false_type{});
+    auto advance = [&](const char* ks, const char* vs, int row) __attribute__((always_inline)) {
+      const f32x16 next = products(ks, row);
+      exponentials();
+      values(vs, row);
+      s = next;
+      largest();
+    };
+    // The same for 16-bit types in an order that gives each matrix instruction vector
+    // operations to run beside.  The last 16 keys' values are left to the next call, whose
+    // score products, a chain, alternate with them; the first 16 keys' values run beside the
+    // split of the others and the next maximum.  extra(i), i < 2 N + 1: what else there is
+    // to do behind the i-th of them.
+    constexpr int N = G::DT * 2;
+    u32x4 v_last[G::DT], p_last[2];
+    auto value_product = [&](int i, const u32x4 (&v)[G::DT], const u32x4 (&p)[2]) __attribute__((always_inline)) {
+      o[i % G::DT] = mfma32<XT>(v[i % G::DT], p[i / G::DT], o[i % G::DT]);
+    };
+    auto split = [&](int u, int e, u32x4 (&p)[2]) __attribute__((always_inline)) {
+      const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
+      p[0][e] = pack<XT>(x, y);
+      p[1][e] = pack<XT>(less<XT, 0>(x, p[0][e], minus_lo), less<XT, 1>(y, p[0][e], minus_hi));
+      asm volatile("" : "+v"(p[0][e]), "+v"(p[1][e]));  // here, not where it is used
+    };
+    auto none_left = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) p_last[0][e] = p_last[1][e] = 0u;
+#pragma unroll
+      for (int dt = 0; dt < G::DT; dt++) v_last[dt] = u32x4{0u, 0u, 0u, 0u};
+    };
+    auto last_values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < N; i++) value_product(i, v_last, p_last);
+    };
+    auto overlapped = [&](const char* ks, const char* vs, int row, auto&& extra) __attribute__((always_inline)) {
+      if (__any(mt > m)) {
+        last_values();
+        none_left();
+        grow();
+      }
+      constexpr int AHEAD = 4;  // K reads on their way
+      u32x4 kf[N], v_first[G::DT], p_first[2];
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) kf[i] = read_k(ks, row, i);
+      f32x16 next;
+#pragma unroll
+      for (int e = 0; e < 16; e++) next[e] = 0.f;
+      float sum = 0.f;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i <= N; i++) {
+        if (i < N) value_product(i, v_last, p_last);
+        if (i > 0) next = mfma32<XT>(kf[i - 1], qf[i - 1], next);
+        if (i > 0 && i - 1 + AHEAD < N) kf[i - 1 + AHEAD] = read_k(ks, row, i - 1 + AHEAD);
+#pragma unroll
+        for (int dt = 0; dt < G::DT; dt++)
+          if (i == N / 2 + 1 + dt % (N / 2)) v_first[dt] = read_v(vs, row, 0, dt);
+#pragma unroll
+        for (int e = 16 * i / (N + 1); e < 16 * (i + 1) / (N + 1); e++) {
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, off));
+          sum += s[e];
+        }
+        if (2 * i > N) {
+          constexpr int half = N / 2 + 1, many = N + 1 - half;
+#pragma unroll
+          for (int e = 4 * (i - half) / many; e < 4 * (i + 1 - half) / many; e++) split(0, e, p_first);
+        }
+        extra(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      l += sum;
+      mt = next[0];
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        value_product(i, v_first, p_first);
+#pragma unroll
+        for (int dt = 0; dt < G::DT; dt++)
+          if (i == dt) v_last[dt] = read_v(vs, row, 1, dt);
+#pragma unroll
+        for (int e = 4 * i / N; e < 4 * (i + 1) / N; e++) split(1, e, p_last);
+#pragma unroll
+        for (int e = 16 * i / N; e < 16 * (i + 1) / N; e++) mt = fmaxf(mt, next[e]);
+        extra(N + 1 + i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      mt = fmaxf(mt, lane_xor<32>(mt, lane)) * scale;
+      s = next;
+    };
+    // 32 keys from k on: their values, and the scores of the 32 after them (K and V rows of one step)
+    auto half_step = [&](const char* ks, const char* vs, int row, int k) __attribute__((always_inline)) {
+      if (seen(k)) {
+        grow();
+        advance(ks, vs, row);
+      } else if (seen(k + 32)) {
+        s = products(ks, row);
+        largest();
+      }
+      if (seen(k + 32)) special(k + 32);
+    };
+    auto step = [&](const char* ks, const char* vs, int k) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < G::KT; t++) half_step(ks, vs, 32 * t, k + 32 * t);
+    };
+    reset();
+    bring(k_lds0, v_lds0);
+    look(k0 + 32 + kKeys);
+    step_barrier();
+    if (seen(k0)) {
+      s = products(k_lds1, 0);
+      largest();
+      special(k0);
+    }
+    step_barrier();
+    // Steps whose keys, and the 32 after them, are all seen by every row of the tile, with others
+    // behind them: no masks, nothing to decide.
+    const int all_hi = min(k1, sq.p0 + tok0 + 1), all_lo = a.window > 0 ? max(0, hi - a.window) : 0;
+    const bool easy = !G::F32 && a.direct && a.same && a.D == DP && a.softcap == 0.f;
+    auto easy_step = [&](const char* ks, const char* vs, char* k_next, char* v_next, int k) __attribute__((always_inline)) {
+      if constexpr (!G::F32) {
+        int64_t k_off = 0;
+        auto rest = [&](int i) __attribute__((always_inline)) {  // brings the next step, a piece at a time
+#pragma unroll
+          for (int t = 0; t < G::KT; t++) {
+            if (i == 3 * t) k_off = (int64_t)((uint64_t)(uint32_t)min(max(entry[t], 0), a.pages - 1) * (uint32_t)a.k_page +
+                                              (uint64_t)(uint32_t)in_page[t] * (uint32_t)a.k_tok);
+            if (i == 3 * t + 1) rows_to_lds(vb + v_off, v_chunk, v_next, 32 * t);
+            if (i == 3 * t + 2) {
+              rows_to_lds(kb + k_off, k_chunk, k_next, 32 * t);
+              v_off = k_off;
+            }
+          }
+          if (i == 3 * G::KT) look(k + 32 + 2 * kKeys);
+        };
+        if (busy) {
+          overlapped(ks, vs, 0, rest);
+          if constexpr (G::KT > 1) overlapped(ks, vs, 32, [](int) {});
+        } else {
+#pragma unroll
+          for (int i = 0; i <= 3 * G::KT; i++) rest(i);
+        }
+        step_barrier();
+      }
+    };
+    // while a step is worked on the next is brought, and the one after it looked up
+    for (int k = k0; k < k1; k += 2 * kKeys) {
+      if (easy && k + 32 >= all_lo && k + 3 * kKeys + 32 <= all_hi) {
+        none_left();
+        do {
+          easy_step(k_lds0, v_lds0, k_lds1, v_lds1, k);
+          easy_step(k_lds1, v_lds1, k_lds0, v_lds0, k + kKeys);
+          k += 2 * kKeys;
+        } while (k + 3 * kKeys + 32 <= all_hi);
+        if constexpr (!G::F32) last_values();
+      }
+      if (k + kKeys < k1) {
+        bring(k_lds1, v_lds1);
+        look(k + 32 + 2 * kKeys);
+      }
+      step(k_lds0, v_lds0, k);
+      step_barrier();
+      if (k + kKeys >= k1) break;
+      if (k + 2 * kKeys < k1) {
+        bring(k_lds0, v_lds0);
+        look(k + 32 + 3 * kKeys);
+      }
+      step(k_lds1, v_lds1, k + kKeys);
+      step_barrier();
+    }
+    l += lane_xor<32>(l, lane);
     float x = l;  // not finite where some value is not
 #pragma unroll
     for (int i = 0; i < G::DT; i++)
 #pragma unroll
       for (int e = 0; e < 16; e++) x = fmaf(o[i][e], 0.f, x);
-    if (__syncthreads_or(r0 + c < rows && !isfinite(x))) run(std::true_type{});
+    if (__syncthreads_or(r0 + c < rows && !isfinite(x))) {
+      // again, 32 keys at a time
+      reset();
+      for (int k = k0; k < k1; k += 32) {
+        if (k > k0) {
+          bring_k(0, k_lds1, 0);
+          look(k + 32);
+        }
+        bring_v(v_lds1, 0);
+        step_barrier();
+        if (seen(k)) {
+          s = products(k_lds1, 0);
+          largest();
+          special(k);
+          grow();
+          exponentials();
+          if (k + 32 > first_hi || k < last_lo) values_safe(v_lds1);
+          else values(v_lds1, 0);
+        }
+        step_barrier();
+      }
+      l += lane_xor<32>(l, lane);
+    }
 
     // row r of the tile: its place in out, its head
     auto finish = [&](int r, int d, float M, float L, f32x4 acc) __attribute__((always_inline)) {
@@ -728,11 +944,13 @@ bool chunk_attention_plan(ChunkAttnArgs& a, int cus, int64_t* part_bytes) {
   const int esz = a.type == GEN_F32 ? 4 : 2;
   uint64_t bits = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
   a.direct = 1;
-  for (int64_t st : {a.k_page, a.k_head, a.k_tok, a.v_page, a.v_head, a.v_tok}) {
-    bits |= (uint64_t)(st * esz);
-    if (st < 0 || st * esz > 0xFFFFFFFFll) a.direct = 0;
+  for (int64_t* st : {&a.k_page, &a.k_head, &a.k_tok, &a.v_page, &a.v_head, &a.v_tok}) {
+    *st *= esz;
+    bits |= (uint64_t)*st;
+    if (*st < 0 || *st > 0xFFFFFFFFll) a.direct = 0;
   }
   if (bits & 15) a.direct = 0;
+  a.same = a.k_page == a.v_page && a.k_tok == a.v_tok;
   const int per = a.Hq / a.Hkv;
   a.tile_heads = std::min(per, kRows);
   a.tile_tokens = kRows / a.tile_heads;

@@ -706,7 +706,7 @@ struct ChunkAttnArgs {
   const int32_t *lengths, *starts;  // [B], [B + 1]
   const float* sinks;      // [Hq] or null
   int64_t q_tok, q_head;   // strides in elements
-  int64_t k_page, k_head, k_tok, v_page, v_head, v_tok;
+  int64_t k_page, k_head, k_tok, v_page, v_head, v_tok;  // in elements; the plan makes them bytes
   int64_t table_row;
   int T, B, Hq, Hkv, D, pages, page, width;
   int window;              // keys a token sees, itself the last (0: all)
@@ -714,7 +714,7 @@ struct ChunkAttnArgs {
   int type;
   // how the work is split (chunk_attention_plan)
   int tile_heads, tile_tokens;  // rows of a tile
-  int direct;              // pools of 16-byte alignment and strides of 32 bits
+  int direct, same;        // pools of 16-byte alignment and strides of 32 bits; of the same strides
   uint32_t page_mul;       // as PagedAttnArgs
   int page_shift;
   int wgs;                 // workgroups
