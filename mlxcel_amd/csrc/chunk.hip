@@ -44,12 +44,13 @@ constexpr int kWaves = 4, kRows = 32 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // What a tile's start and end cost, in keys.
-constexpr int kAround = 64;
-// Keys of a tile that is not cut, and the least that a workgroup takes.
-constexpr int kWhole = 128, kLeast = 128;
+constexpr int kAround = 192;
+// Keys of a tile that is not cut, and the least units that a workgroup takes.
+constexpr int kWhole = 256, kLeast = 128;
 
-// Workgroups whose results one of them joins, and how many are read at a time.
-constexpr int kJoin = 16, kFlight = 8;
+// Workgroups whose results one of them joins, how many are read at a time, and how
+// many times 16 bytes of each lane.
+constexpr int kJoin = 16, kFlight = 8, kUnits = 4;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -111,14 +112,25 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// LDS by pointers of its own: 32 bits, and what is constant goes into the instruction.
+typedef __attribute__((address_space(3))) char Lds;
+template <typename T>
+__device__ __forceinline__ T lds_read(const Lds* p) {
+  return *(const __attribute__((address_space(3))) T*)p;
+}
+template <typename T>
+__device__ __forceinline__ void lds_write(Lds* p, T v) {
+  *(__attribute__((address_space(3))) T*)p = v;
+}
+
 // Four rows of the lane's column: row i of the 16 lanes' 4 x 16 elements is read
 // by lanes 4 i .. 4 i + 3, lane j gets column j.
-__device__ __forceinline__ u32x2 read_transposed(const char* p) {
+__device__ __forceinline__ u32x2 read_transposed(const Lds* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
 // 16 bytes a lane to LDS, in the order of the lanes.
-__device__ __forceinline__ void to_lds(const char* from, char* to) {
+__device__ __forceinline__ void to_lds(const char* from, Lds* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
@@ -144,6 +156,12 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
   }
 }
 
+// Two values as a pair of 16-bit results, rounded as store4 does.
+template <int XT>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+  return f32_to_xt<XT == GEN_F16 ? 1 : 0>(lo) | f32_to_xt<XT == GEN_F16 ? 1 : 0>(hi) << 16;
+}
+
 // Probabilities are held as 2^lift p: in float16 their largest is then 2^14, and
 // those down to 2^-28 of it keep all their bits (smaller ones differ by 2^-39 of it).
 template <int XT>
@@ -157,11 +175,10 @@ __device__ __forceinline__ float exp2_diff(float a, float b) {
 // The new tokens of a sequence that have a position, and its tiles.
 struct Seq {
   int first, n, p0;  // row of the first of n tokens, its position
-  int tiles;         // of a head
+  int tiles;         // of a head: tile_tokens tokens each
+  int late;          // tiles up to this one see key 0
   int skip;          // rows before `first` without a position
 };
-
-// Rows of a tile: tt tokens of hp heads.
 __device__ __forceinline__ Seq seq_of(const ChunkAttnArgs& a, int start, int end, int length) {
   const int st = min(max(start, 0), a.T), all = min(max(end, st), a.T) - st;
   const int len = (int)min((int64_t)max(length, 0), (int64_t)a.width * a.page);
@@ -170,7 +187,10 @@ __device__ __forceinline__ Seq seq_of(const ChunkAttnArgs& a, int start, int end
   s.n = all - s.skip;
   s.first = st + s.skip;
   s.p0 = len - s.n;
-  s.tiles = (s.n + a.tile_tokens - 1) / a.tile_tokens;
+  // v / tile_tokens: (v + 1/2) / tile_tokens is no nearer to a whole number than 1/2 of one
+  s.tiles = (int)((s.n + a.tile_tokens - 0.5) * a.inv_tile_tokens);
+  const int lo = s.p0 - a.window + 1;
+  s.late = a.window == 0 ? s.tiles : lo > 0 ? 0 : (int)((0.5 - lo) * a.inv_tile_tokens) + 1;
   return s;
 }
 __device__ __forceinline__ int tile_lo(const ChunkAttnArgs& a, const Seq& s, int j) {
@@ -179,41 +199,47 @@ __device__ __forceinline__ int tile_lo(const ChunkAttnArgs& a, const Seq& s, int
 __device__ __forceinline__ int tile_hi(const ChunkAttnArgs& a, const Seq& s, int j) {
   return s.p0 + min(s.n, (j + 1) * a.tile_tokens);
 }
+// The units of a tile are its keys and kAround more.  All counts of units are whole
+// numbers below 2^52, held as doubles: their products and sums cost a fraction of 64-bit ones.
 // sum over tiles i < j of kAround + tile_hi(i) - tile_lo(i)
-__device__ __forceinline__ int64_t before(const ChunkAttnArgs& a, const Seq& s, int j) {
-  const int64_t tt = a.tile_tokens;
-  int64_t sum = j * (int64_t)(kAround + s.p0) + tt * ((int64_t)j * (j + 1) / 2);
-  if (j == s.tiles) sum -= j * tt - s.n;
-  if (a.window > 0) {
-    const int64_t lo = (int64_t)s.p0 - a.window + 1;
-    const int i0 = lo > 0 ? 0 : (int)((uint32_t)-lo / (uint32_t)tt) + 1;  // the first tile that does not begin at key 0
-    if (j > i0) sum -= (j - i0) * lo + tt * ((int64_t)j * (j - 1) / 2 - (int64_t)i0 * (i0 - 1) / 2);
-  }
+__device__ __forceinline__ double before(const ChunkAttnArgs& a, const Seq& s, int j) {
+  const double tt = a.tile_tokens, J = j, L = s.late;
+  double sum = J * (kAround + s.p0) + tt * (J * (J + 1) * 0.5);
+  if (j == s.tiles) sum -= J * tt - s.n;
+  if (j > s.late) sum -= (J - L) * (s.p0 - a.window + 1) + tt * ((J * (J - 1) - L * (L - 1)) * 0.5);
   return sum;
 }
 // The tiles of a head are taken shortest, longest, second shortest, ..: tile number q
 // in that order, and the units of those before it.  Two neighbours together then cost
 // about the same everywhere, so that workgroups begin near the same key of their tiles
-// and find each other's keys in L2 (2048 tokens of 32768: misses XX of XX).
+// and find each other's keys in L2 (2048 tokens of 32768: 6% of the requests missed it
+// instead of 66%).
 __device__ __forceinline__ int tile_at(const Seq& s, int q) { return q & 1 ? s.tiles - 1 - q / 2 : q / 2; }
-__device__ __forceinline__ int64_t units_before(const ChunkAttnArgs& a, const Seq& s, int q) {
-  return before(a, s, (q + 1) / 2) + (q > 1 ? before(a, s, s.tiles) - before(a, s, s.tiles - q / 2) : 0);
+__device__ __forceinline__ double units_before(const ChunkAttnArgs& a, const Seq& s, double head, int q) {
+  return before(a, s, (q + 1) / 2) + (q > 1 ? head - before(a, s, s.tiles - q / 2) : 0.0);
 }
-// v / d for 0 <= v < 2^52
-__device__ __forceinline__ int64_t divide(int64_t v, int64_t d) {
-  int64_t q = (int64_t)((double)v / (double)d);
-  while (q * d > v) q--;
-  while ((q + 1) * d <= v) q++;
+// v / d, whole
+__device__ __forceinline__ double divide(double v, double d) {
+  double q = floor(v / d);
+  if (q * d > v) q -= 1.0;
+  if ((q + 1.0) * d <= v) q += 1.0;
   return q;
 }
 
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
+__device__ __forceinline__ double lane_value(double v, int from) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, from), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), from);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ Seq lane_value(const Seq& s, int from) {
+  return Seq{(int)__builtin_amdgcn_readlane(s.first, from), (int)__builtin_amdgcn_readlane(s.n, from),
+             (int)__builtin_amdgcn_readlane(s.p0, from),    (int)__builtin_amdgcn_readlane(s.tiles, from),
+             (int)__builtin_amdgcn_readlane(s.late, from),  (int)__builtin_amdgcn_readlane(s.skip, from)};
 }
 
-// Words of one partial result: O [rows][DP], then (m, l) [rows][2].
-constexpr int part_words(int rows, int DP) { return rows * (DP + 2); }
+// Words of one partial result: O as the registers of `waves` waves hold it, 16 bytes of
+// each lane after the other, then (m, l) of their rows.
+constexpr int part_words(int waves, int DP) { return waves * (32 * DP + 64); }
 
 template <int XT, int DP>
 __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kernel(const ChunkAttnArgs a) {
@@ -222,7 +248,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
   // Keys and values of two steps.  Objects of their own, with one sum from each to what is
   // read of it, so that the compiler sees that what is being filled is not what is read and
   // does not wait for it (it did, at 1700 us for 2048 tokens of 32768).
-  __shared__ __align__(16) char k_lds0[G::TILE], v_lds0[G::TILE], k_lds1[G::TILE], v_lds1[G::TILE];
+  __shared__ __align__(16) char k_obj0[G::TILE], v_obj0[G::TILE], k_obj1[G::TILE], v_obj1[G::TILE];
+  Lds *const k_lds0 = (Lds*)k_obj0, *const v_lds0 = (Lds*)v_obj0, *const k_lds1 = (Lds*)k_obj1, *const v_lds1 = (Lds*)v_obj1;
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, g = lane >> 5;
@@ -230,98 +257,109 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
   const int w = a.wgs % 8 == 0 ? (int)(blockIdx.x % 8) * (a.wgs / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
   const int per = a.Hq / a.Hkv, hp = a.tile_heads, tiles_h = (per + hp - 1) / hp, heads_b = a.Hkv * tiles_h;
 
-  // Where this workgroup's work begins and ends: tile among those of sequence b, key of its range.
+  // Where this workgroup's work begins and ends: head and tile number of sequence b (past
+  // the last: the next one's first), key of its range.
   struct Bound {
-    int b, tile, key;
-    int64_t base;  // of the sequence, among all units
-  };
-  auto load_seq = [&](int b) -> Seq {
-    const int s = __builtin_amdgcn_readfirstlane(a.starts[b]), e = __builtin_amdgcn_readfirstlane(a.starts[b + 1]);
-    return seq_of(a, s, e, __builtin_amdgcn_readfirstlane(a.lengths[b]));
-  };
-  auto bound_at = [&](int64_t off, int b, int64_t base) -> Bound {
-    const Seq s = load_seq(b);
-    const int64_t head = before(a, s, s.tiles);
-    const int hh = (int)divide(off, head);
-    off -= hh * head;
-    int lo = 0, hi = s.tiles - 1;  // the last tile that begins at or before off
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (units_before(a, s, mid) <= off) lo = mid;
-      else hi = mid - 1;
+    int b, hh, nth, key;
+    double base;  // of the sequence, among all units
+    __device__ __forceinline__ bool ahead_of(const Bound& o) const {
+      return b != o.b ? b < o.b : hh != o.hh ? hh < o.hh : nth != o.nth ? nth < o.nth : key < o.key;
     }
-    off -= units_before(a, s, lo);
-    const int j = tile_at(s, lo), keys = tile_hi(a, s, j) - tile_lo(a, s, j);
-    const int64_t r = off - kAround;
-    int key = r > 0 ? (int)r / kKeys * kKeys : 0, tile = hh * s.tiles + lo;
-    if (keys <= kWhole && off > 0) key = 0, tile++;  // it belongs to the workgroup that begins it
-    return Bound{b, tile, key, base};
   };
-  auto clear = [&](const Seq& s) {  // rows without a position
+  auto load_seq = [&](int b) __attribute__((always_inline)) -> Seq {
+    const int s = __builtin_amdgcn_readfirstlane(a.starts[b]), e = __builtin_amdgcn_readfirstlane(a.starts[b + 1]);
+    return lane_value(seq_of(a, s, e, __builtin_amdgcn_readfirstlane(a.lengths[b])), 0);
+  };
+  auto bound_at = [&](double off, int b, const Seq& s, double base) __attribute__((always_inline)) -> Bound {
+    const double head = before(a, s, s.tiles), hh = divide(off, head);
+    off -= hh * head;
+    int lo = 0, hi = s.tiles;  // the last tile that begins at or before off: a lane looks at each
+    while (hi - lo > 1) {
+      const int by = (hi - lo + 63) >> 6, q = lo + lane * by;
+      const int n = __popcll(__ballot(q < hi && units_before(a, s, head, q) <= off));
+      hi = min(hi, lo + n * by);
+      lo += (n - 1) * by;
+    }
+    off -= units_before(a, s, head, lo);
+    const int j = tile_at(s, lo), keys = tile_hi(a, s, j) - tile_lo(a, s, j), r = (int)off - kAround;
+    // a tile that is not cut belongs to the workgroup that begins it
+    const bool past = keys <= kWhole && off > 0.0;
+    return Bound{b, (int)__builtin_amdgcn_readfirstlane((int)hh), (int)__builtin_amdgcn_readfirstlane(lo + past),
+                 (int)__builtin_amdgcn_readfirstlane(past || r <= 0 ? 0 : r / kKeys * kKeys), base};
+  };
+  auto clear = [&](const Seq& s) __attribute__((always_inline)) {  // rows without a position
     const int64_t from = (int64_t)(s.first - s.skip) * a.Hq * a.D, n = (int64_t)s.skip * a.Hq * a.D;
     for (int64_t i = 4 * tid; i < n; i += 1024) store4<XT>(a.out, from + i, f32x4{0.f, 0.f, 0.f, 0.f});
   };
-  int64_t total, n;
+  double total, n;
   Bound at, end;
+  Seq sq{};  // sequence at.b
   {
-    auto units_of = [&](const Seq& s) { return heads_b * before(a, s, s.tiles); };
-    auto per_group = [&]() { return max((int64_t)((double)total * a.inv_wgs) + 1, (int64_t)kLeast); };
-    int64_t sum, mine;
-    auto scan = [&]() {
-#pragma unroll
-      for (int s = 1; s < 64; s <<= 1) {
-        const int64_t o = __shfl_up(sum, s);
+    auto units_of = [&](const Seq& s) __attribute__((always_inline)) { return heads_b * before(a, s, s.tiles); };
+    auto per_group = [&]() __attribute__((always_inline)) { return fmax(floor(total * a.inv_wgs) + 1.0, (double)kLeast); };
+    double sum, mine;
+    auto scan = [&](int lanes) __attribute__((always_inline)) {
+      for (int s = 1; s < lanes; s <<= 1) {
+        const double o = __shfl_up(sum, s);
         if (lane >= s) sum += o;
       }
     };
     if (a.B <= 64) {  // each wave finds them by itself, sequence i in lane i
-      const Seq s = lane < a.B ? seq_of(a, a.starts[lane], a.starts[lane + 1], a.lengths[lane]) : Seq{0, 0, 0, 0, 0};
+      const Seq s = lane < a.B ? seq_of(a, a.starts[lane], a.starts[lane + 1], a.lengths[lane]) : Seq{};
       sum = mine = units_of(s);
-      scan();
-      total = __shfl(sum, 63);
-      total = uniform(total);
-      n = per_group();
-      auto find = [&](int64_t p) -> Bound {
-        if (p >= total) return Bound{a.B, 0, 0, total};
-        const int i = __builtin_ctzll(__ballot(sum - mine <= p && p < sum));
-        const int64_t base = uniform(__shfl(sum - mine, i));
-        return bound_at(p - base, i, base);
-      };
-      at = find(w * n);
-      end = find((w + 1) * n);
+      scan(a.B);
+      total = lane_value(sum, a.B - 1);
+      n = lane_value(per_group(), 0);
+      end = Bound{a.B, 0, 0, 0, total};
+#pragma unroll 1
+      for (int i = 0; i < 2; i++) {
+        at = end;
+        const double p = (w + 1 - i) * n;
+        end = Bound{a.B, 0, 0, 0, total};
+        if (p < total) {
+          const int b = __builtin_ctzll(__ballot(sum - mine <= p && p < sum));
+          const double base = lane_value(sum - mine, b);
+          sq = lane_value(s, b);
+          end = bound_at(p - base, b, sq, base);
+        }
+      }
+      const Bound first = end;  // the second round looked for the beginning
+      end = at;
+      at = first;
       for (uint64_t none = __ballot(s.skip > 0); none; none &= none - 1) {
         const int b = __builtin_ctzll(none);
-        if (b % a.wgs == w) clear(load_seq(b));
+        if (b % a.wgs == w) clear(lane_value(s, b));
       }
     } else {  // thread i sums those of its share
-      int64_t* sums = reinterpret_cast<int64_t*>(k_lds0);
-      Bound* bound = reinterpret_cast<Bound*>(k_lds0 + 64);
+      double* sums = reinterpret_cast<double*>(k_obj0);
+      Bound* bound = reinterpret_cast<Bound*>(k_obj0 + 64);
       const int share = (a.B + 255) / 256, b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
-      mine = 0;
+      mine = 0.0;
       for (int b = b0; b < b1; b++) mine += units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
       sum = mine;
-      scan();
+      scan(64);
       if (lane == 63) sums[wave] = sum;
       __syncthreads();
-      int64_t ahead = sum - mine;
-      total = 0;
+      double ahead = sum - mine;
+      total = 0.0;
 #pragma unroll
       for (int i = 0; i < kWaves; i++) {
         if (i < wave) ahead += sums[i];
         total += sums[i];
       }
-      total = uniform(total);
-      n = per_group();
+      total = lane_value(total, 0);
+      n = lane_value(per_group(), 0);
+#pragma unroll 1
       for (int i = 0; i < 2; i++) {
-        const int64_t p = (w + i) * n;
+        const double p = (w + i) * n;
         if (p >= total) {
-          if (tid == 0) bound[i] = Bound{a.B, 0, 0, total};
+          if (tid == 0) bound[i] = Bound{a.B, 0, 0, 0, total};
         } else if (ahead <= p && p < ahead + mine) {
-          int64_t base = ahead;
+          double base = ahead;
           for (int b = b0; b < b1; b++) {
-            const int64_t u = units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
+            const double u = units_of(seq_of(a, a.starts[b], a.starts[b + 1], a.lengths[b]));
             if (p < base + u) {
-              bound[i] = Bound{b, 0, 0, base};
+              bound[i] = Bound{b, 0, 0, 0, base};
               break;
             }
             base += u;
@@ -333,26 +371,43 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         if (s.skip > 0) clear(s);
       }
       __syncthreads();
-      auto find = [&](int i) -> Bound {
-        const int b = __builtin_amdgcn_readfirstlane(bound[i].b);
-        const int64_t base = uniform(bound[i].base);
-        return b >= a.B ? Bound{b, 0, 0, base} : bound_at((w + i) * n - base, b, base);
-      };
-      at = find(0);
-      end = find(1);
+#pragma unroll 1
+      for (int i = 1; i >= 0; i--) {
+        end = at;
+        at.b = __builtin_amdgcn_readfirstlane(bound[i].b);
+        at.hh = at.nth = at.key = 0;
+        at.base = lane_value(bound[i].base, 0);
+        if (at.b < a.B) {
+          sq = load_seq(at.b);
+          at = bound_at((w + i) * n - at.base, at.b, sq, at.base);
+        }
+      }
       __syncthreads();  // the LDS is free again
     }
   }
+  if (!at.ahead_of(end)) return;
 
   uint32_t minus_lo = 0x0000BF80u, minus_hi = 0xBF800000u;
   asm volatile("" : "+s"(minus_lo), "+s"(minus_hi));
   // A thread brings place lane % 8 of every block of rows 8 wave + lane / 8 (+ 32) of a step.
   const int my_row8 = 8 * wave + (lane >> 3), k_chunk = (lane & 7) ^ swizzle_k(my_row8), v_chunk = (lane & 7) ^ swizzle_v(my_row8);
   const int chunks = a.D / G::CE;
+  // What a lane reads of a block: chunk 2 i + g of K's row c, i < 4; the row and the 8 bytes of
+  // V's 32 columns, even and odd ones of two.  One sum each, which the compiler leaves alone: of
+  // the parts it would make pointers that it no longer knows to be V's.
+  int k_lane[4], v_lane[2];
+  {
+    const int i16 = lane & 15, r = 4 * g + (i16 >> 2), ch = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+#pragma unroll
+    for (int i = 0; i < 4; i++) k_lane[i] = c * 128 + ((2 * i + g) ^ swizzle_k(c)) * 16;
+#pragma unroll
+    for (int i = 0; i < 2; i++) v_lane[i] = r * 128 + ((4 * i + ch) ^ swizzle_v(r)) * 16 + (i16 & 1) * 8;
+    asm volatile("" : "+v"(k_lane[0]), "+v"(k_lane[1]), "+v"(k_lane[2]), "+v"(k_lane[3]), "+v"(v_lane[0]), "+v"(v_lane[1]));
+  }
   if (DP != a.D) {  // K's chunks past the head are zero and stay so
     for (int i = tid; i < G::TILE / 16; i += 256) {
-      reinterpret_cast<u32x4*>(k_lds0)[i] = u32x4{0u, 0u, 0u, 0u};
-      reinterpret_cast<u32x4*>(k_lds1)[i] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(k_obj0)[i] = u32x4{0u, 0u, 0u, 0u};
+      reinterpret_cast<u32x4*>(k_obj1)[i] = u32x4{0u, 0u, 0u, 0u};
     }
   }
   // Scores in units of log2 e are `scale` times the product (the tanh of a soft
@@ -362,39 +417,42 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
   const float cap_in = a.softcap > 0.f ? fminf(2.f * kLog2e * fabsf(a.scale) / a.softcap, FLT_MAX) : 0.f;
   const __amdgpu_buffer_rsrc_t parts = buffer_rsrc(a.part, (uint32_t)((int64_t)4 * a.wgs * a.slot_words * 4));
 
-  Seq sq = at.b < a.B ? load_seq(at.b) : Seq{};
-  int64_t head_units = at.b < a.B ? before(a, sq, sq.tiles) : 0;
-  while (at.b < a.B && (at.b < end.b || (at.b == end.b && (at.tile < end.tile || (at.tile == end.tile && at.key < end.key))))) {
-    if (at.tile >= heads_b * sq.tiles) {
-      at.base += heads_b * head_units;
-      at.b++;
-      at.tile = at.key = 0;
-      if (at.b < a.B) {
+  double head_units = lane_value(before(a, sq, sq.tiles), 0);
+  while (at.ahead_of(end)) {
+    if (at.nth >= sq.tiles) {
+      at.nth = at.key = 0;
+      if (++at.hh >= heads_b || sq.tiles == 0) {
+        at.hh = 0;
+        at.base = lane_value(at.base + heads_b * head_units, 0);
+        if (++at.b >= a.B) break;
         sq = load_seq(at.b);
-        head_units = before(a, sq, sq.tiles);
+        head_units = lane_value(before(a, sq, sq.tiles), 0);
       }
       continue;
     }
-    const int hh = at.tile / sq.tiles, nth = at.tile - hh * sq.tiles, j = tile_at(sq, nth);
-    const int hk = hh / tiles_h, ht = hh - hk * tiles_h;
+    const int j = tile_at(sq, at.nth), hk = tiles_h == 1 ? at.hh : at.hh / tiles_h, ht = at.hh - hk * tiles_h;
     const int heads = min(hp, per - hp * ht), head0 = hk * per + hp * ht;
     const int tok0 = j * a.tile_tokens, toks = min(a.tile_tokens, sq.n - tok0), rows = toks * heads;
     const int lo = tile_lo(a, sq, j), hi = tile_hi(a, sq, j);
-    const int k0 = lo + at.key, k1 = at.b == end.b && at.tile == end.tile ? min(hi, lo + end.key) : hi;
+    const bool ends = at.b == end.b && at.hh == end.hh && at.nth == end.nth;
+    const int k0 = lo + at.key, k1 = ends ? min(hi, lo + end.key) : hi;
     // the tile's workgroups
-    const int64_t p0 = at.base + hh * head_units + units_before(a, sq, nth) + kAround;
     int w0 = w, w1 = w;
-    if (hi - lo > kWhole && (k0 > lo || k1 < hi)) {
-      w0 = (int)divide(p0 + kKeys + n - 1, n) - 1;
-      w1 = (int)divide(p0 + (hi - lo) + n - 1, n) - 1;
+    if (k0 > lo || k1 < hi) {
+      const double p0 = at.base + at.hh * head_units + units_before(a, sq, head_units, at.nth) + kAround;
+      w0 = __builtin_amdgcn_readfirstlane((int)divide(p0 + kKeys + n - 1.0, n)) - 1;
+      w1 = __builtin_amdgcn_readfirstlane((int)divide(p0 + (hi - lo) + n - 1.0, n)) - 1;
     }
 
     // this wave's rows, and the keys that any of them sees
-    const int r0 = 32 * wave, my_row = min(r0 + c, rows - 1), my_tok = my_row / heads;
+    // row / heads for rows below 128 and at most 128 heads
+    const uint32_t inv_heads = heads == hp ? a.inv_tile_heads : (65536 + heads - 1) / heads;
+    auto token_of = [&](int row) __attribute__((always_inline)) -> int { return (int)(row * inv_heads >> 16); };
+    const int r0 = 32 * wave, my_row = min(r0 + c, rows - 1), my_tok = token_of(my_row);
     const int pos = sq.p0 + tok0 + my_tok;
     const bool busy = r0 < rows;
-    const int see1 = pos + 1, see0 = a.window > 0 ? max(0, see1 - a.window) : 0;
-    const int wave_hi = sq.p0 + tok0 + min(r0 + 31, rows - 1) / heads + 1, first_hi = sq.p0 + tok0 + min(r0, rows - 1) / heads + 1;
+    const int see1 = min(pos + 1, k1), see0 = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+    const int wave_hi = sq.p0 + tok0 + token_of(min(r0 + 31, rows - 1)) + 1, first_hi = sq.p0 + tok0 + token_of(min(r0, rows - 1)) + 1;
     const int wave_lo = a.window > 0 ? max(0, first_hi - a.window) : 0, last_lo = a.window > 0 ? max(0, wave_hi - a.window) : 0;
 
     const char* qp = static_cast<const char*>(a.q) +
@@ -415,17 +473,18 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     const char* vb = static_cast<const char*>(a.v) + hk * a.v_head + v_chunk * 16;
     // A thread's rows of a step from key k on are k + my_row8 (+ 32) of V and 32 keys more of K:
     // the scores of 32 keys are worked out beside the values of the 32 before them.
-    int entry[G::KT], in_page[G::KT];
+    int entry[G::KT + 1], in_page[G::KT + 1];
     int64_t v_off = 0;  // bytes to the V row that comes next
     // table entries of keys from + my_row8 (+ 32); past the range they are the last key's
+    auto look_row = [&](int from, int t) __attribute__((always_inline)) {
+      const uint32_t key = min(from + my_row8, hi - 1);
+      const uint32_t slot = __umulhi(key << 2, a.page_mul) >> (a.page_shift - 30);
+      in_page[t] = key - slot * a.page;
+      entry[t] = table[slot];
+    };
     auto look = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < G::KT; t++) {
-        const uint32_t key = min(from + 32 * t + my_row8, hi - 1);
-        const uint32_t slot = __umulhi(key << 2, a.page_mul) >> (a.page_shift - 30);
-        in_page[t] = key - slot * a.page;
-        entry[t] = table[slot];
-      }
+      for (int t = 0; t < G::KT; t++) look_row(from + 32 * t, t);
     };
     // bytes to the looked-up row t in a pool of these strides
     auto place = [&](int t, int64_t page_bytes, int64_t tok_bytes) __attribute__((always_inline)) -> int64_t {
@@ -434,13 +493,13 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       return pid * page_bytes + in_page[t] * tok_bytes;
     };
     // a row of full width to LDS without passing through registers
-    auto rows_to_lds = [&](const char* from, int chunk, char* to, int row) __attribute__((always_inline)) {
+    auto rows_to_lds = [&](const char* from, int chunk, Lds* to, int row) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < G::NC; i++)
         if (8 * i + 8 <= G::C || 8 * i + chunk < G::C) to_lds(from + i * 128, to + (i * kKeys + row + 8 * wave) * 128);
     };
     // a row to LDS, rows `row` on of the blocks
-    auto bring_row = [&](const char* from, int chunk, char* to, int row) __attribute__((always_inline)) {
+    auto bring_row = [&](const char* from, int chunk, Lds* to, int row) __attribute__((always_inline)) {
       if (a.direct) {  // 16-byte aligned, strides of 32 bits
         if (DP == a.D) {
           rows_to_lds(from, chunk, to, row);
@@ -454,19 +513,19 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         for (int i = 0; i < G::NC; i++)
           if (8 * i + chunk < chunks) {
             const u32x4_e x = *reinterpret_cast<const u32x4_e*>(from + i * 128);
-            *reinterpret_cast<u32x4*>(to + (i * kKeys + row + my_row8) * 128 + (lane & 7) * 16) = u32x4{x[0], x[1], x[2], x[3]};
+            lds_write(to + ((i * kKeys + row + my_row8) * 128 + (lane & 7) * 16), u32x4{x[0], x[1], x[2], x[3]});
           }
       }
     };
     // K of looked-up row t, V of the one before
-    auto bring_k = [&](int t, char* to, int row) __attribute__((always_inline)) {
+    auto bring_k = [&](int t, Lds* to, int row) __attribute__((always_inline)) {
       const int64_t off = place(t, a.k_page, a.k_tok);
       bring_row(kb + off, k_chunk, to, row);
       v_off = a.same ? off : place(t, a.v_page, a.v_tok);
     };
-    auto bring_v = [&](char* to, int row) __attribute__((always_inline)) { bring_row(vb + v_off, v_chunk, to, row); };
+    auto bring_v = [&](Lds* to, int row) __attribute__((always_inline)) { bring_row(vb + v_off, v_chunk, to, row); };
     // a step to LDS
-    auto bring = [&](char* ks, char* vs) __attribute__((always_inline)) {
+    auto bring = [&](Lds* ks, Lds* vs) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < G::KT; t++) {
         bring_v(vs, 32 * t);
@@ -476,18 +535,16 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
 
     f32x16 s;  // scores of 32 keys
     float mt;  // and their largest
-    auto read_k = [&](const char* ks, int row, int i) __attribute__((always_inline)) -> u32x4 {
-      return *reinterpret_cast<const u32x4*>(ks + ((i / 4 * kKeys + row + c) * 128 + (((2 * i + g) & 7) ^ swizzle_k(c)) * 16));
+    auto read_k = [&](const Lds* ks, int row, int i) __attribute__((always_inline)) -> u32x4 {
+      return lds_read<u32x4>(ks + k_lane[i & 3] + (i / 4 * kKeys + row) * 128);
     };
     // 16 u + the lane's eight keys of column 32 dt + c
-    auto read_v = [&](const char* vs, int row, int u, int dt) __attribute__((always_inline)) -> u32x4 {
-      const int i16 = lane & 15, r = 4 * g + (i16 >> 2);  // the row and the 8 bytes of it that this lane reads
-      const int ch = 4 * (dt & 1) + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-      const int at = (dt / 2 * kKeys + row + 16 * u + r) * 128 + (ch ^ swizzle_v(r)) * 16 + (i16 & 1) * 8;
-      const u32x2 x = read_transposed(vs + at), y = read_transposed(vs + (at + 8 * 128));
+    auto read_v = [&](const Lds* vs, int row, int u, int dt) __attribute__((always_inline)) -> u32x4 {
+      const Lds* p = vs + v_lane[dt & 1] + (dt / 2 * kKeys + row + 16 * u) * 128;
+      const u32x2 x = read_transposed(p), y = read_transposed(p + 8 * 128);
       return u32x4{x[0], x[1], y[0], y[1]};
     };
-    auto products = [&](const char* ks, int row) __attribute__((always_inline)) -> f32x16 {
+    auto products = [&](const Lds* ks, int row) __attribute__((always_inline)) -> f32x16 {
       f32x16 r;
 #pragma unroll
       for (int e = 0; e < 16; e++) r[e] = 0.f;
@@ -520,10 +577,11 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           s[e] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[e] * cap_in) + 1.f);
       }
       if (hidden) {
+        const int from = see0 - k - 4 * g, to = see1 - k - 4 * g;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-          const int key = k + 8 * (e / 4) + 4 * g + e % 4;
-          s[e] = key < see1 && key >= see0 && key < k1 ? s[e] : -INFINITY;
+          const int key = 8 * (e / 4) + e % 4;  // after k + 4 g
+          s[e] = key >= from && key < to ? s[e] : -INFINITY;
         }
       }
       if (a.softcap > 0.f || hidden) largest();
@@ -551,14 +609,14 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       }
       l += sum;
     };
-    auto values = [&](const char* vs, int row) __attribute__((always_inline)) {
+    auto values = [&](const Lds* vs, int row) __attribute__((always_inline)) {
       if constexpr (G::F32) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           const int key = 8 * (e / 4) + 4 * g + e % 4;
 #pragma unroll
           for (int dt = 0; dt < G::DT; dt++) {
-            const float v = *reinterpret_cast<const float*>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
+            const float v = lds_read<float>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
             o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[dt], 0, 0, 0);
           }
         }
@@ -583,7 +641,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       }
     };
     // The same where values that are not finite must count only for the rows that see their key: one key at a time
-    auto values_safe = [&](const char* vs) __attribute__((always_inline)) {
+    auto values_safe = [&](const Lds* vs, int g) __attribute__((always_inline)) {
       for (int i = 0; i < 16; i++) {
         const float other = lane_xor<32>(s[0], lane);
         for (int gg = 0; gg < 2; gg++) {
@@ -594,10 +652,10 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               const int d = 32 * dt + 8 * (e / 4) + 4 * g + e % 4, ch = d / G::CE;
-              const char* vp = vs + (ch / 8 * kKeys + key) * 128 + ((ch & 7) ^ swizzle_v(key)) * 16 + d % G::CE * G::ES;
+              const Lds* vp = vs + ((ch / 8 * kKeys + key) * 128 + ((ch & 7) ^ swizzle_v(key)) * 16 + d % G::CE * G::ES);
               float v;
-              if constexpr (G::F32) v = *reinterpret_cast<const float*>(vp);
-              else v = half<XT>(*reinterpret_cast<const uint16_t*>(vp), 0);
+              if constexpr (G::F32) v = lds_read<float>(vp);
+              else v = half<XT>(lds_read<uint16_t>(vp), 0);
               o[dt][e] = p == 0.f ? o[dt][e] : fmaf(p, v, o[dt][e]);
             }
         }
@@ -611,76 +669,52 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
 #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = 0.f;
       m = -INFINITY, l = 0.f, off = kLift<XT>;
-      look(k0);
-      __syncthreads();  // the last tile's steps have been read
-      bring_k(0, k_lds1, 0);
+      look_row(k0, G::KT);
       look(k0 + 32);
+      __syncthreads();  // the last tile's steps have been read
+      bring_k(G::KT, k_lds1, 0);
     };
-    auto advance = [&](const char* ks, const char* vs, int row) __attribute__((always_inline)) {
-      const f32x16 next = products(ks, row);
-      exponentials();
-      values(vs, row);
-      s = next;
-      largest();
-    };
-    // The same for 16-bit types in an order that gives each matrix instruction vector
-    // operations to run beside.  The last 16 keys' values are left to the next call, whose
-    // score products, a chain, alternate with them; the first 16 keys' values run beside the
-    // split of the others and the next maximum.  extra(i), i < 2 N + 1: what else there is
-    // to do behind the i-th of them.
-    constexpr int N = G::DT * 2;
-    u32x4 v_last[G::DT], p_last[2];
-    auto value_product = [&](int i, const u32x4 (&v)[G::DT], const u32x4 (&p)[2]) __attribute__((always_inline)) {
-      o[i % G::DT] = mfma32<XT>(v[i % G::DT], p[i / G::DT], o[i % G::DT]);
-    };
-    auto split = [&](int u, int e, u32x4 (&p)[2]) __attribute__((always_inline)) {
-      const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
-      p[0][e] = pack<XT>(x, y);
-      p[1][e] = pack<XT>(less<XT, 0>(x, p[0][e], minus_lo), less<XT, 1>(y, p[0][e], minus_hi));
-      asm volatile("" : "+v"(p[0][e]), "+v"(p[1][e]));  // here, not where it is used
-    };
-    auto none_left = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) p_last[0][e] = p_last[1][e] = 0u;
-#pragma unroll
-      for (int dt = 0; dt < G::DT; dt++) v_last[dt] = u32x4{0u, 0u, 0u, 0u};
-    };
-    auto last_values = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < N; i++) value_product(i, v_last, p_last);
-    };
-    auto overlapped = [&](const char* ks, const char* vs, int row, auto&& extra) __attribute__((always_inline)) {
-      if (__any(mt > m)) {
-        last_values();
-        none_left();
-        grow();
-      }
-      constexpr int AHEAD = 4;  // K reads on their way
-      u32x4 kf[N], v_first[G::DT], p_first[2];
+    // The values of 32 keys and the scores of the 32 after them, for 16-bit types in an order
+    // that gives each matrix instruction vector operations to run beside: the score products
+    // take the exponentials and the split of the first 16 keys, their values the split of the
+    // others, theirs the next maximum.  extra(i), i < 3 N: what else there is to do behind
+    // the i-th of them.
+    auto overlapped = [&](const Lds* ks, const Lds* vs, int row, auto&& extra) __attribute__((always_inline)) {
+      constexpr int N = G::DT * 2, AHEAD = 4;  // K reads on their way
+      grow();
+      u32x4 kf[N], vf[2][G::DT], pt[2][2];
+      auto split = [&](int u, int e) __attribute__((always_inline)) {
+        const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
+        pt[u][0][e] = pack<XT>(x, y);
+        pt[u][1][e] = pack<XT>(less<XT, 0>(x, pt[u][0][e], minus_lo), less<XT, 1>(y, pt[u][0][e], minus_hi));
+        asm volatile("" : "+v"(pt[u][0][e]), "+v"(pt[u][1][e]));  // here, not where it is used
+      };
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) kf[i] = read_k(ks, row, i);
       f32x16 next;
 #pragma unroll
       for (int e = 0; e < 16; e++) next[e] = 0.f;
       float sum = 0.f;
+      auto exponential = [&](int e) __attribute__((always_inline)) {
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, off));
+        sum += s[e];
+      };
+      // some before the first product, whose operand is on its way
+#pragma unroll
+      for (int e = 0; e < 4; e++) exponential(e);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i <= N; i++) {
-        if (i < N) value_product(i, v_last, p_last);
-        if (i > 0) next = mfma32<XT>(kf[i - 1], qf[i - 1], next);
-        if (i > 0 && i - 1 + AHEAD < N) kf[i - 1 + AHEAD] = read_k(ks, row, i - 1 + AHEAD);
+      for (int i = 0; i < N; i++) {
+        next = mfma32<XT>(kf[i], qf[i], next);
+        if (i + AHEAD < N) kf[i + AHEAD] = read_k(ks, row, i + AHEAD);
 #pragma unroll
         for (int dt = 0; dt < G::DT; dt++)
-          if (i == N / 2 + 1 + dt % (N / 2)) v_first[dt] = read_v(vs, row, 0, dt);
+          if (i == N / 2 + dt % (N / 2)) vf[0][dt] = read_v(vs, row, 0, dt);
 #pragma unroll
-        for (int e = 16 * i / (N + 1); e < 16 * (i + 1) / (N + 1); e++) {
-          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, off));
-          sum += s[e];
-        }
-        if (2 * i > N) {
-          constexpr int half = N / 2 + 1, many = N + 1 - half;
+        for (int e = 4 + 12 * i / N; e < 4 + 12 * (i + 1) / N; e++) exponential(e);
+        if (i >= N / 2) {
 #pragma unroll
-          for (int e = 4 * (i - half) / many; e < 4 * (i + 1 - half) / many; e++) split(0, e, p_first);
+          for (int e = 4 * (i - N / 2) / (N - N / 2); e < 4 * (i + 1 - N / 2) / (N - N / 2); e++) split(0, e);
         }
         extra(i);
         __builtin_amdgcn_sched_barrier(0);
@@ -688,33 +722,46 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       l += sum;
       mt = next[0];
 #pragma unroll
-      for (int i = 0; i < N; i++) {
-        value_product(i, v_first, p_first);
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int dt = 0; dt < G::DT; dt++)
-          if (i == dt) v_last[dt] = read_v(vs, row, 1, dt);
+        for (int i = 0; i < N; i++) {
+          o[i % G::DT] = mfma32<XT>(vf[u][i % G::DT], pt[u][i / G::DT], o[i % G::DT]);
+          if (u == 0) {
 #pragma unroll
-        for (int e = 4 * i / N; e < 4 * (i + 1) / N; e++) split(1, e, p_last);
+            for (int dt = 0; dt < G::DT; dt++)
+              if (i == dt) vf[1][dt] = read_v(vs, row, 1, dt);
 #pragma unroll
-        for (int e = 16 * i / N; e < 16 * (i + 1) / N; e++) mt = fmaxf(mt, next[e]);
-        extra(N + 1 + i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+            for (int e = 4 * i / N; e < 4 * (i + 1) / N; e++) split(1, e);
+          } else {
+#pragma unroll
+            for (int e = 16 * i / N; e < 16 * (i + 1) / N; e++) mt = fmaxf(mt, next[e]);
+          }
+          extra((u + 1) * N + i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       mt = fmaxf(mt, lane_xor<32>(mt, lane)) * scale;
       s = next;
     };
     // 32 keys from k on: their values, and the scores of the 32 after them (K and V rows of one step)
-    auto half_step = [&](const char* ks, const char* vs, int row, int k) __attribute__((always_inline)) {
+    auto half_step = [&](const Lds* ks, const Lds* vs, int row, int k) __attribute__((always_inline)) {
       if (seen(k)) {
-        grow();
-        advance(ks, vs, row);
+        if constexpr (G::F32) {
+          grow();
+          const f32x16 next = products(ks, row);
+          exponentials();
+          values(vs, row);
+          s = next;
+          largest();
+        } else {
+          overlapped(ks, vs, row, [](int) {});
+        }
       } else if (seen(k + 32)) {
         s = products(ks, row);
         largest();
       }
       if (seen(k + 32)) special(k + 32);
     };
-    auto step = [&](const char* ks, const char* vs, int k) __attribute__((always_inline)) {
+    auto step = [&](const Lds* ks, const Lds* vs, int k) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < G::KT; t++) half_step(ks, vs, 32 * t, k + 32 * t);
     };
@@ -732,7 +779,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     // behind them: no masks, nothing to decide.
     const int all_hi = min(k1, sq.p0 + tok0 + 1), all_lo = a.window > 0 ? max(0, hi - a.window) : 0;
     const bool easy = !G::F32 && a.direct && a.same && a.D == DP && a.softcap == 0.f;
-    auto easy_step = [&](const char* ks, const char* vs, char* k_next, char* v_next, int k) __attribute__((always_inline)) {
+    auto easy_step = [&](const Lds* ks, const Lds* vs, Lds* k_next, Lds* v_next, int k) __attribute__((always_inline)) {
       if constexpr (!G::F32) {
         int64_t k_off = 0;
         auto rest = [&](int i) __attribute__((always_inline)) {  // brings the next step, a piece at a time
@@ -761,13 +808,11 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     // while a step is worked on the next is brought, and the one after it looked up
     for (int k = k0; k < k1; k += 2 * kKeys) {
       if (easy && k + 32 >= all_lo && k + 3 * kKeys + 32 <= all_hi) {
-        none_left();
         do {
           easy_step(k_lds0, v_lds0, k_lds1, v_lds1, k);
           easy_step(k_lds1, v_lds1, k_lds0, v_lds0, k + kKeys);
           k += 2 * kKeys;
         } while (k + 3 * kKeys + 32 <= all_hi);
-        if constexpr (!G::F32) last_values();
       }
       if (k + kKeys < k1) {
         bring(k_lds1, v_lds1);
@@ -792,6 +837,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     if (__syncthreads_or(r0 + c < rows && !isfinite(x))) {
       // again, 32 keys at a time
       reset();
+      int g_safe = g;
+      asm volatile("" : "+v"(g_safe));
       for (int k = k0; k < k1; k += 32) {
         if (k > k0) {
           bring_k(0, k_lds1, 0);
@@ -805,7 +852,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           special(k);
           grow();
           exponentials();
-          if (k + 32 > first_hi || k < last_lo) values_safe(v_lds1);
+          if (k + 32 > first_hi || k < last_lo) values_safe(v_lds1, g_safe);
           else values(v_lds1, 0);
         }
         step_barrier();
@@ -813,50 +860,89 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       l += lane_xor<32>(l, lane);
     }
 
-    // row r of the tile: its place in out, its head
-    auto finish = [&](int r, int d, float M, float L, f32x4 acc) __attribute__((always_inline)) {
-      const int tok = r / heads, h = head0 + r - tok * heads;
+    // From here on by another copy of the lane's number: addresses worked out from the first
+    // would be kept in registers all through the steps, which do not have them.
+    int lane2 = lane;
+    asm volatile("" : "+v"(lane2));
+    const int c2 = lane2 & 31, g2 = lane2 >> 5;
+    // A row's result is its sum times finish(row, M, L); where it lies.
+    auto finish = [&](int r, float M, float L) __attribute__((always_inline)) -> float {
       float f = 1.f;
       if (a.sinks) {
-        const float x = a.sinks[h];
+        const float x = a.sinks[head0 + r - token_of(r) * heads];
         // the largest finite sinks stay finite in the other base
         const float sink = isinf(x) ? x : fminf(fmaxf(x * kLog2e, -FLT_MAX), FLT_MAX), M2 = fmaxf(M, sink);
         f = exp2_diff(M, M2);
         L = L * f + exp2_diff(sink, M2);
       }
-      if (d < a.D) store4<XT>(a.out, ((int64_t)(sq.first + tok0 + tok) * a.Hq + h) * a.D + d, acc * (f / L));
+      return f / L;
     };
-    const bool mine = r0 + c < rows;
+    auto out_at = [&](int r) __attribute__((always_inline)) -> int64_t {
+      const int tok = token_of(r);
+      return ((int64_t)(sq.first + tok0 + tok) * a.Hq + head0 + r - tok * heads) * a.D;
+    };
     if (w0 == w1) {
-      if (mine) {
+      if (busy) {
+        const int row2 = min(r0 + c2, rows - 1);
+        const float f = finish(row2, m - kLift<XT>, l);
+        if constexpr (G::F32) {
+          const int64_t to = out_at(row2);
+          if (r0 + c2 < rows) {
 #pragma unroll
-        for (int dt = 0; dt < G::DT; dt++)
+            for (int dt = 0; dt < G::DT; dt++)
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            finish(r0 + c, 32 * dt + 2 * e + 4 * g, m - kLift<XT>, l, f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]});
+              for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * dt + 2 * e + 4 * g2;
+                if (d < a.D) store4<XT>(a.out, to + d, f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * f);
+              }
+          }
+        } else {
+          // through LDS, so that whole rows are written: chunk i of row r at place i ^ swizzle(r); the V rows have been read
+          constexpr int LOW = (G::C & -G::C) < 8 ? (G::C & -G::C) : 8;
+          Lds* mine = (wave < 2 ? v_lds0 : v_lds1) + (wave & 1) * (32 * G::C * 16);
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+              lds_write(mine + ((c2 * G::C + ((4 * dt + q) ^ (c2 & (LOW - 1)))) * 16 + g2 * 8),
+                        u32x2{pack_out<XT>(o[dt][4 * q] * f, o[dt][4 * q + 1] * f), pack_out<XT>(o[dt][4 * q + 2] * f, o[dt][4 * q + 3] * f)});
+          const int live = min(32, rows - r0);
+#pragma unroll
+          for (int i = 0; i < G::C / 2; i++) {
+            const int at16 = i * 64 + lane2, r = at16 / G::C, ch = at16 - r * G::C;
+            const u32x4 v = lds_read<u32x4>(mine + (r * G::C + (ch ^ (r & (LOW - 1)))) * 16);
+            if (r < live && ch < chunks)
+              *reinterpret_cast<u32x4_e*>(static_cast<uint16_t*>(a.out) + out_at(r0 + r) + ch * 8) = u32x4_e{v[0], v[1], v[2], v[3]};
+          }
+        }
       }
     } else {
       // bytes of a workgroup's partial result: of its last tile (slot 1), or of one that began before it (slot 0)
-      auto part_at = [&](int v) -> uint32_t { return (uint32_t)((2 * v + (v == w0)) * a.slot_words) * 4u; };
+      auto part_at = [&](int v) __attribute__((always_inline)) -> uint32_t { return (uint32_t)((2 * v + (v == w0)) * a.slot_words) * 4u; };
       // and of the neighbours that it leads, in a place of its own: others of the joining threads may still read the first
       const uint32_t joined = (uint32_t)(2 * a.wgs * a.slot_words) * 4u;
-      auto put_part = [&](uint32_t p, int r, int d, float M, float L, f32x4 acc) {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + (r * DP + d) * 4, 0, kAgentScope);
-        if (d == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts,
-                                                p + (rows * DP + 2 * r) * 4, 0, kAgentScope);
+      const int waves = (rows + 31) >> 5;
+      // of wave v: 16 bytes of each lane, i-th of 4 DT; its rows' maxima and sums
+      auto sum_at = [&](int v, int i) __attribute__((always_inline)) -> uint32_t { return (uint32_t)((v * 4 * G::DT + i) * 64 + lane2) * 16u; };
+      auto ml_at = [&](int v) __attribute__((always_inline)) -> uint32_t { return (uint32_t)(waves * 32 * DP + (v * 32 + c2) * 2) * 4u; };
+      auto put = [&](uint32_t p, int v, int i, f32x4 acc) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), parts, p + sum_at(v, i), 0, kAgentScope);
       };
-      if (mine) {
+      auto put_ml = [&](uint32_t p, int v, float M, float L) __attribute__((always_inline)) {
+        if (g2 == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, parts, p + ml_at(v), 0, kAgentScope);
+      };
+      if (busy) {
 #pragma unroll
         for (int dt = 0; dt < G::DT; dt++)
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            put_part(part_at(w), r0 + c, 32 * dt + 2 * e + 4 * g, m - kLift<XT>, l,
-                     f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]});
+          for (int q = 0; q < 4; q++)
+            put(part_at(w), wave, 4 * dt + q, f32x4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]});
+        put_ml(part_at(w), wave, m - kLift<XT>, l);
       }
       // The last of up to kJoin neighbours to arrive joins them; of more, the
       // last to have joined its neighbours joins the results.
-      auto last_of = [&](uint32_t* cnt, int of) -> bool {
+      auto last_of = [&](uint32_t* cnt, int of) __attribute__((always_inline)) -> bool {
         __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
         __syncthreads();
         if (tid == 0) {
@@ -867,54 +953,66 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         __syncthreads();
         return arrived != 0;
       };
-      // sum of the results, from byte `from` on, of workgroups v, v + by, .. (of them), in the order of the keys
-      auto join = [&](uint32_t from, int v, int by, int of, int r, int d, float& M, float& L, f32x4& acc) {
-        M = -INFINITY, L = 0.f, acc = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 0; i0 < of; i0 += kFlight) {
-          u32x4 ow[kFlight];
-          u32x2 mw[kFlight];
+      // Sums the results, from byte `from` on, of workgroups v, v + by, .. (of them), in the
+      // order of the keys: a wave takes kUnits times 16 bytes of each lane at a time.
+      auto join = [&](uint32_t from, int v, int by, int of, bool last) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int u0 = wave * kUnits; u0 < waves * 4 * G::DT; u0 += kWaves * kUnits) {
+          const int bw = u0 / (4 * G::DT), i = u0 - bw * (4 * G::DT);
+          float M = -INFINITY, L = 0.f;
+          f32x4 acc[kUnits];
 #pragma unroll
-          for (int i = 0; i < kFlight; i++) {
-            const uint32_t p = from + part_at(v + by * min(i0 + i, of - 1));
-            mw[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + (rows * DP + 2 * r) * 4, 0,
-                                                                                   kAgentScope));
-            ow[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + (r * DP + d) * 4, 0, kAgentScope));
+          for (int q = 0; q < kUnits; q++) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int i0 = 0; i0 < of; i0 += kFlight) {
+            u32x4 ow[kFlight][kUnits];
+            u32x2 mw[kFlight];
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+              const uint32_t p = from + part_at(v + by * min(i0 + k, of - 1));
+              mw[k] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, p + ml_at(bw), 0, kAgentScope));
+#pragma unroll
+              for (int q = 0; q < kUnits; q++)
+                ow[k][q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, p + sum_at(bw, i + q), 0, kAgentScope));
+            }
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+              if (i0 + k >= of) break;
+              const float mi = __uint_as_float(mw[k][0]), M2 = fmaxf(M, mi);
+              const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
+              M = M2;
+              L = L * f + __uint_as_float(mw[k][1]) * fi;
+#pragma unroll
+              for (int q = 0; q < kUnits; q++) acc[q] = acc[q] * f + __builtin_bit_cast(f32x4, ow[k][q]) * fi;
+            }
           }
+          if (last) {
+            const int r = 32 * bw + c2;
+            const float by_row = finish(min(r, rows - 1), M, L);
+            const int64_t to = out_at(min(r, rows - 1));
 #pragma unroll
-          for (int i = 0; i < kFlight; i++) {
-            if (i0 + i >= of) break;
-            const float mi = __uint_as_float(mw[i][0]), M2 = fmaxf(M, mi);
-            const float f = exp2_diff(M, M2), fi = exp2_diff(mi, M2);
-            M = M2;
-            L = L * f + __uint_as_float(mw[i][1]) * fi;
-            acc = acc * f + __builtin_bit_cast(f32x4, ow[i]) * fi;
+            for (int q = 0; q < kUnits; q++) {
+              const int d = 8 * (i + q) + 4 * g2;  // 32 (i / 4) + 8 (i % 4)
+              if (r < rows && d < a.D) store4<XT>(a.out, to + d, acc[q] * by_row);
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < kUnits; q++) put(joined + part_at(v), bw, i + q, acc[q]);
+            if (i == 0) put_ml(joined + part_at(v), bw, M, L);
           }
         }
       };
       const int of = w1 - w0 + 1, lead = (w - w0) / kJoin * kJoin, near = min(kJoin, of - lead);
       // a workgroup may lead neighbours of a tile that began before it and of its last one
       if (last_of(a.cnt + 2 * (w0 + lead) + (lead == 0), near)) {
-        for (int e = tid; e < rows * (DP / 4); e += 256) {
-          const int r = e / (DP / 4), d = 4 * (e - r * (DP / 4));
-          float M, L;
-          f32x4 acc;
-          join(0, w0 + lead, 1, near, r, d, M, L, acc);
-          if (of <= kJoin) finish(r, d, M, L, acc);
-          else put_part(joined + part_at(w0 + lead), r, d, M, L, acc);
-        }
-        const int groups = (of + kJoin - 1) / kJoin;
-        if (of > kJoin && last_of(a.cnt + 2 * a.wgs + w0, groups)) {
-          for (int e = tid; e < rows * (DP / 4); e += 256) {
-            const int r = e / (DP / 4), d = 4 * (e - r * (DP / 4));
-            float M, L;
-            f32x4 acc;
-            join(joined, w0, kJoin, groups, r, d, M, L, acc);
-            finish(r, d, M, L, acc);
-          }
+        join(0, w0 + lead, 1, near, of <= kJoin);
+        if (of > kJoin) {
+          const int groups = (of + kJoin - 1) / kJoin;
+          if (last_of(a.cnt + 2 * a.wgs + w0, groups)) join(joined, w0, kJoin, groups, true);
         }
       }
     }
-    at.tile++;
+    at.nth++;
     at.key = 0;
   }
 }
@@ -954,17 +1052,19 @@ bool chunk_attention_plan(ChunkAttnArgs& a, int cus, int64_t* part_bytes) {
   const int per = a.Hq / a.Hkv;
   a.tile_heads = std::min(per, kRows);
   a.tile_tokens = kRows / a.tile_heads;
+  a.inv_tile_heads = (65536 + a.tile_heads - 1) / a.tile_heads;
+  a.inv_tile_tokens = 1.0 / a.tile_tokens;
   const int64_t cap = (int64_t)a.width * a.page;
   const int64_t keys = a.window > 0 ? std::min<int64_t>(cap, (int64_t)a.window + a.tile_tokens) : cap;
   const int64_t heads = (int64_t)a.Hkv * ((per + a.tile_heads - 1) / a.tile_heads);
   const int64_t tiles = heads * (((int64_t)a.T + a.tile_tokens - 1) / a.tile_tokens + std::min(a.B, a.T));
   const int resident = with_kernel(a, [](auto xt, auto dp) { return Geo<decltype(xt)::value, decltype(dp)::value>::WGS; });
-  // tiles are counted in 32 bits, keys of all of them below 2^52
-  if (tiles > (1 << 30) || tiles * (double)(keys + kAround) > 4e15) return false;
+  // tiles of a sequence are counted in 32 bits, keys of all of them, without a window, below 2^52
+  if (tiles > (1 << 30) || tiles * (double)(cap + kAround) > 4e15) return false;
   a.wgs = (int)std::max<int64_t>(1, std::min<int64_t>((tiles * (keys + kAround) + kLeast - 1) / kLeast, (int64_t)cus * resident));
   a.inv_wgs = 1.0 / a.wgs;
-  const int rows = (int)std::min<int64_t>(kRows, (int64_t)a.T * a.tile_heads);
-  a.slot_words = with_kernel(a, [&](auto, auto dp) { return part_words(rows, decltype(dp)::value); });
+  const int waves = (int)((std::min<int64_t>(kRows, (int64_t)a.T * a.tile_heads) + 31) / 32);
+  a.slot_words = with_kernel(a, [&](auto, auto dp) { return part_words(waves, decltype(dp)::value); });
   *part_bytes = (int64_t)4 * a.wgs * a.slot_words * 4;
   return *part_bytes < ((int64_t)1 << 32);
 }

@@ -718,7 +718,8 @@ struct ChunkAttnArgs {
   uint32_t page_mul;       // as PagedAttnArgs
   int page_shift;
   int wgs;                 // workgroups
-  double inv_wgs;
+  double inv_wgs, inv_tile_tokens;
+  uint32_t inv_tile_heads; // 2^16 / tile_heads, rounded up
   int slot_words;          // of a partial result
   float* part;             // [4 wgs][slot_words]
   uint32_t* cnt;           // [3 wgs], zero between launches
