@@ -71,8 +71,9 @@ struct Geo {
   // A step in LDS: K, then V; each in blocks [8 chunks of the row][KEYS rows][128 bytes],
   // so that a wave's 64 lanes fill 8 rows of a block in their order.
   static constexpr int TILE = NC * KEYS * 128;
-  // Workgroups a CU holds: by registers
-  static constexpr int WGS = DP * ES <= 256 ? 2 : 1;
+  // Workgroups a CU holds: by registers.  16-bit heads of 64, 2 instead of 3: short tiles (five
+  // prompts of 1500 with a window of 128) take 109 us instead of 96, long ones (2048 tokens of 32768) 1002 instead of 1015.
+  static constexpr int WGS = DP * ES <= 128 ? 3 : DP * ES <= 256 ? 2 : 1;
 };
 // Chunk p of row r of a block lies at place p ^ swizzle(r).  K is read one chunk
 // of 16 rows at a time, which then hit all banks; V four rows of 64 bytes.
@@ -94,14 +95,15 @@ __device__ __forceinline__ float half(uint32_t w, int hi) {
   return xt_to_f32<XT == GEN_F16 ? 1 : 0>(hi ? w >> 16 : w & 0xFFFFu);
 }
 
-// v less the low (high) half of w, exact where w holds v rounded.  minus: -1 in
-// that half, 0 in the other, in a register: the compiler writes a low bfloat16 -1 as
-// the inline constant -1.0, whose bits are in the high half.
+// v less the low (high) half of w, exact where w holds v rounded; one instruction.  minus
+// is in a register.  bfloat16: -1 in that half, 0 in the other (the compiler writes a low
+// bfloat16 -1 as the inline constant -1.0, whose bits are in the high half).  float16: -1 in
+// 32 bits (of a subtraction the compiler makes a conversion more).
 template <int XT, int HI>
 __device__ __forceinline__ float less(float v, uint32_t w, uint32_t minus) {
   if constexpr (XT == GEN_BF16)
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, minus), v, false);
-  else return fmaf((float)__builtin_bit_cast(_Float16, (uint16_t)(HI ? w >> 16 : w)), -1.f, v);
+  else return fmaf((float)__builtin_bit_cast(_Float16, (uint16_t)(HI ? w >> 16 : w)), __uint_as_float(minus), v);
 }
 
 template <int XT>
@@ -387,7 +389,10 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
   }
   if (!at.ahead_of(end)) return;
 
-  uint32_t minus_lo = 0x0000BF80u, minus_hi = 0xBF800000u;
+  // Of two workgroups of a CU the older one's waves go first, and it is done at 3/4 of the
+  // time (205 of 270 us); so the younger one goes first in every other step.
+  const bool later = blockIdx.x >= gridDim.x / 2;
+  uint32_t minus_lo = XT == GEN_F16 ? 0xBF800000u : 0x0000BF80u, minus_hi = 0xBF800000u;
   asm volatile("" : "+s"(minus_lo), "+s"(minus_hi));
   // A thread brings place lane % 8 of every block of rows 8 wave + lane / 8 (+ 32) of a step.
   const int my_row8 = 8 * wave + (lane >> 3), k_chunk = (lane & 7) ^ swizzle_k(my_row8), v_chunk = (lane & 7) ^ swizzle_v(my_row8);
@@ -628,6 +633,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           for (int e = 0; e < 4; e++) {
             const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
             p0[e] = pack<XT>(x, y);
+            if constexpr (XT == GEN_F16) asm volatile("" : "+v"(p0[e]));  // or it is converted again
             p1[e] = pack<XT>(less<XT, 0>(x, p0[e], minus_lo), less<XT, 1>(y, p0[e], minus_hi));
           }
           u32x4 vf[G::DT];
@@ -686,6 +692,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       auto split = [&](int u, int e) __attribute__((always_inline)) {
         const float x = s[8 * u + 2 * e], y = s[8 * u + 2 * e + 1];
         pt[u][0][e] = pack<XT>(x, y);
+        if constexpr (XT == GEN_F16) asm volatile("" : "+v"(pt[u][0][e]));  // or it is converted again
         pt[u][1][e] = pack<XT>(less<XT, 0>(x, pt[u][0][e], minus_lo), less<XT, 1>(y, pt[u][0][e], minus_hi));
         asm volatile("" : "+v"(pt[u][0][e]), "+v"(pt[u][1][e]));  // here, not where it is used
       };
@@ -809,7 +816,9 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     for (int k = k0; k < k1; k += 2 * kKeys) {
       if (easy && k + 32 >= all_lo && k + 3 * kKeys + 32 <= all_hi) {
         do {
+          if (G::WGS == 2 && later) __builtin_amdgcn_s_setprio(1);
           easy_step(k_lds0, v_lds0, k_lds1, v_lds1, k);
+          if (G::WGS == 2 && later) __builtin_amdgcn_s_setprio(0);
           easy_step(k_lds1, v_lds1, k_lds0, v_lds0, k + kKeys);
           k += 2 * kKeys;
         } while (k + 3 * kKeys + 32 <= all_hi);
