@@ -6,7 +6,10 @@
 // for pairs i < n of a head: elements (i, n + i), or (2 i, 2 i + 1) interleaved;
 // the elements from 2 n on are copied.  An element is read and written once,
 // which is the bound; a workgroup takes one token's heads, so a token's n
-// angles are worked out once for all of them and shared through LDS.
+// angles are worked out once for all of them and shared through LDS, while 16 bytes (32 of
+// a pair of halves) a thread are on their way: 8191 tokens of 32 heads of 96 in 16 bits
+// (101 MB) 24 us, 4.2 TB/s, instead of 27.5 with the loads behind the angles.  A thread
+// for two (four) heads, so half (a quarter) of the angles and workgroups: 24.5 (33.2) us.
 //
 // The angle of a far position needs more than 32 bits (2^20 * 1.0f is off by
 // whole steps of 1/16): it is taken in turns in 64 bits, whole turns and
@@ -71,7 +74,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   extern __shared__ float2 turn[];  // [n] factor * (cos, sin)
   const int tid = threadIdx.x, unit = tid & ((1 << a.unit_shift) - 1);
   const int pairs = INTER ? 2 * a.n : a.n, rot = (pairs + W - 1) / W, units = rotary_units(a, W);
-  const int h0 = blockIdx.y * (256 >> a.unit_shift) + (tid >> a.unit_shift), heads = a.Hq + 2 * a.Hkv;
+  const int at = blockIdx.y * (256 >> a.unit_shift) + (tid >> a.unit_shift), heads = a.Hq + 2 * a.Hkv;
+  const float freq = tid < a.n ? a.inv_freq[tid] : 0.f;
+  // first element of unit u, and whether all of it is there
+  auto first_of = [&](int u) -> int { return u < rot ? u * W : 2 * a.n + (u - rot) * W; };
+  auto whole = [&](int u) -> bool { return (u < rot ? pairs : a.D) - first_of(u) >= W; };
   for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
     const int pos = a.positions[t];
     // where the token's keys and values go (-1: nowhere)
@@ -84,78 +91,58 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         if (pid >= a.pages) pid = -1;
       }
     }
+    const int kind = at < a.Hq ? 0 : at < a.Hq + a.Hkv ? 1 : 2, h = at - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv);
+    const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                   (kind == 0 ? t * a.q_tok + h * a.q_head : kind == 1 ? t * a.k_tok + h * a.k_head : t * a.v_tok + h * a.v_head);
+    Vec v, w;
+    auto load = [&](int u) {
+      v = *reinterpret_cast<const Vec*>(src + first_of(u));
+      if (!INTER && u < rot) w = *reinterpret_cast<const Vec*>(src + a.n + first_of(u));
+    };
+    // a thread's first unit is on its way while the angles are worked out
+    if (at < heads && unit < units && whole(unit)) load(unit);
     for (int i = tid; i < a.n; i += 256) {
-      const float2 r = cos_sin((double)pos * ((double)a.inv_freq[i] * 0.15915494309189533577));
+      const float2 r = cos_sin((double)pos * ((double)(i == tid ? freq : a.inv_freq[i]) * 0.15915494309189533577));
       turn[i] = float2{r.x * a.factor, r.y * a.factor};
     }
     __syncthreads();
-    if (h0 < heads) {
-      const int kind = h0 < a.Hq ? 0 : h0 < a.Hq + a.Hkv ? 1 : 2, h = h0 - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv);
-      const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                     (kind == 0 ? t * a.q_tok + h * a.q_head : kind == 1 ? t * a.k_tok + h * a.k_head : t * a.v_tok + h * a.v_head);
+    auto rotate = [&](T& x, T& y, int i) {
+      const float2 r = turn[i];
+      const float p = E::up(x), q = E::up(y);
+      x = E::down(p * r.x - q * r.y);
+      y = E::down(q * r.x + p * r.y);
+    };
+    if (at < heads && (kind == 0 || pid >= 0)) {
       T* dst = static_cast<T*>(kind == 0 ? a.out : kind == 1 ? a.kp : a.vp) +
                (kind == 0   ? t * a.out_tok + h * a.out_head
                 : kind == 1 ? pid * a.kp_page + h * a.kp_head + off * a.kp_tok
                             : pid * a.vp_page + h * a.vp_head + off * a.vp_tok);
-      if (kind == 0 || pid >= 0) {
-        const bool turned = kind < 2;
-        auto rotate = [&](T& x, T& y, int i) {
-          const float2 r = turn[i];
-          const float p = E::up(x), q = E::up(y);
-          x = E::down(p * r.x - q * r.y);
-          y = E::down(q * r.x + p * r.y);
-        };
-        for (int u = unit; u < units; u += 1 << a.unit_shift) {
-          const int e0 = u < rot ? u * W : 2 * a.n + (u - rot) * W, many = (u < rot ? pairs : a.D) - e0;
-          if (u >= rot) {  // the rest
-            if (many >= W) {
-              *reinterpret_cast<Vec*>(dst + e0) = *reinterpret_cast<const Vec*>(src + e0);
-            } else {
-              for (int e = e0; e < a.D; e++) dst[e] = src[e];
+      const bool turned = kind < 2;
+      for (int u = unit; u < units; u += 1 << a.unit_shift) {
+        const int e0 = first_of(u);
+        if (whole(u)) {
+          if (u != unit) load(u);
+          if (turned && u < rot) {
+#pragma unroll
+            for (int e = 0; e < W; e += INTER ? 2 : 1) {
+              T x = v[e], y = INTER ? v[e + 1] : w[e];
+              rotate(x, y, INTER ? (e0 + e) / 2 : e0 + e);
+              v[e] = x;
+              if constexpr (INTER) v[e + 1] = y;
+              else w[e] = y;
             }
-          } else if constexpr (INTER) {
-            if (many >= W) {
-              Vec v = *reinterpret_cast<const Vec*>(src + e0);
-              T x[W];
-#pragma unroll
-              for (int e = 0; e < W; e++) x[e] = v[e];
-              if (turned) {
-#pragma unroll
-                for (int e = 0; e < W; e += 2) rotate(x[e], x[e + 1], (e0 + e) / 2);
-              }
-#pragma unroll
-              for (int e = 0; e < W; e++) v[e] = x[e];
-              *reinterpret_cast<Vec*>(dst + e0) = v;
-            } else {
-              for (int e = e0; e < pairs; e += 2) {
-                T x = src[e], y = src[e + 1];
-                if (turned) rotate(x, y, e / 2);
-                dst[e] = x;
-                dst[e + 1] = y;
-              }
-            }
-          } else {
-            if (many >= W) {
-              Vec v = *reinterpret_cast<const Vec*>(src + e0), w = *reinterpret_cast<const Vec*>(src + a.n + e0);
-              if (turned) {
-#pragma unroll
-                for (int e = 0; e < W; e++) {
-                  T x = v[e], y = w[e];
-                  rotate(x, y, e0 + e);
-                  v[e] = x;
-                  w[e] = y;
-                }
-              }
-              *reinterpret_cast<Vec*>(dst + e0) = v;
-              *reinterpret_cast<Vec*>(dst + a.n + e0) = w;
-            } else {
-              for (int e = e0; e < pairs; e++) {
-                T x = src[e], y = src[a.n + e];
-                if (turned) rotate(x, y, e);
-                dst[e] = x;
-                dst[a.n + e] = y;
-              }
-            }
+          }
+          *reinterpret_cast<Vec*>(dst + e0) = v;
+          if (!INTER && u < rot) *reinterpret_cast<Vec*>(dst + a.n + e0) = w;
+        } else if (u >= rot) {
+          for (int e = e0; e < a.D; e++) dst[e] = src[e];
+        } else {
+          for (int e = e0; e < pairs; e += INTER ? 2 : 1) {
+            const int other = INTER ? e + 1 : a.n + e;
+            T x = src[e], y = src[other];
+            if (turned) rotate(x, y, INTER ? e / 2 : e);
+            dst[e] = x;
+            dst[other] = y;
           }
         }
       }
