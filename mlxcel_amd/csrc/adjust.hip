@@ -6,11 +6,13 @@
 //   x' += bias                                   for tokens with one
 //   x' = -inf                                    for tokens whose bit of the mask is 0
 //
-// A logit is read and written once, which is the bound.  A workgroup takes 16 bytes of one
+// A logit is read and written once, which is the floor; what it takes beyond that are the
+// vector operations of looking through the history.  A workgroup takes 16 bytes of one
 // row a thread and counts the history's tokens that fall into them in LDS, a word a
 // token: whole numbers, so the order of the atomic operations does not matter.  Of
 // several biases of one token the last in the list counts: LDS keeps the largest
-// place, which then makes way for the value.
+// place.  Whoever finds a token first puts it on a list; a thread for each of the list
+// works out its logit and leaves it in the word.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -22,7 +24,6 @@ namespace mlxq {
 
 namespace {
 
-constexpr uint32_t kNoBias = 0xFFFFFFFFu;  // -1 as a place, a NaN that is not written as a value
 constexpr uint32_t kSeen = 0x80000000u;  // in the prompt; the bits below count the places after it
 
 typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
@@ -30,15 +31,19 @@ typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
 // Entries of the history and of the biases that a thread asks for before anything else.
 constexpr int kAhead = 4;
 
-template <int XT>
-constexpr int kChunk = 256 * (XT == GEN_F32 ? 4 : 8);
+constexpr int kThreads = 256;
 
-// One workgroup: logits [first, first + 256 W) of row t, W in 16 bytes.  All that does not
-// depend on something else is asked for first: the logits, the mask, the beginning of the
-// history and of the biases, the row's numbers.  128 rows of 151936 with 2 (4) times as many
-// logits a workgroup, so half as many of them: 40 (67) us instead of 33.5; one row 6.8 (12.3) instead of 5.1.
 template <int XT>
-__global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) {
+constexpr int kChunk = kThreads * (XT == GEN_F32 ? 4 : 8);
+
+// One workgroup: logits [first, first + CHUNK) of row t, 16 bytes a thread.  All that does not
+// depend on something else is asked for first: the logits, the mask, the beginning of the
+// history and of the biases, the row's numbers.  128 rows of 151936 in bfloat16 with 4000 tokens
+// of history, 300 biases and a mask: 29.7 us (81 MB); every thread working out its own logits instead of a list, in which
+// most lanes wait for the few that have one: 35; workgroups of 512 (1024) threads, half (a quarter) of the
+// looking through the history: 30.3 (39.7); two (four) times 16 bytes a thread: 40 (67), the tables leave too few waves.
+template <int XT>
+__global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const AdjustArgs a) {
   constexpr int ES = XT == GEN_F32 ? 4 : 2, W = 16 / ES, CHUNK = kChunk<XT>;
   extern __shared__ __align__(16) uint32_t lds[];
   const int tid = threadIdx.x, chunks = (a.V + CHUNK - 1) / CHUNK, t = blockIdx.x / chunks;
@@ -49,12 +54,10 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) 
   const int32_t *h = a.history + t * a.history_row, *ids = a.bias_ids + t * a.bias_ids_row;
   const float* values = a.bias + t * a.bias_row;
   int32_t early[kAhead], early_id[kAhead];
-  float early_bias[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; k++) {
-    early[k] = k * 256 + tid < a.n ? h[k * 256 + tid] : -1;
-    early_id[k] = k * 256 + tid < a.m ? ids[k * 256 + tid] : -1;
-    early_bias[k] = k * 256 + tid < a.m ? values[k * 256 + tid] : 0.f;
+    early[k] = k * kThreads + tid < a.n ? h[k * kThreads + tid] : -1;
+    early_id[k] = k * kThreads + tid < a.m ? ids[k * kThreads + tid] : -1;
   }
   int n = a.n, prompt = 0;
   float rep = 1.f, pres = 0.f, freq = 0.f;
@@ -80,95 +83,94 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) 
         else v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[e + i] << (16 * (i & 1));
       }
   }
-  // a word a token: how often the history has it; its last place among the biases, then the bias (kNoBias: none)
-  uint32_t *times = lds, *place = lds + (a.n > 0 ? CHUNK : 0);
   if (edits) {
-    if (a.n > 0) {
+    // A word a token: how often the history has it, then the bits of its new logit, made other than 0; its last
+    // place among the biases (-1: none).  The history's tokens, each once.
+    uint32_t* times = lds;
+    int* place = reinterpret_cast<int*>(lds + CHUNK);
+    uint16_t* list = reinterpret_cast<uint16_t*>(lds + (a.m > 0 ? 2 : 1) * CHUNK);
+    __shared__ uint32_t listed;
+    const uint32_t here = (uint32_t)min(CHUNK, a.V - first);  // tokens past the row's end count for nothing
+    if (tid == 0) listed = 0u;
 #pragma unroll
-      for (int i = 0; i < CHUNK / 1024; i++) reinterpret_cast<u32x4*>(times)[i * 256 + tid] = u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int i = 0; i < CHUNK / (4 * kThreads); i++) reinterpret_cast<u32x4*>(times)[i * kThreads + tid] = u32x4{0u, 0u, 0u, 0u};
     if (a.m > 0) {
 #pragma unroll
-      for (int i = 0; i < CHUNK / 1024; i++)
-        reinterpret_cast<u32x4*>(place)[i * 256 + tid] = u32x4{kNoBias, kNoBias, kNoBias, kNoBias};
+      for (int i = 0; i < CHUNK / (4 * kThreads); i++) reinterpret_cast<u32x4*>(place)[i * kThreads + tid] = u32x4{~0u, ~0u, ~0u, ~0u};
     }
     __syncthreads();
     auto count = [&](int i, int32_t token) {
       const uint32_t at = (uint32_t)token - (uint32_t)first;
-      if (i < n && at < (uint32_t)CHUNK) {  // past the row's end it counts for nothing
-        if (i < prompt) atomicOr(times + at, kSeen);
-        else atomicAdd(times + at, 1u);
+      if (i < n && at < here) {
+        const uint32_t had = i < prompt ? atomicOr(times + at, kSeen) : atomicAdd(times + at, 1u);
+        if (had == 0u) list[atomicAdd(&listed, 1u)] = (uint16_t)at;
       }
     };
     auto mark = [&](int i, int32_t token) {
       const uint32_t at = (uint32_t)token - (uint32_t)first;
-      if (i < a.m && at < (uint32_t)CHUNK) atomicMax(reinterpret_cast<int*>(place) + at, i);
+      if (i < a.m && at < here) atomicMax(place + at, i);
     };
     if (a.n > 0) {
 #pragma unroll
-      for (int k = 0; k < kAhead; k++) count(k * 256 + tid, early[k]);
-      for (int i0 = kAhead * 256; i0 < n; i0 += kAhead * 256) {
+      for (int k = 0; k < kAhead; k++) count(k * kThreads + tid, early[k]);
+      for (int i0 = kAhead * kThreads; i0 < n; i0 += kAhead * kThreads) {
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) early[k] = i0 + k * 256 + tid < n ? h[i0 + k * 256 + tid] : -1;
+        for (int k = 0; k < kAhead; k++) early[k] = i0 + k * kThreads + tid < n ? h[i0 + k * kThreads + tid] : -1;
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) count(i0 + k * 256 + tid, early[k]);
+        for (int k = 0; k < kAhead; k++) count(i0 + k * kThreads + tid, early[k]);
       }
     }
     if (a.m > 0) {
 #pragma unroll
-      for (int k = 0; k < kAhead; k++) mark(k * 256 + tid, early_id[k]);
-      for (int i = kAhead * 256 + tid; i < a.m; i += 256) mark(i, ids[i]);
-      __syncthreads();
-      // A value whose bits are a place that is looked for later would be taken for one: past the
-      // first kAhead * 256 places values stay in memory (places are what is left in LDS).
-      if (a.m <= kAhead * 256) {
-        bool mine[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-          const uint32_t at = (uint32_t)early_id[k] - (uint32_t)first;
-          mine[k] = k * 256 + tid < a.m && at < (uint32_t)CHUNK && place[at] == (uint32_t)(k * 256 + tid);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kAhead; k++)
-          if (mine[k]) place[early_id[k] - first] = early_bias[k] == early_bias[k] ? __float_as_uint(early_bias[k]) : 0x7FC00000u;
-      }
+      for (int k = 0; k < kAhead; k++) mark(k * kThreads + tid, early_id[k]);
+      for (int i = kAhead * kThreads + tid; i < a.m; i += kThreads) mark(i, ids[i]);
     }
     __syncthreads();
-  }
-  auto get = [&](const u32x4& w, int i) -> float {
-    if constexpr (ES == 4) return __uint_as_float(w[i]);
-    else return xt_to_f32<XT == GEN_F16 ? 1 : 0>((w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
-  };
-  auto put = [&](u32x4& w, int i, float x) {
-    if constexpr (ES == 4) w[i] = __float_as_uint(x);
-    else w[i / 2] = (w[i / 2] & (i & 1 ? 0x0000FFFFu : 0xFFFF0000u)) | f32_to_xt<XT == GEN_F16 ? 1 : 0>(x) << (16 * (i & 1));
-  };
-  constexpr uint32_t kNone = XT == GEN_F32 ? 0xFF800000u : XT == GEN_F16 ? 0xFC00u : 0xFF80u;  // -inf
-  if (first + e >= a.V) return;
-  if (edits) {
-    uint32_t c[W], p[W];
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < W; i++) {
-      c[i] = a.n > 0 ? times[e + i] : 0u;
-      p[i] = a.m > 0 ? place[e + i] : kNoBias;
-      any |= c[i] != 0u || p[i] != kNoBias;
+    auto logit = [&](uint32_t at) -> float {
+      if constexpr (ES == 4) return reinterpret_cast<const float*>(src)[at];
+      else return xt_to_f32<XT == GEN_F16 ? 1 : 0>(reinterpret_cast<const uint16_t*>(src)[at]);
+    };
+    auto leave = [&](uint32_t at, float x) {
+      if constexpr (ES == 4) times[at] = ~(x == x ? __float_as_uint(x) : 0x7FC00000u);
+      else times[at] = 0x10000u | f32_to_xt<XT == GEN_F16 ? 1 : 0>(x);
+    };
+    for (uint32_t i = tid; i < listed; i += kThreads) {
+      const uint32_t at = list[i], c = times[at];
+      const int p = a.m > 0 ? place[at] : -1;
+      float x = logit(at);
+      x = x > 0.f ? x / rep : x * rep;
+      if (c & ~kSeen) x -= pres + freq * (float)(c & ~kSeen);
+      if (p >= 0) x += values[p];
+      leave(at, x);
     }
-    if (any) {
+    // tokens with a bias alone
+    auto alone = [&](int i, int32_t token) {
+      const uint32_t at = (uint32_t)token - (uint32_t)first;
+      if (i < a.m && at < here && place[at] == i && times[at] == 0u) leave(at, logit(at) + values[i]);
+    };
+    if (a.m > 0) {
 #pragma unroll
-      for (int i = 0; i < W; i++) {
-        if (c[i] == 0u && p[i] == kNoBias) continue;
-        float x = get(v, i);
-        if (c[i]) {
-          x = x > 0.f ? x / rep : x * rep;
-          if (c[i] & ~kSeen) x -= pres + freq * (float)(c[i] & ~kSeen);
+      for (int k = 0; k < kAhead; k++) alone(k * kThreads + tid, early_id[k]);
+      for (int i = kAhead * kThreads + tid; i < a.m; i += kThreads) alone(i, ids[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const u32x4 r = *reinterpret_cast<const u32x4*>(times + e + i);
+      if constexpr (ES == 4) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) v[q] = r[q] ? ~r[q] : v[q];
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const uint32_t both = r[q] ? (v[(i + q) / 2] & 0xFFFF0000u) | (r[q] & 0xFFFFu) : v[(i + q) / 2];
+          v[(i + q) / 2] = r[q + 1] ? (both & 0xFFFFu) | r[q + 1] << 16 : both;
         }
-        if (p[i] != kNoBias) x += a.m <= kAhead * 256 ? __uint_as_float(p[i]) : values[p[i]];
-        put(v, i, x);
       }
     }
   }
+  constexpr uint32_t kNone = XT == GEN_F32 ? 0xFF800000u : XT == GEN_F16 ? 0xFC00u : 0xFF80u;  // -inf
+  if (first + e >= a.V) return;
   if (a.mask) {
 #pragma unroll
     for (int i = 0; i < W; i++) {
@@ -210,8 +212,8 @@ hipError_t launch_adjust_logits(const AdjustArgs& a, hipStream_t stream) {
   if (groups > kMaxGroups) return hipErrorInvalidValue;
   return with_kernel(a, [&](auto xt) {
     constexpr int XT = decltype(xt)::value;
-    const size_t bytes = (size_t)((a.n > 0) + (a.m > 0)) * kChunk<XT> * 4;
-    hipLaunchKernelGGL((adjust_logits_kernel<XT>), dim3((unsigned)groups), dim3(256), bytes, stream, a);
+    const size_t bytes = a.n > 0 || a.m > 0 ? (size_t)kChunk<XT> * (4 + (a.m > 0 ? 4 : 0) + (a.n > 0 ? 2 : 0)) : 0;
+    hipLaunchKernelGGL((adjust_logits_kernel<XT>), dim3((unsigned)groups), dim3(kThreads), bytes, stream, a);
     return hipGetLastError();
   });
 }
