@@ -442,9 +442,12 @@ mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* toke
  * and values are in the pages already; each sees the keys up to its own (of
  * which the last `window`, where that is not 0).  starts (B + 1) int32
  * ascending; rows of no sequence are left as they were, tokens before a
- * sequence's first (more rows than its length) give zeros.  The result does not
- * depend on how a prompt is cut into calls, up to the order of 32-bit sums.
- * Types, layouts, sinks, infinities: as there. */
+ * sequence's first (more rows than its length) give zeros.  out may be q.  The
+ * result does not depend on how a prompt is cut into calls, up to the order of 32-bit sums.
+ * Types, layouts, sinks and infinities as there; in a product of 16-bit values a
+ * probability differs by at most 2^-17 of itself (bfloat16), 2^-23 of itself or
+ * 2^-39 of the largest (float16).  Values that are not finite among a token's
+ * keys or its neighbours' make the call slower, not other tokens' results wrong. */
 mlxq_status mlxq_paged_attention_chunk(const mlxq_array* q, const mlxq_array* k_pool,
                                        const mlxq_array* v_pool, const mlxq_array* table,
                                        const mlxq_array* lengths, const mlxq_array* starts,

@@ -5,10 +5,12 @@
 //   o_i = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m))
 //
 // A tile is up to 128 rows, (token, query head) pairs of one key head, over the
-// keys that any of them sees.  Its workgroup takes 32 keys a step: the step's K
-// and V rows are loaded while the step before is worked on and go to LDS in the
-// order of their keys, whatever pages they come from.  Each of the four waves has
-// 32 rows, with O, the running maximum and the running sum in registers.  Both
+// keys that any of them sees.  Its workgroup takes 64 keys a step (32 of wide
+// 32-bit heads): the step's K and V rows go to LDS directly while the step before
+// is worked on, in the order of their keys, whatever pages they come from.  K is
+// 32 keys ahead of V, so that the scores of 32 keys are worked out beside the
+// values of the 32 before.  Each of the four waves has 32 rows, with O, the
+// running maximum and the running sum in registers.  Both
 // products are 32x32 MFMAs whose operands need no exchange between lanes:
 //   S^T[key][row] = K Q^T: lane (c, g) = (lane % 32, lane / 32) ends with keys
 //     8 i + 4 g + e (i, e < 4) of row c, so a row's maximum and sum are taken
@@ -16,7 +18,20 @@
 //   O^T[d][row] += V^T P^T: the lane's keys are those it holds P of; V comes out
 //     of LDS transposed (16-bit types: four keys of a column a read).
 // 16-bit products take P as the sum of two 16-bit numbers: bfloat16 ones leave
-// out at most 2^-17 of it, float16 ones 2^-23 or 2^-39 of the largest.
+// out at most 2^-17 of it, float16 ones 2^-23 or 2^-39 of the largest.  One number
+// would leave out 2^-9, as much as the result's own rounding, for a third of the
+// matrix work.
+//
+// Values that are not finite would reach the rows that do not see their key (0 inf):
+// a tile whose results are not all finite is worked out again, where keys are hidden one at a time.
+//
+// Many new tokens are bound by the matrix instructions, at the clock that the
+// card keeps under them: 2048 tokens of 32768 of 32 heads of 128 (8 key heads) in
+// bfloat16 1427 us, that is 746 TFLOP/s or, with P's second number counted, 1119
+// (the matrix instructions alone: 1170 us).  Few are bound by HBM
+// and by the join of what was cut: 16 sequences of 5 tokens over 43000 keys of 4
+// key heads 44 us for 88 MB.  Short tiles (a window of 128 tokens) are bound by their vector
+// operations and by what a tile's start waits for: five prompts of 1500 tokens of 64 heads of 64, 94 us.
 //
 // The work is cut evenly whatever the lengths: a tile counts its keys and kAround
 // more, and workgroup w takes [w n, (w + 1) n) of all tiles laid end to end,

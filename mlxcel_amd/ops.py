@@ -550,8 +550,8 @@ def paged_attention_chunk(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     sequence b's ``lengths[b]`` tokens, whose keys and values are in the pages
     already; each sees the keys up to its own (the last ``window`` of them).
     ``starts`` (B + 1) int32, ascending.  Rows of no sequence are left as they were
-    in ``out`` (undefined in a new one); tokens before a sequence's first give
-    zeros."""
+    in ``out`` (undefined in a new one), which may be q; tokens before a sequence's
+    first give zeros."""
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     r = _native.paged_attention_chunk(q, k_pool, v_pool, table, lengths, starts, sinks, scale, softcap, window, out)
