@@ -6,7 +6,7 @@
 //   x' += bias                                   for tokens with one
 //   x' = -inf                                    for tokens whose bit of the mask is 0
 //
-// A logit is read and written once, which is the floor; what it takes beyond that are the
+// A logit is read and written once, which is the floor; beyond that it takes the
 // vector operations of looking through the history.  A workgroup takes 16 bytes of one
 // row a thread and counts the history's tokens that fall into them in LDS, a word a
 // token: whole numbers, so the order of the atomic operations does not matter.  Of
@@ -27,9 +27,10 @@ namespace {
 constexpr uint32_t kSeen = 0x80000000u;  // in the prompt; the bits below count the places after it
 
 typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
+typedef int32_t i32x4_e __attribute__((ext_vector_type(4), aligned(4)));
 
-// Entries of the history and of the biases that a thread asks for before anything else.
-constexpr int kAhead = 4;
+// Biases that a thread asks for before anything else, beside four tokens of the history.
+constexpr int kAhead = 2;
 
 constexpr int kThreads = 256;
 
@@ -39,9 +40,12 @@ constexpr int kChunk = kThreads * (XT == GEN_F32 ? 4 : 8);
 // One workgroup: logits [first, first + CHUNK) of row t, 16 bytes a thread.  All that does not
 // depend on something else is asked for first: the logits, the mask, the beginning of the
 // history and of the biases, the row's numbers.  128 rows of 151936 in bfloat16 with 4000 tokens
-// of history, 300 biases and a mask: 29.7 us (81 MB); every thread working out its own logits instead of a list, in which
-// most lanes wait for the few that have one: 35; workgroups of 512 (1024) threads, half (a quarter) of the
-// looking through the history: 30.3 (39.7); two (four) times 16 bytes a thread: 40 (67), the tables leave too few waves.
+// of history, 300 biases and a mask: 28.5 us (81 MB), of which 11 are the history past its first
+// 1024 tokens, a dozen vector operations each in every workgroup of a row.  Every thread working out its own logits instead of a
+// list, in which most lanes wait for the few that have one: 35; the list made from the words afterwards: 29.8;
+// the whole history asked for ahead: 28.5, but a mask alone then takes 5.3 instead of 4.7; workgroups of 512 (1024) threads,
+// half (a quarter) of the looking through the history: 30.3 (39.7); two (four) times 16 bytes a thread: 40 (67), the tables
+// leave too few waves.
 template <int XT>
 __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const AdjustArgs a) {
   constexpr int ES = XT == GEN_F32 ? 4 : 2, W = 16 / ES, CHUNK = kChunk<XT>;
@@ -53,12 +57,22 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const AdjustArg
   const bool edits = a.n > 0 || a.m > 0;
   const int32_t *h = a.history + t * a.history_row, *ids = a.bias_ids + t * a.bias_ids_row;
   const float* values = a.bias + t * a.bias_row;
-  int32_t early[kAhead], early_id[kAhead];
+  // entries 4 i .. 4 i + 3 of the history, -1 past its end
+  auto four = [&](int i) -> i32x4_e {
+    i32x4_e r = {-1, -1, -1, -1};
+    if (4 * i + 3 < a.n) {
+      r = *reinterpret_cast<const i32x4_e*>(h + 4 * i);
+    } else {
 #pragma unroll
-  for (int k = 0; k < kAhead; k++) {
-    early[k] = k * kThreads + tid < a.n ? h[k * kThreads + tid] : -1;
-    early_id[k] = k * kThreads + tid < a.m ? ids[k * kThreads + tid] : -1;
-  }
+      for (int q = 0; q < 3; q++)
+        if (4 * i + q < a.n) r[q] = h[4 * i + q];
+    }
+    return r;
+  };
+  i32x4_e early = four(tid);
+  int32_t early_id[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; k++) early_id[k] = k * kThreads + tid < a.m ? ids[k * kThreads + tid] : -1;
   int n = a.n, prompt = 0;
   float rep = 1.f, pres = 0.f, freq = 0.f;
   if (a.n > 0) {
@@ -110,15 +124,10 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const AdjustArg
       const uint32_t at = (uint32_t)token - (uint32_t)first;
       if (i < a.m && at < here) atomicMax(place + at, i);
     };
-    if (a.n > 0) {
+    for (int i = tid; 4 * (i - tid) < n; i += kThreads) {
+      if (i != tid) early = four(i);
 #pragma unroll
-      for (int k = 0; k < kAhead; k++) count(k * kThreads + tid, early[k]);
-      for (int i0 = kAhead * kThreads; i0 < n; i0 += kAhead * kThreads) {
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) early[k] = i0 + k * kThreads + tid < n ? h[i0 + k * kThreads + tid] : -1;
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) count(i0 + k * kThreads + tid, early[k]);
-      }
+      for (int q = 0; q < 4; q++) count(4 * i + q, early[q]);
     }
     if (a.m > 0) {
 #pragma unroll

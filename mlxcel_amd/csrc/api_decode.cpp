@@ -869,7 +869,8 @@ mlxq_status mlxq_adjust_logits(const mlxq_array* logits, const mlxq_array* histo
         (Refusal(tag) << name << " must have one row a row of logits (" << T << ") but has shape " << fmt_shape(v.shape())
                       << ".").invalid();
       if (!unit_last(v)) (Refusal(tag) << name << "'s rows must be contiguous.").unsupported();
-      fits_int(v.dim(1), tag, name);
+      if (v.dim(1) > ((int64_t)1 << 30))
+        (Refusal(tag) << name << "'s rows of " << v.dim(1) << " entries are too long.").unsupported();
       stride = r->strides[0];
       return r->data;
     };

@@ -131,6 +131,8 @@ ADJUST = dict(x=((3, 100), BF), history=((3, 7), I32), lengths=None, prompts=Non
     (dict(out=((3, 100), F32)), EINVAL, "out must have shape"),
     (dict(x=((1, (1 << 30) + 8), BF), history=None, out=((1, (1 << 30) + 8), BF)), EUNSUPPORTED, "too long"),
     (dict(x=((1 << 30, 100), BF), history=None, out=((1 << 30, 100), BF)), EUNSUPPORTED, "too many logits"),
+    (dict(history=((3, (1 << 30) + 1), I32)), EUNSUPPORTED, "too long"),
+    (dict(ids=((3, 1 << 31), I32), bias=((3, 1 << 31), F32)), EUNSUPPORTED, "too long"),
 ])
 def test_adjust_logits(lib, change, code, text):
     refused(lib, "mlxq_adjust_logits", code, text, *args_of(ADJUST, change))
