@@ -423,10 +423,11 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     for (int i = 0; i < 2; i++) v_lane[i] = r * 128 + ((4 * i + ch) ^ swizzle_v(r)) * 16 + (i16 & 1) * 8;
     asm volatile("" : "+v"(k_lane[0]), "+v"(k_lane[1]), "+v"(k_lane[2]), "+v"(k_lane[3]), "+v"(v_lane[0]), "+v"(v_lane[1]));
   }
-  if (DP != a.D) {  // K's chunks past the head are zero and stay so
+  // The chunks past the head are zero and stay so: K's count in the scores, and values that are
+  // not finite, whatever lay there, would send every tile the slow way.
+  if (DP != a.D) {
     for (int i = tid; i < G::TILE / 16; i += 256) {
-      reinterpret_cast<u32x4*>(k_obj0)[i] = u32x4{0u, 0u, 0u, 0u};
-      reinterpret_cast<u32x4*>(k_obj1)[i] = u32x4{0u, 0u, 0u, 0u};
+      for (char* p : {k_obj0, v_obj0, k_obj1, v_obj1}) reinterpret_cast<u32x4*>(p)[i] = u32x4{0u, 0u, 0u, 0u};
     }
   }
   // Scores in units of log2 e are `scale` times the product (the tanh of a soft
@@ -567,16 +568,22 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       f32x16 r;
 #pragma unroll
       for (int e = 0; e < 16; e++) r[e] = 0.f;
+      if constexpr (G::F32) {
+        u32x4 kf = read_k(ks, row, 0);
 #pragma unroll
-      for (int i = 0; i < G::C / 2; i++) {
-        const u32x4 kf = read_k(ks, row, i);
-        if constexpr (G::F32) {
+        for (int i = 0; i < G::C / 2; i++) {
+          const u32x4 next = read_k(ks, row, min(i + 1, G::C / 2 - 1));
 #pragma unroll
           for (int e = 0; e < 4; e++)
             r = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), r, 0, 0, 0);
-        } else {
-          r = mfma32<XT>(kf, qf[i], r);
+          kf = next;
+          // One read ahead: all of them would take the registers of Q.  Heads of 128 721 us with them all, 683
+          // so; of 64, where registers are left, 339 and 385 (300 tokens of 14636, 32 heads).
+          if constexpr (G::WGS == 1) __builtin_amdgcn_sched_barrier(0);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < G::C / 2; i++) r = mfma32<XT>(read_k(ks, row, i), qf[i], r);
       }
       return r;
     };
@@ -630,14 +637,23 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     };
     auto values = [&](const Lds* vs, int row) __attribute__((always_inline)) {
       if constexpr (G::F32) {
+        auto read = [&](int e, int dt) __attribute__((always_inline)) -> float {
+          const int key = 8 * (e / 4) + 4 * g + e % 4;
+          return lds_read<float>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
+        };
+        float v[G::DT], next[G::DT];
+#pragma unroll
+        for (int dt = 0; dt < G::DT; dt++) v[dt] = read(0, dt);
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-          const int key = 8 * (e / 4) + 4 * g + e % 4;
+#pragma unroll
+          for (int dt = 0; dt < G::DT; dt++) next[dt] = read(min(e + 1, 15), dt);
 #pragma unroll
           for (int dt = 0; dt < G::DT; dt++) {
-            const float v = lds_read<float>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[dt], s[e], o[dt], 0, 0, 0);
+            v[dt] = next[dt];
           }
+          if constexpr (G::WGS == 1) __builtin_amdgcn_sched_barrier(0);
         }
       } else {
 #pragma unroll
@@ -660,27 +676,42 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         }
       }
     };
-    // The same where values that are not finite must count only for the rows that see their key: one key at a time
+    // The same where values that are not finite must count only for the rows that see their key: one
+    // key at a time, and 32 columns after the other (registers would be taken from the steps).
     auto values_safe = [&](const Lds* vs, int g) __attribute__((always_inline)) {
-      for (int i = 0; i < 16; i++) {
-        const float other = lane_xor<32>(s[0], lane);
-        for (int gg = 0; gg < 2; gg++) {
-          const int key = 8 * (i / 4) + 4 * gg + i % 4;
-          const float p = gg == g ? s[0] : other;
 #pragma unroll
-          for (int dt = 0; dt < G::DT; dt++)
+      for (int dt = 0; dt < G::DT; dt++) {
+        f32x16 ps = s;
+#pragma unroll 1
+        for (int i = 0; i < 16; i++) {
+          const float other = lane_xor<32>(ps[0], lane);
+#pragma unroll 1
+          for (int gg = 0; gg < 2; gg++) {
+            const int key = 8 * (i / 4) + 4 * gg + i % 4;
+            const float p = gg == g ? ps[0] : other;
+            int at = (key * 128 + g * 4 * G::ES) ^ (swizzle_v(key) * 16);
+            asm volatile("" : "+v"(at));
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-              const int d = 32 * dt + 8 * (e / 4) + 4 * g + e % 4, ch = d / G::CE;
-              const Lds* vp = vs + ((ch / 8 * kKeys + key) * 128 + ((ch & 7) ^ swizzle_v(key)) * 16 + d % G::CE * G::ES);
-              float v;
-              if constexpr (G::F32) v = lds_read<float>(vp);
-              else v = half<XT>(lds_read<uint16_t>(vp), 0);
-              o[dt][e] = p == 0.f ? o[dt][e] : fmaf(p, v, o[dt][e]);
+            for (int q = 0; q < 4; q++) {  // columns 32 dt + 8 q + 4 g and the three after it
+              const int ch = (32 * dt + 8 * q) / G::CE;
+              const Lds* vp = vs + ((at ^ (ch & 7) * 16) + (32 * dt + 8 * q) / (8 * G::CE) * kKeys * 128);
+              float v[4];
+              if constexpr (G::F32) {
+                const f32x4 w = lds_read<f32x4>(vp);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = w[e];
+              } else {
+                const u32x2 w = lds_read<u32x2>(vp);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = half<XT>(w[e / 2], e % 2);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e++) o[dt][4 * q + e] = p == 0.f ? o[dt][4 * q + e] : fmaf(p, v[e], o[dt][4 * q + e]);
             }
-        }
+          }
 #pragma unroll
-        for (int e = 0; e < 15; e++) s[e] = s[e + 1];
+          for (int e = 0; e < 15; e++) ps[e] = ps[e + 1];
+        }
       }
     };
     auto reset = [&]() __attribute__((always_inline)) {
