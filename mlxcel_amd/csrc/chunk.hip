@@ -478,13 +478,25 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     const char* qp = static_cast<const char*>(a.q) +
                      ((int64_t)(sq.first + tok0 + my_tok) * a.q_tok + (head0 + my_row - my_tok * heads) * a.q_head) * G::ES;
     u32x4 qf[G::C / 2];
+    // Q is asked for behind the first K and looked at when that is there, not before (3% of short tiles)
+    auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < G::C / 2; i++) {
-      const int d = (2 * i + g) * G::CE;
-      const u32x4_e v = *reinterpret_cast<const u32x4_e*>(qp + (d < a.D ? d : 0) * G::ES);
-      qf[i] = d < a.D ? u32x4{v[0], v[1], v[2], v[3]} : u32x4{0u, 0u, 0u, 0u};
-      if (a.scale < 0.f) qf[i] ^= G::F32 ? 0x80000000u : 0x80008000u;
-    }
+      for (int i = 0; i < G::C / 2; i++) {
+        const int d = (2 * i + g) * G::CE;
+        const u32x4_e v = *reinterpret_cast<const u32x4_e*>(qp + (DP == a.D || d < a.D ? d : 0) * G::ES);
+        qf[i] = u32x4{v[0], v[1], v[2], v[3]};
+      }
+    };
+    auto finish_q = [&]() __attribute__((always_inline)) {
+      if (DP != a.D) {
+#pragma unroll
+        for (int i = 0; i < G::C / 2; i++) qf[i] = (2 * i + g) * G::CE < a.D ? qf[i] : u32x4{0u, 0u, 0u, 0u};
+      }
+      if (a.scale < 0.f) {
+#pragma unroll
+        for (int i = 0; i < G::C / 2; i++) qf[i] ^= G::F32 ? 0x80000000u : 0x80008000u;
+      }
+    };
     f32x16 o[G::DT];
     float m, l, off;  // off: what is added to a score before its exponential is taken
 
@@ -821,9 +833,11 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       for (int t = 0; t < G::KT; t++) half_step(ks, vs, 32 * t, k + 32 * t);
     };
     reset();
+    load_q();
     bring(k_lds0, v_lds0);
     look(k0 + 32 + kKeys);
     step_barrier();
+    finish_q();
     if (seen(k0)) {
       s = products(k_lds1, 0);
       largest();
