@@ -6,8 +6,8 @@
 //   x' += bias                                   for tokens with one
 //   x' = -inf                                    for tokens whose bit of the mask is 0
 //
-// A logit is read and written once, which is the floor; beyond that it takes the
-// vector operations of looking through the history.  A workgroup takes 16 bytes of one
+// A logit is read and written once, which is the floor; beyond that it takes
+// looking through the history.  A workgroup takes 16 bytes of one
 // row a thread and counts the history's tokens that fall into them in LDS, a word a
 // token: whole numbers, so the order of the atomic operations does not matter.  Of
 // several biases of one token the last in the list counts: LDS keeps the largest
@@ -40,8 +40,8 @@ constexpr int kChunk = kThreads * (XT == GEN_F32 ? 4 : 8);
 // One workgroup: logits [first, first + CHUNK) of row t, 16 bytes a thread.  All that does not
 // depend on something else is asked for first: the logits, the mask, the beginning of the
 // history and of the biases, the row's numbers.  128 rows of 151936 in bfloat16 with 4000 tokens
-// of history, 300 biases and a mask: 28.5 us (81 MB), of which 11 are the history past its first
-// 1024 tokens, a dozen vector operations each in every workgroup of a row.  Every thread working out its own logits instead of a
+// of history, 300 biases and a mask: 28 us (81 MB), of which 11 are the history past its first
+// 1024 tokens, a dozen vector operations and a wait for LDS each in every workgroup of a row.  Every thread working out its own logits instead of a
 // list, in which most lanes wait for the few that have one: 35; the list made from the words afterwards: 29.8;
 // the whole history asked for ahead: 28.5, but a mask alone then takes 5.3 instead of 4.7; workgroups of 512 (1024) threads,
 // half (a quarter) of the looking through the history: 30.3 (39.7); two (four) times 16 bytes a thread: 40 (67), the tables

@@ -27,11 +27,11 @@
 //
 // Many new tokens are bound by the matrix instructions, at the clock that the
 // card keeps under them: 2048 tokens of 32768 of 32 heads of 128 (8 key heads) in
-// bfloat16 1427 us, that is 746 TFLOP/s or, with P's second number counted, 1119
+// bfloat16 1400 us, that is 762 TFLOP/s or, with P's second number counted, 1144
 // (the matrix instructions alone: 1170 us).  Few are bound by HBM
 // and by the join of what was cut: 16 sequences of 5 tokens over 43000 keys of 4
-// key heads 44 us for 88 MB.  Short tiles (a window of 128 tokens) are bound by their vector
-// operations and by what a tile's start waits for: five prompts of 1500 tokens of 64 heads of 64, 94 us.
+// key heads 45 us for 88 MB.  Short tiles (a window of 128 tokens) are bound by their vector
+// operations and by what a tile's start waits for: five prompts of 1500 tokens of 64 heads of 64, 90 us.
 //
 // The work is cut evenly whatever the lengths: a tile counts its keys and kAround
 // more, and workgroup w takes [w n, (w + 1) n) of all tiles laid end to end,
