@@ -80,14 +80,16 @@ struct Geo {
   static constexpr int C = DP / CE;             // 16-byte chunks of a row
   static constexpr int NC = (C + 7) / 8;        // blocks of 8 chunks
   static constexpr int DT = DP / 32;            // 32-column tiles of O
-  static constexpr int KEYS = DP * ES <= 512 ? 64 : 32;  // of a step
+  static constexpr int KEYS = DP * ES <= (F32 ? 256 : 512) ? 64 : 32;  // of a step
   static constexpr int KT = KEYS / 32;
   // A step in LDS: K, then V; each in blocks [8 chunks of the row][KEYS rows][128 bytes],
   // so that a wave's 64 lanes fill 8 rows of a block in their order.
   static constexpr int TILE = NC * KEYS * 128;
   // Workgroups a CU holds: by registers.  16-bit heads of 64, 2 instead of 3: short tiles (five
   // prompts of 1500 with a window of 128) take 109 us instead of 96, long ones (2048 tokens of 32768) 1002 instead of 1015.
-  static constexpr int WGS = DP * ES <= 128 ? 3 : DP * ES <= 256 ? 2 : 1;
+  // float32 heads of 96 (128), 64 keys a step and one workgroup instead of 32 keys and two: 300 tokens
+  // of 14636 590 (747) us instead of 550 (710), 5 new ones of each of 16 sequences 114 (141) instead of 102 (137).
+  static constexpr int WGS = DP * ES <= 128 ? 3 : DP * ES <= (F32 ? 512 : 256) ? 2 : 1;
 };
 // Chunk p of row r of a block lies at place p ^ swizzle(r).  K is read one chunk
 // of 16 rows at a time, which then hit all banks; V four rows of 64 bytes.
@@ -592,9 +594,9 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           for (int e = 0; e < 4; e++)
             r = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), r, 0, 0, 0);
           kf = next;
-          // One read ahead: all of them would take the registers of Q.  Heads of 128 721 us with them all, 683
-          // so; of 64, where registers are left, 339 and 385 (300 tokens of 14636, 32 heads).
-          if constexpr (G::WGS == 1) __builtin_amdgcn_sched_barrier(0);
+          // One read ahead: all of them would take the registers of Q (300 tokens of 14636, 32 heads
+          // of 192: 1090 us instead of 1050; of 64, where registers are left, the same).
+          __builtin_amdgcn_sched_barrier(0);
         }
       } else {
 #pragma unroll
@@ -668,7 +670,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
             o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[dt], s[e], o[dt], 0, 0, 0);
             v[dt] = next[dt];
           }
-          if constexpr (G::WGS == 1) __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_sched_barrier(0);
         }
       } else {
 #pragma unroll
