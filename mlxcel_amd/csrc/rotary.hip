@@ -79,7 +79,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   // first element of unit u, and whether all of it is there
   auto first_of = [&](int u) -> int { return u < rot ? u * W : 2 * a.n + (u - rot) * W; };
   auto whole = [&](int u) -> bool { return (u < rot ? pairs : a.D) - first_of(u) >= W; };
-  for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+  // tokens without a sign: the step past the last of 2^31 - 1 stays below 2^32
+  for (uint32_t t = blockIdx.x; t < (uint32_t)a.T; t += gridDim.x) {
     const int pos = a.positions[t];
     // where the token's keys and values go (-1: nowhere)
     int pid = -1, off = 0;
