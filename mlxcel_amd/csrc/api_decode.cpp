@@ -745,7 +745,8 @@ mlxq_status mlxq_rotary_frequencies(int32_t dims, double base, int32_t scaling, 
       if (scaling == MLXQ_ROTARY_BANDS) keep = std::min(std::max((original * f / turn - low) / (high - low), 0.0), 1.0);
       if (scaling == MLXQ_ROTARY_RAMP)
         keep = 1.0 - std::min(std::max((i - first) / std::max(last - first, 1e-3), 0.0), 1.0);
-      inv_freq[i] = (float)(keep * f + (1.0 - keep) * f / factor);
+      // nothing is divided where all is kept: a factor that the scaling does not name may be anything
+      inv_freq[i] = (float)(keep < 1.0 ? keep * f + (1.0 - keep) * f / factor : f);
     }
     *attention_factor = scaling == MLXQ_ROTARY_RAMP ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
   });
