@@ -22,8 +22,9 @@
 // would leave out 2^-9, as much as the result's own rounding, for a third of the
 // matrix work.
 //
-// Values that are not finite would reach the rows that do not see their key (0 inf):
-// a tile whose results are not all finite is worked out again, where keys are hidden one at a time.
+// Values that are not finite would reach the rows that do not see their key (0 inf), and scores past
+// 2^25 would take probabilities out of their type: a tile whose results are not all finite, or one of whose rows has a
+// largest probability far from 1, is worked out again, where keys are hidden one at a time and exponents are exact.
 //
 // Many new tokens are bound by the matrix instructions, at the clock that the
 // card keeps under them: 2048 tokens of 32768 of 32 heads of 128 (8 key heads) in
@@ -652,6 +653,21 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       }
       l += sum;
     };
+    // The same with the product of large scores rounded as the maximum was: the largest exponent is kLift itself.
+    // exponentials() takes the product as it is, and the exponents of a row are off by half a step of its maximum
+    // (2^22: 1/4), all by the same.
+    auto exponentials_safe = [&]() __attribute__((always_inline)) {
+      const float from = m == -INFINITY ? 0.f : m;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        float x = s[e] * scale;
+        asm volatile("" : "+v"(x));  // or the product and the difference are one operation again
+        s[e] = __builtin_amdgcn_exp2f(fabsf(from) < 4194304.f ? fmaf(s[e], scale, off) : (x - from) + kLift<XT>);
+        sum += s[e];
+      }
+      l += sum;
+    };
     auto values = [&](const Lds* vs, int row) __attribute__((always_inline)) {
       if constexpr (G::F32) {
         auto read = [&](int e, int dt) __attribute__((always_inline)) -> float {
@@ -907,7 +923,10 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     for (int i = 0; i < G::DT; i++)
 #pragma unroll
       for (int e = 0; e < 16; e++) x = fmaf(o[i][e], 0.f, x);
-    if (__syncthreads_or(r0 + c < rows && !isfinite(x))) {
+    // A row's largest probability is 2^kLift, more or less by a factor of 2 while scores are below 2^25 (in
+    // base 2).  Of larger ones it may have left the type: upwards it is found in x, downwards here.
+    const float least = kLift<XT> == 0.f ? 0.25f : 4096.f;
+    if (__syncthreads_or(r0 + c < rows && (!isfinite(x) || (l < least && m != -INFINITY)))) {
       // again, 32 keys at a time
       reset();
       int g_safe = g;
@@ -924,7 +943,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           largest();
           special(k);
           grow();
-          exponentials();
+          exponentials_safe();
           if (k + 32 > first_hi || k < last_lo) values_safe(v_lds1, g_safe);
           else values(v_lds1, 0);
         }
