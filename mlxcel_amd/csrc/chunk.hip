@@ -23,8 +23,9 @@
 // matrix work.
 //
 // Values that are not finite would reach the rows that do not see their key (0 inf), and scores past
-// 2^25 would take probabilities out of their type: a tile whose results are not all finite, or one of whose rows has a
-// largest probability far from 1, is worked out again, where keys are hidden one at a time and exponents are exact.
+// 2^25 would take probabilities out of their type: a tile whose results are not all finite, or one of whose rows has
+// a largest probability far from 1, is worked out again, where exponents are exact and 32 keys with such a value
+// are taken one at a time, each for the rows that see it.
 //
 // Many new tokens are bound by the matrix instructions, at the clock that the
 // card keeps under them: 2048 tokens of 32768 of 32 heads of 128 (8 key heads) in
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
   // does not wait for it (it did, at 1700 us for 2048 tokens of 32768).
   __shared__ __align__(16) char k_obj0[G::TILE], v_obj0[G::TILE], k_obj1[G::TILE], v_obj1[G::TILE];
   Lds *const k_lds0 = (Lds*)k_obj0, *const v_lds0 = (Lds*)v_obj0, *const k_lds1 = (Lds*)k_obj1, *const v_lds1 = (Lds*)v_obj1;
-  __shared__ uint32_t arrived;
+  __shared__ uint32_t arrived, odd;  // odd: the tile has to be worked out again
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, g = lane >> 5;
   // neighbours in the order of the keys on one XCD
@@ -582,6 +583,11 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       const u32x2 x = read_transposed(p), y = read_transposed(p + 8 * 128);
       return u32x4{x[0], x[1], y[0], y[1]};
     };
+    // the lane's e-th key of that column, 32-bit types
+    auto read_v32 = [&](const Lds* vs, int row, int e, int dt) __attribute__((always_inline)) -> float {
+      const int key = 8 * (e / 4) + 4 * g + e % 4;
+      return lds_read<float>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
+    };
     auto products = [&](const Lds* ks, int row) __attribute__((always_inline)) -> f32x16 {
       f32x16 r;
 #pragma unroll
@@ -670,10 +676,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     };
     auto values = [&](const Lds* vs, int row) __attribute__((always_inline)) {
       if constexpr (G::F32) {
-        auto read = [&](int e, int dt) __attribute__((always_inline)) -> float {
-          const int key = 8 * (e / 4) + 4 * g + e % 4;
-          return lds_read<float>(vs + ((dt * kKeys + row + key) * 128 + ((c >> 2) ^ swizzle_v(e)) * 16 + (c & 3) * 4));
-        };
+        auto read = [&](int e, int dt) __attribute__((always_inline)) -> float { return read_v32(vs, row, e, dt); };
         float v[G::DT], next[G::DT];
 #pragma unroll
         for (int dt = 0; dt < G::DT; dt++) v[dt] = read(0, dt);
@@ -709,9 +712,10 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         }
       }
     };
-    // The same where values that are not finite must count only for the rows that see their key: one
-    // key at a time, and 32 columns after the other (registers would be taken from the steps).
-    auto values_safe = [&](const Lds* vs, int g) __attribute__((always_inline)) {
+    // The same where values that are not finite must count only for the rows that see their key (bit e of `see`:
+    // the lane's e-th key): one key at a time, and 32 columns after the other (registers would be taken from the steps).
+    auto values_safe = [&](const Lds* vs, int g, uint32_t see) __attribute__((always_inline)) {
+      const uint32_t see_other = lane_xor<32>(see, lane);
 #pragma unroll
       for (int dt = 0; dt < G::DT; dt++) {
         f32x16 ps = s;
@@ -722,6 +726,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           for (int gg = 0; gg < 2; gg++) {
             const int key = 8 * (i / 4) + 4 * gg + i % 4;
             const float p = gg == g ? ps[0] : other;
+            const bool sees = (gg == g ? see : see_other) >> i & 1u;
             int at = (key * 128 + g * 4 * G::ES) ^ (swizzle_v(key) * 16);
             asm volatile("" : "+v"(at));
 #pragma unroll
@@ -739,13 +744,37 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
                 for (int e = 0; e < 4; e++) v[e] = half<XT>(w[e / 2], e % 2);
               }
 #pragma unroll
-              for (int e = 0; e < 4; e++) o[dt][4 * q + e] = p == 0.f ? o[dt][4 * q + e] : fmaf(p, v[e], o[dt][4 * q + e]);
+              for (int e = 0; e < 4; e++) o[dt][4 * q + e] = sees ? fmaf(p, v[e], o[dt][4 * q + e]) : o[dt][4 * q + e];
             }
           }
 #pragma unroll
           for (int e = 0; e < 15; e++) ps[e] = ps[e + 1];
         }
       }
+    };
+    // Whether some of the 32 V rows' values is not finite, each looked at by the lane that multiplies it.
+    auto wild = [&](const Lds* vs, int c) __attribute__((always_inline)) -> bool {
+      uint32_t kExp = G::F32 ? 0x7F800000u : XT == GEN_BF16 ? 0x7F80u : 0x7C00u;
+      int head = a.D - c;
+      asm volatile("" : "+s"(kExp), "+v"(head));  // or they would be in registers all through the steps
+      bool found = false;
+#pragma unroll
+      for (int dt = 0; dt < G::DT; dt++) {
+        bool here = false;
+        if constexpr (G::F32) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) here |= (__float_as_uint(read_v32(vs, 0, e, dt)) & kExp) == kExp;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const u32x4 w = read_v(vs, 0, u, dt);
+#pragma unroll
+            for (int e = 0; e < 4; e++) here |= (w[e] & kExp) == kExp || (w[e] >> 16 & kExp) == kExp;
+          }
+        }
+        found |= here && 32 * dt < head;
+      }
+      return __any(found);
     };
     auto reset = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -756,6 +785,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       look_row(k0, G::KT);
       look(k0 + 32);
       __syncthreads();  // the last tile's steps have been read
+      if (tid == 0) odd = 0u;
       bring_k(G::KT, k_lds1, 0);
     };
     // The values of 32 keys and the scores of the 32 after them, for 16-bit types in an order
@@ -926,11 +956,13 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     // A row's largest probability is 2^kLift, more or less by a factor of 2 while scores are below 2^25 (in
     // base 2).  Of larger ones it may have left the type: upwards it is found in x, downwards here.
     const float least = kLift<XT> == 0.f ? 0.25f : 4096.f;
-    if (__syncthreads_or(r0 + c < rows && (!isfinite(x) || (l < least && m != -INFINITY)))) {
+    if (r0 + c < rows && (!isfinite(x) || (l < least && m != -INFINITY))) odd = 1u;
+    __syncthreads();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd), 0)) {
       // again, 32 keys at a time
       reset();
-      int g_safe = g;
-      asm volatile("" : "+v"(g_safe));
+      int g_safe = g, c_safe = c;
+      asm volatile("" : "+v"(g_safe), "+v"(c_safe));
       for (int k = k0; k < k1; k += 32) {
         if (k > k0) {
           bring_k(0, k_lds1, 0);
@@ -943,8 +975,11 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
           largest();
           special(k);
           grow();
+          uint32_t see = 0u;  // a score of -inf is a key that is not seen, or one that has no part
+#pragma unroll
+          for (int e = 15; e >= 0; e--) see = 2 * see + (s[e] != -INFINITY ? 1u : 0u);
           exponentials_safe();
-          if (k + 32 > first_hi || k < last_lo) values_safe(v_lds1, g_safe);
+          if (wild(v_lds1, c_safe)) values_safe(v_lds1, g_safe, see);
           else values(v_lds1, 0);
         }
         step_barrier();
