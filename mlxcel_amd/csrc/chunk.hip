@@ -424,11 +424,15 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
 #pragma unroll
     for (int i = 0; i < 4; i++) k_lane[i] = c * 128 + ((2 * i + g) ^ swizzle_k(c)) * 16;
 #pragma unroll
-    for (int i = 0; i < 2; i++) v_lane[i] = r * 128 + ((4 * i + ch) ^ swizzle_v(r)) * 16 + (i16 & 1) * 8;
+    for (int i = 0; i < 2; i++) {
+      // of one block past the head the last chunk of the head instead
+      const int at = DP == 64 ? min(4 * i + ch, a.D / G::CE - 1) : 4 * i + ch;
+      v_lane[i] = r * 128 + (at ^ swizzle_v(r)) * 16 + (i16 & 1) * 8;
+    }
     asm volatile("" : "+v"(k_lane[0]), "+v"(k_lane[1]), "+v"(k_lane[2]), "+v"(k_lane[3]), "+v"(v_lane[0]), "+v"(v_lane[1]));
   }
-  // The chunks past the head are zero and stay so: K's count in the scores, and values that are
-  // not finite, whatever lay there, would send every tile the slow way.
+  // The chunks past the head are zero and stay so: K's count in the scores, and values that are not finite, whatever
+  // lay there, would send every tile the slow way.  (V's of a kernel of one block, where results go through, are not read.)
   if (DP != a.D) {
     for (int i = tid; i < G::TILE / 16; i += 256) {
       for (char* p : {k_obj0, v_obj0, k_obj1, v_obj1}) reinterpret_cast<u32x4*>(p)[i] = u32x4{0u, 0u, 0u, 0u};
@@ -1024,9 +1028,12 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
               }
           }
         } else {
-          // through LDS, so that whole rows are written: chunk i of row r at place i ^ swizzle(r); the V rows have been read
+          // through LDS, so that whole rows are written: chunk i of row r at place i ^ swizzle(r); the step's rows have
+          // been read.  In blocks that the head fills: what lies past it stays.
           constexpr int LOW = (G::C & -G::C) < 8 ? (G::C & -G::C) : 8;
-          Lds* mine = (wave < 2 ? v_lds0 : v_lds1) + (wave & 1) * (32 * G::C * 16);
+          static_assert(DP == 64 || 32 * G::C * 16 <= (G::NC - 1) * kKeys * 128, "");
+          Lds* mine = DP == 64 ? (wave < 2 ? v_lds0 : v_lds1) + (wave & 1) * (32 * G::C * 16)
+                               : wave < 2 ? (wave == 0 ? v_lds0 : v_lds1) : (wave == 2 ? k_lds0 : k_lds1);
 #pragma unroll
           for (int dt = 0; dt < G::DT; dt++)
 #pragma unroll
