@@ -449,7 +449,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void paged_attention_kerne
         for (int t = 0; t < G::KT; t++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            s[t][r] = exp2_diff(s[t][r] + kLift<XT>, m);
+            // the lift comes last: beside scores past 2^25 it would be rounded to 16, and the largest p to infinity
+            s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - (m == -INFINITY ? 0.f : m) + kLift<XT>);
             l += s[t][r];
           }
         if constexpr (G::F32) {
