@@ -142,28 +142,31 @@ class PagedDecoder:
         answers, score = [ids.reshape(-1)], top.reshape(-1)
         live = (self.rows >= n) & (self.rows < n * (1 + ways))
         tokens = torch.zeros(len(self.rows), dtype=torch.int64, device=dev)
-        # what each answer's choice looks back on: the prompt, then the answer
-        longest = max(map(len, prompts))
-        history = torch.zeros(n * ways, longest + steps, dtype=torch.int32, device=dev)
-        for i, p in enumerate(prompts):
-            history[i * ways:(i + 1) * ways, :len(p)] = torch.tensor(p, dtype=torch.int32, device=dev)
-        seen = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=dev).repeat_interleave(ways)
-        penalty = torch.full((n * ways,), repetition, device=dev)
-        each = torch.arange(n * ways, device=dev)
+        if repetition != 1.0:
+            # what each answer's choice looks back on: the prompt, then the answer
+            longest = max(map(len, prompts))
+            history = torch.zeros(n * ways, longest + steps, dtype=torch.int32, device=dev)
+            for i, p in enumerate(prompts):
+                history[i * ways:(i + 1) * ways, :len(p)] = torch.tensor(p, dtype=torch.int32, device=dev)
+            seen = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=dev).repeat_interleave(ways)
+            penalty = torch.full((n * ways,), repetition, device=dev)
+            each = torch.arange(n * ways, device=dev)
         for _ in range(steps - 1):
-            history[each, seen.long()] = answers[-1]
-            seen = seen + 1
             tokens[n:n + n * ways] = answers[-1].long()
             out, granted = self.step(tokens, live)
             if not bool(granted.all()):
                 raise RuntimeError("the cache has no page left")
             out = out[n:n + n * ways]
-            choice = out
             if repetition != 1.0:
+                history[each, seen.long()] = answers[-1]
+                seen = seen + 1
                 choice = mq.adjust_logits(out, history=history, history_lengths=seen, repetition=penalty)
-            _, _, _, ids = mq.token_logprobs(choice, answers[-1][:, None].contiguous(), top_k=1)
+                _, _, _, ids = mq.token_logprobs(choice, answers[-1][:, None].contiguous(), top_k=1)
+                given, _ = mq.token_logprobs(out, ids.contiguous())[:2]
+            else:
+                _, _, given, ids = mq.token_logprobs(out, answers[-1][:, None].contiguous(), top_k=1)
             answers.append(ids[:, 0].contiguous())
-            score = score + mq.token_logprobs(out, ids.contiguous())[0][:, 0]
+            score = score + given[:, 0]
         mq.cache_free(self.table, self.lengths, self.refs, dst, self.page)
         answers = torch.stack(answers, 1).tolist()
         return [(i // ways, a, s) for i, (a, s) in enumerate(zip(answers, score.tolist()))]
