@@ -357,8 +357,9 @@ mlxq_status mlxq_fused_moe_geglu(const mlxq_array* x, const mlxq_array* indices,
  * 256.  table (B, n), lengths (B): a length is cut to the n pages, one of 0 or
  * less gives zeros.  window > 0: only the last `window` keys.  sinks: NULL or
  * float32 (query heads), logits that join each head's sum without a value.
- * Keys whose score is -inf have no part in it; scores (and sink) that are all
- * -inf give NaN, as softmax of them.
+ * Keys whose score is -inf have no part in it (a value of theirs that is not
+ * finite gives NaN); scores (and sink) that are all -inf give NaN, as softmax of
+ * them.
  * Keys outside the sequence are not read; page numbers out of range are
  * clamped.  Scores, probabilities and sums are held in 32 bits (in a product of
  * 16-bit values a probability differs by at most 2^-24 of itself or 2^-39 of the
@@ -446,8 +447,9 @@ mlxq_status mlxq_token_logprobs(const mlxq_array* logits, const mlxq_array* toke
  * result does not depend on how a prompt is cut into calls, up to the order of 32-bit sums.
  * Types, layouts, sinks and infinities as there; in a product of 16-bit values a
  * probability differs by at most 2^-17 of itself (bfloat16), 2^-23 of itself or
- * 2^-39 of the largest (float16).  Values that are not finite among a token's
- * keys or its neighbours' make the call slower, not other tokens' results wrong. */
+ * 2^-39 of the largest (float16).  A value that is not finite reaches the tokens
+ * that see its key with a score above -inf, however small its probability, and
+ * no others; such values, and scores past 2^24, may make the call slower. */
 mlxq_status mlxq_paged_attention_chunk(const mlxq_array* q, const mlxq_array* k_pool,
                                        const mlxq_array* v_pool, const mlxq_array* table,
                                        const mlxq_array* lengths, const mlxq_array* starts,

@@ -40,12 +40,14 @@ constexpr int kChunk = kThreads * (XT == GEN_F32 ? 4 : 8);
 // One workgroup: logits [first, first + CHUNK) of row t, 16 bytes a thread.  All that does not
 // depend on something else is asked for first: the logits, the mask, the beginning of the
 // history and of the biases, the row's numbers.  128 rows of 151936 in bfloat16 with 4000 tokens
-// of history, 300 biases and a mask: 28 us (81 MB), of which 11 are the history past its first
-// 1024 tokens, a dozen vector operations and a wait for LDS each in every workgroup of a row.  Every thread working out its own logits instead of a
-// list, in which most lanes wait for the few that have one: 35; the list made from the words afterwards: 29.8;
-// the whole history asked for ahead: 28.5, but a mask alone then takes 5.3 instead of 4.7; workgroups of 512 (1024) threads,
-// half (a quarter) of the looking through the history: 30.3 (39.7); two (four) times 16 bytes a thread: 40 (67), the tables
-// leave too few waves.
+// of history, 300 biases and a mask: 27 us a launch among others (81 MB; 27.6 traced), of which 11
+// are the history past its first 1024 tokens, a dozen vector operations and a wait for LDS each
+// in every workgroup of a row.  Others, where this took 28.3: every thread working out its own
+// logits instead of a list, in which most lanes wait for the few that have one, 35; the list made
+// from the words afterwards 29.8; the whole history asked for ahead 28.5, but a mask alone then
+// takes 5.3 instead of 4.7; workgroups of 512 (1024) threads, half (a quarter) of the looking
+// through the history, 30.3 (39.7); two (four) times 16 bytes a thread 40 (67), the tables leave
+// too few waves.
 template <int XT>
 __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const AdjustArgs a) {
   constexpr int ES = XT == GEN_F32 ? 4 : 2, W = 16 / ES, CHUNK = kChunk<XT>;

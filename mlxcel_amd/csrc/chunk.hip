@@ -29,11 +29,11 @@
 //
 // Many new tokens are bound by the matrix instructions, at the clock that the
 // card keeps under them: 2048 tokens of 32768 of 32 heads of 128 (8 key heads) in
-// bfloat16 1400 us, that is 762 TFLOP/s or, with P's second number counted, 1144
-// (the matrix instructions alone: 1170 us).  Few are bound by HBM
+// bfloat16 1400 us (1385 to 1470 by the card), that is 762 TFLOP/s or, with P's second number
+// counted, 1144 (the matrix instructions alone: 1170 us).  Few are bound by HBM
 // and by the join of what was cut: 16 sequences of 5 tokens over 43000 keys of 4
-// key heads 45 us for 88 MB.  Short tiles (a window of 128 tokens) are bound by their vector
-// operations and by what a tile's start waits for: five prompts of 1500 tokens of 64 heads of 64, 90 us.
+// key heads 42 us for 88 MB.  Short tiles (a window of 128 tokens) are bound by their vector
+// operations and by what a tile's start waits for: five prompts of 1500 tokens of 64 heads of 64, 83 us.
 //
 // The work is cut evenly whatever the lengths: a tile counts its keys and kAround
 // more, and workgroup w takes [w n, (w + 1) n) of all tiles laid end to end,
@@ -88,9 +88,10 @@ struct Geo {
   // so that a wave's 64 lanes fill 8 rows of a block in their order.
   static constexpr int TILE = NC * KEYS * 128;
   // Workgroups a CU holds: by registers.  16-bit heads of 64, 2 instead of 3: short tiles (five
-  // prompts of 1500 with a window of 128) take 109 us instead of 96, long ones (2048 tokens of 32768) 1002 instead of 1015.
-  // float32 heads of 96 (128), 64 keys a step and one workgroup instead of 32 keys and two: 300 tokens
-  // of 14636 590 (747) us instead of 550 (710), 5 new ones of each of 16 sequences 114 (141) instead of 102 (137).
+  // prompts of 1500 with a window of 128) take 101 us instead of 83, 5 tokens of each of 16 sequences
+  // 28.2 instead of 27.0, long ones (2048 tokens of 32768) 899 either way.  float32 heads of 96 (128), 64
+  // keys a step and one workgroup instead of 32 keys and two: 300 tokens of 14636 537 (681) us
+  // instead of 472 (630), 5 new ones of each of 16 sequences 112 (141) instead of 98 (135).
   static constexpr int WGS = DP * ES <= 128 ? 3 : DP * ES <= (F32 ? 512 : 256) ? 2 : 1;
 };
 // Chunk p of row r of a block lies at place p ^ swizzle(r).  K is read one chunk
@@ -408,7 +409,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
   if (!at.ahead_of(end)) return;
 
   // Of two workgroups of a CU the older one's waves go first, and it is done at 3/4 of the
-  // time (205 of 270 us); so the younger one goes first in every other step.
+  // time (205 of 270 us); so the younger one goes first in every other step (three prompts of 1000 tokens
+  // beside 61 single tokens 254 us instead of 258, 2048 tokens of 32768 1390 instead of 1411).
   const bool later = blockIdx.x >= gridDim.x / 2;
   uint32_t minus_lo = XT == GEN_F16 ? 0xBF800000u : 0x0000BF80u, minus_hi = 0xBF800000u;
   asm volatile("" : "+s"(minus_lo), "+s"(minus_hi));
@@ -486,7 +488,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
     const char* qp = static_cast<const char*>(a.q) +
                      ((int64_t)(sq.first + tok0 + my_tok) * a.q_tok + (head0 + my_row - my_tok * heads) * a.q_head) * G::ES;
     u32x4 qf[G::C / 2];
-    // Q is asked for behind the first K and looked at when that is there, not before (3% of short tiles)
+    // Q is asked for behind the first K and looked at when that is there (before it: short tiles 81.9 us
+    // instead of 83.0, prompts beside single tokens 255 instead of 254)
     auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < G::C / 2; i++) {
@@ -533,7 +536,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
       return pid * page_bytes + in_page[t] * tok_bytes;
     };
     // Of a row only the last block may be part full.  It is looked at where the kernel's width has a part
-    // full one anyway, or the head is narrower (heads of 128 with a look in every step: 2048 tokens of 32768 2% slower).
+    // full one anyway, or the head is narrower (heads of 128 take the same with a look in every step: 2048
+    // tokens of 32768 1383 and 1388 us).
     constexpr bool kLook = G::C % 8 != 0;
     // a row to LDS without passing through registers
     auto rows_to_lds = [&](const char* from, int chunk, Lds* to, int row) __attribute__((always_inline)) {
@@ -606,7 +610,7 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
             r = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[i][e]), r, 0, 0, 0);
           kf = next;
           // One read ahead: all of them would take the registers of Q (300 tokens of 14636, 32 heads
-          // of 192: 1090 us instead of 1050; of 64, where registers are left, the same).
+          // of 192: 995 us instead of 984; of 64 and 128 within 1%; of 256 1391 instead of 1410).
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
@@ -1083,7 +1087,8 @@ __global__ __launch_bounds__(256, (Geo<XT, DP>::WGS)) void chunk_attention_kerne
         put_ml(part_at(w), wave, m - kLift<XT>, l);
       }
       // The last of up to kFlight neighbours to arrive joins them; more are joined in two steps, the
-      // root of their number at a time (16 sequences of 5 tokens over 43000 keys in all: 45 us, with up to 16 in the first step 50.5).
+      // root of their number at a time (16 sequences of 5 tokens over 43000 keys in all: 42.1 us, with
+      // up to 16 in the first step 46.8).
       auto last_of = [&](uint32_t* cnt, int of) __attribute__((always_inline)) -> bool {
         __builtin_amdgcn_s_waitcnt(0);  // this thread's partial stores have completed
         __syncthreads();

@@ -8,8 +8,9 @@
 // which is the bound; a workgroup takes one token's heads, so a token's n
 // angles are worked out once for all of them and shared through LDS, while 16 bytes (32 of
 // a pair of halves) a thread are on their way: 8191 tokens of 32 heads of 96 in 16 bits
-// (101 MB) 24 us, 4.2 TB/s, instead of 27.5 with the loads behind the angles.  A thread
-// for two (four) heads, so half (a quarter) of the angles and workgroups: 24.5 (33.2) us.
+// (101 MB) 23.3 us a launch among others, 4.3 TB/s (24.6 traced); with the loads behind the
+// angles 24.0.  A thread for two (four) heads, so half (a quarter) of the angles and
+// workgroups: 1.05 (1.4) times as long.
 //
 // The angle of a far position needs more than 32 bits (2^20 * 1.0f is off by
 // whole steps of 1/16): it is taken in turns in 64 bits, whole turns and
